@@ -186,6 +186,115 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
                         void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Operators of the training pass: the gradients of the two scans, dropout and
+ * the loss.  Device pointers, asynchronous on `stream`, no allocation: scratch
+ * is a caller-owned device buffer (256-byte aligned) of the size that the
+ * matching *_workspace function gives (0 for sizes that the operator refuses).
+ * It holds nothing between calls; calls that may overlap (other streams, other
+ * captured graphs) need a buffer each.
+ * ------------------------------------------------------------------------- */
+
+/*
+ * Gradients of yuf_wkv7_scan_f32 (the backward half of the reference operator,
+ * `yufmusicgen_rwkv7::backward`, yufmusicgen/cuda/rwkv7_clampw.cpp:40-63; with
+ * a carried state, which that one lacks).
+ *   r, w_raw, k, v, a, b, state_in : the forward call's inputs.
+ *   dy          : device [B, T, H, N], gradient of y.
+ *   dstate_out  : device [B, H, N, N], gradient of the final state, or NULL.
+ *   dr .. db    : device [B, T, H, N] outputs (none may alias an input).
+ *   dstate_in   : device [B, H, N, N], gradient of the initial state, or NULL;
+ *                 may alias dstate_out.
+ *   workspace   : yuf_wkv7_scan_backward_workspace(B, T, H, N) bytes.
+ * With G_t the gradient of S_t:  G_t += dy_t r_t^T;  dr = S_t^T dy, dv = G k,
+ * dk = G^T v, da = S_{t-1}^T (G b), db = G^T (S_{t-1} a),
+ * dd_j = sum_i G_ij S_{t-1,ij};  G_{t-1} = G_t (diag(d_t) + b_t a_t^T).
+ * Same head sizes and lengths as the scan.
+ */
+size_t yuf_wkv7_scan_backward_workspace(int B, int T, int H, int N);
+int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,
+                               const float *r, const float *w_raw, const float *k,
+                               const float *v, const float *a, const float *b,
+                               const float *state_in, const float *dy, const float *dstate_out,
+                               float *dr, float *dw_raw, float *dk, float *dv, float *da, float *db,
+                               float *dstate_in, void *workspace, void *stream);
+
+/*
+ * Gradients of yuf_rosa_scan_f32 (`yufmusicgen_rosa::backward`,
+ * yufmusicgen/cuda/rosa_householder.cpp:52-83, with the read gate as an option).
+ *   cand .. memory_in : the forward call's inputs; read_raw NULL where the read
+ *                       is ungated, memory_in NULL for a zero memory.
+ *   dread             : device [B, T, D], gradient of read_out.
+ *   dmemory           : device [B, D], gradient of memory_out, or NULL.
+ *   dcand, dwrite     : device [B, T, D]; dread_raw too where read_raw is given,
+ *                       else NULL.
+ *   ddecay, ddirection: device [D]: of lambda (post-sigmoid) and of u as it
+ *                       stands in H(x) = x - 2 (x.u) u (not renormalised);
+ *                       zero for B = 0.
+ *   dmemory_in        : device [B, D] or NULL; may alias dmemory.
+ *   workspace         : yuf_rosa_scan_backward_workspace(B, T, D) bytes.
+ * Supported D: 1 .. 1024.
+ */
+size_t yuf_rosa_scan_backward_workspace(int B, int T, int D);
+int yuf_rosa_scan_backward_f32(int B, int T, int D,
+                               const float *cand, const float *write, const float *read_raw,
+                               const float *decay, const float *direction, const float *memory_in,
+                               const float *dread, const float *dmemory,
+                               float *dcand, float *dwrite, float *dread_raw,
+                               float *ddecay, float *ddirection, float *dmemory_in,
+                               void *workspace, void *stream);
+
+/*
+ * Dropout with a generated mask (the reference block's nn.Dropout,
+ * yufmusicgen/config.py:82): out = (keep ? x / (1 - p) : 0) + residual.
+ *   x, out   : device [n] fp32, or bf16 bit patterns; residual [n] or NULL.
+ *              out may be x or residual.  Any element alignment.
+ *   p        : in [0, 1]; an element is dropped where its random word is below
+ *              p 2^32 (p = 1: always).
+ *   seed, counter, counter_dev : the mask: element i takes word i % 4 of
+ *              Philox4x32-10 with counter (i / 4, counter + *counter_dev) and key
+ *              seed.  counter_dev (device [1], or NULL for 0) is read when the
+ *              kernel runs, so a captured graph can be replayed with new masks.
+ * The gradient of x is the same call on the gradient of out without residual.
+ * bf16 sums in fp32 and rounds once.
+ */
+int yuf_dropout_f32(int64_t n, const float *x, const float *residual, double p, uint64_t seed,
+                    uint64_t counter, const uint64_t *counter_dev, float *out, void *stream);
+int yuf_dropout_bf16(int64_t n, const uint16_t *x, const uint16_t *residual, double p, uint64_t seed,
+                     uint64_t counter, const uint64_t *counter_dev, uint16_t *out, void *stream);
+
+enum { YUF_LOSS_NONE = 0, YUF_LOSS_MEAN = 1, YUF_LOSS_SUM = 2 };
+
+/*
+ * Cross-entropy of logits and token ids, and the logits' gradient in the same
+ * pass over them (the training loop's F.cross_entropy,
+ * yufmusicgen/training.py:295-306).
+ *   logits     : device [M, V] fp32 (or bf16), rows ld elements apart (ld >= V).
+ *   targets    : device [M] int32 or int64 (target_bits 32 or 64).  A row whose
+ *                target is ignore_index has loss 0 and gradient 0 and is not
+ *                read; a target outside [0, V) gives NaN in that row's loss and
+ *                gradient.  A row of nothing but -inf, or with a NaN or +inf,
+ *                gives NaN, as its softmax does.
+ *   reduction  : YUF_LOSS_NONE (loss [M]), _SUM or _MEAN over the rows that are
+ *                not ignored (loss [1]; no such row: NaN).
+ *   loss       : device fp32, or NULL where only the gradient is wanted.
+ *   dloss      : device, gradient of the loss: [M] without reduction, else [1];
+ *                NULL for ones.
+ *   dlogits    : device [M, V] of the logits' type, rows ld_out apart, or NULL;
+ *                may be logits (then ld_out = ld).
+ *   workspace  : yuf_cross_entropy_workspace(M) bytes for _MEAN and _SUM.
+ * Exponentials and row sums in fp32, the sum over rows in fp64, in one order.
+ */
+size_t yuf_cross_entropy_workspace(int M);
+int yuf_cross_entropy_f32(int M, int V, const float *logits, int64_t ld, const void *targets,
+                          int target_bits, int64_t ignore_index, int reduction, float *loss,
+                          const float *dloss, float *dlogits, int64_t ld_out, void *workspace,
+                          void *stream);
+int yuf_cross_entropy_bf16(int M, int V, const uint16_t *logits, int64_t ld, const void *targets,
+                           int target_bits, int64_t ignore_index, int reduction, float *loss,
+                           const float *dloss, uint16_t *dlogits, int64_t ld_out, void *workspace,
+                           void *stream);
+
+/* ---------------------------------------------------------------------------
  * Checkpoints (.yuf).  Replaces `Checkpoint::load / tensor / tensor_dims`
  * (vulkan/src/checkpoint.rs:90-176).
  * ------------------------------------------------------------------------- */

@@ -1,0 +1,121 @@
+"""The training pass's operators without a GPU: what they refuse, before any device call."""
+
+import ctypes
+
+import pytest
+import torch
+
+from yufmusicgen_amd import ops
+from yufmusicgen_amd._lib import lib
+
+DUMMY = 256  # never dereferenced: each call returns before any device work
+
+
+def refused(status, *words):
+    message = lib().yuf_last_error().decode()
+    assert status == -1, (status, message)
+    assert all(w in message for w in words), message
+
+
+def test_wkv7_backward_refusals():
+    call = lib().yuf_wkv7_scan_backward_f32
+    full = [DUMMY] * 17 + [None]
+    refused(call(1, 1, 1, 12, *full), "head size")
+    refused(call(-1, 1, 1, 40, *full), "negative")
+    refused(call(1, 1, 1, 40, *[None] * 18), "null")
+    refused(call(1, 0, 1, 40, *[None] * 18), "workspace")
+    refused(call(1, 1, 1, 40, *[DUMMY] * 16, None, None), "workspace")
+    refused(call(1, 1, 1 << 20, 40, *full), "H * N")
+    refused(call(1 << 14, 1 << 12, 1 << 10, 40, *full), "chunks")
+    for missing in (0, 1, 2, 3, 4, 5, 7, 9, 10, 11, 12, 13, 14):
+        args = list(full)
+        args[missing] = None
+        refused(call(1, 1, 1, 40, *args), "null")
+    assert call(0, 5, 3, 40, *[None] * 18) == 0 and call(5, 5, 0, 40, *[None] * 18) == 0
+    space = lib().yuf_wkv7_scan_backward_workspace
+    assert space(1, 16, 1, 12) == space(0, 16, 1, 40) == space(1, -1, 1, 40) == 0
+    assert space(1, 0, 1, 40) > 0 and space(8, 2048, 16, 40) > space(8, 1024, 16, 40)
+
+
+def test_rosa_backward_refusals():
+    call = lib().yuf_rosa_scan_backward_f32
+    full = [DUMMY] * 15 + [None]
+    refused(call(1, 1, 2048, *full), "D must be")
+    refused(call(1, 1, 0, *full), "D must be")
+    refused(call(1, -1, 64, *full), "negative")
+    for missing in (0, 1, 3, 4, 6, 8, 9, 11, 12):
+        args = list(full)
+        args[missing] = None
+        refused(call(1, 1, 64, *args), "null")
+    args = list(full)
+    args[10] = None  # dread_raw without its read_raw's gradient
+    refused(call(1, 1, 64, *args), "read_raw")
+    refused(call(1, 1, 64, *[DUMMY] * 14, None, None), "workspace")
+    refused(call(1 << 20, 1 << 20, 64, *full), "segments")
+    space = lib().yuf_rosa_scan_backward_workspace
+    assert space(1, 16, 1025) == space(0, 16, 64) == space(1, -1, 64) == 0 and space(1, 0, 64) > 0
+
+
+def test_dropout_refusals():
+    for name in ("yuf_dropout_f32", "yuf_dropout_bf16"):
+        call = getattr(lib(), name)
+        refused(call(-1, DUMMY, None, 0.5, 0, 0, None, DUMMY, None), "negative")
+        for p in (-0.1, 1.1, float("nan")):
+            refused(call(8, DUMMY, None, p, 0, 0, None, DUMMY, None), "p must be")
+        refused(call(8, None, None, 0.5, 0, 0, None, DUMMY, None), "null")
+        refused(call(8, DUMMY, None, 0.5, 0, 0, None, None, None), "null")
+        refused(call(1 << 62, DUMMY, None, 0.5, 0, 0, None, DUMMY, None), "too many")
+        assert call(0, None, None, 0.5, 0, 0, None, None, None) == 0
+
+
+def test_cross_entropy_refusals():
+    for name in ("yuf_cross_entropy_f32", "yuf_cross_entropy_bf16"):
+        call = getattr(lib(), name)
+
+        def bad(*words, M=4, V=10, logits=DUMMY, ld=10, targets=DUMMY, bits=32, reduction=1, loss=DUMMY, dlogits=None,
+                ld_out=0, space=DUMMY):
+            refused(call(M, V, logits, ld, targets, bits, -100, reduction, loss, None, dlogits, ld_out, space, None), *words)
+
+        bad("negative", M=-1)
+        bad("negative", V=-1, ld=0)
+        bad("without logits", V=0, ld=0)
+        bad("stride", ld=9)
+        bad("stride", dlogits=DUMMY * 2, ld_out=9)
+        bad("in place", dlogits=DUMMY, ld_out=12)
+        bad("target_bits", bits=16)
+        bad("reduction", reduction=3)
+        bad("null", logits=None)
+        bad("null", targets=None)
+        bad("neither", loss=None)
+        bad("workspace", space=None)
+    assert lib().yuf_cross_entropy_workspace(-1) == 0 and lib().yuf_cross_entropy_workspace(10) >= 44
+
+
+def test_python_refusals():
+    x = torch.zeros(1, 4, 2, 40)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.rwkv7_scan_backward(*[x] * 7)
+    with pytest.raises(ValueError, match="head size"):
+        ops.rwkv7_scan_backward(*[torch.zeros(1, 4, 2, 12)] * 7)
+    with pytest.raises(ValueError, match="shape"):
+        ops.rwkv7_scan_backward(*[torch.zeros(4, 2, 40)] * 7)
+    seq, vec = torch.zeros(1, 4, 64), torch.zeros(64)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.rosa_householder_scan_backward(seq, seq, seq, vec, vec, torch.zeros(1, 64), seq)
+    with pytest.raises(ValueError, match="shape"):
+        ops.rosa_householder_scan_backward(vec, vec, vec, vec, vec, vec, vec)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.dropout(vec, 0.5, 1)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.cross_entropy(torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="shape"):
+        ops.cross_entropy(vec, torch.zeros(64, dtype=torch.int64))
+
+
+def test_the_abi_takes_ctypes_integers_of_full_width():
+    """Seeds and counters are 64-bit: a cut one would repeat masks."""
+    from yufmusicgen_amd._lib import SIGNATURES
+
+    for name in ("yuf_dropout_f32", "yuf_dropout_bf16"):
+        args = SIGNATURES[name][1]
+        assert args[0] is ctypes.c_int64 and args[4] is args[5] is ctypes.c_uint64 and args[3] is ctypes.c_double

@@ -46,6 +46,21 @@ SIGNATURES = {
     "yuf_wkv7_scan_f32": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p] * 10),
     "yuf_rosa_scan_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 9),
     "yuf_rosa_scan_f32_noalloc": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 9),
+    "yuf_wkv7_scan_backward_workspace": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "yuf_wkv7_scan_backward_f32": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p] * 18),
+    "yuf_rosa_scan_backward_workspace": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "yuf_rosa_scan_backward_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 16),
+    "yuf_dropout_f32": (ctypes.c_int, [ctypes.c_int64, c_void_p, c_void_p, ctypes.c_double, ctypes.c_uint64,
+                                       ctypes.c_uint64, c_void_p, c_void_p, c_void_p]),
+    "yuf_dropout_bf16": (ctypes.c_int, [ctypes.c_int64, c_void_p, c_void_p, ctypes.c_double, ctypes.c_uint64,
+                                        ctypes.c_uint64, c_void_p, c_void_p, c_void_p]),
+    "yuf_cross_entropy_workspace": (ctypes.c_size_t, [ctypes.c_int]),
+    "yuf_cross_entropy_f32": (ctypes.c_int, [ctypes.c_int] * 2 + [c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int,
+                                                                  ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3 +
+                              [ctypes.c_int64, c_void_p, c_void_p]),
+    "yuf_cross_entropy_bf16": (ctypes.c_int, [ctypes.c_int] * 2 + [c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int,
+                                                                   ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3 +
+                               [ctypes.c_int64, c_void_p, c_void_p]),
     "yuf_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 3 + [ctypes.c_int] + [c_void_p] * 3),
     "yuf_ln_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 9),
     "yuf_x3_planes_elems": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),

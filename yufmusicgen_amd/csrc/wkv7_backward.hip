@@ -1,0 +1,533 @@
+// Gradients of the WKV-7 scan, in chunks of 16 tokens on the fp32 matrix cores.
+//
+// Forward, per (b, h):  S_t = S_{t-1} (diag(d_t) + a_t b_t^T) + v_t k_t^T,  y_t = S_t r_t,
+// d = exp(-e^{-0.5} sigmoid(w_raw)).  With the running decay products D_t of a chunk and,
+// as rows per token, A = a D_{t-1}, R = r D_t, B = b / D_t, K = k / D_t (d >= 0.545 keeps
+// 1 / D below 2^14):
+//     Lab = strict(A B^T), Lak = strict(A K^T), Mrb = incl(R B^T), Mrk = incl(R K^T)
+//     T = (I - Lab)^{-1},  C = T Lak
+//     U = T A S0^T + C V                  (rows S_{t-1} a_t)
+//     S1 = (S0 + U^T B + V^T K) diag(D_15)
+// With G1, G0 the gradients of S1 and S0, G = G1 diag(D_15), and the same letters with a
+// prime for gradients:
+//     F = Mrb^T Y' + B G^T,   E = T^T F                    (E = U')
+//     V' = Mrk^T Y' + K G^T + C^T F
+//     G0 = G + Y'^T R + E^T A
+//     Mrb' = incl(Y' U^T), Mrk' = incl(Y' V^T), Lab' = strict(E U^T), Lak' = strict(E V^T)
+//     R' = Y' S0 + Mrb' B + Mrk' K        A' = E S0 + Lab' B + Lak' K
+//     B' = U G + Mrb'^T R + Lab'^T A      K' = V G + Mrk'^T R + Lak'^T A
+//     r' = R' D_t, a' = A' D_{t-1}, b' = B' / D_t, k' = K' / D_t
+//     (log d_t)' = sum_i (G0 S0)_i - sum_{s < t} (R R' - B B' - K K')_s - sum_{s <= t} (A A')_s
+//     w' = (log d)' (-e^{-0.5}) sigmoid(w) (1 - sigmoid(w))
+// The last but one: scaling S0 by x and every D_t by 1 / x per key column changes nothing, so
+// the log D_t' of a chunk add up to the share of S0.  Summed from the chunk's start, and not from its
+// end, a zero state's first token gets its exact 0.
+//
+// Kernels:
+//   wkv7_grad_gram_kernel  what no state enters, for every chunk at once: T, C, Mrb, Mrk.
+//   wkv7_grad_kernel       a workgroup per head: S forward over the chunks (kept per
+//                          chunk, with U), then G and the gradients backward.
+//
+// MFMA layouts (16x16x4 f32; lane l, g = l / 16, li = l % 16): A[m = li][k = g],
+// B[k = g][n = li], register r of the result D[m = 4 g + r][n = li].  k-step r of a
+// product means rows {4 g + r}, so a result is the next product's B operand as it is,
+// and an A operand is four consecutive k per lane.  Wave q of NB = ceil(N / 16) owns key
+// tile q and value tile q; its stage-0 registers hold (token 4 g + r, column 16 q + li)
+// of every input, which is at once the B operand of the products that contract tokens.
+#include "common.h"
+#include "kernels.h"
+
+namespace yuf {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kC = 16;     // tokens of a chunk
+constexpr int kWave = 64;
+constexpr int kXcds = 8;
+constexpr int kST = 20;    // row stride of the 16 x 16 tiles in LDS
+constexpr int kFrag = kWave * 4;  // floats of a 16 x 16 fragment
+// Fragments of a chunk.  "Row": lane holds X[li][4 g + r]; "Col": X[4 g + r][li].
+enum { kTRow, kCRow, kTCol, kCCol, kMrbCol, kMrkCol, kFrags };
+
+struct GradParams {
+    int B, T, H, N;
+    int chunks;  // of a sequence
+    const float *r, *w, *k, *v, *a, *b, *dy;
+    const float *state_in, *dstate_out;
+    float *dr, *dw, *dk, *dv, *da, *db, *dstate_in;
+    float *frags;   // [B H][chunks][kFrags][kFrag]
+    float *states;  // [B H][chunks][N][N]: the state before each chunk
+    float *u;       // [B H][chunks][NB][kFrag]
+};
+
+__device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+// c += sum over the 16 values of k of a (lane: 4 consecutive k of row li) and b.
+__device__ __forceinline__ floatx4 mul16(floatx4 a, floatx4 b, floatx4 c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = mfma(a[r], b[r], c);
+    return c;
+}
+__device__ __forceinline__ floatx4 ld4(const float *p) { return *reinterpret_cast<const floatx4 *>(p); }
+__device__ __forceinline__ void st4(float *p, floatx4 v) { *reinterpret_cast<floatx4 *>(p) = v; }
+// Four rows of a column, `stride` apart.
+__device__ __forceinline__ floatx4 ldcol(const float *p, int stride) {
+    return floatx4{p[0], p[stride], p[2 * stride], p[3 * stride]};
+}
+__device__ __forceinline__ void stcol(float *p, int stride, floatx4 v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r * stride] = v[r];
+}
+__device__ __forceinline__ floatx4 buf_load4(__amdgpu_buffer_rsrc_t rsrc, uint32_t byte_offset) {
+    return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, byte_offset, 0, 0));
+}
+__device__ __forceinline__ void buf_store4(floatx4 v, __amdgpu_buffer_rsrc_t rsrc, uint32_t byte_offset) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc, byte_offset, 0, 0);
+}
+
+// The 16 tokens x 16 columns of one wave in a chunk of a [B, T, H, N] tensor: lane
+// (g, li) holds tokens 4 g + r of its column.  Tokens past T and columns past N read as
+// 0 and are not written.
+struct Tile {
+    uint32_t offset[4];  // bytes from the head's row of the chunk's first token
+    uint32_t bytes;      // range of the chunk
+    size_t base;         // elements
+
+    __device__ __forceinline__ void at(const GradParams &p, int b, int h, int chunk, int col, int g) {
+        const int t0 = chunk * kC, nt = min(kC, p.T - t0), HN = p.H * p.N;
+        base = (((size_t)b * p.T + t0) * p.H + h) * p.N;
+        bytes = (uint32_t)((nt - 1) * HN + p.N) * 4u;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) offset[r] = col < p.N ? (uint32_t)((4 * g + r) * HN + col) * 4u : kBufferOob;
+    }
+    __device__ __forceinline__ floatx4 load(const float *x) const {
+        const auto rs = make_rsrc(x + base, bytes);
+        floatx4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = buf_load(rs, offset[r]);
+        return v;
+    }
+    __device__ __forceinline__ void store(float *x, floatx4 v) const {
+        const auto rs = make_rsrc(x + base, bytes);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) buf_store(v[r], rs, offset[r]);
+    }
+};
+
+// Running decay products of a chunk for the lane's column.
+struct Decays {
+    floatx4 now, before, inv;  // D_t, D_{t-1}, 1 / D_t
+    float last;                // D_15
+    floatx4 slope;             // d log d / d w = -e^{-0.5} sigmoid(w) (1 - sigmoid(w))
+
+    // valid: tokens of the chunk; the rest keep the state (d = 1).
+    __device__ __forceinline__ void set(floatx4 w, int valid, int g) {
+        float run[4], acc = 1.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            // exp(-w) stays finite, so that 1 - sigmoid(w) = exp(-w) sigmoid(w) keeps its relative precision.
+            const float e = __expf(w[r] < -80.0f ? 80.0f : -w[r]);
+            const float sig = __builtin_amdgcn_rcpf(1.0f + e);
+            const float d = __builtin_amdgcn_exp2f(-0.8750387749f * sig);  // e^{-0.5} log2(e)
+            slope[r] = -0.6065306597f * sig * (e * sig);
+            acc *= 4 * g + r < valid ? d : 1.0f;
+            run[r] = acc;
+        }
+        // Products of the earlier lane groups' tokens (rows of 16 lanes): pairs, then halves.
+        const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc), __float_as_uint(acc), false, false);
+        const float even = __uint_as_float(s16[0]), odd = __uint_as_float(s16[1]);
+        const float pair = even * odd;
+        const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair), __float_as_uint(pair), false, false);
+        const float low = __uint_as_float(s32[0]);
+        const float base = g == 0 ? 1.0f : g == 1 ? even : g == 2 ? low : low * even;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            before[r] = r == 0 ? base : base * run[r - 1];
+            now[r] = base * run[r];
+            inv[r] = __builtin_amdgcn_rcpf(now[r]);
+        }
+        last = __shfl(now[3], 48 + (threadIdx.x & 15));
+    }
+};
+
+// Sum over the four lanes of a column (one per row of 16 lanes), to all of them.
+__device__ __forceinline__ float rows_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// Sum over the earlier lane groups of a column.
+__device__ __forceinline__ float rows_before(float x, int g) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float even = __uint_as_float(a[0]), pair = even + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair), __float_as_uint(pair), false, false);
+    const float low = __uint_as_float(b[0]);
+    return g == 0 ? 0.0f : g == 1 ? even : g == 2 ? low : low + even;
+}
+
+// Units dealt so that consecutive ones (the chunks of a head, the heads of a batch row)
+// share an XCD's L2.
+__device__ __forceinline__ int xcd_unit(int per_xcd) { return (blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds; }
+
+// One wave per chunk of a head.
+template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int SA = 16 * NB + 4;
+    __shared__ __attribute__((aligned(16))) float tiles[4 * kC * SA + 3 * kC * kST];
+    float *sA = tiles, *sR = sA + kC * SA, *sB = sR + kC * SA, *sK = sB + kC * SA;
+    float *sL = sK + kC * SA, *sP = sL + kC * kST, *sT = sP + kC * kST;
+    const int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;
+    const int head = unit / p.chunks, chunk = unit - head * p.chunks;
+    const int bb = head / p.H, h = head - bb * p.H;
+    const int lane = threadIdx.x, g = lane >> 4, li = lane & 15;
+    const int valid = min(kC, p.T - chunk * kC);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+        Tile tile;
+        tile.at(p, bb, h, chunk, 16 * q + li, g);
+        Decays d;
+        d.set(tile.load(p.w), valid, g);
+        const int at = 4 * g * SA + 16 * q + li;
+        stcol(sA + at, SA, tile.load(p.a) * d.before);
+        stcol(sR + at, SA, tile.load(p.r) * d.now);
+        stcol(sB + at, SA, tile.load(p.b) * d.inv);
+        stcol(sK + at, SA, tile.load(p.k) * d.inv);
+    }
+    lds_barrier();
+    floatx4 ab = {0.f, 0.f, 0.f, 0.f}, ak = ab, rb = ab, rk = ab;
+#pragma unroll
+    for (int jb = 0; jb < NB; ++jb) {
+        const int at = li * SA + 16 * jb + 4 * g;
+        const floatx4 a4 = ld4(sA + at), r4 = ld4(sR + at), b4 = ld4(sB + at), k4 = ld4(sK + at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            ab = mfma(a4[r], b4[r], ab);
+            ak = mfma(a4[r], k4[r], ak);
+            rb = mfma(r4[r], b4[r], rb);
+            rk = mfma(r4[r], k4[r], rk);
+        }
+    }
+    // Register r: row t = 4 g + r, column s = li.
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = 4 * g + r;
+        ab[r] = li < t ? ab[r] : 0.0f;
+        ak[r] = li < t ? ak[r] : 0.0f;
+        rb[r] = li <= t ? rb[r] : 0.0f;
+        rk[r] = li <= t ? rk[r] : 0.0f;
+    }
+    st4(sL + li * kST + 4 * g, ab);  // Lab^T: column s of Lab in row s
+    st4(sP + li * kST + 4 * g, ak);  // Lak^T
+    lds_barrier();
+    {
+        // Column li of T by forward substitution, right-looking (the four lane groups alike).
+        float x[kC];
+#pragma unroll
+        for (int t = 0; t < kC; ++t) x[t] = li == t ? 1.0f : 0.0f;
+#pragma unroll
+        for (int s = 0; s < kC - 1; ++s)
+#pragma unroll
+            for (int m = s / 4; m < 4; ++m) {
+                const floatx4 col = ld4(sL + s * kST + 4 * m);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (4 * m + e > s) x[4 * m + e] = fmaf(col[e], x[s], x[4 * m + e]);
+            }
+        // T^T, row s = li: each lane group writes its four tokens.
+        const floatx4 own = g == 0 ? floatx4{x[0], x[1], x[2], x[3]}
+                          : g == 1 ? floatx4{x[4], x[5], x[6], x[7]}
+                          : g == 2 ? floatx4{x[8], x[9], x[10], x[11]}
+                                   : floatx4{x[12], x[13], x[14], x[15]};
+        st4(sT + li * kST + 4 * g, own);
+    }
+    lds_barrier();
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const floatx4 t_col = ld4(sT + li * kST + 4 * g);            // T[4 g + r][li]
+    const floatx4 t_row = ldcol(sT + 4 * g * kST + li, kST);     // T[li][4 g + r]
+    // C[t][s] = sum T[t][m] Lak[m][s]: B operand Lak[m = 4 g + r][s = li] = the Gram's registers.
+    const floatx4 c_col = mul16(t_row, ak, zero);
+    // C^T[s][t] = sum Lak^T[s][m] T^T[m][t]: its registers, [s = 4 g + r][t = li], are C's row fragment.
+    // Its B operand T^T[m = 4 g + r][t = li] is the same four values as T's row fragment.
+    const floatx4 c_row = mul16(ld4(sP + li * kST + 4 * g), t_row, zero);
+    float *out = p.frags + ((size_t)head * p.chunks + chunk) * kFrags * kFrag + 4 * lane;
+    st4(out + kTRow * kFrag, t_row);
+    st4(out + kCRow * kFrag, c_row);
+    st4(out + kTCol * kFrag, t_col);
+    st4(out + kCCol * kFrag, c_col);
+    st4(out + kMrbCol * kFrag, rb);
+    st4(out + kMrkCol * kFrag, rk);
+}
+
+// A workgroup of NB waves per head.
+template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
+    // Forward: two buffers of A, B, K and D_15.  Backward: B, K, V, Y', U, E, G [value][key]
+    // and the four 16 x 16 gradients.
+    constexpr int kForward = 2 * (3 * kTok + NP), kBackward = 6 * kTok + NP * SA + 4 * kC * kST;
+    __shared__ __attribute__((aligned(16))) float lds[kForward > kBackward ? kForward : kBackward];
+    static_assert(sizeof(lds) <= 160 * 1024, "LDS of one CU");
+    const int head = xcd_unit(per_xcd);
+    if (head >= units) return;  // uniform over the workgroup
+    const int bb = head / p.H, h = head - bb * p.H;
+    const int q = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const int N = p.N, nc = p.chunks;
+    const int col = 16 * q + li;
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const float *frags = p.frags + (size_t)head * nc * kFrags * kFrag + 4 * lane;
+    float *states = p.states + (size_t)head * nc * N * N;
+    float *us = p.u + ((size_t)head * nc * NB + q) * kFrag + 4 * lane;
+    const uint32_t state_bytes = (uint32_t)(N * N * 4);
+    // (value 16 q + li, keys 16 jb + 4 g ..) and (value 16 ib + 4 g + r, key 16 q + li) of a state.
+    auto rows_at = [&](int jb) { return col < N && 16 * jb + 4 * g < N ? (uint32_t)(col * N + 16 * jb + 4 * g) * 4u : kBufferOob; };
+    auto cols_at = [&](int ib, int r) {
+        const int i = 16 * ib + 4 * g + r;
+        return col < N && i < N ? (uint32_t)(i * N + col) * 4u : kBufferOob;
+    };
+    auto load_cols = [&](const float *s, floatx4 (&x)[NB]) {
+        const auto rs = make_rsrc(s, s ? state_bytes : 0u);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[ib][r] = buf_load(rs, cols_at(ib, r));
+    };
+
+    {
+        // --------------------------------------------------------------- forward
+        // S^T[:, value tile q] as NB tiles of 16 keys.
+        floatx4 S[NB];
+        {
+            const float *s0 = p.state_in ? p.state_in + (size_t)head * N * N : nullptr;
+            const auto rs = make_rsrc(s0, s0 ? state_bytes : 0u);
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb) S[jb] = buf_load4(rs, rows_at(jb));
+        }
+        auto keep = [&](int slot) {
+            const auto rs = make_rsrc(states + (size_t)slot * N * N, state_bytes);
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb) buf_store4(S[jb], rs, rows_at(jb));
+        };
+        floatx4 w, k, v, a, b;
+        auto fetch = [&](int c) {
+            Tile tile;
+            tile.at(p, bb, h, c, col, g);
+            w = tile.load(p.w);
+            k = tile.load(p.k);
+            v = tile.load(p.v);
+            a = tile.load(p.a);
+            b = tile.load(p.b);
+        };
+        if (nc > 0) fetch(0);
+        for (int c = 0; c < nc; ++c) {
+            float *sA = lds + (c & 1) * (3 * kTok + NP), *sB = sA + kTok, *sK = sB + kTok, *sD = sK + kTok;
+            const floatx4 t_row = ld4(frags + ((size_t)c * kFrags + kTRow) * kFrag);
+            const floatx4 c_row = ld4(frags + ((size_t)c * kFrags + kCRow) * kFrag);
+            keep(c);
+            Decays d;
+            d.set(w, min(kC, p.T - c * kC), g);
+            const int at = 4 * g * SA + col;
+            stcol(sA + at, SA, a * d.before);
+            stcol(sB + at, SA, b * d.inv);
+            stcol(sK + at, SA, k * d.inv);
+            if (g == 3) sD[col] = d.last;
+            const floatx4 v4 = v;
+            if (c + 1 < nc) fetch(c + 1);
+            lds_barrier();
+            floatx4 X = zero;
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb) X = mul16(ld4(sA + li * SA + 16 * jb + 4 * g), S[jb], X);
+            floatx4 U = mul16(c_row, v4, zero);
+            U = mul16(t_row, X, U);
+            st4(us + (size_t)c * NB * kFrag, U);
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb) {
+                floatx4 s = mul16(ldcol(sK + 4 * g * SA + 16 * jb + li, SA), v4, S[jb]);
+                s = mul16(ldcol(sB + 4 * g * SA + 16 * jb + li, SA), U, s);
+                S[jb] = s * ld4(sD + 16 * jb + 4 * g);
+            }
+        }
+    }
+    __syncthreads();  // the states are read across waves, and LDS is used anew
+
+    // ----------------------------------------------------------------- backward
+    float *sB = lds, *sK = sB + kTok, *sV = sK + kTok, *sY = sV + kTok, *sU = sY + kTok, *sE = sU + kTok;
+    float *sG = sE + kTok;  // G, [value][key]
+    float *sMrb = sG + NP * SA, *sMrk = sMrb + kC * kST, *sLab = sMrk + kC * kST, *sLak = sLab + kC * kST;
+    // G[:, key tile q] as NB tiles of 16 values, and S0 in the same layout.
+    floatx4 G[NB], S0[NB];
+    load_cols(p.dstate_out ? p.dstate_out + (size_t)head * N * N : nullptr, G);
+    for (int c = nc - 1; c >= 0; --c) {
+        Tile tile;
+        tile.at(p, bb, h, c, col, g);
+        const float *fr = frags + (size_t)c * kFrags * kFrag;
+        const floatx4 w = tile.load(p.w), rr = tile.load(p.r), aa = tile.load(p.a), bv = tile.load(p.b);
+        const floatx4 kv = tile.load(p.k), vv = tile.load(p.v), yv = tile.load(p.dy);
+        const floatx4 uv = ld4(us + (size_t)c * NB * kFrag);
+        load_cols(states + (size_t)c * N * N, S0);
+        Decays d;
+        d.set(w, min(kC, p.T - c * kC), g);
+        const floatx4 A = aa * d.before, R = rr * d.now, B = bv * d.inv, K = kv * d.inv;
+        const int at = 4 * g * SA + col;
+        stcol(sB + at, SA, B);
+        stcol(sK + at, SA, K);
+        stcol(sV + at, SA, vv);
+        stcol(sY + at, SA, yv);
+        stcol(sU + at, SA, uv);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib) {
+            G[ib] *= d.last;
+            stcol(sG + (16 * ib + 4 * g) * SA + col, SA, G[ib]);
+        }
+        const floatx4 t_col = ld4(fr + kTCol * kFrag), c_col = ld4(fr + kCCol * kFrag);
+        const floatx4 rb_col = ld4(fr + kMrbCol * kFrag), rk_col = ld4(fr + kMrkCol * kFrag);
+        lds_barrier();
+        // Value tile q: F, E, V'.
+        floatx4 F = mul16(rb_col, yv, zero), dV = mul16(rk_col, yv, zero);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) {
+            const floatx4 g4 = ld4(sG + col * SA + 16 * jb + 4 * g);
+            F = mul16(ld4(sB + li * SA + 16 * jb + 4 * g), g4, F);
+            dV = mul16(ld4(sK + li * SA + 16 * jb + 4 * g), g4, dV);
+        }
+        const floatx4 E = mul16(t_col, F, zero);
+        stcol(sE + at, SA, E);
+        dV = mul16(c_col, F, dV);
+        tile.store(p.dv, dV);
+        // Key tile q: Y' S0, U G, V G.
+        floatx4 dR = zero, dA = zero, dB = zero, dK = zero;
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib) {
+            const int o = li * SA + 16 * ib + 4 * g;
+            dR = mul16(ld4(sY + o), S0[ib], dR);
+            dB = mul16(ld4(sU + o), G[ib], dB);
+            dK = mul16(ld4(sV + o), G[ib], dK);
+        }
+        // Rows t = 4 g + r, columns s = li of X Z^T, kept where s <= t (s < t).
+        auto gram = [&](const float *x, const float *z, float *out, bool strict) {
+            floatx4 m = zero;
+#pragma unroll
+            for (int ib = 0; ib < NB; ++ib) m = mul16(ld4(x + li * SA + 16 * ib + 4 * g), ld4(z + li * SA + 16 * ib + 4 * g), m);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) out[(4 * g + r) * kST + li] = li < 4 * g + r + !strict ? m[r] : 0.0f;
+        };
+        if (q == 0) gram(sY, sU, sMrb, false);
+        if (q == (NB > 1 ? 1 : 0)) gram(sY, sV, sMrk, false);
+        lds_barrier();
+        if (q == (NB > 2 ? 2 : 0)) gram(sE, sU, sLab, true);
+        if (q == (NB > 3 ? 3 : NB > 1 ? 1 : 0)) gram(sE, sV, sLak, true);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib) {
+            dA = mul16(ld4(sE + li * SA + 16 * ib + 4 * g), S0[ib], dA);
+            // G0 = G + Y'^T R + E^T A
+            floatx4 n = mul16(ldcol(sY + 4 * g * SA + 16 * ib + li, SA), R, G[ib]);
+            G[ib] = mul16(ldcol(sE + 4 * g * SA + 16 * ib + li, SA), A, n);
+        }
+        dR = mul16(ld4(sMrb + li * kST + 4 * g), B, dR);
+        dR = mul16(ld4(sMrk + li * kST + 4 * g), K, dR);
+        dB = mul16(ldcol(sMrb + 4 * g * kST + li, kST), R, dB);
+        dK = mul16(ldcol(sMrk + 4 * g * kST + li, kST), R, dK);
+        lds_barrier();
+        dA = mul16(ld4(sLab + li * kST + 4 * g), B, dA);
+        dA = mul16(ld4(sLak + li * kST + 4 * g), K, dA);
+        dB = mul16(ldcol(sLab + 4 * g * kST + li, kST), A, dB);
+        dK = mul16(ldcol(sLak + 4 * g * kST + li, kST), A, dK);
+        tile.store(p.dr, dR * d.now);
+        tile.store(p.da, dA * d.before);
+        tile.store(p.db, dB * d.inv);
+        tile.store(p.dk, dK * d.inv);
+        // (log d_t)': sums over the chunk's earlier tokens.
+        const floatx4 ya = A * dA, z = R * dR - B * dB - K * dK + ya;
+        float share = 0.0f;  // sum_i (G0 S0)_i of the lane's key
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) share = fmaf(G[ib][r], S0[ib][r], share);
+        float run = rows_sum(share) - rows_before((z[0] + z[1]) + (z[2] + z[3]), g);
+        floatx4 dw;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            dw[r] = (run - ya[r]) * d.slope[r];
+            run -= z[r];
+        }
+        tile.store(p.dw, dw);
+    }
+    if (p.dstate_in) {
+        const auto rs = make_rsrc(p.dstate_in + (size_t)head * N * N, state_bytes);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) buf_store(G[ib][r], rs, cols_at(ib, r));
+    }
+}
+
+struct Scratch {
+    size_t frags, states, u, bytes;
+};
+
+Scratch scratch_of(int B, int T, int H, int N) {
+    const size_t heads = (size_t)B * H, chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Scratch o{};
+    o.frags = 0;
+    o.states = o.frags + up(heads * chunks * kFrags * kFrag * sizeof(float));
+    o.u = o.states + up(heads * chunks * N * N * sizeof(float));
+    o.bytes = o.u + up(heads * chunks * NB * kFrag * sizeof(float)) + 256;  // some buffer for T = 0 too
+    return o;
+}
+
+template <int NB> void launch(const GradParams &p, hipStream_t s) {
+    const int heads = p.B * p.H, grams = heads * p.chunks;
+    auto per_xcd = [](int units) { return (units + kXcds - 1) / kXcds; };
+    if (grams > 0)
+        hipLaunchKernelGGL((wkv7_grad_gram_kernel<NB>), dim3(per_xcd(grams) * kXcds), dim3(kWave), 0, s, p, grams, per_xcd(grams));
+    hipLaunchKernelGGL((wkv7_grad_kernel<NB>), dim3(per_xcd(heads) * kXcds), dim3(NB * kWave), 0, s, p, heads, per_xcd(heads));
+}
+
+}  // namespace
+}  // namespace yuf
+
+extern "C" size_t yuf_wkv7_scan_backward_workspace(int B, int T, int H, int N) {
+    using namespace yuf;
+    if (B <= 0 || T < 0 || H <= 0 || !wkv7_supported(N)) return 0;
+    return scratch_of(B, T, H, N).bytes;
+}
+
+extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const float *r, const float *w_raw, const float *k,
+                                          const float *v, const float *a, const float *b, const float *state_in,
+                                          const float *dy, const float *dstate_out, float *dr, float *dw_raw, float *dk,
+                                          float *dv, float *da, float *db, float *dstate_in, void *workspace,
+                                          void *stream) {
+    using namespace yuf;
+    if (B < 0 || T < 0 || H < 0) return fail(YUF_ERR_INVALID, "wkv7 backward: negative size");
+    if (!wkv7_supported(N)) return fail(YUF_ERR_INVALID, "wkv7 backward: unsupported head size N=" + std::to_string(N));
+    if (B == 0 || H == 0) return YUF_OK;
+    if (T > 0 && (!r || !w_raw || !k || !v || !a || !b || !dy || !dr || !dw_raw || !dk || !dv || !da || !db))
+        return fail(YUF_ERR_INVALID, "wkv7 backward: null input/output pointer");
+    if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
+    // Offsets inside a chunk of one head are 32-bit, workgroups are counted in int.
+    if ((int64_t)H * N > (1 << 24)) return fail(YUF_ERR_INVALID, "wkv7 backward: H * N above 2^24");
+    if ((int64_t)B * H * ((T + kC - 1) / kC) > (1 << 30)) return fail(YUF_ERR_INVALID, "wkv7 backward: too many chunks");
+    GradParams p{};
+    p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = (T + kC - 1) / kC;
+    p.r = r; p.w = w_raw; p.k = k; p.v = v; p.a = a; p.b = b; p.dy = dy;
+    p.state_in = state_in; p.dstate_out = dstate_out;
+    p.dr = dr; p.dw = dw_raw; p.dk = dk; p.dv = dv; p.da = da; p.db = db; p.dstate_in = dstate_in;
+    const Scratch o = scratch_of(B, T, H, N);
+    char *base = static_cast<char *>(workspace);
+    p.frags = reinterpret_cast<float *>(base + o.frags);
+    p.states = reinterpret_cast<float *>(base + o.states);
+    p.u = reinterpret_cast<float *>(base + o.u);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch ((N + 15) / 16) {
+        case 1: launch<1>(p, s); break;
+        case 2: launch<2>(p, s); break;
+        case 3: launch<3>(p, s); break;
+        case 4: launch<4>(p, s); break;
+        default: launch<8>(p, s); break;
+    }
+    YUF_LAUNCH_CHECK("wkv7 backward");
+    return YUF_OK;
+}
