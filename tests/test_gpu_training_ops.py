@@ -105,6 +105,26 @@ def test_wkv7_gradients_of_no_token():
     assert rwkv7_scan_backward(*none)[0].shape == (0, 5, 3, 40)
 
 
+@pytest.mark.parametrize("size", [8, 40, 64])
+@pytest.mark.parametrize("steps", [21, 200])
+def test_wkv7_gradients_stay_inside_their_outputs(size, steps):
+    """Ragged last chunk and padded columns: what lies behind each output, and behind the
+    workspace, stays as it was; an output may start at any element."""
+    from yufmusicgen_amd._lib import check, lib
+
+    arrs, s0, dy, ds = wkv_case(size, 2, steps, 3, size)
+    expect = wkv_grads(arrs, s0, dy, ds)
+    held = [torch.full((e.numel() + 133,), 7.0, device="cuda") for e in expect]
+    space = torch.full((lib().yuf_wkv7_scan_backward_workspace(2, steps, 3, size) + 4096,), 7, dtype=torch.uint8, device="cuda")
+    inputs = [cuda(x) for x in (*arrs, s0, dy, ds)]
+    check(lib().yuf_wkv7_scan_backward_f32(2, steps, 3, size, *(x.data_ptr() for x in inputs),
+                                           *(h[3:].data_ptr() for h in held), space.data_ptr(),
+                                           torch.cuda.current_stream().cuda_stream))
+    for h, e in zip(held, expect):
+        assert torch.equal(h[3 : 3 + e.numel()], e.reshape(-1)) and (h[:3] == 7).all() and (h[3 + e.numel() :] == 7).all()
+    assert (space[-4096:] == 7).all()
+
+
 def test_wkv7_gradients_at_extreme_decays():
     """w at both ends of the decay's range (0.545 and 1) and beyond: the gradients stay
     finite, and dw vanishes where the sigmoid is flat."""

@@ -23,10 +23,17 @@
 // the log D_t' of a chunk add up to the share of S0.  Summed from the chunk's start, and not from its
 // end, a zero state's first token gets its exact 0.
 //
-// Kernels:
-//   wkv7_grad_gram_kernel  what no state enters, for every chunk at once: T, C, Mrb, Mrk.
-//   wkv7_grad_kernel       a workgroup per head: S forward over the chunks (kept per
-//                          chunk, with U), then G and the gradients backward.
+// The sequence is cut into segments of whole chunks that run side by side:
+//   wkv7_grad_gram_kernel   what no state enters, for every chunk at once: T, C, Mrb, Mrk.
+//   wkv7_grad_local_kernel  per segment: its end state from a zero start, the gradient of its
+//                           start from a zero one at its end, and its transition Pi (the end
+//                           state of S = I with v = 0), where S1 = S0 Pi + local and G0 =
+//                           G1 Pi^T + local.  The first segment starts from the call's state
+//                           and the last from its gradient, so that these two are final.
+//   wkv7_grad_carry_kernel  both recurrences over the segments, a wave per value tile.
+//   wkv7_grad_kernel        per segment: S forward over its chunks (kept per chunk, with U),
+//                           then G and the gradients backward.
+// One segment needs the first and the last alone, two no carry.
 //
 // MFMA layouts (16x16x4 f32; lane l, g = l / 16, li = l % 16): A[m = li][k = g],
 // B[k = g][n = li], register r of the result D[m = 4 g + r][n = li].  k-step r of a
@@ -53,13 +60,18 @@ enum { kTRow, kCRow, kTCol, kCCol, kMrbCol, kMrkCol, kFrags };
 
 struct GradParams {
     int B, T, H, N;
-    int chunks;  // of a sequence
+    int chunks;    // of a sequence
+    int segments;  // of a sequence, of seg_chunks chunks each (the last may have fewer)
+    int seg_chunks;
     const float *r, *w, *k, *v, *a, *b, *dy;
     const float *state_in, *dstate_out;
     float *dr, *dw, *dk, *dv, *da, *db, *dstate_in;
     float *frags;   // [B H][chunks][kFrags][kFrag]
     float *states;  // [B H][chunks][N][N]: the state before each chunk
     float *u;       // [B H][chunks][NB][kFrag]
+    // [B H][segments][N][N]: the state before segment s >= 1, the gradient of the state after
+    // segment s <= segments - 2, and Pi of the segments between the first and the last.
+    float *starts, *ends, *powers;
 };
 
 __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
@@ -262,93 +274,284 @@ template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel
     st4(out + kMrkCol * kFrag, rk);
 }
 
-// A workgroup of NB waves per head.
-template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
-    constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
-    // Forward: two buffers of A, B, K and D_15.  Backward: B, K, V, Y', U, E, G [value][key]
-    // and the four 16 x 16 gradients.
-    constexpr int kForward = 2 * (3 * kTok + NP), kBackward = 6 * kTok + NP * SA + 4 * kC * kST;
-    __shared__ __attribute__((aligned(16))) float lds[kForward > kBackward ? kForward : kBackward];
-    static_assert(sizeof(lds) <= 160 * 1024, "LDS of one CU");
-    const int head = xcd_unit(per_xcd);
-    if (head >= units) return;  // uniform over the workgroup
-    const int bb = head / p.H, h = head - bb * p.H;
-    const int q = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
-    const int N = p.N, nc = p.chunks;
-    const int col = 16 * q + li;
-    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-    const float *frags = p.frags + (size_t)head * nc * kFrags * kFrag + 4 * lane;
-    float *states = p.states + (size_t)head * nc * N * N;
-    float *us = p.u + ((size_t)head * nc * NB + q) * kFrag + 4 * lane;
-    const uint32_t state_bytes = (uint32_t)(N * N * 4);
-    // (value 16 q + li, keys 16 jb + 4 g ..) and (value 16 ib + 4 g + r, key 16 q + li) of a state.
-    auto rows_at = [&](int jb) { return col < N && 16 * jb + 4 * g < N ? (uint32_t)(col * N + 16 * jb + 4 * g) * 4u : kBufferOob; };
-    auto cols_at = [&](int ib, int r) {
-        const int i = 16 * ib + 4 * g + r;
-        return col < N && i < N ? (uint32_t)(i * N + col) * 4u : kBufferOob;
-    };
-    auto load_cols = [&](const float *s, floatx4 (&x)[NB]) {
-        const auto rs = make_rsrc(s, s ? state_bytes : 0u);
+// What a wave of the segment kernels is: its head, segment, tile and place in it.
+struct Place {
+    int head, bb, h, q, g, li, lane, col;
+    int c0, c1;  // chunks of the segment
+    __device__ __forceinline__ Place(const GradParams &p, int head_, int seg) {
+        head = head_;
+        bb = head / p.H;
+        h = head - bb * p.H;
+        q = threadIdx.x >> 6;
+        lane = threadIdx.x & 63;
+        g = lane >> 4;
+        li = lane & 15;
+        col = 16 * q + li;
+        c0 = seg * p.seg_chunks;
+        c1 = min(p.chunks, c0 + p.seg_chunks);
+    }
+};
+
+// State tiles and memory.  "Rows": value 16 q + li, keys 16 jb + 4 g ..; "columns": value
+// 16 ib + 4 g + r, key 16 q + li.  A null state reads as zeros.
+template <int NB> struct StateIo {
+    int N, col, g;
+    uint32_t bytes;
+    __device__ __forceinline__ StateIo(const GradParams &p, const Place &w) : N(p.N), col(w.col), g(w.g), bytes((uint32_t)(p.N * p.N * 4)) {}
+    __device__ __forceinline__ uint32_t row(int jb) const {
+        return col < N && 16 * jb + 4 * g < N ? (uint32_t)(col * N + 16 * jb + 4 * g) * 4u : kBufferOob;
+    }
+    // Column elements share a lane offset; their rows' uniform part goes into the scalar offset, which
+    // stays below the range (16 (NB - 1) + 3 < N), while values past N end beyond it.
+    __device__ __forceinline__ uint32_t column() const { return col < N ? (uint32_t)(4 * g * N + col) * 4u : kBufferOob; }
+    __device__ __forceinline__ uint32_t row_part(int ib, int r) const { return (uint32_t)((16 * ib + r) * N) * 4u; }
+    __device__ __forceinline__ void load_rows(const float *s, floatx4 (&x)[NB]) const {
+        const auto rs = make_rsrc(s, s ? bytes : 0u);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) x[jb] = buf_load4(rs, row(jb));
+    }
+    __device__ __forceinline__ void store_rows(const floatx4 (&x)[NB], float *s) const {
+        const auto rs = make_rsrc(s, bytes);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) buf_store4(x[jb], rs, row(jb));
+    }
+    __device__ __forceinline__ void load_columns(const float *s, floatx4 (&x)[NB]) const {
+        const auto rs = make_rsrc(s, s ? bytes : 0u);
 #pragma unroll
         for (int ib = 0; ib < NB; ++ib)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[ib][r] = buf_load(rs, cols_at(ib, r));
+            for (int r = 0; r < 4; ++r)
+                x[ib][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, column(), row_part(ib, r), 0));
+    }
+    __device__ __forceinline__ void store_columns(const floatx4 (&x)[NB], float *s) const {
+        const auto rs = make_rsrc(s, bytes);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float v = x[ib][r];  // __builtin_bit_cast of a vector's element itself takes its first one
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rs, column(), row_part(ib, r), 0);
+            }
+    }
+};
+
+__device__ __forceinline__ const float *head_state(const float *s, const GradParams &p, int head) {
+    return s ? s + (size_t)head * p.N * p.N : nullptr;
+}
+__device__ __forceinline__ float *seg_state(float *s, const GradParams &p, int head, int seg) {
+    return s + ((size_t)head * p.segments + seg) * p.N * p.N;
+}
+
+template <int NB> struct Sweep {
+    static constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
+    static constexpr int kBuf = 3 * kTok + NP;  // three token tiles and D_15
+    static constexpr int kFloats = 2 * kBuf;    // two of them: one barrier per chunk
+};
+
+// S^T[:, value tile q], as NB tiles of 16 keys, over the segment's chunks; KEEP: the state
+// before each chunk and U go to memory; POWER: P likewise, with v = 0.
+template <int NB, bool KEEP, bool POWER>
+__device__ __forceinline__ void sweep_forward(const GradParams &p, const Place &w, float *lds, floatx4 (&S)[NB], floatx4 (&P)[NB]) {
+    using Ly = Sweep<NB>;
+    constexpr int SA = Ly::SA, kTok = Ly::kTok;
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const float *frags = p.frags + (size_t)w.head * p.chunks * kFrags * kFrag + 4 * w.lane;
+    float *us = p.u + ((size_t)w.head * p.chunks * NB + w.q) * kFrag + 4 * w.lane;
+    const StateIo<NB> io(p, w);
+    floatx4 wv, k, v, a, b;
+    auto fetch = [&](int c) {
+        Tile tile;
+        tile.at(p, w.bb, w.h, c, w.col, w.g);
+        wv = tile.load(p.w);
+        k = tile.load(p.k);
+        v = tile.load(p.v);
+        a = tile.load(p.a);
+        b = tile.load(p.b);
     };
+    if (w.c0 < w.c1) fetch(w.c0);
+    for (int c = w.c0; c < w.c1; ++c) {
+        float *sA = lds + ((c - w.c0) & 1) * Ly::kBuf, *sB = sA + kTok, *sK = sB + kTok, *sD = sK + kTok;
+        const floatx4 t_row = ld4(frags + ((size_t)c * kFrags + kTRow) * kFrag);
+        const floatx4 c_row = ld4(frags + ((size_t)c * kFrags + kCRow) * kFrag);
+        if constexpr (KEEP) io.store_rows(S, p.states + ((size_t)w.head * p.chunks + c) * p.N * p.N);
+        Decays d;
+        d.set(wv, min(kC, p.T - c * kC), w.g);
+        const int at = 4 * w.g * SA + w.col;
+        stcol(sA + at, SA, a * d.before);
+        stcol(sB + at, SA, b * d.inv);
+        stcol(sK + at, SA, k * d.inv);
+        if (w.g == 3) sD[w.col] = d.last;
+        const floatx4 v4 = v;
+        if (c + 1 < w.c1) fetch(c + 1);
+        lds_barrier();
+        floatx4 X = zero, XP = zero;
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) {
+            const floatx4 a4 = ld4(sA + w.li * SA + 16 * jb + 4 * w.g);
+            X = mul16(a4, S[jb], X);
+            if constexpr (POWER) XP = mul16(a4, P[jb], XP);
+        }
+        floatx4 U = mul16(c_row, v4, zero), UP;
+        U = mul16(t_row, X, U);
+        if constexpr (POWER) UP = mul16(t_row, XP, zero);
+        if constexpr (KEEP) st4(us + (size_t)c * NB * kFrag, U);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) {
+            const int o = 4 * w.g * SA + 16 * jb + w.li;
+            const floatx4 d4 = ld4(sD + 16 * jb + 4 * w.g), b4 = ldcol(sB + o, SA);
+            S[jb] = mul16(b4, U, mul16(ldcol(sK + o, SA), v4, S[jb])) * d4;
+            if constexpr (POWER) P[jb] = mul16(b4, UP, P[jb]) * d4;
+        }
+    }
+}
+
+// G^T[:, value tile q] backward over the segment's chunks.
+template <int NB>
+__device__ __forceinline__ void sweep_backward(const GradParams &p, const Place &w, float *lds, floatx4 (&G)[NB]) {
+    using Ly = Sweep<NB>;
+    constexpr int SA = Ly::SA, kTok = Ly::kTok;
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const float *frags = p.frags + (size_t)w.head * p.chunks * kFrags * kFrag + 4 * w.lane;
+    floatx4 wv, r, y, a, b;
+    auto fetch = [&](int c) {
+        Tile tile;
+        tile.at(p, w.bb, w.h, c, w.col, w.g);
+        wv = tile.load(p.w);
+        r = tile.load(p.r);
+        y = tile.load(p.dy);
+        a = tile.load(p.a);
+        b = tile.load(p.b);
+    };
+    if (w.c0 < w.c1) fetch(w.c1 - 1);
+    for (int c = w.c1 - 1; c >= w.c0; --c) {
+        float *sA = lds + ((c - w.c0) & 1) * Ly::kBuf, *sB = sA + kTok, *sR = sB + kTok, *sD = sR + kTok;
+        const floatx4 t_col = ld4(frags + ((size_t)c * kFrags + kTCol) * kFrag);
+        const floatx4 rb_col = ld4(frags + ((size_t)c * kFrags + kMrbCol) * kFrag);
+        Decays d;
+        d.set(wv, min(kC, p.T - c * kC), w.g);
+        const int at = 4 * w.g * SA + w.col;
+        stcol(sA + at, SA, a * d.before);
+        stcol(sB + at, SA, b * d.inv);
+        stcol(sR + at, SA, r * d.now);
+        if (w.g == 3) sD[w.col] = d.last;
+        const floatx4 y4 = y;
+        if (c > w.c0) fetch(c - 1);
+        lds_barrier();
+        floatx4 F = mul16(rb_col, y4, zero);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) {
+            G[jb] *= ld4(sD + 16 * jb + 4 * w.g);
+            F = mul16(ld4(sB + w.li * SA + 16 * jb + 4 * w.g), G[jb], F);
+        }
+        const floatx4 E = mul16(t_col, F, zero);
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) {
+            const int o = 4 * w.g * SA + 16 * jb + w.li;
+            G[jb] = mul16(ldcol(sA + o, SA), E, mul16(ldcol(sR + o, SA), y4, G[jb]));
+        }
+    }
+}
+
+// Workgroups: the segments 0 .. segments - 2 of every head forward, then 1 .. segments - 1 backward.
+template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_local_kernel(GradParams p, int units, int per_xcd) {
+    __shared__ __attribute__((aligned(16))) float lds[Sweep<NB>::kFloats];
+    int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;
+    const int per_head = p.segments - 1, half = units / 2;
+    const bool back = unit >= half;
+    if (back) unit -= half;
+    const int head = unit / per_head, seg = unit - head * per_head + back;
+    const Place w(p, head, seg);
+    const StateIo<NB> io(p, w);
+    floatx4 S[NB], P[NB];
+    if (back) {
+        io.load_rows(seg == p.segments - 1 ? head_state(p.dstate_out, p, head) : nullptr, S);
+        sweep_backward<NB>(p, w, lds, S);
+        io.store_rows(S, seg_state(p.ends, p, head, seg - 1));
+        return;
+    }
+    io.load_rows(seg == 0 ? head_state(p.state_in, p, head) : nullptr, S);
+    if (seg == 0) {
+        sweep_forward<NB, false, false>(p, w, lds, S, P);
+    } else {
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) P[jb][r] = 16 * jb + 4 * w.g + r == w.col ? 1.0f : 0.0f;
+        sweep_forward<NB, false, true>(p, w, lds, S, P);
+        io.store_rows(P, seg_state(p.powers, p, head, seg));
+    }
+    io.store_rows(S, seg_state(p.starts, p, head, seg + 1));
+}
+
+// A wave per (head, value tile, direction): x <- x Pi + local (x Pi^T backward) over the
+// segments between the first and the last.
+template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_carry_kernel(GradParams p, int units, int per_xcd) {
+    int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;
+    const int head = unit / (2 * NB);
+    unit -= head * 2 * NB;
+    const bool back = unit >= NB;
+    const int q = back ? unit - NB : unit;
+    Place w(p, head, 0);
+    w.q = q;
+    w.col = 16 * q + w.li;
+    const StateIo<NB> io(p, w);
+    const int N = p.N, dir = back ? -1 : 1;
+    float *slots = back ? p.ends : p.starts;
+    // Forward: slot 1 is final, slot s + 1 += slot s Pi_s; backward: slot segments - 2 is, slot
+    // s - 1 += slot s Pi_s^T.
+    int s = back ? p.segments - 2 : 1;
+    floatx4 x[NB], local[NB];
+    io.load_rows(seg_state(slots, p, head, s), x);
+    for (int n = 0; n < p.segments - 2; ++n, s += dir) {
+        const auto rs = make_rsrc(seg_state(p.powers, p, head, s), io.bytes);
+        float *next = seg_state(slots, p, head, s + dir);
+        io.load_rows(next, local);
+        // x^T[j][i] = sum_k Pi[k][j] x^T[k][i], and Pi[j][k] backward: rows j = 16 jb + li, four k.
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb)
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                const int j = 16 * jb + w.li, k = 16 * kb + 4 * w.g;
+                const bool in = j < N && k < N;  // N % 4 == 0
+                floatx4 m;
+                if (back) {
+                    m = buf_load4(rs, in ? (uint32_t)(j * N + k) * 4u : kBufferOob);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m[r] = buf_load(rs, in ? (uint32_t)((k + r) * N + j) * 4u : kBufferOob);
+                }
+                local[jb] = mul16(m, x[kb], local[jb]);
+            }
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) x[jb] = local[jb];
+        io.store_rows(x, next);
+    }
+}
+
+// A workgroup of NB waves per segment of a head.
+template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
+    // Backward: B, K, V, Y', U, E, G [value][key] and the four 16 x 16 gradients.
+    constexpr int kBackward = 6 * kTok + NP * SA + 4 * kC * kST;
+    __shared__ __attribute__((aligned(16))) float lds[Sweep<NB>::kFloats > kBackward ? Sweep<NB>::kFloats : kBackward];
+    static_assert(sizeof(lds) <= 160 * 1024, "LDS of one CU");
+    const int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;  // uniform over the workgroup
+    const int head = unit / p.segments, seg = unit - head * p.segments;
+    const Place w(p, head, seg);
+    const StateIo<NB> io(p, w);
+    const int q = w.q, g = w.g, li = w.li, col = w.col, N = p.N;
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const float *frags = p.frags + (size_t)head * p.chunks * kFrags * kFrag + 4 * w.lane;
+    const float *states = p.states + (size_t)head * p.chunks * N * N;
+    const float *us = p.u + ((size_t)head * p.chunks * NB + q) * kFrag + 4 * w.lane;
 
     {
-        // --------------------------------------------------------------- forward
-        // S^T[:, value tile q] as NB tiles of 16 keys.
-        floatx4 S[NB];
-        {
-            const float *s0 = p.state_in ? p.state_in + (size_t)head * N * N : nullptr;
-            const auto rs = make_rsrc(s0, s0 ? state_bytes : 0u);
-#pragma unroll
-            for (int jb = 0; jb < NB; ++jb) S[jb] = buf_load4(rs, rows_at(jb));
-        }
-        auto keep = [&](int slot) {
-            const auto rs = make_rsrc(states + (size_t)slot * N * N, state_bytes);
-#pragma unroll
-            for (int jb = 0; jb < NB; ++jb) buf_store4(S[jb], rs, rows_at(jb));
-        };
-        floatx4 w, k, v, a, b;
-        auto fetch = [&](int c) {
-            Tile tile;
-            tile.at(p, bb, h, c, col, g);
-            w = tile.load(p.w);
-            k = tile.load(p.k);
-            v = tile.load(p.v);
-            a = tile.load(p.a);
-            b = tile.load(p.b);
-        };
-        if (nc > 0) fetch(0);
-        for (int c = 0; c < nc; ++c) {
-            float *sA = lds + (c & 1) * (3 * kTok + NP), *sB = sA + kTok, *sK = sB + kTok, *sD = sK + kTok;
-            const floatx4 t_row = ld4(frags + ((size_t)c * kFrags + kTRow) * kFrag);
-            const floatx4 c_row = ld4(frags + ((size_t)c * kFrags + kCRow) * kFrag);
-            keep(c);
-            Decays d;
-            d.set(w, min(kC, p.T - c * kC), g);
-            const int at = 4 * g * SA + col;
-            stcol(sA + at, SA, a * d.before);
-            stcol(sB + at, SA, b * d.inv);
-            stcol(sK + at, SA, k * d.inv);
-            if (g == 3) sD[col] = d.last;
-            const floatx4 v4 = v;
-            if (c + 1 < nc) fetch(c + 1);
-            lds_barrier();
-            floatx4 X = zero;
-#pragma unroll
-            for (int jb = 0; jb < NB; ++jb) X = mul16(ld4(sA + li * SA + 16 * jb + 4 * g), S[jb], X);
-            floatx4 U = mul16(c_row, v4, zero);
-            U = mul16(t_row, X, U);
-            st4(us + (size_t)c * NB * kFrag, U);
-#pragma unroll
-            for (int jb = 0; jb < NB; ++jb) {
-                floatx4 s = mul16(ldcol(sK + 4 * g * SA + 16 * jb + li, SA), v4, S[jb]);
-                s = mul16(ldcol(sB + 4 * g * SA + 16 * jb + li, SA), U, s);
-                S[jb] = s * ld4(sD + 16 * jb + 4 * g);
-            }
-        }
+        floatx4 S[NB], none[NB];
+        io.load_rows(seg == 0 ? head_state(p.state_in, p, head) : seg_state(p.starts, p, head, seg), S);
+        sweep_forward<NB, true, false>(p, w, lds, S, none);
     }
     __syncthreads();  // the states are read across waves, and LDS is used anew
 
@@ -358,17 +561,17 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(
     float *sMrb = sG + NP * SA, *sMrk = sMrb + kC * kST, *sLab = sMrk + kC * kST, *sLak = sLab + kC * kST;
     // G[:, key tile q] as NB tiles of 16 values, and S0 in the same layout.
     floatx4 G[NB], S0[NB];
-    load_cols(p.dstate_out ? p.dstate_out + (size_t)head * N * N : nullptr, G);
-    for (int c = nc - 1; c >= 0; --c) {
+    io.load_columns(seg == p.segments - 1 ? head_state(p.dstate_out, p, head) : seg_state(p.ends, p, head, seg), G);
+    for (int c = w.c1 - 1; c >= w.c0; --c) {
         Tile tile;
-        tile.at(p, bb, h, c, col, g);
+        tile.at(p, w.bb, w.h, c, col, g);
         const float *fr = frags + (size_t)c * kFrags * kFrag;
-        const floatx4 w = tile.load(p.w), rr = tile.load(p.r), aa = tile.load(p.a), bv = tile.load(p.b);
+        const floatx4 wv = tile.load(p.w), rr = tile.load(p.r), aa = tile.load(p.a), bv = tile.load(p.b);
         const floatx4 kv = tile.load(p.k), vv = tile.load(p.v), yv = tile.load(p.dy);
         const floatx4 uv = ld4(us + (size_t)c * NB * kFrag);
-        load_cols(states + (size_t)c * N * N, S0);
+        io.load_columns(states + (size_t)c * N * N, S0);
         Decays d;
-        d.set(w, min(kC, p.T - c * kC), g);
+        d.set(wv, min(kC, p.T - c * kC), g);
         const floatx4 A = aa * d.before, R = rr * d.now, B = bv * d.inv, K = kv * d.inv;
         const int at = 4 * g * SA + col;
         stcol(sB + at, SA, B);
@@ -454,36 +657,63 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(
         }
         tile.store(p.dw, dw);
     }
-    if (p.dstate_in) {
-        const auto rs = make_rsrc(p.dstate_in + (size_t)head * N * N, state_bytes);
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) buf_store(G[ib][r], rs, cols_at(ib, r));
-    }
+    if (p.dstate_in && seg == 0) io.store_columns(G, p.dstate_in + (size_t)head * N * N);
+}
+
+// Segments so that the last kernel's workgroups fill the GPU (about as many as it holds at
+// once), of at least four chunks each.
+int segments_of(int B, int T, int H, int N) {
+    const int64_t heads = (int64_t)B * H;
+    const int chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
+    const int resident = 256 * (NB <= 3 ? 4 : NB == 4 ? 3 : 1);
+    const int64_t want = (resident + heads - 1) / heads;
+    const int most = chunks / 4 > 1 ? chunks / 4 : 1;
+    return (int)(want < most ? want : most);
 }
 
 struct Scratch {
-    size_t frags, states, u, bytes;
+    size_t frags, states, u, starts, ends, powers, bytes;
+    int segments, seg_chunks;
 };
 
 Scratch scratch_of(int B, int T, int H, int N) {
     const size_t heads = (size_t)B * H, chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Scratch o{};
-    o.frags = 0;
-    o.states = o.frags + up(heads * chunks * kFrags * kFrag * sizeof(float));
-    o.u = o.states + up(heads * chunks * N * N * sizeof(float));
-    o.bytes = o.u + up(heads * chunks * NB * kFrag * sizeof(float)) + 256;  // some buffer for T = 0 too
+    const int most = segments_of(B, T, H, N);
+    o.seg_chunks = (int)(chunks + most - 1) / most;
+    o.segments = chunks ? (int)(chunks + o.seg_chunks - 1) / o.seg_chunks : 1;
+    size_t at = 0;
+    auto take = [&](size_t floats) {
+        const size_t here = at;
+        at += up(floats * sizeof(float));
+        return here;
+    };
+    o.frags = take(heads * chunks * kFrags * kFrag);
+    o.states = take(heads * chunks * N * N);
+    o.u = take(heads * chunks * NB * kFrag);
+    const size_t per_seg = o.segments > 1 ? heads * o.segments * N * N : 0;
+    o.starts = take(per_seg);
+    o.ends = take(per_seg);
+    o.powers = take(per_seg);
+    o.bytes = at + 256;  // some buffer for T = 0 too
     return o;
 }
 
 template <int NB> void launch(const GradParams &p, hipStream_t s) {
-    const int heads = p.B * p.H, grams = heads * p.chunks;
+    const int heads = p.B * p.H, grams = heads * p.chunks, segs = heads * p.segments;
     auto per_xcd = [](int units) { return (units + kXcds - 1) / kXcds; };
     if (grams > 0)
         hipLaunchKernelGGL((wkv7_grad_gram_kernel<NB>), dim3(per_xcd(grams) * kXcds), dim3(kWave), 0, s, p, grams, per_xcd(grams));
-    hipLaunchKernelGGL((wkv7_grad_kernel<NB>), dim3(per_xcd(heads) * kXcds), dim3(NB * kWave), 0, s, p, heads, per_xcd(heads));
+    if (p.segments > 1) {
+        const int locals = 2 * heads * (p.segments - 1);
+        hipLaunchKernelGGL((wkv7_grad_local_kernel<NB>), dim3(per_xcd(locals) * kXcds), dim3(NB * kWave), 0, s, p, locals, per_xcd(locals));
+    }
+    if (p.segments > 2) {
+        const int waves = heads * 2 * NB;
+        hipLaunchKernelGGL((wkv7_grad_carry_kernel<NB>), dim3(per_xcd(waves) * kXcds), dim3(kWave), 0, s, p, waves, per_xcd(waves));
+    }
+    hipLaunchKernelGGL((wkv7_grad_kernel<NB>), dim3(per_xcd(segs) * kXcds), dim3(NB * kWave), 0, s, p, segs, per_xcd(segs));
 }
 
 }  // namespace
@@ -520,6 +750,11 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     p.frags = reinterpret_cast<float *>(base + o.frags);
     p.states = reinterpret_cast<float *>(base + o.states);
     p.u = reinterpret_cast<float *>(base + o.u);
+    p.starts = reinterpret_cast<float *>(base + o.starts);
+    p.ends = reinterpret_cast<float *>(base + o.ends);
+    p.powers = reinterpret_cast<float *>(base + o.powers);
+    p.segments = o.segments;
+    p.seg_chunks = o.seg_chunks;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch ((N + 15) / 16) {
         case 1: launch<1>(p, s); break;
