@@ -30,7 +30,7 @@
 //                           state of S = I with v = 0), where S1 = S0 Pi + local and G0 =
 //                           G1 Pi^T + local.  The first segment starts from the call's state
 //                           and the last from its gradient, so that these two are final.
-//   wkv7_grad_carry_kernel  both recurrences over the segments, a wave per value tile.
+//   wkv7_grad_carry_kernel  both recurrences over the segments, a workgroup per value tile.
 //   wkv7_grad_kernel        per segment: S forward over its chunks (kept per chunk, with U),
 //                           then G and the gradients backward.
 // One segment needs the first and the last alone, two no carry.
@@ -70,8 +70,8 @@ struct GradParams {
     float *states;  // [B H][chunks][N][N]: the state before each chunk
     float *u;       // [B H][chunks][NB][kFrag]
     // [B H][segments][N][N]: the state before segment s >= 1, the gradient of the state after
-    // segment s <= segments - 2, and Pi of the segments between the first and the last.
-    float *starts, *ends, *powers;
+    // segment s <= segments - 2, and Pi and Pi^T of the segments between the first and the last.
+    float *starts, *ends, *powers, *powers_t;
 };
 
 __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
@@ -82,6 +82,21 @@ __device__ __forceinline__ floatx4 mul16(floatx4 a, floatx4 b, floatx4 c) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) c = mfma(a[r], b[r], c);
     return c;
+}
+// Products side by side: an MFMA waits for the one before it where it adds to the same
+// accumulator, so independent sums take turns.
+__device__ __forceinline__ void mul16(floatx4 a0, floatx4 b0, floatx4 &c0, floatx4 a1, floatx4 b1, floatx4 &c1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        c0 = mfma(a0[r], b0[r], c0);
+        c1 = mfma(a1[r], b1[r], c1);
+    }
+}
+template <int NB> __device__ __forceinline__ void mul16_tiles(const floatx4 (&a)[NB], floatx4 b, floatx4 (&c)[NB]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < NB; ++t) c[t] = mfma(a[t][r], b[r], c[t]);
 }
 __device__ __forceinline__ floatx4 ld4(const float *p) { return *reinterpret_cast<const floatx4 *>(p); }
 __device__ __forceinline__ void st4(float *p, floatx4 v) { *reinterpret_cast<floatx4 *>(p) = v; }
@@ -329,7 +344,7 @@ template <int NB> struct StateIo {
         for (int ib = 0; ib < NB; ++ib)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float v = x[ib][r];  // __builtin_bit_cast of a vector's element itself takes its first one
+                const float v = x[ib][r];  // a copy: __builtin_bit_cast takes a vector element in place for the first one
                 __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rs, column(), row_part(ib, r), 0);
             }
     }
@@ -384,23 +399,41 @@ __device__ __forceinline__ void sweep_forward(const GradParams &p, const Place &
         const floatx4 v4 = v;
         if (c + 1 < w.c1) fetch(c + 1);
         lds_barrier();
-        floatx4 X = zero, XP = zero;
+        floatx4 X = zero, Y = zero, U = zero, UP = zero;  // POWER: Y is X of P, else X's odd k-steps
 #pragma unroll
         for (int jb = 0; jb < NB; ++jb) {
             const floatx4 a4 = ld4(sA + w.li * SA + 16 * jb + 4 * w.g);
-            X = mul16(a4, S[jb], X);
-            if constexpr (POWER) XP = mul16(a4, P[jb], XP);
+            if constexpr (POWER) {
+                mul16(a4, S[jb], X, a4, P[jb], Y);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    X = mfma(a4[r], S[jb][r], X);
+                    Y = mfma(a4[r + 1], S[jb][r + 1], Y);
+                }
+            }
         }
-        floatx4 U = mul16(c_row, v4, zero), UP;
-        U = mul16(t_row, X, U);
-        if constexpr (POWER) UP = mul16(t_row, XP, zero);
+        U = mul16(c_row, v4, U);
+        floatx4 k4[NB], b4[NB];
+#pragma unroll
+        for (int jb = 0; jb < NB; ++jb) k4[jb] = ldcol(sK + 4 * w.g * SA + 16 * jb + w.li, SA);
+        mul16_tiles<NB>(k4, v4, S);
+        if constexpr (POWER) {
+            mul16(t_row, X, U, t_row, Y, UP);
+        } else {
+            X += Y;
+            U = mul16(t_row, X, U);
+        }
         if constexpr (KEEP) st4(us + (size_t)c * NB * kFrag, U);
 #pragma unroll
+        for (int jb = 0; jb < NB; ++jb) b4[jb] = ldcol(sB + 4 * w.g * SA + 16 * jb + w.li, SA);
+        mul16_tiles<NB>(b4, U, S);
+        if constexpr (POWER) mul16_tiles<NB>(b4, UP, P);
+#pragma unroll
         for (int jb = 0; jb < NB; ++jb) {
-            const int o = 4 * w.g * SA + 16 * jb + w.li;
-            const floatx4 d4 = ld4(sD + 16 * jb + 4 * w.g), b4 = ldcol(sB + o, SA);
-            S[jb] = mul16(b4, U, mul16(ldcol(sK + o, SA), v4, S[jb])) * d4;
-            if constexpr (POWER) P[jb] = mul16(b4, UP, P[jb]) * d4;
+            const floatx4 d4 = ld4(sD + 16 * jb + 4 * w.g);
+            S[jb] *= d4;
+            if constexpr (POWER) P[jb] *= d4;
         }
     }
 }
@@ -437,18 +470,28 @@ __device__ __forceinline__ void sweep_backward(const GradParams &p, const Place 
         const floatx4 y4 = y;
         if (c > w.c0) fetch(c - 1);
         lds_barrier();
-        floatx4 F = mul16(rb_col, y4, zero);
+        floatx4 F = zero, F1 = zero;  // even and odd k-steps
+        F1 = mul16(rb_col, y4, F1);
 #pragma unroll
         for (int jb = 0; jb < NB; ++jb) {
             G[jb] *= ld4(sD + 16 * jb + 4 * w.g);
-            F = mul16(ld4(sB + w.li * SA + 16 * jb + 4 * w.g), G[jb], F);
+            const floatx4 b4 = ld4(sB + w.li * SA + 16 * jb + 4 * w.g);
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                F = mfma(b4[r], G[jb][r], F);
+                F1 = mfma(b4[r + 1], G[jb][r + 1], F1);
+            }
         }
-        const floatx4 E = mul16(t_col, F, zero);
+        F += F1;
+        floatx4 r4[NB], a4[NB];
 #pragma unroll
         for (int jb = 0; jb < NB; ++jb) {
             const int o = 4 * w.g * SA + 16 * jb + w.li;
-            G[jb] = mul16(ldcol(sA + o, SA), E, mul16(ldcol(sR + o, SA), y4, G[jb]));
+            r4[jb] = ldcol(sR + o, SA);
+            a4[jb] = ldcol(sA + o, SA);
         }
+        mul16_tiles<NB>(r4, y4, G);
+        mul16_tiles<NB>(a4, mul16(t_col, F, zero), G);
     }
 }
 
@@ -480,53 +523,69 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_local_k
             for (int r = 0; r < 4; ++r) P[jb][r] = 16 * jb + 4 * w.g + r == w.col ? 1.0f : 0.0f;
         sweep_forward<NB, false, true>(p, w, lds, S, P);
         io.store_rows(P, seg_state(p.powers, p, head, seg));
+        io.store_columns(P, seg_state(p.powers_t, p, head, seg));
     }
     io.store_rows(S, seg_state(p.starts, p, head, seg + 1));
 }
 
-// A wave per (head, value tile, direction): x <- x Pi + local (x Pi^T backward) over the
-// segments between the first and the last.
-template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_carry_kernel(GradParams p, int units, int per_xcd) {
+// A workgroup per (head, value tile, direction): x <- x Pi + local (x Pi^T backward) over the
+// segments between the first and the last; wave q computes key tile q, and the tiles of x go round
+// through LDS.  Each step waits for memory longer than for its products, so loads run kAhead steps ahead.
+template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_carry_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int kAhead = 3;
+    __shared__ __attribute__((aligned(16))) float tiles[2][NB][kFrag];
     int unit = xcd_unit(per_xcd);
-    if (unit >= units) return;
+    if (unit >= units) return;  // uniform over the workgroup
     const int head = unit / (2 * NB);
     unit -= head * 2 * NB;
     const bool back = unit >= NB;
-    const int q = back ? unit - NB : unit;
-    Place w(p, head, 0);
-    w.q = q;
-    w.col = 16 * q + w.li;
-    const StateIo<NB> io(p, w);
-    const int N = p.N, dir = back ? -1 : 1;
+    const int i = 16 * (back ? unit - NB : unit) + (threadIdx.x & 15);  // value of the lane's column
+    const Place w(p, head, 0);
+    const int N = p.N, dir = back ? -1 : 1, steps = p.segments - 2;
+    const uint32_t bytes = (uint32_t)(N * N * 4);
     float *slots = back ? p.ends : p.starts;
+    // Element offsets of (value i, keys 16 q + 4 g ..) of a state and (row 16 q + li, 16 kb + 4 g ..) of Pi.
+    const uint32_t own = i < N && 16 * w.q + 4 * w.g < N ? (uint32_t)(i * N + 16 * w.q + 4 * w.g) * 4u : kBufferOob;
+    uint32_t at[NB];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+        at[kb] = w.col < N && 16 * kb + 4 * w.g < N ? (uint32_t)(w.col * N + 16 * kb + 4 * w.g) * 4u : kBufferOob;
     // Forward: slot 1 is final, slot s + 1 += slot s Pi_s; backward: slot segments - 2 is, slot
-    // s - 1 += slot s Pi_s^T.
-    int s = back ? p.segments - 2 : 1;
-    floatx4 x[NB], local[NB];
-    io.load_rows(seg_state(slots, p, head, s), x);
-    for (int n = 0; n < p.segments - 2; ++n, s += dir) {
-        const auto rs = make_rsrc(seg_state(p.powers, p, head, s), io.bytes);
-        float *next = seg_state(slots, p, head, s + dir);
-        io.load_rows(next, local);
-        // x^T[j][i] = sum_k Pi[k][j] x^T[k][i], and Pi[j][k] backward: rows j = 16 jb + li, four k.
+    // s - 1 += slot s Pi_s^T.  x^T[j][i] = sum_k Pi^T[j][k] x^T[k][i] (Pi[j][k] backward).
+    const int first = back ? p.segments - 2 : 1;
+    floatx4 pi[kAhead][NB], local[kAhead];
+    auto fetch = [&](int n, floatx4 (&m)[NB], floatx4 &l) {
+        const int s = first + min(n, steps - 1) * dir;  // past the last step: its values again, unused
+        const auto rs = make_rsrc(seg_state(back ? p.powers : p.powers_t, p, head, s), bytes);
 #pragma unroll
-        for (int jb = 0; jb < NB; ++jb)
+        for (int kb = 0; kb < NB; ++kb) m[kb] = buf_load4(rs, at[kb]);
+        l = buf_load4(make_rsrc(seg_state(slots, p, head, s + dir), bytes), own);
+    };
+    floatx4 x = buf_load4(make_rsrc(seg_state(slots, p, head, first), bytes), own);
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) {
-                const int j = 16 * jb + w.li, k = 16 * kb + 4 * w.g;
-                const bool in = j < N && k < N;  // N % 4 == 0
-                floatx4 m;
-                if (back) {
-                    m = buf_load4(rs, in ? (uint32_t)(j * N + k) * 4u : kBufferOob);
-                } else {
+    for (int n = 0; n < kAhead; ++n) fetch(n, pi[n], local[n]);
+    auto step = [&](int n, floatx4 (&m)[NB], floatx4 &l) {
+        st4(&tiles[n & 1][w.q][4 * w.lane], x);
+        lds_barrier();
+        floatx4 y0 = l, y1 = {0.f, 0.f, 0.f, 0.f};  // even and odd k-steps
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) m[r] = buf_load(rs, in ? (uint32_t)((k + r) * N + j) * 4u : kBufferOob);
-                }
-                local[jb] = mul16(m, x[kb], local[jb]);
+        for (int kb = 0; kb < NB; ++kb) {
+            const floatx4 k4 = ld4(&tiles[n & 1][kb][4 * w.lane]);
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                y0 = mfma(m[kb][r], k4[r], y0);
+                y1 = mfma(m[kb][r + 1], k4[r + 1], y1);
             }
+        }
+        x = y0 + y1;
+        // Loads of a slot that this step writes were issued before its store: each slot is read once, ahead.
+        fetch(n + kAhead, m, l);
+        buf_store4(x, make_rsrc(seg_state(slots, p, head, first + (n + 1) * dir), bytes), own);
+    };
+    for (int n = 0; n < steps; n += kAhead) {
 #pragma unroll
-        for (int jb = 0; jb < NB; ++jb) x[jb] = local[jb];
-        io.store_rows(x, next);
+        for (int e = 0; e < kAhead; ++e)
+            if (n + e < steps) step(n + e, pi[e], local[e]);
     }
 }
 
@@ -587,32 +646,40 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(
         const floatx4 t_col = ld4(fr + kTCol * kFrag), c_col = ld4(fr + kCCol * kFrag);
         const floatx4 rb_col = ld4(fr + kMrbCol * kFrag), rk_col = ld4(fr + kMrkCol * kFrag);
         lds_barrier();
-        // Value tile q: F, E, V'.
-        floatx4 F = mul16(rb_col, yv, zero), dV = mul16(rk_col, yv, zero);
+        // Value tile q: F, V'; key tile q: Y' S0, U G, V G.
+        floatx4 F = zero, dV = zero, dR = zero, dA = zero, dB = zero, dK = zero;
+        mul16(rb_col, yv, F, rk_col, yv, dV);
 #pragma unroll
-        for (int jb = 0; jb < NB; ++jb) {
-            const floatx4 g4 = ld4(sG + col * SA + 16 * jb + 4 * g);
-            F = mul16(ld4(sB + li * SA + 16 * jb + 4 * g), g4, F);
-            dV = mul16(ld4(sK + li * SA + 16 * jb + 4 * g), g4, dV);
+        for (int t = 0; t < NB; ++t) {
+            const int o = li * SA + 16 * t + 4 * g;
+            const floatx4 g4 = ld4(sG + col * SA + 16 * t + 4 * g), b4 = ld4(sB + o), k4 = ld4(sK + o);
+            const floatx4 y4 = ld4(sY + o), u4 = ld4(sU + o), v4 = ld4(sV + o);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                F = mfma(b4[r], g4[r], F);
+                dV = mfma(k4[r], g4[r], dV);
+                dR = mfma(y4[r], S0[t][r], dR);
+                dB = mfma(u4[r], G[t][r], dB);
+                dK = mfma(v4[r], G[t][r], dK);
+            }
         }
-        const floatx4 E = mul16(t_col, F, zero);
+        floatx4 E = zero;
+        mul16(t_col, F, E, c_col, F, dV);
         stcol(sE + at, SA, E);
-        dV = mul16(c_col, F, dV);
         tile.store(p.dv, dV);
-        // Key tile q: Y' S0, U G, V G.
-        floatx4 dR = zero, dA = zero, dB = zero, dK = zero;
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib) {
-            const int o = li * SA + 16 * ib + 4 * g;
-            dR = mul16(ld4(sY + o), S0[ib], dR);
-            dB = mul16(ld4(sU + o), G[ib], dB);
-            dK = mul16(ld4(sV + o), G[ib], dK);
-        }
         // Rows t = 4 g + r, columns s = li of X Z^T, kept where s <= t (s < t).
         auto gram = [&](const float *x, const float *z, float *out, bool strict) {
-            floatx4 m = zero;
+            floatx4 m = zero, m1 = zero;  // even and odd k-steps
 #pragma unroll
-            for (int ib = 0; ib < NB; ++ib) m = mul16(ld4(x + li * SA + 16 * ib + 4 * g), ld4(z + li * SA + 16 * ib + 4 * g), m);
+            for (int t = 0; t < NB; ++t) {
+                const floatx4 x4 = ld4(x + li * SA + 16 * t + 4 * g), z4 = ld4(z + li * SA + 16 * t + 4 * g);
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    m = mfma(x4[r], z4[r], m);
+                    m1 = mfma(x4[r + 1], z4[r + 1], m1);
+                }
+            }
+            m += m1;
 #pragma unroll
             for (int r = 0; r < 4; ++r) out[(4 * g + r) * kST + li] = li < 4 * g + r + !strict ? m[r] : 0.0f;
         };
@@ -621,22 +688,32 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(
         lds_barrier();
         if (q == (NB > 2 ? 2 : 0)) gram(sE, sU, sLab, true);
         if (q == (NB > 3 ? 3 : NB > 1 ? 1 : 0)) gram(sE, sV, sLak, true);
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib) {
-            dA = mul16(ld4(sE + li * SA + 16 * ib + 4 * g), S0[ib], dA);
+        {
             // G0 = G + Y'^T R + E^T A
-            floatx4 n = mul16(ldcol(sY + 4 * g * SA + 16 * ib + li, SA), R, G[ib]);
-            G[ib] = mul16(ldcol(sE + 4 * g * SA + 16 * ib + li, SA), A, n);
+            floatx4 x4[NB];
+#pragma unroll
+            for (int t = 0; t < NB; ++t) x4[t] = ldcol(sY + 4 * g * SA + 16 * t + li, SA);
+            mul16_tiles<NB>(x4, R, G);
+#pragma unroll
+            for (int t = 0; t < NB; ++t) x4[t] = ldcol(sE + 4 * g * SA + 16 * t + li, SA);
+            mul16_tiles<NB>(x4, A, G);
         }
-        dR = mul16(ld4(sMrb + li * kST + 4 * g), B, dR);
-        dR = mul16(ld4(sMrk + li * kST + 4 * g), K, dR);
-        dB = mul16(ldcol(sMrb + 4 * g * kST + li, kST), R, dB);
-        dK = mul16(ldcol(sMrk + 4 * g * kST + li, kST), R, dK);
+        mul16(ld4(sMrb + li * kST + 4 * g), B, dR, ldcol(sMrb + 4 * g * kST + li, kST), R, dB);
+        mul16(ld4(sMrk + li * kST + 4 * g), K, dR, ldcol(sMrk + 4 * g * kST + li, kST), R, dK);
+        floatx4 dA1 = zero;
+#pragma unroll
+        for (int t = 0; t < NB; ++t) {
+            const floatx4 e4 = ld4(sE + li * SA + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                dA = mfma(e4[r], S0[t][r], dA);
+                dA1 = mfma(e4[r + 1], S0[t][r + 1], dA1);
+            }
+        }
         lds_barrier();
-        dA = mul16(ld4(sLab + li * kST + 4 * g), B, dA);
-        dA = mul16(ld4(sLak + li * kST + 4 * g), K, dA);
-        dB = mul16(ldcol(sLab + 4 * g * kST + li, kST), A, dB);
-        dK = mul16(ldcol(sLak + 4 * g * kST + li, kST), A, dK);
+        mul16(ld4(sLab + li * kST + 4 * g), B, dA, ldcol(sLab + 4 * g * kST + li, kST), A, dB);
+        mul16(ld4(sLak + li * kST + 4 * g), K, dA1, ldcol(sLak + 4 * g * kST + li, kST), A, dK);
+        dA += dA1;
         tile.store(p.dr, dR * d.now);
         tile.store(p.da, dA * d.before);
         tile.store(p.db, dB * d.inv);
@@ -672,7 +749,7 @@ int segments_of(int B, int T, int H, int N) {
 }
 
 struct Scratch {
-    size_t frags, states, u, starts, ends, powers, bytes;
+    size_t frags, states, u, starts, ends, powers, powers_t, bytes;
     int segments, seg_chunks;
 };
 
@@ -696,6 +773,7 @@ Scratch scratch_of(int B, int T, int H, int N) {
     o.starts = take(per_seg);
     o.ends = take(per_seg);
     o.powers = take(per_seg);
+    o.powers_t = take(per_seg);
     o.bytes = at + 256;  // some buffer for T = 0 too
     return o;
 }
@@ -710,8 +788,8 @@ template <int NB> void launch(const GradParams &p, hipStream_t s) {
         hipLaunchKernelGGL((wkv7_grad_local_kernel<NB>), dim3(per_xcd(locals) * kXcds), dim3(NB * kWave), 0, s, p, locals, per_xcd(locals));
     }
     if (p.segments > 2) {
-        const int waves = heads * 2 * NB;
-        hipLaunchKernelGGL((wkv7_grad_carry_kernel<NB>), dim3(per_xcd(waves) * kXcds), dim3(kWave), 0, s, p, waves, per_xcd(waves));
+        const int carries = heads * 2 * NB;
+        hipLaunchKernelGGL((wkv7_grad_carry_kernel<NB>), dim3(per_xcd(carries) * kXcds), dim3(NB * kWave), 0, s, p, carries, per_xcd(carries));
     }
     hipLaunchKernelGGL((wkv7_grad_kernel<NB>), dim3(per_xcd(segs) * kXcds), dim3(NB * kWave), 0, s, p, segs, per_xcd(segs));
 }
@@ -753,6 +831,7 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     p.starts = reinterpret_cast<float *>(base + o.starts);
     p.ends = reinterpret_cast<float *>(base + o.ends);
     p.powers = reinterpret_cast<float *>(base + o.powers);
+    p.powers_t = reinterpret_cast<float *>(base + o.powers_t);
     p.segments = o.segments;
     p.seg_chunks = o.seg_chunks;
     hipStream_t s = static_cast<hipStream_t>(stream);
