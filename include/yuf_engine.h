@@ -201,9 +201,8 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
  *   r, w_raw, k, v, a, b, state_in : the forward call's inputs.
  *   dy          : device [B, T, H, N], gradient of y.
  *   dstate_out  : device [B, H, N, N], gradient of the final state, or NULL.
- *   dr .. db    : device [B, T, H, N] outputs (none may alias an input).
- *   dstate_in   : device [B, H, N, N], gradient of the initial state, or NULL;
- *                 may alias dstate_out.
+ *   dr .. db    : device [B, T, H, N] outputs (no output may alias an input).
+ *   dstate_in   : device [B, H, N, N], gradient of the initial state, or NULL.
  *   workspace   : yuf_wkv7_scan_backward_workspace(B, T, H, N) bytes.
  * With G_t the gradient of S_t:  G_t += dy_t r_t^T;  dr = S_t^T dy, dv = G k,
  * dk = G^T v, da = S_{t-1}^T (G b), db = G^T (S_{t-1} a),
@@ -230,7 +229,7 @@ int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,
  *   ddecay, ddirection: device [D]: of lambda (post-sigmoid) and of u as it
  *                       stands in H(x) = x - 2 (x.u) u (not renormalised);
  *                       zero for B = 0.
- *   dmemory_in        : device [B, D] or NULL; may alias dmemory.
+ *   dmemory_in        : device [B, D] or NULL.  No output may alias an input.
  *   workspace         : yuf_rosa_scan_backward_workspace(B, T, D) bytes.
  * Supported D: 1 .. 1024.
  */

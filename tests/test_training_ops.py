@@ -19,12 +19,14 @@ def refused(status, *words):
 
 def test_wkv7_backward_refusals():
     call = lib().yuf_wkv7_scan_backward_f32
-    full = [DUMMY] * 17 + [None]
+    full = [DUMMY] * 9 + [2 * DUMMY] * 8 + [None]  # inputs, then outputs and workspace: none aliases
     refused(call(1, 1, 1, 12, *full), "head size")
     refused(call(-1, 1, 1, 40, *full), "negative")
     refused(call(1, 1, 1, 40, *[None] * 18), "null")
     refused(call(1, 0, 1, 40, *[None] * 18), "workspace")
-    refused(call(1, 1, 1, 40, *[DUMMY] * 16, None, None), "workspace")
+    refused(call(1, 1, 1, 40, *full[:16], None, None), "workspace")
+    aliased = full[:15] + [full[8]] + full[16:]
+    refused(call(1, 1, 1, 40, *aliased), "dstate_in")
     refused(call(1, 1, 1 << 20, 40, *full), "H * N")
     refused(call(1 << 14, 1 << 12, 1 << 10, 40, *full), "chunks")
     for missing in (0, 1, 2, 3, 4, 5, 7, 9, 10, 11, 12, 13, 14):
@@ -39,7 +41,7 @@ def test_wkv7_backward_refusals():
 
 def test_rosa_backward_refusals():
     call = lib().yuf_rosa_scan_backward_f32
-    full = [DUMMY] * 15 + [None]
+    full = [DUMMY] * 8 + [2 * DUMMY] * 7 + [None]
     refused(call(1, 1, 2048, *full), "D must be")
     refused(call(1, 1, 0, *full), "D must be")
     refused(call(1, -1, 64, *full), "negative")
@@ -50,8 +52,9 @@ def test_rosa_backward_refusals():
     args = list(full)
     args[10] = None  # dread_raw without its read_raw's gradient
     refused(call(1, 1, 64, *args), "read_raw")
-    refused(call(1, 1, 64, *[DUMMY] * 14, None, None), "workspace")
-    refused(call(1 << 20, 1 << 20, 64, *full), "segments")
+    refused(call(1, 1, 64, *full[:14], None, None), "workspace")
+    refused(call(1, 1, 64, *full[:13], full[7], *full[14:]), "dmemory_in")
+    refused(call(1 << 20, 1 << 20, 64, *full), "blocks")
     space = lib().yuf_rosa_scan_backward_workspace
     assert space(1, 16, 1025) == space(0, 16, 64) == space(1, -1, 64) == 0 and space(1, 0, 64) > 0
 

@@ -814,6 +814,7 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     if (B == 0 || H == 0) return YUF_OK;
     if (T > 0 && (!r || !w_raw || !k || !v || !a || !b || !dy || !dr || !dw_raw || !dk || !dv || !da || !db))
         return fail(YUF_ERR_INVALID, "wkv7 backward: null input/output pointer");
+    if (dstate_in && dstate_in == dstate_out) return fail(YUF_ERR_INVALID, "wkv7 backward: dstate_in may not be dstate_out");
     if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
     // Offsets inside a chunk of one head are 32-bit, workgroups are counted in int.
     if ((int64_t)H * N > (1 << 24)) return fail(YUF_ERR_INVALID, "wkv7 backward: H * N above 2^24");
