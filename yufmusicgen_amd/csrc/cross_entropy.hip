@@ -20,6 +20,7 @@ namespace {
 constexpr int kWave = 64;
 constexpr int kRowsPerWg = 4;    // rows of a workgroup where a row is one wave
 constexpr int kMaxWaves = 16;
+constexpr int kBatch = 8;        // loads of a lane in flight where rows are counted and summed
 constexpr int kCountInline = 4096;  // up to so many rows each workgroup counts the valid targets itself
 
 // Vectors with the alignment of their elements: a row of an odd vocabulary starts anywhere.
@@ -81,10 +82,23 @@ __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 
 // all of them is `all` (its sum is 0 and has to stay so where it saw no finite logit).
 __device__ __forceinline__ float rescale(float m, float all) { return m == -INFINITY ? 0.0f : expf(m - all); }
 
+template <typename I> __device__ __forceinline__ int count_mine(const I *targets, int M, int64_t ignore) {
+    int mine = 0;
+    // kBatch loads in flight: one at a time, each waits for memory (16384 rows: 10.5 us, so 5).
+    for (int i0 = threadIdx.x; i0 < M; i0 += kBatch * blockDim.x) {
+        I t[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) t[e] = targets[min(i0 + e * (int)blockDim.x, M - 1)];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) mine += i0 + e * (int)blockDim.x < M && (int64_t)t[e] != ignore;
+    }
+    return mine;
+}
+
 // Rows whose target counts, seen by every lane of the workgroup (all its threads call this).
 __device__ __forceinline__ float count_valid(const LossParams &p, int *partial) {
-    int mine = 0;
-    for (int i = threadIdx.x; i < p.M; i += blockDim.x) mine += target_of(p.targets, p.wide, i) != p.ignore;
+    int mine = p.wide ? count_mine(static_cast<const int64_t *>(p.targets), p.M, p.ignore)
+                      : count_mine(static_cast<const int32_t *>(p.targets), p.M, p.ignore);
 #pragma unroll
     for (int s = 1; s < kWave; s <<= 1) mine += __shfl_xor(mine, s);
     if ((threadIdx.x & 63) == 0) partial[threadIdx.x >> 6] = mine;
@@ -245,7 +259,13 @@ __global__ void __launch_bounds__(kReduceThreads) loss_sum_kernel(LossParams p, 
     __shared__ double sums[kReduceThreads / kWave];
     __shared__ int partial[kReduceThreads / kWave];
     double s = 0.0;
-    for (int i = threadIdx.x; i < p.M; i += kReduceThreads) s += (double)p.row_loss[i];
+    for (int i0 = threadIdx.x; i0 < p.M; i0 += kBatch * kReduceThreads) {
+        float v[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) v[e] = p.row_loss[min(i0 + e * kReduceThreads, p.M - 1)];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) s += i0 + e * kReduceThreads < p.M ? (double)v[e] : 0.0;
+    }
     s = wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     float n = 1.0f;

@@ -256,7 +256,12 @@ template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel
 #pragma unroll
         for (int t = 0; t < kC; ++t) x[t] = li == t ? 1.0f : 0.0f;
 #pragma unroll
-        for (int s = 0; s < kC - 1; ++s)
+        for (int s = 0; s < kC - 1; ++s) {
+            // Two steps' columns at a time: the compiler would load them all first and add them last, which
+            // takes 126 registers, so 70 and more waves at once.
+            if (s % 2 == 0)
+#pragma unroll
+                for (int t = 0; t < kC; ++t) asm volatile("" : "+v"(x[t])::"memory");
 #pragma unroll
             for (int m = s / 4; m < 4; ++m) {
                 const floatx4 col = ld4(sL + s * kST + 4 * m);
@@ -264,6 +269,7 @@ template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel
                 for (int e = 0; e < 4; ++e)
                     if (4 * m + e > s) x[4 * m + e] = fmaf(col[e], x[s], x[4 * m + e]);
             }
+        }
         // T^T, row s = li: each lane group writes its four tokens.
         const floatx4 own = g == 0 ? floatx4{x[0], x[1], x[2], x[3]}
                           : g == 1 ? floatx4{x[4], x[5], x[6], x[7]}
@@ -289,6 +295,9 @@ template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel
     st4(out + kMrkCol * kFrag, rk);
 }
 
+// The wave's number, known to be the same for its lanes: descriptors and branches made from it stay scalar.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // What a wave of the segment kernels is: its head, segment, tile and place in it.
 struct Place {
     int head, bb, h, q, g, li, lane, col;
@@ -297,7 +306,7 @@ struct Place {
         head = head_;
         bb = head / p.H;
         h = head - bb * p.H;
-        q = threadIdx.x >> 6;
+        q = wave_id();
         lane = threadIdx.x & 63;
         g = lane >> 4;
         li = lane & 15;

@@ -34,6 +34,25 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+class _on:
+    """The device's raw current stream, with the device made current if another is."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -147,8 +166,11 @@ def rwkv7_scan_backward(r, w, k, v, a, b, dy, state=None, dstate=None):
     batch, steps, heads, size = r.shape
     if size not in SUPPORTED_HEAD_SIZES:
         raise ValueError(f"head size {size} not supported (supported: {SUPPORTED_HEAD_SIZES})")
-    for name, x in zip(("r", "w", "k", "v", "a", "b", "dy"), tensors):
-        _check_like(name, x, r.shape, r.device)
+    shape, device = r.shape, r.device
+    for x in tensors:
+        if x.shape != shape or x.device != device or x.dtype != torch.float32 or not device.type == "cuda":
+            for name, t in zip(("r", "w", "k", "v", "a", "b", "dy"), tensors):
+                _check_like(name, t, shape, device)
         if not x.is_contiguous():
             raise ValueError("RWKV-7 inputs must be contiguous")
     for name, x in (("state", state), ("dstate", dstate)):
@@ -156,13 +178,13 @@ def rwkv7_scan_backward(r, w, k, v, a, b, dy, state=None, dstate=None):
             _check_like(name, x, (batch, heads, size, size), r.device)
     state = None if state is None else state.contiguous()
     dstate = None if dstate is None else dstate.contiguous()
-    with torch.cuda.device(r.device):
+    with _on(r.device) as stream:
         grads = [torch.empty_like(r) for _ in range(6)]
         dstate_in = torch.empty(batch, heads, size, size, device=r.device, dtype=torch.float32)
         space = _scratch(lib().yuf_wkv7_scan_backward_workspace(batch, steps, heads, size), r.device)
         check(lib().yuf_wkv7_scan_backward_f32(
             batch, steps, heads, size, *(x.data_ptr() for x in tensors[:6]), _ptr(state), dy.data_ptr(), _ptr(dstate),
-            *(x.data_ptr() for x in grads), dstate_in.data_ptr(), space.data_ptr(), _stream()))
+            *(x.data_ptr() for x in grads), dstate_in.data_ptr(), space.data_ptr(), stream))
     return (*grads, dstate_in)
 
 
@@ -207,7 +229,7 @@ def rosa_householder_scan_backward(cand, write, read_raw, decay, direction, memo
         dmemory = dmemory.float().contiguous()
         _check_like("dmemory", dmemory, (batch, dim), cand.device)
     cand, write, read_raw, decay, direction, memory, dread = tensors
-    with torch.cuda.device(cand.device):
+    with _on(cand.device) as stream:
         dcand, dwrite, dmemory_in = torch.empty_like(cand), torch.empty_like(cand), torch.empty_like(memory)
         dread_raw = torch.empty_like(cand) if gated else None
         ddecay, ddirection = torch.empty_like(decay), torch.empty_like(decay)
@@ -216,7 +238,7 @@ def rosa_householder_scan_backward(cand, write, read_raw, decay, direction, memo
             batch, steps, dim, cand.data_ptr(), write.data_ptr(), read_raw.data_ptr() if gated else None,
             decay.data_ptr(), direction.data_ptr(), memory.data_ptr(), dread.data_ptr(), _ptr(dmemory),
             dcand.data_ptr(), dwrite.data_ptr(), _ptr(dread_raw), ddecay.data_ptr(), ddirection.data_ptr(),
-            dmemory_in.data_ptr(), space.data_ptr(), _stream()))
+            dmemory_in.data_ptr(), space.data_ptr(), stream))
     return dcand, dwrite, dread_raw, ddecay, ddirection, dmemory_in
 
 
@@ -239,7 +261,7 @@ class _RosaScan(torch.autograd.Function):
 
 
 # -------------------------------------------------------------------- dropout
-_FLOATS = {torch.float32: "f32", torch.bfloat16: "bf16"}
+_FLOATS = (torch.float32, torch.bfloat16)
 
 
 def dropout(x, p: float, seed: int, counter=0, residual=None):
@@ -273,11 +295,11 @@ def dropout(x, p: float, seed: int, counter=0, residual=None):
 def _dropout_forward(x, residual, p, seed, counter, counter_dev):
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
-    with torch.cuda.device(x.device):
+    with _on(x.device) as stream:
         out = torch.empty_like(x)
-        entry = getattr(lib(), f"yuf_dropout_{_FLOATS[x.dtype]}")
+        entry = lib().yuf_dropout_f32 if x.dtype == torch.float32 else lib().yuf_dropout_bf16
         check(entry(x.numel(), x.data_ptr(), _ptr(residual), float(p), int(seed) & _U64, int(counter) & _U64,
-                    _ptr(counter_dev), out.data_ptr(), _stream()))
+                    _ptr(counter_dev), out.data_ptr(), stream))
     return out
 
 
@@ -320,16 +342,18 @@ def _loss_rows(logits, targets, reduction):
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if logits.shape[-1] == 0:
         raise ValueError("logits must have at least one column")
-    rows = logits.reshape(targets.numel(), logits.shape[-1])
+    if logits.ndim > 2:
+        logits, targets = logits.reshape(targets.numel(), logits.shape[-1]), targets.reshape(-1)
+    rows = logits
     if rows.stride(-1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()
-    return rows, targets.reshape(-1).contiguous()
+    return rows, targets.contiguous()
 
 
 def _loss_call(rows, targets, ignore_index, reduction, dloss, dlogits, want_loss: bool):
     """Loss of the rows (or None), and their gradient into ``dlogits`` where it is given."""
     count, vocab = rows.shape
-    with torch.cuda.device(rows.device):
+    with _on(rows.device) as stream:
         loss = space = None
         if want_loss:
             loss = torch.empty((count,) if reduction == "none" else (), device=rows.device, dtype=torch.float32)
@@ -337,12 +361,12 @@ def _loss_call(rows, targets, ignore_index, reduction, dloss, dlogits, want_loss
             space = _scratch(lib().yuf_cross_entropy_workspace(count), rows.device)
         if count == 0 and reduction == "none":
             return loss
-        entry = getattr(lib(), f"yuf_cross_entropy_{_FLOATS[rows.dtype]}")
+        entry = lib().yuf_cross_entropy_f32 if rows.dtype == torch.float32 else lib().yuf_cross_entropy_bf16
         stride = max(rows.stride(0), vocab)  # the stride of a single row says nothing
         stride_out = 0 if dlogits is None else max(dlogits.stride(0), vocab)
         check(entry(count, vocab, rows.data_ptr(), stride, targets.data_ptr(), 8 * targets.element_size(),
                     int(ignore_index), _REDUCTIONS[reduction], _ptr(loss), _ptr(dloss), _ptr(dlogits), stride_out,
-                    _ptr(space), _stream()))
+                    _ptr(space), stream))
     return loss
 
 
