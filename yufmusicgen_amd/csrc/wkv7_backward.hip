@@ -44,6 +44,8 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <algorithm>
+
 namespace yuf {
 namespace {
 
@@ -746,15 +748,27 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(
     if (p.dstate_in && seg == 0) io.store_columns(G, p.dstate_in + (size_t)head * N * N);
 }
 
-// Segments so that the last kernel's workgroups fill the GPU (about as many as it holds at
-// once), of at least four chunks each.
-int segments_of(int B, int T, int H, int N) {
+// Chunks of a segment.  The last kernel takes as long as its fullest CU, w = ceil(heads segments / 256)
+// workgroups of c chunks, a third longer alone on it (5.6 us a chunk at N = 40, 7.4 alone); the local pass
+// adds 0.45 of that (a quarter of it for two segments, which have no Pi), the carry 4 us and 0.35 a segment.
+// Measured so: 8 x 2048 x 16 x 40, 2 / 4 / 8 / 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x
+// 16 x 64, 8 / 10 / 13: 160 / 143 / 169; 1 x 2048 x 16 x 64, 8 / 16 / 32: 190 / 143 / 136.
+int segment_chunks(int B, int T, int H, int N) {
     const int64_t heads = (int64_t)B * H;
-    const int chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
-    const int resident = 256 * (NB <= 3 ? 4 : NB == 4 ? 3 : 1);
-    const int64_t want = (resident + heads - 1) / heads;
-    const int most = chunks / 4 > 1 ? chunks / 4 : 1;
-    return (int)(want < most ? want : most);
+    const int chunks = (T + kC - 1) / kC;
+    int best = std::max(chunks, 1);
+    double least = 1e30;
+    for (int64_t want = 1; want <= std::max<int64_t>(1, 1024 / heads) && (want == 1 || want * 4 <= chunks); ++want) {
+        const int c = std::max<int>(1, (int)((chunks + want - 1) / want)), S = std::max(1, (chunks + c - 1) / c);
+        const int64_t w = (heads * S + 255) / 256;
+        const double last = (double)w * c * (w == 1 && N <= 64 ? 1.3 : 1.0);
+        const double cost = last * (S == 1 ? 1.0 : S == 2 ? 1.25 : 1.0 + 0.45 * (S - 1) / S) + (S > 2 ? 0.7 + 0.06 * S : 0.0);
+        if (cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    return best;
 }
 
 struct Scratch {
@@ -766,8 +780,7 @@ Scratch scratch_of(int B, int T, int H, int N) {
     const size_t heads = (size_t)B * H, chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Scratch o{};
-    const int most = segments_of(B, T, H, N);
-    o.seg_chunks = (int)(chunks + most - 1) / most;
+    o.seg_chunks = segment_chunks(B, T, H, N);
     o.segments = chunks ? (int)(chunks + o.seg_chunks - 1) / o.seg_chunks : 1;
     size_t at = 0;
     auto take = [&](size_t floats) {
