@@ -668,3 +668,78 @@ def test_operators_captured_and_replayed():
         torch.cuda.synchronize()
         for i, (g, e) in enumerate(zip(out, expect)):
             assert torch.equal(g, e), (step, i)
+
+
+def test_a_captured_backward_pass_is_refused():
+    """backward() under capture raises (and the process lives), also beside an eager graph of the
+    same leaves; a captured forward pass of leaves that want gradients works as without them."""
+    from yufmusicgen_amd import ops
+
+    leaves = [cuda(x).requires_grad_() for x in wkv_inputs(3, 1, 40, 2, 16)]
+    eager, _ = ops.rwkv7_scan(*leaves)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.rwkv7_scan(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    for take in (lambda y: y.sum().backward(), lambda y: torch.autograd.grad(y.sum(), leaves)):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                take(ops.rwkv7_scan(*leaves)[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = ops.rwkv7_scan(*leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, eager)
+    torch.autograd.grad(eager.sum(), leaves)
+
+
+# ------------------------------------------------------------------ a sequence in pieces
+@pytest.mark.parametrize("steps,dim", [(3000, 128), (40000, 8), (1500, 300)])
+def test_rosa_gradients_of_a_sequence_in_two_pieces(steps, dim):
+    """The whole sequence's gradients are those of its pieces, joined by the memory and its
+    gradient: other cuts into blocks and ranges, the same sums."""
+    from yufmusicgen_amd.ops import rosa_householder_scan, rosa_householder_scan_backward
+
+    arrs, dread, dmem = rosa_case(5, 1, steps, dim)
+    cand, write, rr, decay, u, memory = (cuda(x) for x in arrs)
+    dread, dmem, cut = cuda(dread), cuda(dmem), steps * 5 // 8 + 3
+    whole = rosa_householder_scan_backward(cand, write, rr, decay, u, memory, dread, dmem, gated=True)
+    head, tail = slice(None, cut), slice(cut, None)
+    _, middle = rosa_householder_scan(cand[:, head], write[:, head], rr[:, head], decay, u, memory, gated=True)
+    late = rosa_householder_scan_backward(cand[:, tail], write[:, tail], rr[:, tail], decay, u, middle, dread[:, tail], dmem, gated=True)
+    early = rosa_householder_scan_backward(cand[:, head], write[:, head], rr[:, head], decay, u, memory, dread[:, head], late[5], gated=True)
+    for i, name in enumerate(ROSA_NAMES):
+        joined = torch.cat([early[i], late[i]], 1) if i < 3 else early[i].double() + late[i].double() if i < 5 else early[i]
+        close(whole[i], joined, 2 * (dim + 32), name)  # the errors of both
+
+
+@pytest.mark.parametrize("steps,size", [(2000, 40), (700, 64), (500, 128)])
+def test_wkv7_gradients_of_a_sequence_in_two_pieces(steps, size):
+    from yufmusicgen_amd.ops import rwkv7_scan, rwkv7_scan_backward
+
+    arrs, s0, dy, ds = wkv_case(9, 1, steps, 2, size)
+    x, state, dy, ds, cut = [cuda(a) for a in arrs], cuda(s0), cuda(dy), cuda(ds), steps * 5 // 8 + 3
+    whole = rwkv7_scan_backward(*x, dy, state=state, dstate=ds)
+    head, tail = [a[:, :cut].contiguous() for a in (*x, dy)], [a[:, cut:].contiguous() for a in (*x, dy)]
+    _, middle = rwkv7_scan(*head[:6], state=state)
+    late = rwkv7_scan_backward(*tail, state=middle, dstate=ds)
+    early = rwkv7_scan_backward(*head, state=state, dstate=late[6])
+    for i, name in enumerate(WKV_NAMES):
+        close(whole[i], torch.cat([early[i], late[i]], 1) if i < 6 else early[i], 2 * (size + 32), name)
+
+
+def test_cross_entropy_of_more_rows_than_a_launch_takes():
+    """2^21 rows are one launch; the rows behind them get theirs too."""
+    from yufmusicgen_amd.ops import cross_entropy_grad
+
+    rows = (1 << 21) + 5
+    x, t = torch.randn(rows, 3, device="cuda"), torch.randint(0, 3, (rows,), device="cuda")
+    loss, grad = cross_entropy_grad(x, t, reduction="none")
+    logp = torch.log_softmax(x.double(), -1)
+    expect = -logp.gather(-1, t[:, None])[:, 0]
+    assert (loss.double() - expect).abs().max() <= 60 * EPS32 * (1 + expect.abs().max())
+    one = torch.zeros_like(logp).scatter_(-1, t[:, None], 1.0)
+    assert (grad.double() - (logp.exp() - one)).abs().max() <= 60 * EPS32

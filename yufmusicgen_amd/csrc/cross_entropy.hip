@@ -45,6 +45,7 @@ template <> struct MinusInf<uint16_t> { static __device__ uint16_t get() { retur
 
 struct LossParams {
     int M, V;
+    int row0;  // first row of this launch
     const void *logits;
     int64_t ld;
     const void *targets;
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? kRowsPerWg * kWave : WAVES * kWav
     float count = 1.0f;
     if (p.reduction == YUF_LOSS_MEAN && p.dlogits)
         count = p.count ? *p.count : count_valid(p, counts);
-    const int row = WAVES == 1 ? (int)blockIdx.x * kRowsPerWg + (threadIdx.x >> 6) : (int)blockIdx.x;
+    const int row = p.row0 + (WAVES == 1 ? (int)blockIdx.x * kRowsPerWg + (int)(threadIdx.x >> 6) : (int)blockIdx.x);
     const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     if (row >= p.M) return;  // whole waves of a one-wave form, which has no barrier below
     const int64_t target = target_of(p.targets, p.wide, row);
@@ -279,10 +280,14 @@ __global__ void __launch_bounds__(kReduceThreads) loss_sum_kernel(LossParams p, 
 }
 
 template <typename T, int WAVES, int NV>
-void launch_form(const LossParams &p, hipStream_t s) {
-    const int per_wg = WAVES == 1 ? kRowsPerWg : 1;
-    hipLaunchKernelGGL((loss_kernel<T, WAVES, NV>), dim3((p.M + per_wg - 1) / per_wg), dim3((WAVES == 1 ? kRowsPerWg : WAVES) * kWave), 0,
-                       s, p);
+void launch_form(LossParams p, hipStream_t s) {
+    constexpr int kPerWg = WAVES == 1 ? kRowsPerWg : 1;
+    constexpr int kRows = 1 << 21;  // of a launch, which has at most 2^32 threads
+    for (; p.row0 < p.M; p.row0 += kRows) {
+        const int rows = std::min(p.M - p.row0, kRows);
+        hipLaunchKernelGGL((loss_kernel<T, WAVES, NV>), dim3((rows + kPerWg - 1) / kPerWg), dim3(kPerWg * WAVES * kWave), 0, s, p);
+        if (p.M - p.row0 <= kRows) break;
+    }
 }
 
 // The fewest waves whose registers hold the row.
@@ -313,6 +318,7 @@ int cross_entropy(int M, int V, const T *logits, int64_t ld, const void *targets
         return fail(YUF_ERR_INVALID, "cross entropy: reduction must be YUF_LOSS_NONE, _MEAN or _SUM");
     if (target_bits != 32 && target_bits != 64) return fail(YUF_ERR_INVALID, "cross entropy: target_bits must be 32 or 64");
     if (ld < V || (dlogits && ld_out < V)) return fail(YUF_ERR_INVALID, "cross entropy: row stride below V");
+    if (V > 1 << 30) return fail(YUF_ERR_INVALID, "cross entropy: V above 2^30");
     if (M > 0 && V == 0) return fail(YUF_ERR_INVALID, "cross entropy: rows without logits");
     if (M > 0 && (!logits || !targets)) return fail(YUF_ERR_INVALID, "cross entropy: null logits or targets");
     if (!loss && !dlogits) return fail(YUF_ERR_INVALID, "cross entropy: neither a loss nor a gradient asked for");

@@ -125,7 +125,7 @@ int dropout(int64_t n, const T *x, const T *residual, double p, uint64_t seed, u
     if (!x || !out) return fail(YUF_ERR_INVALID, "dropout: null input/output pointer");
     constexpr int64_t kPerBlock = (int64_t)kThreads * kUnits * Vec<T>::kN;
     const int64_t blocks = (n + kPerBlock - 1) / kPerBlock;
-    if (blocks > 0x7FFFFFFF) return fail(YUF_ERR_INVALID, "dropout: too many elements");
+    if (blocks * kThreads >= (int64_t)1 << 32) return fail(YUF_ERR_INVALID, "dropout: too many elements");  // threads of a launch
     DropoutParams<T> q{};
     q.n = n; q.x = x; q.residual = residual; q.out = out;
     q.seed = seed; q.counter = counter; q.counter_dev = counter_dev;

@@ -493,7 +493,7 @@ struct Cut {
 Cut cut_of(int T, int D) {
     const int tok = block_tokens(epl_of(D));
     Cut c{};
-    c.S = std::max(1, (T + tok - 1) / tok);
+    c.S = std::max(1, T / tok + (T % tok != 0));
     c.R = D > kMaxCarryDim ? c.S : c.S <= 128 ? 1 : c.S <= 1024 ? 8 : 32;
     c.NR = (c.S + c.R - 1) / c.R;
     return c;
@@ -563,7 +563,7 @@ extern "C" int yuf_rosa_scan_backward_f32(int B, int T, int D, const float *cand
     if (B > 0 && !workspace) return fail(YUF_ERR_INVALID, "rosa backward: null workspace");
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Cut cut = cut_of(T, D);
-    if ((int64_t)B * cut.S > (1 << 29)) return fail(YUF_ERR_INVALID, "rosa backward: too many blocks");
+    if ((int64_t)B * cut.S >= (1 << 22)) return fail(YUF_ERR_INVALID, "rosa backward: too many blocks");  // 2^32 threads a launch
     RosaGradParams p{};
     p.B = B; p.T = T; p.D = D; p.S = cut.S; p.R = cut.R; p.NR = cut.NR;
     p.cand = cand; p.write = write; p.read_raw = read_raw; p.decay = decay; p.direction = direction;

@@ -838,9 +838,10 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
         return fail(YUF_ERR_INVALID, "wkv7 backward: null input/output pointer");
     if (dstate_in && dstate_in == dstate_out) return fail(YUF_ERR_INVALID, "wkv7 backward: dstate_in may not be dstate_out");
     if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
-    // Offsets inside a chunk of one head are 32-bit, workgroups are counted in int.
+    // Offsets inside a chunk of one head are 32-bit.
     if ((int64_t)H * N > (1 << 24)) return fail(YUF_ERR_INVALID, "wkv7 backward: H * N above 2^24");
-    if ((int64_t)B * H * ((T + kC - 1) / kC) > (1 << 30)) return fail(YUF_ERR_INVALID, "wkv7 backward: too many chunks");
+    if ((int64_t)B * H * std::max(1, T / kC + (T % kC != 0)) > (1 << 25))  // a launch has at most 2^32 threads
+        return fail(YUF_ERR_INVALID, "wkv7 backward: too many chunks");
     GradParams p{};
     p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = (T + kC - 1) / kC;
     p.r = r; p.w = w_raw; p.k = k; p.v = v; p.a = a; p.b = b; p.dy = dy;

@@ -30,10 +30,6 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
-
-
 class _on:
     """The device's raw current stream, with the device made current if another is."""
 
@@ -110,8 +106,9 @@ def _rwkv7_forward(r, w, k, v, a, b, state):
     batch, steps, heads, size = r.shape
     y = torch.empty_like(r)
     final = torch.empty(batch, heads, size, size, device=r.device, dtype=torch.float32)
-    check(lib().yuf_wkv7_scan_f32(batch, steps, heads, size, *(x.data_ptr() for x in (r, w, k, v, a, b)),
-                                  _ptr(state), final.data_ptr(), y.data_ptr(), _stream()))
+    with _on(r.device) as stream:
+        check(lib().yuf_wkv7_scan_f32(batch, steps, heads, size, *(x.data_ptr() for x in (r, w, k, v, a, b)),
+                                      _ptr(state), final.data_ptr(), y.data_ptr(), stream))
     return y, final
 
 
@@ -143,10 +140,11 @@ def _rosa_forward(cand, write, read_raw, decay, direction, memory, gated):
     batch, steps, dim = cand.shape
     read = torch.empty_like(cand)
     final = torch.empty(batch, dim, device=cand.device, dtype=torch.float32)
-    check(lib().yuf_rosa_scan_f32(batch, steps, dim, cand.data_ptr(), write.data_ptr(),
-                                  read_raw.data_ptr() if gated else None, decay.data_ptr(),
-                                  direction.data_ptr(), memory.data_ptr(), final.data_ptr(),
-                                  read.data_ptr(), _stream()))
+    with _on(cand.device) as stream:
+        check(lib().yuf_rosa_scan_f32(batch, steps, dim, cand.data_ptr(), write.data_ptr(),
+                                      read_raw.data_ptr() if gated else None, decay.data_ptr(),
+                                      direction.data_ptr(), memory.data_ptr(), final.data_ptr(),
+                                      read.data_ptr(), stream))
     return read, final
 
 
