@@ -564,39 +564,48 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_carry_k
     // Forward: slot 1 is final, slot s + 1 += slot s Pi_s; backward: slot segments - 2 is, slot
     // s - 1 += slot s Pi_s^T.  x^T[j][i] = sum_k Pi^T[j][k] x^T[k][i] (Pi[j][k] backward).
     const int first = back ? p.segments - 2 : 1;
+    const float *powers = seg_state(back ? p.powers : p.powers_t, p, head, 0);
+    slots = seg_state(slots, p, head, 0);
     floatx4 pi[kAhead][NB], local[kAhead];
     auto fetch = [&](int n, floatx4 (&m)[NB], floatx4 &l) {
         const int s = first + min(n, steps - 1) * dir;  // past the last step: its values again, unused
-        const auto rs = make_rsrc(seg_state(back ? p.powers : p.powers_t, p, head, s), bytes);
+        const auto rs = make_rsrc(powers + (size_t)s * N * N, bytes);
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) m[kb] = buf_load4(rs, at[kb]);
-        l = buf_load4(make_rsrc(seg_state(slots, p, head, s + dir), bytes), own);
+        l = buf_load4(make_rsrc(slots + (size_t)(s + dir) * N * N, bytes), own);
     };
-    floatx4 x = buf_load4(make_rsrc(seg_state(slots, p, head, first), bytes), own);
+    floatx4 x = buf_load4(make_rsrc(slots + (size_t)first * N * N, bytes), own);
+    // The waits for loads count exactly where the loop has no branch (steps past the last one store nothing)
+    // and the loads before it are issued in its order (the scheduling barriers).
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) fetch(n, pi[n], local[n]);
-    auto step = [&](int n, floatx4 (&m)[NB], floatx4 &l) {
-        st4(&tiles[n & 1][w.q][4 * w.lane], x);
-        lds_barrier();
-        floatx4 y0 = l, y1 = {0.f, 0.f, 0.f, 0.f};  // even and odd k-steps
+    for (int n = 0; n < kAhead; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(n, pi[n], local[n]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    for (int n0 = 0; n0 < steps; n0 += kAhead) {
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-            const floatx4 k4 = ld4(&tiles[n & 1][kb][4 * w.lane]);
+        for (int e = 0; e < kAhead; ++e) {
+            const int n = n0 + e;
+            float *tile = &tiles[n & 1][0][4 * w.lane];
+            st4(tile + w.q * kFrag, x);
+            lds_barrier();
+            floatx4 y0 = local[e], y1 = {0.f, 0.f, 0.f, 0.f};  // even and odd k-steps
 #pragma unroll
-            for (int r = 0; r < 4; r += 2) {
-                y0 = mfma(m[kb][r], k4[r], y0);
-                y1 = mfma(m[kb][r + 1], k4[r + 1], y1);
+            for (int kb = 0; kb < NB; ++kb) {
+                const floatx4 k4 = ld4(tile + kb * kFrag);
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    y0 = mfma(pi[e][kb][r], k4[r], y0);
+                    y1 = mfma(pi[e][kb][r + 1], k4[r + 1], y1);
+                }
             }
+            x = y0 + y1;
+            // Loads of a slot that a step writes were issued before its store: each slot is read once, ahead.
+            fetch(n + kAhead, pi[e], local[e]);
+            const int to = first + (min(n, steps - 1) + 1) * dir;
+            buf_store4(x, make_rsrc(slots + (size_t)to * N * N, n < steps ? bytes : 0u), own);
         }
-        x = y0 + y1;
-        // Loads of a slot that this step writes were issued before its store: each slot is read once, ahead.
-        fetch(n + kAhead, m, l);
-        buf_store4(x, make_rsrc(seg_state(slots, p, head, first + (n + 1) * dir), bytes), own);
-    };
-    for (int n = 0; n < steps; n += kAhead) {
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e)
-            if (n + e < steps) step(n + e, pi[e], local[e]);
     }
 }
 

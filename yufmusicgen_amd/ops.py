@@ -174,6 +174,11 @@ def rwkv7_scan_backward(r, w, k, v, a, b, dy, state=None, dstate=None):
     for name, x in (("state", state), ("dstate", dstate)):
         if x is not None:
             _check_like(name, x, (batch, heads, size, size), r.device)
+    return _rwkv7_backward(*tensors, state, dstate)
+
+
+def _rwkv7_backward(r, w, k, v, a, b, dy, state, dstate):
+    batch, steps, heads, size = r.shape
     state = None if state is None else state.contiguous()
     dstate = None if dstate is None else dstate.contiguous()
     with _on(r.device) as stream:
@@ -181,7 +186,7 @@ def rwkv7_scan_backward(r, w, k, v, a, b, dy, state=None, dstate=None):
         dstate_in = torch.empty(batch, heads, size, size, device=r.device, dtype=torch.float32)
         space = _scratch(lib().yuf_wkv7_scan_backward_workspace(batch, steps, heads, size), r.device)
         check(lib().yuf_wkv7_scan_backward_f32(
-            batch, steps, heads, size, *(x.data_ptr() for x in tensors[:6]), _ptr(state), dy.data_ptr(), _ptr(dstate),
+            batch, steps, heads, size, *(x.data_ptr() for x in (r, w, k, v, a, b)), _ptr(state), dy.data_ptr(), _ptr(dstate),
             *(x.data_ptr() for x in grads), dstate_in.data_ptr(), space.data_ptr(), stream))
     return (*grads, dstate_in)
 
@@ -199,7 +204,7 @@ class _Rwkv7Scan(torch.autograd.Function):
         _not_captured("rwkv7_scan")
         *inputs, state = ctx.saved_tensors
         dy = torch.zeros_like(inputs[0]) if dy is None else dy.contiguous()
-        *grads, dstate_in = rwkv7_scan_backward(*inputs, dy, state, dstate)
+        *grads, dstate_in = _rwkv7_backward(*inputs, dy, state, dstate)
         grads.append(None if state is None else dstate_in)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad))
 
