@@ -408,7 +408,7 @@ __device__ __forceinline__ void sweep_forward(const GradParams &p, const Place &
         stcol(sK + at, SA, k * d.inv);
         if (w.g == 3) sD[w.col] = d.last;
         const floatx4 v4 = v;
-        if (c + 1 < w.c1) fetch(c + 1);
+        fetch(min(c + 1, w.c1 - 1));
         lds_barrier();
         floatx4 X = zero, Y = zero, U = zero, UP = zero;  // POWER: Y is X of P, else X's odd k-steps
 #pragma unroll
@@ -479,7 +479,7 @@ __device__ __forceinline__ void sweep_backward(const GradParams &p, const Place 
         stcol(sR + at, SA, r * d.now);
         if (w.g == 3) sD[w.col] = d.last;
         const floatx4 y4 = y;
-        if (c > w.c0) fetch(c - 1);
+        fetch(max(c - 1, w.c0));
         lds_barrier();
         floatx4 F = zero, F1 = zero;  // even and odd k-steps
         F1 = mul16(rb_col, y4, F1);
