@@ -609,8 +609,10 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_carry_k
     }
 }
 
-// A workgroup of NB waves per segment of a head.
-template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
+// A workgroup of NB waves per segment of a head.  Two waves per SIMD saturate it (the fp32 MFMAs, the VALU
+// and LDS instructions of a SIMD go one after the other: 60, 15 and 15 % of its time), and scheduled for two
+// instead of three the operands come from LDS in time: 8 x 2048 x 16 x 40 360 us, so 345.
+template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
     constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
     // Backward: B, K, V, Y', U, E, G [value][key] and the four 16 x 16 gradients.
     constexpr int kBackward = 6 * kTok + NP * SA + 4 * kC * kST;
