@@ -10,6 +10,8 @@
 // waves' registers are read twice.  Each wave takes its own maximum and sum, and
 // the waves of a row join them through LDS with one barrier.  Everything is summed
 // in fp32 inside a row and in fp64 over the rows, always in the same order.
+// 16384 x 20480 fp32 with the gradient: 575 us = 4.7 TB/s (a large copy: 4.8), and 10 us
+// to count the rows before and to sum their losses behind.
 #include "common.h"
 
 #include <algorithm>
@@ -85,7 +87,7 @@ __device__ __forceinline__ float rescale(float m, float all) { return m == -INFI
 
 template <typename I> __device__ __forceinline__ int count_mine(const I *targets, int M, int64_t ignore) {
     int mine = 0;
-    // kBatch loads in flight: one at a time, each waits for memory (16384 rows: 10.5 us, so 5).
+    // kBatch loads in flight: one at a time, each waits for memory (16384 rows: 10.5 us, so 6.2).
     for (int i0 = threadIdx.x; i0 < M; i0 += kBatch * blockDim.x) {
         I t[kBatch];
 #pragma unroll

@@ -8,9 +8,11 @@
 // (i / 4, counter) under a 64-bit key gives four 32-bit words, one per element,
 // and an element is dropped where its word is below p 2^32.
 //
-// Bound: HBM, 8 or 12 bytes an element in fp32 (half of it in bf16).  Philox costs
+// Bound: memory, 8 or 12 bytes an element in fp32 (half of it in bf16).  Philox costs
 // 20 32 x 32 -> 64-bit products per four elements.  A thread handles kUnits groups
-// of a 16-byte vector, all loads issued before the first product.
+// of a 16-byte vector, all loads issued before the first product.  16384 x 640 fp32
+// with the residual: 19.4 us = 6.5 TB/s, as long as an addition of the two tensors
+// (they fit the memory-side cache).
 #include "common.h"
 
 #include <cmath>

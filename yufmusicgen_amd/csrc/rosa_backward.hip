@@ -22,6 +22,9 @@
 //   5  those sums over the blocks, in fp64 and one order.
 // With R = 1 the carry's states are the blocks' and 3 is left out; with one range (D > 256, whose
 // power does not fit a workgroup's registers) 1 and 2 are, and a sequence of one block is 4 and 5.
+// 8 x 2048 x 128 with the gate (64 blocks a sequence): 13.0 + 22.6 + 22.2 + 4.1 us, 59 MB at 0.95 TB/s;
+// 3 x 777 x 256: 11.0 + 22.1 + 18.5 + 4.0.  Whole segments of 64 tokens by one wave, elementwise parts
+// included, took 39 + 12.6 + 93 + 6.4 us of the former.
 #include "common.h"
 #include "kernels.h"
 
@@ -247,9 +250,10 @@ __global__ void __launch_bounds__(block_waves(EPL) * kWave) rosa_grad_range_kern
 }
 
 // Phase 2.  DP = D padded to 64, 128 or 256.  Wave w holds columns 16 w + li of the power, lane
-// row q (16 lanes) the rows [q DP / 4, ..) of them.  A lane reads 16 x-values per 64 of DP and the
+// row q (16 lanes) the rows [q DP / 4, ..) of them.  A lane reads one x-value per 64 of DP and the
 // multiplications take them from their lanes by row broadcast, so that x costs LDS one word per lane and
-// not per product; the four lane rows add up by row swaps: one barrier a step.
+// not per product; the four lane rows add up by row swaps: one barrier a step, 0.33 us at D = 128 (0.44 with
+// every lane reading its 16 values from LDS).
 // acc += sum_r (x of lane r of the lane row) w[r], even and odd r apart.  The compiler splits a row
 // broadcast and its multiplication into two instructions; the s_nop covers a move of x just before.
 __device__ __forceinline__ void mac_rows(float x, const float (&w)[16], float (&acc)[2]) {
@@ -485,8 +489,9 @@ __global__ void __launch_bounds__(1024) rosa_grad_sum_kernel(const double *sums,
 
 int epl_of(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : D <= 512 ? 8 : 16; }
 
-// Blocks of a sequence and of a range.  A range costs the carry one step and its blocks cost the
-// local pass and the walk a block each, so R grows with the sequence; without a walk up to 128 blocks.
+// Blocks of a sequence and of a range.  A range costs the carry a step (0.33 us at D = 128) and its blocks
+// cost the local pass and the walk a block (about 3 us with its neighbours beside it) each, so R grows with
+// the sequence; without a walk up to 128 blocks.
 struct Cut {
     int S, R, NR;
 };

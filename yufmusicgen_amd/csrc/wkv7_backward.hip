@@ -35,6 +35,11 @@
 //                           then G and the gradients backward.
 // One segment needs the first and the last alone, two no carry.
 //
+// 8 x 2048 x 16 x 40 (four segments): 77 + 136 + 6 + 341 us; 3 x 777 x 16 x 64 (ten): 16 + 46 + 18 + 66;
+// 1 x 2048 x 16 x 64 (32): 17 + 39 + 22 + 55.  The first is bound by memory (300 MB at 3.9 TB/s), the second
+// and the last by their SIMDs' issue: an fp32 MFMA takes 32 cycles of one, a VALU instruction 4 and a 16-byte
+// LDS read about 18, none beside another, and a wave's chunk in the last kernel has 266 of the first at N = 64.
+//
 // MFMA layouts (16x16x4 f32; lane l, g = l / 16, li = l % 16): A[m = li][k = g],
 // B[k = g][n = li], register r of the result D[m = 4 g + r][n = li].  k-step r of a
 // product means rows {4 g + r}, so a result is the next product's B operand as it is,
