@@ -301,17 +301,22 @@ def test_rosa_autograd_is_the_operator():
 
 
 # ----------------------------------------------------------------------------- dropout
+def philox_block(block, counter, seed):
+    """Four words of Philox 4x32-10 with Python's integers."""
+    c = [block & 0xFFFFFFFF, block >> 32, counter & 0xFFFFFFFF, counter >> 32]
+    k = [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
 def philox_words(n, counter, seed):
-    """The first n words of Philox 4x32-10 with Python's integers, block by block."""
+    """The first n words, block by block."""
     words = []
     for block in range((n + 3) // 4):
-        c = [block & 0xFFFFFFFF, block >> 32, counter & 0xFFFFFFFF, counter >> 32]
-        k = [seed & 0xFFFFFFFF, seed >> 32]
-        for _ in range(10):
-            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
-            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
-            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
-        words += c
+        words += philox_block(block, counter, seed)
     return torch.tensor(words[:n], dtype=torch.int64)
 
 
@@ -743,3 +748,43 @@ def test_cross_entropy_of_more_rows_than_a_launch_takes():
     assert (loss.double() - expect).abs().max() <= 60 * EPS32 * (1 + expect.abs().max())
     one = torch.zeros_like(logp).scatter_(-1, t[:, None], 1.0)
     assert (grad.double() - (logp.exp() - one)).abs().max() <= 60 * EPS32
+
+
+def test_offsets_beyond_32_bits():
+    """Over 2^31 bf16 elements (4.5 GB, all in one buffer): the last rows' loss and gradient and the
+    last elements' dropout are those of the same rows alone."""
+    from yufmusicgen_amd._lib import check, lib
+    from yufmusicgen_amd.ops import cross_entropy_grad, dropout
+
+    rows, vocab = 110000, 20480
+    x = torch.zeros(rows, vocab, device="cuda", dtype=torch.bfloat16)
+    tail = torch.randn(7, vocab, device="cuda").bfloat16()
+    x[-7:] = tail
+    t = torch.arange(rows, device="cuda") % vocab
+    loss, grad = cross_entropy_grad(x, t, reduction="none", inplace=True)
+    alone = cross_entropy_grad(tail, t[-7:], reduction="none")
+    assert torch.equal(loss[-7:], alone[0]) and torch.equal(grad[-7:], alone[1])
+    assert (loss[:-7] - np.log(vocab)).abs().max() <= 60 * EPS32 * 10
+    x.fill_(1.0)
+    n, check_from = x.numel(), x.numel() - 4096
+    check(lib().yuf_dropout_bf16(n, x.data_ptr(), None, 0.5, 3, 0, None, x.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    words = []
+    for block in range(check_from // 4, n // 4):  # the mask goes by the element's 64-bit place
+        words += philox_block(block, 0, 3)
+    assert torch.equal(x.reshape(-1)[check_from:].cpu() != 0, torch.tensor(words) >= 2**31)
+    assert dropout(x[:1, :8], 0.5, 3).shape == (1, 8)
+
+
+def test_rosa_autograd_takes_the_scans_layouts():
+    """decay, direction and memory in other shapes of the same elements, as the forward call takes them."""
+    from yufmusicgen_amd.ops import rosa_householder_scan
+
+    arrs, dread, _ = rosa_case(3, 1, 70, 64)
+    x = [cuda(a) for a in arrs]
+    odd = [x[0], x[1], x[2], x[3].reshape(1, 64), x[4].reshape(64, 1), x[5].reshape(64)]
+    leaves = [z.clone().requires_grad_() for z in odd]
+    plain = [z.clone().requires_grad_() for z in x]
+    got = torch.autograd.grad(rosa_householder_scan(*leaves, gated=True)[0], leaves, cuda(dread))
+    expect = torch.autograd.grad(rosa_householder_scan(*plain, gated=True)[0], plain, cuda(dread))
+    for g, e, z in zip(got, expect, leaves):
+        assert g.shape == z.shape and torch.equal(g.reshape(-1), e.reshape(-1))

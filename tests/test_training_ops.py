@@ -25,8 +25,10 @@ def test_wkv7_backward_refusals():
     refused(call(1, 1, 1, 40, *[None] * 18), "null")
     refused(call(1, 0, 1, 40, *[None] * 18), "workspace")
     refused(call(1, 1, 1, 40, *full[:16], None, None), "workspace")
-    aliased = full[:15] + [full[8]] + full[16:]
-    refused(call(1, 1, 1, 40, *aliased), "dstate_in")
+    refused(call(1, 1, 1, 40, *full[:16], DUMMY + 64, None), "aligned")
+    apart = [256 * (i + 1) for i in range(17)] + [None]
+    for out, inp in ((9, 0), (14, 7), (15, 8), (10, 6), (13, 9)):  # an output as an input, and as another output
+        refused(call(1, 1, 1, 40, *apart[:out], apart[inp], *apart[out + 1 :]), "may not be")
     refused(call(1, 1, 1 << 20, 40, *full), "H * N")
     refused(call(1 << 14, 1 << 12, 1 << 10, 40, *full), "chunks")
     for missing in (0, 1, 2, 3, 4, 5, 7, 9, 10, 11, 12, 13, 14):
@@ -53,7 +55,10 @@ def test_rosa_backward_refusals():
     args[10] = None  # dread_raw without its read_raw's gradient
     refused(call(1, 1, 64, *args), "read_raw")
     refused(call(1, 1, 64, *full[:14], None, None), "workspace")
-    refused(call(1, 1, 64, *full[:13], full[7], *full[14:]), "dmemory_in")
+    refused(call(1, 1, 64, *full[:14], DUMMY + 64, None), "aligned")
+    apart = [256 * (i + 1) for i in range(15)] + [None]
+    for out, inp in ((8, 0), (9, 6), (10, 2), (11, 3), (13, 7), (12, 11)):
+        refused(call(1, 1, 64, *apart[:out], apart[inp], *apart[out + 1 :]), "may not be")
     refused(call(1 << 20, 1 << 20, 64, *full), "blocks")
     space = lib().yuf_rosa_scan_backward_workspace
     assert space(1, 16, 1025) == space(0, 16, 64) == space(1, -1, 64) == 0 and space(1, 0, 64) > 0

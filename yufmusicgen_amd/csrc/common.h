@@ -151,6 +151,20 @@ __device__ __forceinline__ void buf_store(float value, __amdgpu_buffer_rsrc_t rs
 // later loop (where it would also wait for prefetches issued in that loop).
 __device__ __forceinline__ void wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
+// Whether an output is an input or another output (the pointers themselves; null ones are none).
+template <int NI, int NO> inline bool outputs_alias(const void *const (&in)[NI], const void *const (&out)[NO]) {
+    for (int o = 0; o < NO; ++o) {
+        if (!out[o]) continue;
+        for (const void *i : in)
+            if (i == out[o]) return true;
+        for (int p = 0; p < o; ++p)
+            if (out[p] == out[o]) return true;
+    }
+    return false;
+}
+// Scratch that the kernels take apart in runs of 256 bytes.
+inline bool scratch_aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 256 == 0; }
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace yuf

@@ -564,11 +564,15 @@ extern "C" int yuf_rosa_scan_backward_f32(int B, int T, int D, const float *cand
         return fail(YUF_ERR_INVALID, "rosa backward: null input/output pointer");
     if ((read_raw != nullptr) != (dread_raw != nullptr) && T > 0)
         return fail(YUF_ERR_INVALID, "rosa backward: read_raw and its gradient go together");
-    if (dmemory_in && dmemory_in == dmemory) return fail(YUF_ERR_INVALID, "rosa backward: dmemory_in may not be dmemory");
     if (B > 0 && !workspace) return fail(YUF_ERR_INVALID, "rosa backward: null workspace");
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Cut cut = cut_of(T, D);
     if ((int64_t)B * cut.S >= (1 << 22)) return fail(YUF_ERR_INVALID, "rosa backward: too many blocks");  // 2^32 threads a launch
+    if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "rosa backward: workspace must be 256-byte aligned");
+    // The gradients of one block are written while another still reads the inputs.
+    if (B > 0 && outputs_alias<8, 6>({cand, write, read_raw, decay, direction, memory_in, dread, dmemory},
+                                     {dcand, dwrite, dread_raw, ddecay, ddirection, dmemory_in}))
+        return fail(YUF_ERR_INVALID, "rosa backward: an output may not be an input or another output");
     RosaGradParams p{};
     p.B = B; p.T = T; p.D = D; p.S = cut.S; p.R = cut.R; p.NR = cut.NR;
     p.cand = cand; p.write = write; p.read_raw = read_raw; p.decay = decay; p.direction = direction;

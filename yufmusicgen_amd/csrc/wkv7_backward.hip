@@ -852,12 +852,15 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     if (B == 0 || H == 0) return YUF_OK;
     if (T > 0 && (!r || !w_raw || !k || !v || !a || !b || !dy || !dr || !dw_raw || !dk || !dv || !da || !db))
         return fail(YUF_ERR_INVALID, "wkv7 backward: null input/output pointer");
-    if (dstate_in && dstate_in == dstate_out) return fail(YUF_ERR_INVALID, "wkv7 backward: dstate_in may not be dstate_out");
     if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
     // Offsets inside a chunk of one head are 32-bit.
     if ((int64_t)H * N > (1 << 24)) return fail(YUF_ERR_INVALID, "wkv7 backward: H * N above 2^24");
     if ((int64_t)B * H * std::max(1, T / kC + (T % kC != 0)) > (1 << 25))  // a launch has at most 2^32 threads
         return fail(YUF_ERR_INVALID, "wkv7 backward: too many chunks");
+    if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "wkv7 backward: workspace must be 256-byte aligned");
+    // The gradients of one segment are written while another still reads the inputs.
+    if (outputs_alias<9, 7>({r, w_raw, k, v, a, b, state_in, dy, dstate_out}, {dr, dw_raw, dk, dv, da, db, dstate_in}))
+        return fail(YUF_ERR_INVALID, "wkv7 backward: an output may not be an input or another output");
     GradParams p{};
     p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = (T + kC - 1) / kC;
     p.r = r; p.w = w_raw; p.k = k; p.v = v; p.a = a; p.b = b; p.dy = dy;

@@ -132,7 +132,10 @@ def rosa_householder_scan(cand, write, read_raw, decay, direction, memory, gated
     if not all(x.is_cuda for x in tensors):
         raise ValueError("ROSA inputs must be on the GPU")
     if _needs_grad(*tensors):
-        return _RosaScan.apply(*tensors, gated)
+        batch, _, dim = cand.shape
+        cand, write, read_raw, decay, direction, memory = tensors
+        return _RosaScan.apply(cand, write, read_raw, decay.reshape(dim), direction.reshape(dim),
+                               memory.reshape(batch, dim), gated)
     return _rosa_forward(*tensors, gated)
 
 
