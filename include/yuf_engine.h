@@ -207,7 +207,8 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
  * With G_t the gradient of S_t:  G_t += dy_t r_t^T;  dr = S_t^T dy, dv = G k,
  * dk = G^T v, da = S_{t-1}^T (G b), db = G^T (S_{t-1} a),
  * dd_j = sum_i G_ij S_{t-1,ij};  G_{t-1} = G_t (diag(d_t) + b_t a_t^T).
- * Same head sizes and lengths as the scan.
+ * Same head sizes and lengths as the scan, up to 2^25 chunks (B H ceil(T / 16))
+ * and H N = 2^24.
  */
 size_t yuf_wkv7_scan_backward_workspace(int B, int T, int H, int N);
 int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,
@@ -231,7 +232,8 @@ int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,
  *                       zero for B = 0.
  *   dmemory_in        : device [B, D] or NULL.  No output may alias an input.
  *   workspace         : yuf_rosa_scan_backward_workspace(B, T, D) bytes.
- * Supported D: 1 .. 1024.
+ * Supported D: 1 .. 1024; B ceil(T / 32) below 2^22 (ceil(T / 16) for D > 256,
+ * ceil(T / 8) for D > 512).
  */
 size_t yuf_rosa_scan_backward_workspace(int B, int T, int D);
 int yuf_rosa_scan_backward_f32(int B, int T, int D,
@@ -267,7 +269,8 @@ enum { YUF_LOSS_NONE = 0, YUF_LOSS_MEAN = 1, YUF_LOSS_SUM = 2 };
  * Cross-entropy of logits and token ids, and the logits' gradient in the same
  * pass over them (the training loop's F.cross_entropy,
  * yufmusicgen/training.py:295-306).
- *   logits     : device [M, V] fp32 (or bf16), rows ld elements apart (ld >= V).
+ *   logits     : device [M, V] fp32 (or bf16), V <= 2^30, rows ld elements apart
+ *                (ld >= V).
  *   targets    : device [M] int32 or int64 (target_bits 32 or 64).  A row whose
  *                target is ignore_index has loss 0 and gradient 0 and is not
  *                read; a target outside [0, V) gives NaN in that row's loss and

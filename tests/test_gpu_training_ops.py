@@ -94,6 +94,20 @@ def test_wkv7_gradients_of_long_and_many_sequences(batch, steps, heads, size):
     wkv_compare(wkv_grads(*case), wkv_exact(*case), size)
 
 
+@pytest.mark.parametrize("steps", [90, 200, 333])
+@pytest.mark.parametrize("size", [8, 16, 32, 40, 48, 64, 128])
+def test_wkv7_gradients_of_many_heads_are_those_of_each(size, steps):
+    """However many heads a call brings -- they choose how long its segments are and which kernels make
+    the local pass -- a sequence's gradients are those of that sequence alone, up to both calls' rounding."""
+    print(f"wkv7 gradients many heads N={size} T={steps}", flush=True)
+    arrs, s0, dy, ds = wkv_case(size + steps, 10, steps, 16, size)
+    many = wkv_grads(arrs, s0, dy, ds)
+    last = slice(9, 10)
+    alone = wkv_grads([a[last] for a in arrs], s0[last], dy[last], ds[last])
+    for name, m, a in zip(WKV_NAMES, many, alone):
+        close(m[last], a, 2 * (size + 32), name)
+
+
 def test_wkv7_gradients_of_no_token():
     from yufmusicgen_amd.ops import rwkv7_scan_backward
 

@@ -33,11 +33,12 @@
 //   wkv7_grad_carry_kernel  both recurrences over the segments, a workgroup per value tile.
 //   wkv7_grad_kernel        per segment: S forward over its chunks (kept per chunk, with U),
 //                           then G and the gradients backward.
-// One segment needs the first and the last alone, two no carry.
+// One segment needs the first and the last alone, two no carry.  Short segments that the GPU holds all at once
+// take the first two as one (wkv7_grad_block_kernel).
 //
 // 8 x 2048 x 16 x 40 (four segments): 77 + 136 + 6 + 341 us; 3 x 777 x 16 x 64 (ten): 16 + 46 + 18 + 66;
-// 1 x 2048 x 16 x 64 (32): 17 + 39 + 22 + 55.  The first is bound by memory (300 MB at 3.9 TB/s), the second
-// and the last by their SIMDs' issue: an fp32 MFMA takes 32 cycles of one, a VALU instruction 4 and a 16-byte
+// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 55.  The first is bound by memory (300 MB at 3.9
+// TB/s), the second and the last by their SIMDs' issue: an fp32 MFMA takes 32 cycles of one, a VALU instruction 4 and a 16-byte
 // LDS read about 18, none beside another, and a wave's chunk in the last kernel has 266 of the first at N = 64.
 //
 // MFMA layouts (16x16x4 f32; lane l, g = l / 16, li = l % 16): A[m = li][k = g],
@@ -207,31 +208,18 @@ __device__ __forceinline__ float rows_before(float x, int g) {
 // share an XCD's L2.
 __device__ __forceinline__ int xcd_unit(int per_xcd) { return (blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds; }
 
-// One wave per chunk of a head.
-template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel(GradParams p, int units, int per_xcd) {
+// A wave's LDS writes before its reads of other lanes' words.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The fragments of one chunk by one wave, from its tiles in LDS; sL and sP: 16 x kST floats each.
+template <int NB>
+__device__ __forceinline__ void chunk_fragments(const float *sA, const float *sR, const float *sB, const float *sK, float *sL, float *sP,
+                                                int lane, float *out) {
     constexpr int SA = 16 * NB + 4;
-    __shared__ __attribute__((aligned(16))) float tiles[4 * kC * SA + 3 * kC * kST];
-    float *sA = tiles, *sR = sA + kC * SA, *sB = sR + kC * SA, *sK = sB + kC * SA;
-    float *sL = sK + kC * SA, *sP = sL + kC * kST, *sT = sP + kC * kST;
-    const int unit = xcd_unit(per_xcd);
-    if (unit >= units) return;
-    const int head = unit / p.chunks, chunk = unit - head * p.chunks;
-    const int bb = head / p.H, h = head - bb * p.H;
-    const int lane = threadIdx.x, g = lane >> 4, li = lane & 15;
-    const int valid = min(kC, p.T - chunk * kC);
-#pragma unroll
-    for (int q = 0; q < NB; ++q) {
-        Tile tile;
-        tile.at(p, bb, h, chunk, 16 * q + li, g);
-        Decays d;
-        d.set(tile.load(p.w), valid, g);
-        const int at = 4 * g * SA + 16 * q + li;
-        stcol(sA + at, SA, tile.load(p.a) * d.before);
-        stcol(sR + at, SA, tile.load(p.r) * d.now);
-        stcol(sB + at, SA, tile.load(p.b) * d.inv);
-        stcol(sK + at, SA, tile.load(p.k) * d.inv);
-    }
-    lds_barrier();
+    const int g = lane >> 4, li = lane & 15;
     floatx4 ab = {0.f, 0.f, 0.f, 0.f}, ak = ab, rb = ab, rk = ab;
 #pragma unroll
     for (int jb = 0; jb < NB; ++jb) {
@@ -254,52 +242,75 @@ template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel
         rb[r] = li <= t ? rb[r] : 0.0f;
         rk[r] = li <= t ? rk[r] : 0.0f;
     }
-    st4(sL + li * kST + 4 * g, ab);  // Lab^T: column s of Lab in row s
-    st4(sP + li * kST + 4 * g, ak);  // Lak^T
-    lds_barrier();
-    {
-        // Column li of T by forward substitution, right-looking (the four lane groups alike).
-        float x[kC];
-#pragma unroll
-        for (int t = 0; t < kC; ++t) x[t] = li == t ? 1.0f : 0.0f;
-#pragma unroll
-        for (int s = 0; s < kC - 1; ++s) {
-            // Two steps' columns at a time: the compiler would load them all first and add them last, which
-            // takes 126 registers, so 70 and more waves at once.
-            if (s % 2 == 0)
-#pragma unroll
-                for (int t = 0; t < kC; ++t) asm volatile("" : "+v"(x[t])::"memory");
-#pragma unroll
-            for (int m = s / 4; m < 4; ++m) {
-                const floatx4 col = ld4(sL + s * kST + 4 * m);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (4 * m + e > s) x[4 * m + e] = fmaf(col[e], x[s], x[4 * m + e]);
-            }
-        }
-        // T^T, row s = li: each lane group writes its four tokens.
-        const floatx4 own = g == 0 ? floatx4{x[0], x[1], x[2], x[3]}
-                          : g == 1 ? floatx4{x[4], x[5], x[6], x[7]}
-                          : g == 2 ? floatx4{x[8], x[9], x[10], x[11]}
-                                   : floatx4{x[12], x[13], x[14], x[15]};
-        st4(sT + li * kST + 4 * g, own);
-    }
-    lds_barrier();
-    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-    const floatx4 t_col = ld4(sT + li * kST + 4 * g);            // T[4 g + r][li]
-    const floatx4 t_row = ldcol(sT + 4 * g * kST + li, kST);     // T[li][4 g + r]
-    // C[t][s] = sum T[t][m] Lak[m][s]: B operand Lak[m = 4 g + r][s = li] = the Gram's registers.
-    const floatx4 c_col = mul16(t_row, ak, zero);
-    // C^T[s][t] = sum Lak^T[s][m] T^T[m][t]: its registers, [s = 4 g + r][t = li], are C's row fragment.
-    // Its B operand T^T[m = 4 g + r][t = li] is the same four values as T's row fragment.
-    const floatx4 c_row = mul16(ld4(sP + li * kST + 4 * g), t_row, zero);
-    float *out = p.frags + ((size_t)head * p.chunks + chunk) * kFrags * kFrag + 4 * lane;
-    st4(out + kTRow * kFrag, t_row);
-    st4(out + kCRow * kFrag, c_row);
-    st4(out + kTCol * kFrag, t_col);
-    st4(out + kCCol * kFrag, c_col);
     st4(out + kMrbCol * kFrag, rb);
     st4(out + kMrkCol * kFrag, rk);
+    st4(sL + li * kST + 4 * g, ab);  // Lab^T: column s of Lab in row s
+    st4(sP + li * kST + 4 * g, ak);  // Lak^T
+    wave_lds_fence();
+    // Column li of T by forward substitution, right-looking (the four lane groups alike).
+    float x[kC];
+#pragma unroll
+    for (int t = 0; t < kC; ++t) x[t] = li == t ? 1.0f : 0.0f;
+#pragma unroll
+    for (int s = 0; s < kC - 1; ++s) {
+        // Two steps' columns at a time: the compiler would load them all first and add them last, which
+        // takes 126 registers, so 70 and more waves at once.
+        if (s % 2 == 0)
+#pragma unroll
+            for (int t = 0; t < kC; ++t) asm volatile("" : "+v"(x[t])::"memory");
+#pragma unroll
+        for (int m = s / 4; m < 4; ++m) {
+            const floatx4 col = ld4(sL + s * kST + 4 * m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * m + e > s) x[4 * m + e] = fmaf(col[e], x[s], x[4 * m + e]);
+        }
+    }
+    wave_lds_fence();
+    // T^T over Lab^T, row s = li: each lane group writes its four tokens.
+    const floatx4 own = g == 0 ? floatx4{x[0], x[1], x[2], x[3]}
+                      : g == 1 ? floatx4{x[4], x[5], x[6], x[7]}
+                      : g == 2 ? floatx4{x[8], x[9], x[10], x[11]}
+                               : floatx4{x[12], x[13], x[14], x[15]};
+    st4(sL + li * kST + 4 * g, own);
+    wave_lds_fence();
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    const floatx4 t_row = ldcol(sL + 4 * g * kST + li, kST);  // T[li][4 g + r]
+    st4(out + kTRow * kFrag, t_row);
+    st4(out + kTCol * kFrag, ld4(sL + li * kST + 4 * g));     // T[4 g + r][li]
+    // C[t][s] = sum T[t][m] Lak[m][s]: B operand Lak[m = 4 g + r][s = li] = the Gram's registers.
+    st4(out + kCCol * kFrag, mul16(t_row, ak, zero));
+    // C^T[s][t] = sum Lak^T[s][m] T^T[m][t]: its registers, [s = 4 g + r][t = li], are C's row fragment.
+    // Its B operand T^T[m = 4 g + r][t = li] is the same four values as T's row fragment.
+    st4(out + kCRow * kFrag, mul16(ld4(sP + li * kST + 4 * g), t_row, zero));
+}
+
+// One wave per chunk of a head.
+template <int NB> __global__ void __launch_bounds__(kWave) wkv7_grad_gram_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int SA = 16 * NB + 4;
+    __shared__ __attribute__((aligned(16))) float tiles[4 * kC * SA + 2 * kC * kST];
+    float *sA = tiles, *sR = sA + kC * SA, *sB = sR + kC * SA, *sK = sB + kC * SA, *scratch = sK + kC * SA;
+    const int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;
+    const int head = unit / p.chunks, chunk = unit - head * p.chunks;
+    const int bb = head / p.H, h = head - bb * p.H;
+    const int lane = threadIdx.x, g = lane >> 4, li = lane & 15;
+    const int valid = min(kC, p.T - chunk * kC);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+        Tile tile;
+        tile.at(p, bb, h, chunk, 16 * q + li, g);
+        Decays d;
+        d.set(tile.load(p.w), valid, g);
+        const int at = 4 * g * SA + 16 * q + li;
+        stcol(sA + at, SA, tile.load(p.a) * d.before);
+        stcol(sR + at, SA, tile.load(p.r) * d.now);
+        stcol(sB + at, SA, tile.load(p.b) * d.inv);
+        stcol(sK + at, SA, tile.load(p.k) * d.inv);
+    }
+    wave_lds_fence();
+    chunk_fragments<NB>(sA, sR, sB, sK, scratch, scratch + kC * kST, lane,
+                        p.frags + ((size_t)head * p.chunks + chunk) * kFrags * kFrag + 4 * lane);
 }
 
 // The wave's number, known to be the same for its lanes: descriptors and branches made from it stay scalar.
@@ -371,6 +382,36 @@ __device__ __forceinline__ const float *head_state(const float *s, const GradPar
 }
 __device__ __forceinline__ float *seg_state(float *s, const GradParams &p, int head, int seg) {
     return s + ((size_t)head * p.segments + seg) * p.N * p.N;
+}
+
+// X S for a row-fragment operand X (tokens, keys) in LDS: its own 16 tokens times the state tiles.
+template <int NB> __device__ __forceinline__ floatx4 times_state(const float *x, const floatx4 (&S)[NB]) {
+    floatx4 even = {0.f, 0.f, 0.f, 0.f}, odd = even;  // k-steps
+#pragma unroll
+    for (int jb = 0; jb < NB; ++jb) {
+        const floatx4 x4 = ld4(x + 16 * jb);
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            even = mfma(x4[r], S[jb][r], even);
+            odd = mfma(x4[r + 1], S[jb][r + 1], odd);
+        }
+    }
+    return even + odd;
+}
+
+// S += X^T b for a column-fragment operand X (tokens, keys) in LDS, four tiles at a time.
+template <int NB> __device__ __forceinline__ void add_to_state(const float *x, floatx4 b, floatx4 (&S)[NB]) {
+    constexpr int SA = 16 * NB + 4, kGroup = NB < 4 ? NB : 4;
+#pragma unroll
+    for (int j0 = 0; j0 < NB; j0 += kGroup) {
+        floatx4 x4[kGroup];
+#pragma unroll
+        for (int t = 0; t < kGroup; ++t) x4[t] = ldcol(x + 16 * (j0 + t), SA);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < kGroup; ++t) S[j0 + t] = mfma(x4[t][r], b[r], S[j0 + t]);
+    }
 }
 
 template <int NB> struct Sweep {
@@ -542,6 +583,118 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_local_k
         io.store_columns(P, seg_state(p.powers_t, p, head, seg));
     }
     io.store_rows(S, seg_state(p.starts, p, head, seg + 1));
+}
+
+// The two kernels above as one, for segments of kBlock chunks, a workgroup each.  Its inputs are read
+// once, scaled into LDS, and stay there: four waves make the chunks' fragments, then 3 NB
+// independent chains run over them without a barrier, NB tiles each of the segment's end state, its Pi, and
+// the gradient of its start.  1 x 2048 x 16 x 64: 33 us, so 56 with the two kernels; 2 x 1024 x 16 x 40: 31, so
+// 38.  While all segments are resident (two 64 to 81 KB workgroups a CU); 8 x 2048 x 16 x 40 in eight rounds: 269,
+// so 213.
+constexpr int kBlock = 4;
+// Waves of a SIMD that two workgroups of a CU need (their LDS fits up to NB = 4).
+template <int NB> constexpr int kBlockPerSimd = NB >= 8 ? 4 : (2 * (3 * NB < 4 ? 4 : 3 * NB) + 3) / 4;
+template <int NB> constexpr int kBlockWaves = 3 * NB < 4 ? 4 : 3 * NB > 16 ? 16 : 3 * NB;
+
+template <int NB> __global__ void __launch_bounds__(kBlockWaves<NB> *kWave, kBlockPerSimd<NB>) wkv7_grad_block_kernel(GradParams p, int units, int per_xcd) {
+    constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA, kWaves = kBlockWaves<NB>;
+    __shared__ __attribute__((aligned(16))) float lds[kBlock * (4 * kTok + NP + 2 * kC * kST)];
+    static_assert(sizeof(lds) <= 160 * 1024, "LDS of one CU");
+    auto tile_of = [&](int what, int i) { return lds + (4 * i + what) * kTok; };  // 0 A, 1 R, 2 B, 3 K of chunk i
+    float *sD = lds + kBlock * 4 * kTok, *scratch = sD + kBlock * NP;
+    const int unit = xcd_unit(per_xcd);
+    if (unit >= units) return;  // uniform over the workgroup
+    const int blocks = (p.chunks + kBlock - 1) / kBlock;
+    const int head = unit / blocks, seg = unit - head * blocks;
+    const int c0 = seg * kBlock, nc = min(kBlock, p.chunks - c0);
+    const int wave = wave_id();
+    Place w(p, head, 0);
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+
+    for (int i = wave; i < nc * NB; i += kWaves) {
+        const int chunk = i / NB, col = 16 * (i - chunk * NB) + w.li;
+        Tile tile;
+        tile.at(p, w.bb, w.h, c0 + chunk, col, w.g);
+        const floatx4 a = tile.load(p.a), r = tile.load(p.r), b = tile.load(p.b), k = tile.load(p.k);
+        Decays d;
+        d.set(tile.load(p.w), min(kC, p.T - (c0 + chunk) * kC), w.g);
+        const int at = 4 * w.g * SA + col;
+        stcol(tile_of(0, chunk) + at, SA, a * d.before);
+        stcol(tile_of(1, chunk) + at, SA, r * d.now);
+        stcol(tile_of(2, chunk) + at, SA, b * d.inv);
+        stcol(tile_of(3, chunk) + at, SA, k * d.inv);
+        if (w.g == 3) sD[chunk * NP + col] = d.last;
+    }
+    lds_barrier();
+    float *frags = p.frags + ((size_t)head * p.chunks + c0) * kFrags * kFrag + 4 * w.lane;
+    if (wave < nc)
+        chunk_fragments<NB>(tile_of(0, wave), tile_of(1, wave), tile_of(2, wave), tile_of(3, wave), scratch + 2 * wave * kC * kST,
+                            scratch + (2 * wave + 1) * kC * kST, w.lane, frags + (size_t)wave * kFrags * kFrag);
+    __syncthreads();  // the fragments are read back from memory
+
+    for (int task = wave; task < 3 * NB; task += kWaves) {
+        const int kind = task / NB;  // 0: state, 1: Pi, 2: gradient
+        if (kind == 0 && seg == p.segments - 1) continue;
+        if (kind == 1 && (seg == 0 || seg == p.segments - 1)) continue;
+        if (kind == 2 && seg == 0) continue;
+        w.q = task - kind * NB;
+        w.col = 16 * w.q + w.li;
+        const StateIo<NB> io(p, w);
+        const int row = w.li * SA + 4 * w.g, colm = 4 * w.g * SA + w.li;  // operands: rows of tokens, columns of keys
+        auto load_token = [&](const float *x, int i) {
+            Tile tile;
+            tile.at(p, w.bb, w.h, c0 + min(i, nc - 1), w.col, w.g);
+            return tile.load(x);
+        };
+        auto fragment = [&](int i, int which) { return ld4(frags + ((size_t)i * kFrags + which) * kFrag); };
+        floatx4 S[NB];
+        if (kind == 2) {
+            io.load_rows(seg == p.segments - 1 ? head_state(p.dstate_out, p, head) : nullptr, S);
+            floatx4 next = load_token(p.dy, nc - 1);
+            for (int i = nc - 1; i >= 0; --i) {
+                const floatx4 t_col = fragment(i, kTCol), rb_col = fragment(i, kMrbCol), y4 = next;
+                next = load_token(p.dy, max(i - 1, 0));
+#pragma unroll
+                for (int jb = 0; jb < NB; ++jb) S[jb] *= ld4(sD + i * NP + 16 * jb + 4 * w.g);
+                floatx4 F = times_state<NB>(tile_of(2, i) + row, S);
+                F = mul16(rb_col, y4, F);
+                add_to_state<NB>(tile_of(1, i) + colm, y4, S);
+                const floatx4 E = mul16(t_col, F, zero);
+                add_to_state<NB>(tile_of(0, i) + colm, E, S);
+            }
+            io.store_rows(S, seg_state(p.ends, p, head, seg - 1));
+            continue;
+        }
+        if (kind == 0) {
+            io.load_rows(seg == 0 ? head_state(p.state_in, p, head) : nullptr, S);
+        } else {
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[jb][r] = 16 * jb + 4 * w.g + r == w.col ? 1.0f : 0.0f;
+        }
+        floatx4 next = kind == 0 ? load_token(p.v, 0) : zero;
+        for (int i = 0; i < nc; ++i) {
+            const floatx4 t_row = fragment(i, kTRow), v4 = next;
+            floatx4 U = zero;
+            const floatx4 X = times_state<NB>(tile_of(0, i) + row, S);
+            if (kind == 0) {
+                next = load_token(p.v, i + 1);
+                U = mul16(fragment(i, kCRow), v4, U);
+                add_to_state<NB>(tile_of(3, i) + colm, v4, S);
+            }
+            U = mul16(t_row, X, U);
+            add_to_state<NB>(tile_of(2, i) + colm, U, S);
+#pragma unroll
+            for (int jb = 0; jb < NB; ++jb) S[jb] *= ld4(sD + i * NP + 16 * jb + 4 * w.g);
+        }
+        if (kind == 0) {
+            io.store_rows(S, seg_state(p.starts, p, head, seg + 1));
+        } else {
+            io.store_rows(S, seg_state(p.powers, p, head, seg));
+            io.store_columns(S, seg_state(p.powers_t, p, head, seg));
+        }
+    }
 }
 
 // A workgroup per (head, value tile, direction): x <- x Pi + local (x Pi^T backward) over the
@@ -764,21 +917,28 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
     if (p.dstate_in && seg == 0) io.store_columns(G, p.dstate_in + (size_t)head * N * N);
 }
 
+// Whether the segments' local pass and the chunks' matrices are one kernel: four-chunk segments, at most two a CU.
+bool block_form(int64_t heads, int segments, int seg_chunks) {
+    return segments > 1 && seg_chunks == kBlock && heads * segments <= 512;
+}
+
 // Chunks of a segment.  The last kernel takes as long as its fullest CU, w = ceil(heads segments / 256)
 // workgroups of c chunks, a third longer alone on it (5.6 us a chunk at N = 40, 7.4 alone); the local pass
-// adds 0.45 of that (a quarter of it for two segments, which have no Pi), the carry 4 us and 0.35 a segment.
-// Measured so: 8 x 2048 x 16 x 40, 2 / 4 / 8 / 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x
-// 16 x 64, 8 / 10 / 13: 160 / 143 / 169; 1 x 2048 x 16 x 64, 8 / 16 / 32: 190 / 143 / 136.
+// adds 0.45 of that (a quarter of it for two segments, which have no Pi; 0.25 with the chunks' matrices in
+// the block form), the carry 4 us and 0.35 a segment.  Measured so: 8 x 2048 x 16 x 40, 2 / 4 / 8 /
+// 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x 16 x 64, 8 / 10 / 13: 160 / 143 / 169; 1 x 2048 x 16 x 64,
+// 8 / 16 / 32: 190 / 143 / 136.
 int segment_chunks(int B, int T, int H, int N) {
     const int64_t heads = (int64_t)B * H;
-    const int chunks = (T + kC - 1) / kC;
+    const int chunks = T / kC + (T % kC != 0);
     int best = std::max(chunks, 1);
     double least = 1e30;
-    for (int64_t want = 1; want <= std::max<int64_t>(1, 1024 / heads) && (want == 1 || want * 4 <= chunks); ++want) {
-        const int c = std::max<int>(1, (int)((chunks + want - 1) / want)), S = std::max(1, (chunks + c - 1) / c);
+    for (int64_t want = 1; want == 1 || (want <= 1024 / heads && want * kBlock < chunks + kBlock); ++want) {
+        const int c = std::max<int>(want == 1 ? 1 : kBlock, (int)((chunks + want - 1) / want)), S = std::max(1, (chunks + c - 1) / c);
         const int64_t w = (heads * S + 255) / 256;
         const double last = (double)w * c * (w == 1 && N <= 64 ? 1.3 : 1.0);
-        const double cost = last * (S == 1 ? 1.0 : S == 2 ? 1.25 : 1.0 + 0.45 * (S - 1) / S) + (S > 2 ? 0.7 + 0.06 * S : 0.0);
+        const double local = S == 1 ? 0.0 : block_form(heads, S, c) ? 0.25 : S == 2 ? 0.25 : 0.45 * (S - 1) / S;
+        const double cost = last * (1.0 + local) + (S > 2 ? 0.7 + 0.06 * S : 0.0);
         if (cost < least) {
             least = cost;
             best = c;
@@ -793,7 +953,7 @@ struct Scratch {
 };
 
 Scratch scratch_of(int B, int T, int H, int N) {
-    const size_t heads = (size_t)B * H, chunks = (T + kC - 1) / kC, NB = (N + 15) / 16;
+    const size_t heads = (size_t)B * H, chunks = T / kC + (T % kC != 0), NB = (N + 15) / 16;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Scratch o{};
     o.seg_chunks = segment_chunks(B, T, H, N);
@@ -819,11 +979,15 @@ Scratch scratch_of(int B, int T, int H, int N) {
 template <int NB> void launch(const GradParams &p, hipStream_t s) {
     const int heads = p.B * p.H, grams = heads * p.chunks, segs = heads * p.segments;
     auto per_xcd = [](int units) { return (units + kXcds - 1) / kXcds; };
-    if (grams > 0)
-        hipLaunchKernelGGL((wkv7_grad_gram_kernel<NB>), dim3(per_xcd(grams) * kXcds), dim3(kWave), 0, s, p, grams, per_xcd(grams));
-    if (p.segments > 1) {
-        const int locals = 2 * heads * (p.segments - 1);
-        hipLaunchKernelGGL((wkv7_grad_local_kernel<NB>), dim3(per_xcd(locals) * kXcds), dim3(NB * kWave), 0, s, p, locals, per_xcd(locals));
+    if (block_form(heads, p.segments, p.seg_chunks)) {
+        hipLaunchKernelGGL((wkv7_grad_block_kernel<NB>), dim3(per_xcd(segs) * kXcds), dim3(kBlockWaves<NB> * kWave), 0, s, p, segs, per_xcd(segs));
+    } else {
+        if (grams > 0)
+            hipLaunchKernelGGL((wkv7_grad_gram_kernel<NB>), dim3(per_xcd(grams) * kXcds), dim3(kWave), 0, s, p, grams, per_xcd(grams));
+        if (p.segments > 1) {
+            const int locals = 2 * heads * (p.segments - 1);
+            hipLaunchKernelGGL((wkv7_grad_local_kernel<NB>), dim3(per_xcd(locals) * kXcds), dim3(NB * kWave), 0, s, p, locals, per_xcd(locals));
+        }
     }
     if (p.segments > 2) {
         const int carries = heads * 2 * NB;
@@ -862,7 +1026,7 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     if (outputs_alias<9, 7>({r, w_raw, k, v, a, b, state_in, dy, dstate_out}, {dr, dw_raw, dk, dv, da, db, dstate_in}))
         return fail(YUF_ERR_INVALID, "wkv7 backward: an output may not be an input or another output");
     GradParams p{};
-    p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = (T + kC - 1) / kC;
+    p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = T / kC + (T % kC != 0);
     p.r = r; p.w = w_raw; p.k = k; p.v = v; p.a = a; p.b = b; p.dy = dy;
     p.state_in = state_in; p.dstate_out = dstate_out;
     p.dr = dr; p.dw = dw_raw; p.dk = dk; p.dv = dv; p.da = da; p.db = db; p.dstate_in = dstate_in;
