@@ -108,6 +108,18 @@ def test_wkv7_gradients_of_many_heads_are_those_of_each(size, steps):
         close(m[last], a, 2 * (size + 32), name)
 
 
+@pytest.mark.parametrize("steps,heads", [(512, 32), (512, 33), (512, 96), (512, 128), (512, 129)])
+@pytest.mark.parametrize("size", [16, 40, 64, 128])
+def test_wkv7_gradients_at_the_limits_of_the_split(size, steps, heads):
+    """256, 768 and 1024 segments of a call and the next heads after: the last head as alone."""
+    print(f"wkv7 gradients limits {steps} x {heads} x {size}", flush=True)
+    arrs, s0, dy, ds = wkv_case(size + heads, 1, steps, heads, size)
+    many = wkv_grads(arrs, s0, dy, ds)
+    alone = wkv_grads([x[:, :, -1:] for x in arrs], s0[:, -1:], dy[:, :, -1:], ds[:, -1:])
+    for name, m, x in zip(WKV_NAMES, many, alone):
+        close(m[:, -1:] if name == "state" else m[:, :, -1:], x, 2 * (size + 32), name)
+
+
 def test_wkv7_gradients_of_no_token():
     from yufmusicgen_amd.ops import rwkv7_scan_backward
 

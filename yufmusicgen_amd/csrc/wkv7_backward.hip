@@ -589,8 +589,7 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_local_k
 // once, scaled into LDS, and stay there: four waves make the chunks' fragments, then 3 NB
 // independent chains run over them without a barrier, NB tiles each of the segment's end state, its Pi, and
 // the gradient of its start.  1 x 2048 x 16 x 64: 33 us, so 56 with the two kernels; 2 x 1024 x 16 x 40: 31, so
-// 38.  While all segments are resident (two 64 to 81 KB workgroups a CU); 8 x 2048 x 16 x 40 in eight rounds: 269,
-// so 213.
+// 38.  Not for many rounds of workgroups (two of 64 to 81 KB a CU): 8 x 2048 x 16 x 40 in eight: 269, so 213.
 constexpr int kBlock = 4;
 // Waves of a SIMD that two workgroups of a CU need (their LDS fits up to NB = 4).
 template <int NB> constexpr int kBlockPerSimd = NB >= 8 ? 4 : (2 * (3 * NB < 4 ? 4 : 3 * NB) + 3) / 4;
@@ -917,17 +916,22 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
     if (p.dstate_in && seg == 0) io.store_columns(G, p.dstate_in + (size_t)head * N * N);
 }
 
-// Whether the segments' local pass and the chunks' matrices are one kernel: four-chunk segments, at most two a CU.
-bool block_form(int64_t heads, int segments, int seg_chunks) {
-    return segments > 1 && seg_chunks == kBlock && heads * segments <= 512;
+// Whether the segments' local pass and the chunks' matrices are one kernel: four-chunk segments (at most 1024,
+// segment_chunks), and for N > 64, whose LDS leaves room for one a CU, at most 256 of them.  The whole call without
+// it and with it, one sequence of 2048 tokens in 256 / 512 / 768 / 1024 segments: N = 16 39 / 43 / 50 / 63 and
+// 34 / 38 / 44 / 47 us; N = 40 66 / 91 / 142 / 153 and 58 / 85 / 133 / 152; N = 64 87 / 130 / 193 / 224 and
+// 78 / 110 / 169 / 216; N = 128 241 / 368 / 559 / 668 and 210 / 376 / 588 / 759.  (512 tokens, 1024 segments of
+// N = 40: 137 and 143.)
+bool block_form(int64_t heads, int segments, int seg_chunks, int N) {
+    return segments > 1 && seg_chunks == kBlock && (N <= 64 || heads * segments <= 256);
 }
 
 // Chunks of a segment.  The last kernel takes as long as its fullest CU, w = ceil(heads segments / 256)
 // workgroups of c chunks, a third longer alone on it (5.6 us a chunk at N = 40, 7.4 alone); the local pass
 // adds 0.45 of that (a quarter of it for two segments, which have no Pi; 0.25 with the chunks' matrices in
 // the block form), the carry 4 us and 0.35 a segment.  Measured so: 8 x 2048 x 16 x 40, 2 / 4 / 8 /
-// 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x 16 x 64, 8 / 10 / 13: 160 / 143 / 169; 1 x 2048 x 16 x 64,
-// 8 / 16 / 32: 190 / 143 / 136.
+// 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x 16 x 64, 8 / 10 / 13: 160 / 143 / 169 (13 with the chunks'
+// matrices apart); 1 x 2048 x 16 x 64, 8 / 16 / 32: 190 / 143 / 116.
 int segment_chunks(int B, int T, int H, int N) {
     const int64_t heads = (int64_t)B * H;
     const int chunks = T / kC + (T % kC != 0);
@@ -937,7 +941,7 @@ int segment_chunks(int B, int T, int H, int N) {
         const int c = std::max<int>(want == 1 ? 1 : kBlock, (int)((chunks + want - 1) / want)), S = std::max(1, (chunks + c - 1) / c);
         const int64_t w = (heads * S + 255) / 256;
         const double last = (double)w * c * (w == 1 && N <= 64 ? 1.3 : 1.0);
-        const double local = S == 1 ? 0.0 : block_form(heads, S, c) ? 0.25 : S == 2 ? 0.25 : 0.45 * (S - 1) / S;
+        const double local = S == 1 ? 0.0 : block_form(heads, S, c, N) ? 0.25 : S == 2 ? 0.25 : 0.45 * (S - 1) / S;
         const double cost = last * (1.0 + local) + (S > 2 ? 0.7 + 0.06 * S : 0.0);
         if (cost < least) {
             least = cost;
@@ -979,7 +983,7 @@ Scratch scratch_of(int B, int T, int H, int N) {
 template <int NB> void launch(const GradParams &p, hipStream_t s) {
     const int heads = p.B * p.H, grams = heads * p.chunks, segs = heads * p.segments;
     auto per_xcd = [](int units) { return (units + kXcds - 1) / kXcds; };
-    if (block_form(heads, p.segments, p.seg_chunks)) {
+    if (block_form(heads, p.segments, p.seg_chunks, p.N)) {
         hipLaunchKernelGGL((wkv7_grad_block_kernel<NB>), dim3(per_xcd(segs) * kXcds), dim3(kBlockWaves<NB> * kWave), 0, s, p, segs, per_xcd(segs));
     } else {
         if (grams > 0)
