@@ -33,8 +33,8 @@
 //   wkv7_grad_carry_kernel  both recurrences over the segments, a workgroup per value tile.
 //   wkv7_grad_kernel        per segment: S forward over its chunks (kept per chunk, with U),
 //                           then G and the gradients backward.
-// One segment needs the first and the last alone, two no carry.  Short segments that the GPU holds all at once
-// take the first two as one (wkv7_grad_block_kernel).
+// One segment needs the first and the last alone, two no carry.  Four-chunk segments take the first two
+// as one (wkv7_grad_block_kernel, block_form).
 //
 // 8 x 2048 x 16 x 40 (four segments): 77 + 136 + 6 + 341 us; 3 x 777 x 16 x 64 (ten): 16 + 46 + 18 + 66;
 // 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 55.  The first is bound by memory (300 MB at 3.9
