@@ -282,7 +282,8 @@ enum { YUF_LOSS_NONE = 0, YUF_LOSS_MEAN = 1, YUF_LOSS_SUM = 2 };
  *   dloss      : device, gradient of the loss: [M] without reduction, else [1];
  *                NULL for ones.
  *   dlogits    : device [M, V] of the logits' type, rows ld_out apart, or NULL;
- *                may be logits (then ld_out = ld).
+ *                may be logits (then ld_out = ld).  Without rows a gradient alone
+ *                writes nothing.
  *   workspace  : yuf_cross_entropy_workspace(M) bytes for _MEAN and _SUM.
  * Exponentials and row sums in fp32, the sum over rows in fp64, in one order.
  */

@@ -814,3 +814,20 @@ def test_rosa_autograd_takes_the_scans_layouts():
     expect = torch.autograd.grad(rosa_householder_scan(*plain, gated=True)[0], plain, cuda(dread))
     for g, e, z in zip(got, expect, leaves):
         assert g.shape == z.shape and torch.equal(g.reshape(-1), e.reshape(-1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_backward_over_no_rows(reduction, dtype):
+    """As torch's loss: an empty gradient, also through [0, T, V] logits and a head's product."""
+    from yufmusicgen_amd.ops import cross_entropy
+
+    for shape in ((0, 50), (0, 7, 50), (3, 0, 50)):
+        x = torch.empty(*shape, device="cuda", dtype=dtype, requires_grad=True)
+        loss = cross_entropy(x, torch.empty(*shape[:-1], dtype=torch.int64, device="cuda"), reduction=reduction)
+        loss.sum().backward()
+        assert x.grad.shape == x.shape and x.grad.dtype == dtype
+    h = torch.empty(0, 8, device="cuda")
+    head = torch.randn(8, 50, device="cuda", requires_grad=True)
+    cross_entropy(h @ head, torch.empty(0, dtype=torch.int64, device="cuda"), reduction=reduction).sum().backward()
+    assert head.grad.shape == (8, 50) and not head.grad.any()

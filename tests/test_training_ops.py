@@ -127,3 +127,13 @@ def test_the_abi_takes_ctypes_integers_of_full_width():
     for name in ("yuf_dropout_f32", "yuf_dropout_bf16"):
         args = SIGNATURES[name][1]
         assert args[0] is ctypes.c_int64 and args[4] is args[5] is ctypes.c_uint64 and args[3] is ctypes.c_double
+
+
+@pytest.mark.parametrize("reduction", [0, 1, 2])
+def test_cross_entropy_gradient_of_no_rows(reduction):
+    """A backward pass over no rows has an empty gradient, whose pointer is null: there is nothing to do."""
+    for name in ("yuf_cross_entropy_f32", "yuf_cross_entropy_bf16"):
+        call = getattr(lib(), name)
+        for bits in (32, 64):
+            status = call(0, 10, None, 10, None, bits, -100, reduction, None, DUMMY, None, 10, DUMMY, None)
+            assert status == 0, lib().yuf_last_error().decode()

@@ -323,6 +323,7 @@ int cross_entropy(int M, int V, const T *logits, int64_t ld, const void *targets
     if (V > 1 << 30) return fail(YUF_ERR_INVALID, "cross entropy: V above 2^30");
     if (M > 0 && V == 0) return fail(YUF_ERR_INVALID, "cross entropy: rows without logits");
     if (M > 0 && (!logits || !targets)) return fail(YUF_ERR_INVALID, "cross entropy: null logits or targets");
+    if (!loss && M == 0) return YUF_OK;  // the gradient of no rows, whose pointer may well be null
     if (!loss && !dlogits) return fail(YUF_ERR_INVALID, "cross entropy: neither a loss nor a gradient asked for");
     if (dlogits == logits && dlogits && ld_out != ld)
         return fail(YUF_ERR_INVALID, "cross entropy: a gradient in place of the logits has their row stride");
