@@ -207,8 +207,8 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
  * With G_t the gradient of S_t:  G_t += dy_t r_t^T;  dr = S_t^T dy, dv = G k,
  * dk = G^T v, da = S_{t-1}^T (G b), db = G^T (S_{t-1} a),
  * dd_j = sum_i G_ij S_{t-1,ij};  G_{t-1} = G_t (diag(d_t) + b_t a_t^T).
- * Same head sizes and lengths as the scan, up to 2^25 chunks (B H ceil(T / 16))
- * and H N = 2^24.
+ * Same head sizes and lengths as the scan, up to 2^25 chunks (B H ceil(T / 16)),
+ * H N = 2^24 and B H ceil(N / 16) below 2^26.
  */
 size_t yuf_wkv7_scan_backward_workspace(int B, int T, int H, int N);
 int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,

@@ -137,3 +137,26 @@ def test_cross_entropy_gradient_of_no_rows(reduction):
         for bits in (32, 64):
             status = call(0, 10, None, 10, None, bits, -100, reduction, None, DUMMY, None, 10, DUMMY, None)
             assert status == 0, lib().yuf_last_error().decode()
+
+
+def test_scratch_of_refused_sizes_is_none():
+    """A workspace query gives 0 for every size that its operator refuses -- not terabytes that a caller
+    would ask the allocator for -- and the operator names the reason, with or without that buffer."""
+    call, space = lib().yuf_wkv7_scan_backward_f32, lib().yuf_wkv7_scan_backward_workspace
+    full = [256 * (i + 1) for i in range(17)] + [None]
+    for sizes, word in (((1, 1, 1 << 20, 40), "H * N"), ((1 << 14, 1 << 12, 1 << 10, 40), "chunks"),
+                        ((1 << 15, 17, 1 << 10, 8), "chunks"), ((1 << 15, 0, 1 << 10, 128), "heads"),
+                        ((1 << 15, 1, 1 << 10, 32), "heads"), ((1 << 13, 1, 1 << 10, 128), "heads")):
+        assert space(*sizes) == 0, sizes
+        refused(call(*sizes, *full), word)
+        refused(call(*sizes, *full[:16], None, None), word)  # not for want of the buffer
+    for sizes in ((1 << 15, 16, 1 << 10, 8), (1 << 12, 1, 1 << 10, 128), (1, 1, 1 << 17, 128)):
+        assert space(*sizes) > 0, sizes
+    call, space = lib().yuf_rosa_scan_backward_f32, lib().yuf_rosa_scan_backward_workspace
+    full = [256 * (i + 1) for i in range(15)] + [None]
+    for sizes in ((1 << 20, 1 << 20, 64), (1 << 22, 0, 64), (1 << 17, 1024, 256), (1 << 16, 1024, 257)):
+        assert space(*sizes) == 0, sizes
+        refused(call(*sizes, *full), "blocks")
+        refused(call(*sizes, *full[:14], None, None), "blocks")
+    for sizes in (((1 << 22) - 1, 32, 64), ((1 << 17) - 1, 1024, 256), ((1 << 16) - 1, 1024, 512)):
+        assert space(*sizes) > 0, sizes

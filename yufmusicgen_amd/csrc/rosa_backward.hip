@@ -528,6 +528,14 @@ Scratch scratch_of(int B, int T, int D) {
     return o;
 }
 
+// Why the sizes of a call are not supported, or null.
+const char *unsupported(int B, int T, int D) {
+    if (B < 0 || T < 0) return "rosa backward: negative size";
+    if (D < 1 || D > kMaxDim) return "rosa backward: D must be in 1..1024";
+    if ((int64_t)B * cut_of(T, D).S >= (1 << 22)) return "rosa backward: too many blocks";  // 2^32 threads a launch
+    return nullptr;
+}
+
 template <int EPL> void launch(const RosaGradParams &p, hipStream_t s) {
     constexpr int kWaves = block_waves(EPL);
     const dim3 wg(kWaves * kWave);
@@ -546,7 +554,7 @@ template <int EPL> void launch(const RosaGradParams &p, hipStream_t s) {
 
 extern "C" size_t yuf_rosa_scan_backward_workspace(int B, int T, int D) {
     using namespace yuf;
-    if (B <= 0 || T < 0 || D < 1 || D > kMaxDim) return 0;
+    if (B <= 0 || unsupported(B, T, D)) return 0;
     return scratch_of(B, T, D).bytes;
 }
 
@@ -556,8 +564,7 @@ extern "C" int yuf_rosa_scan_backward_f32(int B, int T, int D, const float *cand
                                           float *dcand, float *dwrite, float *dread_raw, float *ddecay,
                                           float *ddirection, float *dmemory_in, void *workspace, void *stream) {
     using namespace yuf;
-    if (B < 0 || T < 0) return fail(YUF_ERR_INVALID, "rosa backward: negative size");
-    if (D < 1 || D > kMaxDim) return fail(YUF_ERR_INVALID, "rosa backward: D must be in 1..1024");
+    if (const char *why = unsupported(B, T, D)) return fail(YUF_ERR_INVALID, why);
     if (!decay || !direction || !ddecay || !ddirection)
         return fail(YUF_ERR_INVALID, "rosa backward: null decay, direction or their gradients");
     if (B > 0 && T > 0 && (!cand || !write || !dread || !dcand || !dwrite))
@@ -567,7 +574,6 @@ extern "C" int yuf_rosa_scan_backward_f32(int B, int T, int D, const float *cand
     if (B > 0 && !workspace) return fail(YUF_ERR_INVALID, "rosa backward: null workspace");
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Cut cut = cut_of(T, D);
-    if ((int64_t)B * cut.S >= (1 << 22)) return fail(YUF_ERR_INVALID, "rosa backward: too many blocks");  // 2^32 threads a launch
     if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "rosa backward: workspace must be 256-byte aligned");
     // The gradients of one block are written while another still reads the inputs.
     if (B > 0 && outputs_alias<8, 6>({cand, write, read_raw, decay, direction, memory_in, dread, dmemory},

@@ -980,6 +980,20 @@ Scratch scratch_of(int B, int T, int H, int N) {
     return o;
 }
 
+// Why the sizes of a call are not supported, or nothing.
+std::string unsupported(int B, int T, int H, int N) {
+    if (B < 0 || T < 0 || H < 0) return "wkv7 backward: negative size";
+    if (!wkv7_supported(N)) return "wkv7 backward: unsupported head size N=" + std::to_string(N);
+    // Offsets inside a chunk of one head are 32-bit.
+    if ((int64_t)H * N > (1 << 24)) return "wkv7 backward: H * N above 2^24";
+    const int64_t heads = (int64_t)B * H;
+    if (heads > (1 << 25) / std::max(1, T / kC + (T % kC != 0))) return "wkv7 backward: too many chunks";
+    // A launch has fewer than 2^32 threads: a chunk is one wave, a segment NB.  (Heads of more than one
+    // segment have at most 1024 segments together.)
+    if ((heads + kXcds - 1) / kXcds * kXcds * ((N + 15) / 16) * kWave >= (int64_t)1 << 32) return "wkv7 backward: too many heads";
+    return "";
+}
+
 template <int NB> void launch(const GradParams &p, hipStream_t s) {
     const int heads = p.B * p.H, grams = heads * p.chunks, segs = heads * p.segments;
     auto per_xcd = [](int units) { return (units + kXcds - 1) / kXcds; };
@@ -1005,7 +1019,7 @@ template <int NB> void launch(const GradParams &p, hipStream_t s) {
 
 extern "C" size_t yuf_wkv7_scan_backward_workspace(int B, int T, int H, int N) {
     using namespace yuf;
-    if (B <= 0 || T < 0 || H <= 0 || !wkv7_supported(N)) return 0;
+    if (B <= 0 || H <= 0 || !unsupported(B, T, H, N).empty()) return 0;
     return scratch_of(B, T, H, N).bytes;
 }
 
@@ -1015,16 +1029,11 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
                                           float *dv, float *da, float *db, float *dstate_in, void *workspace,
                                           void *stream) {
     using namespace yuf;
-    if (B < 0 || T < 0 || H < 0) return fail(YUF_ERR_INVALID, "wkv7 backward: negative size");
-    if (!wkv7_supported(N)) return fail(YUF_ERR_INVALID, "wkv7 backward: unsupported head size N=" + std::to_string(N));
+    if (const std::string why = unsupported(B, T, H, N); !why.empty()) return fail(YUF_ERR_INVALID, why);
     if (B == 0 || H == 0) return YUF_OK;
     if (T > 0 && (!r || !w_raw || !k || !v || !a || !b || !dy || !dr || !dw_raw || !dk || !dv || !da || !db))
         return fail(YUF_ERR_INVALID, "wkv7 backward: null input/output pointer");
     if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
-    // Offsets inside a chunk of one head are 32-bit.
-    if ((int64_t)H * N > (1 << 24)) return fail(YUF_ERR_INVALID, "wkv7 backward: H * N above 2^24");
-    if ((int64_t)B * H * std::max(1, T / kC + (T % kC != 0)) > (1 << 25))  // a launch has at most 2^32 threads
-        return fail(YUF_ERR_INVALID, "wkv7 backward: too many chunks");
     if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "wkv7 backward: workspace must be 256-byte aligned");
     // The gradients of one segment are written while another still reads the inputs.
     if (outputs_alias<9, 7>({r, w_raw, k, v, a, b, state_in, dy, dstate_out}, {dr, dw_raw, dk, dv, da, db, dstate_in}))
