@@ -831,3 +831,94 @@ def test_cross_entropy_backward_over_no_rows(reduction, dtype):
     head = torch.randn(8, 50, device="cuda", requires_grad=True)
     cross_entropy(h @ head, torch.empty(0, dtype=torch.int64, device="cuda"), reduction=reduction).sum().backward()
     assert head.grad.shape == (8, 50) and not head.grad.any()
+
+
+# ---------------------------------------------------------- the decays' gradient, token by token
+def wkv_decay_gradient(arrs, s0, dy, ds):
+    """float64: dw and, per element, the sum of its terms' magnitudes, sum_i |G_ij S_ij| d_j |slope_j|."""
+    r, w, k, v, a, b, dy = (torch.from_numpy(np.asarray(x, np.float64)) for x in (*arrs, dy))
+    batch, steps, heads, size = r.shape
+    sig = torch.sigmoid(w)
+    d, slope = torch.exp(-np.exp(-0.5) * sig), -np.exp(-0.5) * sig * torch.sigmoid(-w)
+    zero = torch.zeros(batch, heads, size, size, dtype=torch.float64)
+    S = zero if s0 is None else torch.from_numpy(np.asarray(s0, np.float64))
+    G = zero if ds is None else torch.from_numpy(np.asarray(ds, np.float64))
+    states = []
+    for t in range(steps):
+        states.append(S)
+        u = S @ a[:, t, :, :, None]
+        S = S * d[:, t, :, None, :] + u @ b[:, t, :, None, :] + v[:, t, :, :, None] @ k[:, t, :, None, :]
+    dw, size_of = torch.empty_like(w), torch.empty_like(w)
+    for t in reversed(range(steps)):
+        G = G + dy[:, t, :, :, None] @ r[:, t, :, None, :]
+        terms = G * states[t] * (d[:, t] * slope[:, t])[:, :, None, :]
+        dw[:, t], size_of[:, t] = terms.sum(-2), terms.abs().sum(-2)
+        G = G * d[:, t, :, None, :] + (G @ b[:, t, :, :, None]) @ a[:, t, :, None, :]
+    return dw, size_of
+
+
+def decay_gradient_close(got, arrs, s0, dy, ds, floor=0.0):
+    """Every token's dw by itself: its error's 2-norm over the columns is at most N + 32 roundings (the terms
+    of the sums that make a state, its gradient and their product) of its own terms' magnitudes -- not of other
+    tokens' -- and so exactly 0 where no term is left.  floor: an absolute error that a test derives."""
+    dw, size_of = wkv_decay_gradient(arrs, s0, dy, ds)
+    err = (got.double().cpu() - dw).norm(dim=-1)
+    terms, size_of = dw.shape[-1] + 32, size_of.norm(dim=-1)
+    bound = terms * EPS32 * size_of + torch.where(size_of > 0, terms * 2.0**-114 + floor, 0.0)
+    worst = ((err - bound) / bound.clamp(min=1e-30)).argmax().item()
+    assert (err <= bound).all(), (worst, err.reshape(-1)[worst].item(), bound.reshape(-1)[worst].item())
+
+
+def decay_inputs(kind, seed, batch, steps, heads, size):
+    """Inputs whose tokens' decay gradients differ by orders of magnitude."""
+    arrs, s0, dy, ds = wkv_case(seed, batch, steps, heads, size)
+    half = np.arange(steps) % 16 < 8
+    if kind.startswith("fast"):  # a state that dies out within a chunk, but for the chunk's last token
+        arrs[1][:] = 30.0
+        arrs[1][:, 15::16] = -1.0
+        arrs[2] *= float(kind[4:])  # writes
+    elif kind == "padded":  # right padding: nothing follows the last token that counts
+        dy[:, steps - steps // 3 :] = 0.0
+        s0 *= 30.0
+        ds = None
+    elif kind == "left":  # nothing before the first token that counts
+        s0 = None
+        arrs[2][:, : steps // 3] = 0.0
+    elif kind == "early":
+        arrs[3][:, half] *= 100.0
+        dy[:, half] *= 100.0
+        arrs[1][:, ~half] = 30.0
+    elif kind == "late":
+        arrs[3][:, ~half] *= 100.0
+        dy[:, ~half] *= 100.0
+    elif kind == "state":
+        s0 *= 30.0
+    return arrs, s0, dy, ds
+
+
+@pytest.mark.parametrize("kind", ["fast0.01", "fast0.001", "fast0", "padded", "left", "early", "late", "state", "plain"])
+@pytest.mark.parametrize("size", [8, 40, 64, 128])
+@pytest.mark.parametrize("steps", [16, 27, 50, 333])
+def test_wkv7_decay_gradient_of_every_token(steps, size, kind):
+    print(f"wkv7 decay gradient {kind} N={size} T={steps}", flush=True)
+    case = decay_inputs(kind, size + steps, 1, steps, 2, size)
+    got = wkv_grads(*case)
+    decay_gradient_close(got[1], *case)
+    expect = wkv_exact(*case)
+    close(got[1], expect[1], size + 32, "w")
+    if kind == "padded":
+        assert not got[1][:, steps - steps // 3 :].any()
+
+
+def test_wkv7_decay_gradient_of_a_zero_states_first_token():
+    arrs, _, dy, ds = wkv_case(4, 2, 40, 3, 40)
+    assert not wkv_grads(arrs, None, dy, ds)[1][:, 0].any()
+
+
+def test_wkv7_decay_gradient_at_extreme_decays():
+    """The values, where the sigmoid is flat too: exp(-80) is the smallest exponential the kernel takes, 1.8e-35,
+    and a gradient below it is the state's and its gradient's product (some 10^3 here) with that."""
+    arrs, s0, dy, ds = wkv_case(3, 1, 64, 2, 40)
+    arrs[1][:, :, 0] = 100.0
+    arrs[1][:, ::2, 1] = -200.0
+    decay_gradient_close(wkv_grads(arrs, s0, dy, ds)[1], arrs, s0, dy, ds, floor=1e-30)

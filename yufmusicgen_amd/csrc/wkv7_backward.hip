@@ -17,11 +17,19 @@
 //     R' = Y' S0 + Mrb' B + Mrk' K        A' = E S0 + Lab' B + Lak' K
 //     B' = U G + Mrb'^T R + Lab'^T A      K' = V G + Mrk'^T R + Lak'^T A
 //     r' = R' D_t, a' = A' D_{t-1}, b' = B' / D_t, k' = K' / D_t
-//     (log d_t)' = sum_i (G0 S0)_i - sum_{s < t} (R R' - B B' - K K')_s - sum_{s <= t} (A A')_s
 //     w' = (log d)' (-e^{-0.5}) sigmoid(w) (1 - sigmoid(w))
-// The last but one: scaling S0 by x and every D_t by 1 / x per key column changes nothing, so
-// the log D_t' of a chunk add up to the share of S0.  Summed from the chunk's start, and not from its
-// end, a zero state's first token gets its exact 0.
+// (log d_t)' per key column is the sum over what enters the state before d_t -- S0 and, at tokens s < t, b_s and
+// k_s -- times what takes from it behind -- G, r_s at tokens s >= t and a_s at tokens s > t.  The pairs with S0 or
+// G are, with R'0 = Y' S0, A'0 = E S0, B'0 = U G and K'0 = V G, the first terms above,
+//     sum_i (G S0)_i + sum_{s >= t} (R R'0)_s + sum_{s > t} (A A'0)_s + sum_{s < t} (B B'0 + K K'0)_s;
+// those inside the chunk, with z = R (R' - R'0) - B (B' - B'0) - K (K' - K'0) + A (A' - A'0), which
+// adds up to 0 over the chunk, are
+//     - sum_{s < t} z_s - (A (A' - A'0))_t  =  sum_{s >= t} z_s - (A (A' - A'0))_t,
+// from its start or from its end, and each token takes the side whose terms are the smaller in sum: terms
+// that cancel are not larger than what they leave behind is made of, and nothing before the first
+// token or behind the last one with a gradient is left of either.  One sum for all pairs, from the start as the
+// difference of sum_i (G0 S0)_i and the earlier tokens' shares, lost up to all digits of a token
+// whose state has died out within the chunk.
 //
 // The sequence is cut into segments of whole chunks that run side by side:
 //   wkv7_grad_gram_kernel   what no state enters, for every chunk at once: T, C, Mrb, Mrk.
@@ -195,14 +203,19 @@ __device__ __forceinline__ float rows_sum(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-// Sum over the earlier lane groups of a column.
-__device__ __forceinline__ float rows_before(float x, int g) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float even = __uint_as_float(a[0]), pair = even + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair), __float_as_uint(pair), false, false);
-    const float low = __uint_as_float(b[0]);
-    return g == 0 ? 0.0f : g == 1 ? even : g == 2 ? low : low + even;
-}
+// Sums over the earlier and over the later lane groups of a column.
+struct Around {
+    float before, after;
+    __device__ __forceinline__ Around(float x, int g) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        const float even = __uint_as_float(a[0]), odd = __uint_as_float(a[1]), pair = even + odd;
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair), __float_as_uint(pair), false, false);
+        const float low = __uint_as_float(b[0]), high = __uint_as_float(b[1]);
+        before = g == 0 ? 0.0f : g == 1 ? even : g == 2 ? low : low + even;
+        after = g == 0 ? odd + high : g == 1 ? high : g == 2 ? odd : 0.0f;
+    }
+};
+__device__ __forceinline__ float sum4(floatx4 x) { return (x[0] + x[1]) + (x[2] + x[3]); }
 
 // Units dealt so that consecutive ones (the chunks of a head, the heads of a batch row)
 // share an XCD's L2.
@@ -827,6 +840,7 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
         lds_barrier();
         // Value tile q: F, V'; key tile q: Y' S0, U G, V G.
         floatx4 F = zero, dV = zero, dR = zero, dA = zero, dB = zero, dK = zero;
+        float share = 0.0f;  // sum_i (G S0)_i of the lane's key
         mul16(rb_col, yv, F, rk_col, yv, dV);
 #pragma unroll
         for (int t = 0; t < NB; ++t) {
@@ -840,6 +854,7 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
                 dR = mfma(y4[r], S0[t][r], dR);
                 dB = mfma(u4[r], G[t][r], dB);
                 dK = mfma(v4[r], G[t][r], dK);
+                share = fmaf(G[t][r], S0[t][r], share);
             }
         }
         floatx4 E = zero;
@@ -877,8 +892,9 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
             for (int t = 0; t < NB; ++t) x4[t] = ldcol(sE + 4 * g * SA + 16 * t + li, SA);
             mul16_tiles<NB>(x4, A, G);
         }
-        mul16(ld4(sMrb + li * kST + 4 * g), B, dR, ldcol(sMrb + 4 * g * kST + li, kST), R, dB);
-        mul16(ld4(sMrk + li * kST + 4 * g), K, dR, ldcol(sMrk + 4 * g * kST + li, kST), R, dK);
+        floatx4 iR = zero, iA = zero, iA1 = zero, iB = zero, iK = zero;  // the chunk's own parts of R', A', B', K'
+        mul16(ld4(sMrb + li * kST + 4 * g), B, iR, ldcol(sMrb + 4 * g * kST + li, kST), R, iB);
+        mul16(ld4(sMrk + li * kST + 4 * g), K, iR, ldcol(sMrk + 4 * g * kST + li, kST), R, iK);
         floatx4 dA1 = zero;
 #pragma unroll
         for (int t = 0; t < NB; ++t) {
@@ -890,26 +906,40 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
             }
         }
         lds_barrier();
-        mul16(ld4(sLab + li * kST + 4 * g), B, dA, ldcol(sLab + 4 * g * kST + li, kST), A, dB);
-        mul16(ld4(sLak + li * kST + 4 * g), K, dA1, ldcol(sLak + 4 * g * kST + li, kST), A, dK);
         dA += dA1;
-        tile.store(p.dr, dR * d.now);
-        tile.store(p.da, dA * d.before);
-        tile.store(p.db, dB * d.inv);
-        tile.store(p.dk, dK * d.inv);
-        // (log d_t)': sums over the chunk's earlier tokens.
-        const floatx4 ya = A * dA, z = R * dR - B * dB - K * dK + ya;
-        float share = 0.0f;  // sum_i (G0 S0)_i of the lane's key
+        mul16(ld4(sLab + li * kST + 4 * g), B, iA, ldcol(sLab + 4 * g * kST + li, kST), A, iB);
+        mul16(ld4(sLak + li * kST + 4 * g), K, iA1, ldcol(sLak + 4 * g * kST + li, kST), A, iK);
+        iA += iA1;
+        tile.store(p.dr, (dR + iR) * d.now);
+        tile.store(p.da, (dA + iA) * d.before);
+        tile.store(p.db, (dB + iB) * d.inv);
+        tile.store(p.dk, (dK + iK) * d.inv);
+        // (log d_t)', in the tokens' order forward for what enters the state and backward for what takes from it.
+        const floatx4 pr = R * dR, pa = A * dA, in = B * dB + K * dK;
+        const floatx4 yr = R * iR, ya = A * iA, yb = B * iB + K * iK, rest = yr - yb, z = rest + ya;
+        floatx4 m;  // magnitude of a token's terms
 #pragma unroll
-        for (int ib = 0; ib < NB; ++ib)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) share = fmaf(G[ib][r], S0[ib][r], share);
-        float run = rows_sum(share) - rows_before((z[0] + z[1]) + (z[2] + z[3]), g);
-        floatx4 dw;
+        for (int r = 0; r < 4; ++r) m[r] = fabsf(yr[r]) + fabsf(yb[r]) + fabsf(ya[r]);
+        const Around az(sum4(z), g), am(sum4(m), g);
+        float before = rows_sum(share) + Around(sum4(in), g).before, after = Around(sum4(pr + pa), g).after;
+        float z_before = az.before, m_before = am.before, z_after = az.after, m_after = am.after;
+        floatx4 dw, inner, low;  // low: magnitude on the start's side
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            dw[r] = (run - ya[r]) * d.slope[r];
-            run -= z[r];
+            dw[r] = before;
+            low[r] = m_before;
+            inner[r] = -z_before - ya[r];
+            before += in[r];
+            m_before += m[r];
+            z_before += z[r];
+        }
+#pragma unroll
+        for (int r = 3; r >= 0; --r) {
+            m_after += m[r];
+            inner[r] = low[r] <= m_after ? inner[r] : z_after + rest[r];
+            z_after += z[r];
+            dw[r] = (dw[r] + (after + pr[r]) + inner[r]) * d.slope[r];
+            after += pr[r] + pa[r];
         }
         tile.store(p.dw, dw);
     }
