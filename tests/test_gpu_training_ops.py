@@ -922,3 +922,53 @@ def test_wkv7_decay_gradient_at_extreme_decays():
     arrs[1][:, :, 0] = 100.0
     arrs[1][:, ::2, 1] = -200.0
     decay_gradient_close(wkv_grads(arrs, s0, dy, ds)[1], arrs, s0, dy, ds, floor=1e-30)
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("dim", [64, 100, 300])
+def test_rosa_gradients_through_open_gates_and_small_candidates(dim, gated):
+    """Every element by itself.  One token, no memory and the first unit vector as direction: H only changes the first
+    element's sign, so each gradient is a product of its own element's factors.  exp of x is off by |x| + 2 roundings
+    (its argument's and its own), a sigmoid, 1 - sigmoid, tanh and 1 - tanh^2 by their exponential's (|x|, 2 |x| for
+    tanh) and at most 8 more (tanh beyond 1/4 divides E - 1 by E + 1, of which the first magnifies E's 2 by up to 3);
+    six factors and their products are within 64 beside the exponentials'.  Below float32's smallest normal number
+    2^-126 a factor is off by that, times factors below 2^4."""
+    from yufmusicgen_amd.ops import rosa_householder_scan_backward
+
+    batch, rng = 40, np.random.default_rng(dim)
+
+    def spread(most):
+        """Either sign, from 1e-6 to `most` evenly in the logarithm."""
+        x = np.exp(rng.uniform(np.log(1e-6), np.log(most), (batch, 1, dim))) * rng.choice([-1.0, 1.0], (batch, 1, dim))
+        return x.astype(np.float32)
+
+    cand, write, rr, dread = spread(30.0), spread(40.0), spread(40.0), rng.uniform(0.5, 2.0, (batch, 1, dim)).astype(np.float32)
+    u, lam = np.zeros(dim, np.float32), np.full(dim, 0.5, np.float32)
+    u[0] = 1.0
+    got = rosa_householder_scan_backward(*(cuda(x) for x in (cand, write, rr, lam, u, np.zeros((batch, dim)), dread)),
+                                         gated=gated)
+    c, w, r, n = (torch.from_numpy(x).double() for x in (cand, write, rr, dread))
+    sign = 1.0 - 2.0 * torch.from_numpy(u).double()
+    g, th, slope = torch.sigmoid(w), torch.tanh(c), 1.0 / torch.cosh(c) ** 2
+    dq = n * torch.sigmoid(r) if gated else n
+    expect = [sign * dq * g * slope, sign * dq * th * g * torch.sigmoid(-w)]
+    if gated:
+        expect.append(n * sign * g * th * torch.sigmoid(r) * torch.sigmoid(-r))
+    roundings = 64 + 2 * w.abs() + 2 * c.abs() + (2 * r.abs() if gated else 0)
+    for name, x, e in zip(("cand", "write", "read_raw"), got, expect):
+        err, bound = (x.double().cpu() - e).abs(), roundings * EPS32 * e.abs() + 2.0**-122
+        at = (err / bound).argmax()
+        assert (err <= bound).all(), (name, *(z.reshape(-1)[at].item() for z in (c, w, r, x.double().cpu(), e)))
+
+
+def test_rosa_gradients_of_saturated_inputs_are_finite():
+    """Infinities and the largest numbers as gates and candidates: no 0 times infinity."""
+    from yufmusicgen_amd.ops import rosa_householder_scan_backward
+
+    ends = torch.tensor([float("inf"), -float("inf"), 3e38, -3e38, 100.0, -100.0, 88.8, -88.8], device="cuda")
+    cand = ends.repeat(8)[None, None]
+    write, rr = ends.repeat_interleave(8)[None, None], ends.roll(3).repeat(8)[None, None]
+    vec, one = torch.full((64,), 0.125, device="cuda"), torch.ones(1, 1, 64, device="cuda")
+    for gated in (True, False):
+        for g in rosa_householder_scan_backward(cand, write, rr, vec, vec, torch.zeros(1, 64, device="cuda"), one, gated=gated):
+            assert g is None or torch.isfinite(g).all()

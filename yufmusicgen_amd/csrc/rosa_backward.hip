@@ -56,16 +56,27 @@ struct RosaGradParams {
     double *sums;         // [B * S][2][D]: dlambda and du of a block
 };
 
-// sigmoid(x) = 1 / (1 + e^{-x}) and, with E = e^{2x}, tanh(x) = (E - 1) / (E + 1) and
-// 1 - tanh(x)^2 = 4 E / (E + 1)^2 from the hardware's exponential and reciprocal, as the
-// scan has them: within 2^-22 of their values' range.
-__device__ __forceinline__ float gate(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+// Each of these keeps its relative precision, up to its exponential's |x| 2^-24 (2 |x| for tanh): the
+// gradients are products of them, and 1 - sigmoid of an open gate, as a difference, would be of its rounding.
+// e stays finite, so that no 0 meets an infinity.
+struct Gate {
+    float value, rest;  // sigmoid(x) = 1 / (1 + e) and 1 - sigmoid(x) = e / (1 + e), e = exp(-x)
+    __device__ __forceinline__ explicit Gate(float x) {
+        const float e = __expf(x < -80.0f ? 80.0f : -x);  // the comparison keeps NaN
+        value = __builtin_amdgcn_rcpf(1.0f + e);
+        rest = e * value;
+    }
+};
+__device__ __forceinline__ float gate(float x) { return Gate(x).value; }
+// With e = exp(2 x): tanh(x) = (e - 1) / (e + 1) and 1 - tanh(x)^2 = 4 e / (e + 1)^2.  e - 1 loses digits near
+// 0, where the first terms of tanh's series do (up to 1/4: the next one is 2^-27 of x).
 struct Tanh {
     float value, slope;
     __device__ __forceinline__ explicit Tanh(float x) {
-        const float e = __expf(2.0f * (x > 10.0f ? 10.0f : x));  // 1 in fp32 from there on; the comparison keeps NaN
-        const float r = __builtin_amdgcn_rcpf(e + 1.0f);
-        value = (e - 1.0f) * r;
+        const float e = __expf(2.0f * (x > 40.0f ? 40.0f : x));
+        const float r = __builtin_amdgcn_rcpf(e + 1.0f), q = x * x;
+        const float series = fmaf(fmaf(fmaf(fmaf(62.0f / 2835.0f, q, -17.0f / 315.0f), q, 2.0f / 15.0f), q, -1.0f / 3.0f), q * x, x);
+        value = fabsf(x) < 0.25f ? series : (e - 1.0f) * r;
         slope = 4.0f * e * r * r;
     }
 };
@@ -378,13 +389,18 @@ template <int EPL> __global__ void __launch_bounds__(block_waves(EPL) * kWave) r
 #pragma unroll
             for (int k = 0; k < EPL; ++k) {
                 const int t = wave + i * kWaves, at = c.lane + kWave * k;
-                const float g = gate(write[i][k]), r = gated ? gate(rr[i][k]) : 1.0f;
+                const Gate g(write[i][k]);
                 const Tanh th(cand[i][k]);
-                block.e[t][at] = c.own(k) ? g * th.value : 0.0f;
-                block.dq[t][at] = c.own(k) ? dread[i][k] * r : 0.0f;
-                dr[i][k] = dread[i][k] * r * (1.0f - r);
-                gc[i][k] = g * th.slope;
-                gw[i][k] = th.value * g * (1.0f - g);
+                block.e[t][at] = c.own(k) ? g.value * th.value : 0.0f;
+                gc[i][k] = g.value * th.slope;
+                gw[i][k] = th.value * g.value * g.rest;
+                float dq = dread[i][k];
+                if (gated) {
+                    const Gate r(rr[i][k]);
+                    dq *= r.value;
+                    dr[i][k] = dq * r.rest;
+                }
+                block.dq[t][at] = c.own(k) ? dq : 0.0f;
             }
     }
     // m before the block, for the first token's q_{t-1} and (block 0) the initial memory's terms.
@@ -429,7 +445,7 @@ template <int EPL> __global__ void __launch_bounds__(block_waves(EPL) * kWave) r
             x[k] = fmaf(-2.0f * sp, c.u[k], pt) + extra[k];
             oc[k] = x[k] * gc[i][k];
             ow[k] = x[k] * gw[i][k];
-            orr[k] = dr[i][k] * fmaf(-2.0f * mu, c.u[k], m);
+            if (gated) orr[k] = dr[i][k] * fmaf(-2.0f * mu, c.u[k], m);
             dlam[k] = fmaf(x[k], fmaf(-2.0f * mu_before, c.u[k], before), dlam[k]);
             du[k] = fmaf(-2.0f * sp, m, fmaf(-2.0f * mu, pt, du[k]));
         }
