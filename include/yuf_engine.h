@@ -201,7 +201,8 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
  *   r, w_raw, k, v, a, b, state_in : the forward call's inputs.
  *   dy          : device [B, T, H, N], gradient of y.
  *   dstate_out  : device [B, H, N, N], gradient of the final state, or NULL.
- *   dr .. db    : device [B, T, H, N] outputs (no output may alias an input).
+ *   dr .. db    : device [B, T, H, N] outputs.  No output, nor the workspace, may
+ *                 share memory with an input or another output.
  *   dstate_in   : device [B, H, N, N], gradient of the initial state, or NULL.
  *   workspace   : yuf_wkv7_scan_backward_workspace(B, T, H, N) bytes.
  * With G_t the gradient of S_t:  G_t += dy_t r_t^T;  dr = S_t^T dy, dv = G k,
@@ -230,7 +231,8 @@ int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N,
  *   ddecay, ddirection: device [D]: of lambda (post-sigmoid) and of u as it
  *                       stands in H(x) = x - 2 (x.u) u (not renormalised);
  *                       zero for B = 0.
- *   dmemory_in        : device [B, D] or NULL.  No output may alias an input.
+ *   dmemory_in        : device [B, D] or NULL.  No output, nor the workspace, may
+ *                       share memory with an input or another output.
  *   workspace         : yuf_rosa_scan_backward_workspace(B, T, D) bytes.
  * Supported D: 1 .. 1024; B ceil(T / 32) below 2^22 (ceil(T / 16) for D > 256,
  * ceil(T / 8) for D > 512).
@@ -248,7 +250,8 @@ int yuf_rosa_scan_backward_f32(int B, int T, int D,
  * Dropout with a generated mask (the reference block's nn.Dropout,
  * yufmusicgen/config.py:82): out = (keep ? x / (1 - p) : 0) + residual.
  *   x, out   : device [n] fp32, or bf16 bit patterns; residual [n] or NULL.
- *              out may be x or residual.  Any element alignment.
+ *              out may be x or residual, but not a part of them.  Any element
+ *              alignment.
  *   p        : in [0, 1]; an element is dropped where its random word is below
  *              p 2^32 (p = 1: always).
  *   seed, counter, counter_dev : the mask: element i takes word i % 4 of
@@ -282,8 +285,8 @@ enum { YUF_LOSS_NONE = 0, YUF_LOSS_MEAN = 1, YUF_LOSS_SUM = 2 };
  *   dloss      : device, gradient of the loss: [M] without reduction, else [1];
  *                NULL for ones.
  *   dlogits    : device [M, V] of the logits' type, rows ld_out apart, or NULL;
- *                may be logits (then ld_out = ld).  Without rows a gradient alone
- *                writes nothing.
+ *                may be logits (then ld_out = ld), but not overlap them otherwise.
+ *                Without rows a gradient alone writes nothing.
  *   workspace  : yuf_cross_entropy_workspace(M) bytes for _MEAN and _SUM.
  * Exponentials and row sums in fp32, the sum over rows in fp64, in one order.
  */

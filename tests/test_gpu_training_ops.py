@@ -972,3 +972,20 @@ def test_rosa_gradients_of_saturated_inputs_are_finite():
     for gated in (True, False):
         for g in rosa_householder_scan_backward(cand, write, rr, vec, vec, torch.zeros(1, 64, device="cuda"), one, gated=gated):
             assert g is None or torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("side", [1, -1])
+def test_gradients_beside_their_logits(side):
+    """Logits and gradient in the two halves of one buffer's rows: of one stride, each between the other's."""
+    from yufmusicgen_amd._lib import check, lib
+    from yufmusicgen_amd.ops import cross_entropy_grad
+
+    logits, targets = loss_case(9, 67)
+    both = torch.full((9, 134), 7.0, device="cuda")
+    x, g = (both[:, :67], both[:, 67:]) if side > 0 else (both[:, 67:], both[:, :67])
+    x.copy_(logits)
+    loss, t = torch.empty(9, device="cuda"), targets.cuda()
+    check(lib().yuf_cross_entropy_f32(9, 67, x.data_ptr(), 134, t.data_ptr(), 64, -100, 0, loss.data_ptr(), None, g.data_ptr(), 134,
+                                      None, torch.cuda.current_stream().cuda_stream))
+    expect = cross_entropy_grad(logits.cuda(), t, reduction="none")
+    assert torch.equal(loss, expect[0]) and torch.equal(g, expect[1]) and torch.equal(x.cpu(), logits)

@@ -160,3 +160,55 @@ def test_scratch_of_refused_sizes_is_none():
         refused(call(*sizes, *full[:14], None, None), "blocks")
     for sizes in (((1 << 22) - 1, 32, 64), ((1 << 17) - 1, 1024, 256), ((1 << 16) - 1, 1024, 512)):
         assert space(*sizes) > 0, sizes
+
+
+def test_outputs_that_share_memory_are_refused():
+    """Not only an output that is an input: one that begins inside of it, or inside of the workspace."""
+    batch, steps, heads, size = 2, 16, 3, 40
+    token, state = 4 * batch * steps * heads * size, 4 * batch * heads * size * size
+    call, space = lib().yuf_wkv7_scan_backward_f32, lib().yuf_wkv7_scan_backward_workspace(batch, steps, heads, size)
+    # r, w, k, v, a, b, state, dy, dstate, then dr, dw, dk, dv, da, db, dstate_in, workspace.
+    sizes = [token] * 6 + [state, token, state] + [token] * 6 + [state, space]
+    at = [1 << 20]
+    for n in sizes:
+        at.append((at[-1] + n + 255) // 256 * 256)
+
+    def overlapping(out, other, by):
+        where = list(at[:17])
+        where[out] = at[other] + by
+        refused(call(batch, steps, heads, size, *where, None), "may not be")
+
+    for out in range(9, 17):
+        for other in (*range(9), *range(9, 17)):
+            if other != out:
+                overlapping(out, other, 0)
+                overlapping(out, other, (sizes[other] - 4) // 256 * 256)  # its last words
+                overlapping(out, other, -((sizes[out] - 4) // 256 * 256))  # the output's last words
+    batch, steps, dim = 2, 40, 64
+    token, memory, vec = 4 * batch * steps * dim, 4 * batch * dim, 4 * dim
+    call, space = lib().yuf_rosa_scan_backward_f32, lib().yuf_rosa_scan_backward_workspace(batch, steps, dim)
+    sizes = [token, token, token, vec, vec, memory, token, memory, token, token, token, vec, vec, memory, space]
+    at = [1 << 20]
+    for n in sizes:
+        at.append((at[-1] + n + 255) // 256 * 256)
+    for out in range(8, 15):
+        for other in range(15):
+            for by in (0, (sizes[other] - 4) // 256 * 256, -((sizes[out] - 4) // 256 * 256)):
+                if other != out:
+                    where = list(at[:15])
+                    where[out] = at[other] + by
+                    refused(call(batch, steps, dim, *where, None), "may not be")
+    for name, size in (("yuf_dropout_f32", 4), ("yuf_dropout_bf16", 2)):
+        call, n, x, far = getattr(lib(), name), 5000, 1 << 20, 1 << 22
+        for by in (size, n * size - size, -size, size - n * size):
+            refused(call(n, x, None, 0.5, 0, 0, None, x + by, None), "not a part")
+            refused(call(n, far, x, 0.5, 0, 0, None, x + by, None), "not a part")
+    for name, size in (("yuf_cross_entropy_f32", 4), ("yuf_cross_entropy_bf16", 2)):
+        call, rows, vocab, ld, x, far = getattr(lib(), name), 7, 50, 100, 1 << 20, 1 << 22
+
+        def grad(by, ld_out=ld):
+            return call(rows, vocab, x, ld, far, 64, -100, 0, far, None, x + by * size, ld_out, None, None)
+
+        for by in (1, 49, -1, -49, 51, -51, 99, 6 * 100 + 49, -6 * 100 - 49):
+            refused(grad(by), "not overlap")
+        refused(grad(50, 99), "not overlap")  # strides that differ: some row meets another

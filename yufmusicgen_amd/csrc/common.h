@@ -151,14 +151,22 @@ __device__ __forceinline__ void buf_store(float value, __amdgpu_buffer_rsrc_t rs
 // later loop (where it would also wait for prefetches issued in that loop).
 __device__ __forceinline__ void wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
-// Whether an output is an input or another output (the pointers themselves; null ones are none).
-template <int NI, int NO> inline bool outputs_alias(const void *const (&in)[NI], const void *const (&out)[NO]) {
+// A run of a call's memory; null or empty ones overlap nothing.
+struct Span {
+    const void *at;
+    size_t bytes;
+};
+inline bool overlap(const Span &a, const Span &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.at && b.at && a.bytes && b.bytes && (x < y ? y - x < a.bytes : x - y < b.bytes);
+}
+// Whether an output shares memory with an input or with another output.
+template <int NI, int NO> inline bool outputs_overlap(const Span (&in)[NI], const Span (&out)[NO]) {
     for (int o = 0; o < NO; ++o) {
-        if (!out[o]) continue;
-        for (const void *i : in)
-            if (i == out[o]) return true;
+        for (const Span &i : in)
+            if (overlap(i, out[o])) return true;
         for (int p = 0; p < o; ++p)
-            if (out[p] == out[o]) return true;
+            if (overlap(out[p], out[o])) return true;
     }
     return false;
 }

@@ -311,6 +311,16 @@ void launch_rows(const LossParams &p, hipStream_t s) {
     }
 }
 
+// Whether M rows of `bytes` at each of two places, a stride apart, share memory.  Rows of one stride may lie
+// between each other's; of two strides, places that reach into each other are taken to overlap.
+bool rows_overlap(int M, size_t bytes, const void *a, size_t stride_a, const void *b, size_t stride_b) {
+    if (!overlap({a, (M - 1) * stride_a + bytes}, {b, (M - 1) * stride_b + bytes})) return false;
+    if (stride_a != stride_b) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const size_t apart = (x < y ? y - x : x - y) % stride_a;
+    return apart < bytes || stride_a - apart < bytes;
+}
+
 template <typename T>
 int cross_entropy(int M, int V, const T *logits, int64_t ld, const void *targets, int target_bits, int64_t ignore,
                   int reduction, float *loss, const float *dloss, T *dlogits, int64_t ld_out, float *workspace,
@@ -327,6 +337,8 @@ int cross_entropy(int M, int V, const T *logits, int64_t ld, const void *targets
     if (!loss && !dlogits) return fail(YUF_ERR_INVALID, "cross entropy: neither a loss nor a gradient asked for");
     if (dlogits == logits && dlogits && ld_out != ld)
         return fail(YUF_ERR_INVALID, "cross entropy: a gradient in place of the logits has their row stride");
+    if (dlogits && dlogits != logits && M > 0 && rows_overlap(M, V * sizeof(T), logits, ld * sizeof(T), dlogits, ld_out * sizeof(T)))
+        return fail(YUF_ERR_INVALID, "cross entropy: the gradient may take the logits' place, but not overlap them otherwise");
     const bool reduced = reduction != YUF_LOSS_NONE;
     if (reduced && !workspace) return fail(YUF_ERR_INVALID, "cross entropy: mean and sum need the workspace");
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -125,6 +125,11 @@ int dropout(int64_t n, const T *x, const T *residual, double p, uint64_t seed, u
     if (!(p >= 0.0 && p <= 1.0)) return fail(YUF_ERR_INVALID, "dropout: p must be in [0, 1]");
     if (n == 0) return YUF_OK;
     if (!x || !out) return fail(YUF_ERR_INVALID, "dropout: null input/output pointer");
+    // A thread reads its elements, and no others, before it writes them.
+    const Span to{out, (size_t)n * sizeof(T)};
+    for (const T *from : {x, residual})
+        if (from != out && overlap({from, to.bytes}, to))
+            return fail(YUF_ERR_INVALID, "dropout: out may be x or residual, but not a part of them");
     constexpr int64_t kPerBlock = (int64_t)kThreads * kUnits * Vec<T>::kN;
     const int64_t blocks = (n + kPerBlock - 1) / kPerBlock;
     if (blocks * kThreads >= (int64_t)1 << 32) return fail(YUF_ERR_INVALID, "dropout: too many elements");  // threads of a launch

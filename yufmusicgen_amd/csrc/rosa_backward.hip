@@ -592,15 +592,16 @@ extern "C" int yuf_rosa_scan_backward_f32(int B, int T, int D, const float *cand
     const Cut cut = cut_of(T, D);
     if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "rosa backward: workspace must be 256-byte aligned");
     // The gradients of one block are written while another still reads the inputs.
-    if (B > 0 && outputs_alias<8, 6>({cand, write, read_raw, decay, direction, memory_in, dread, dmemory},
-                                     {dcand, dwrite, dread_raw, ddecay, ddirection, dmemory_in}))
-        return fail(YUF_ERR_INVALID, "rosa backward: an output may not be an input or another output");
+    const Scratch o = scratch_of(B, T, D);
+    const size_t tok = (size_t)B * T * D * sizeof(float), mem = (size_t)B * D * sizeof(float), vec = (size_t)D * sizeof(float);
+    if (outputs_overlap<8, 7>({{cand, tok}, {write, tok}, {read_raw, tok}, {decay, vec}, {direction, vec}, {memory_in, mem}, {dread, tok}, {dmemory, mem}},
+                              {{dcand, tok}, {dwrite, tok}, {dread_raw, tok}, {ddecay, vec}, {ddirection, vec}, {dmemory_in, mem}, {workspace, o.bytes}}))
+        return fail(YUF_ERR_INVALID, "rosa backward: an output or the workspace may not be (a part of) an input or another output");
     RosaGradParams p{};
     p.B = B; p.T = T; p.D = D; p.S = cut.S; p.R = cut.R; p.NR = cut.NR;
     p.cand = cand; p.write = write; p.read_raw = read_raw; p.decay = decay; p.direction = direction;
     p.memory_in = memory_in; p.dread = dread; p.dmemory = dmemory;
     p.dcand = dcand; p.dwrite = dwrite; p.dread_raw = dread_raw; p.dmemory_in = dmemory_in;
-    const Scratch o = scratch_of(B, T, D);
     char *base = static_cast<char *>(workspace);
     p.sums = reinterpret_cast<double *>(base + o.sums);
     p.fwd = reinterpret_cast<float *>(base + o.fwd);

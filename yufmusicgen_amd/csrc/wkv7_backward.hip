@@ -1066,14 +1066,16 @@ extern "C" int yuf_wkv7_scan_backward_f32(int B, int T, int H, int N, const floa
     if (!workspace) return fail(YUF_ERR_INVALID, "wkv7 backward: null workspace");
     if (!scratch_aligned(workspace)) return fail(YUF_ERR_INVALID, "wkv7 backward: workspace must be 256-byte aligned");
     // The gradients of one segment are written while another still reads the inputs.
-    if (outputs_alias<9, 7>({r, w_raw, k, v, a, b, state_in, dy, dstate_out}, {dr, dw_raw, dk, dv, da, db, dstate_in}))
-        return fail(YUF_ERR_INVALID, "wkv7 backward: an output may not be an input or another output");
+    const Scratch o = scratch_of(B, T, H, N);
+    const size_t tok = (size_t)B * T * H * N * sizeof(float), st = (size_t)B * H * N * N * sizeof(float);
+    if (outputs_overlap<9, 8>({{r, tok}, {w_raw, tok}, {k, tok}, {v, tok}, {a, tok}, {b, tok}, {state_in, st}, {dy, tok}, {dstate_out, st}},
+                              {{dr, tok}, {dw_raw, tok}, {dk, tok}, {dv, tok}, {da, tok}, {db, tok}, {dstate_in, st}, {workspace, o.bytes}}))
+        return fail(YUF_ERR_INVALID, "wkv7 backward: an output or the workspace may not be (a part of) an input or another output");
     GradParams p{};
     p.B = B; p.T = T; p.H = H; p.N = N; p.chunks = T / kC + (T % kC != 0);
     p.r = r; p.w = w_raw; p.k = k; p.v = v; p.a = a; p.b = b; p.dy = dy;
     p.state_in = state_in; p.dstate_out = dstate_out;
     p.dr = dr; p.dw = dw_raw; p.dk = dk; p.dv = dv; p.da = da; p.db = db; p.dstate_in = dstate_in;
-    const Scratch o = scratch_of(B, T, H, N);
     char *base = static_cast<char *>(workspace);
     p.frags = reinterpret_cast<float *>(base + o.frags);
     p.states = reinterpret_cast<float *>(base + o.states);
