@@ -989,3 +989,21 @@ def test_gradients_beside_their_logits(side):
                                       None, torch.cuda.current_stream().cuda_stream))
     expect = cross_entropy_grad(logits.cuda(), t, reduction="none")
     assert torch.equal(loss, expect[0]) and torch.equal(g, expect[1]) and torch.equal(x.cpu(), logits)
+
+
+@pytest.mark.parametrize("rows", [(1 << 31) - 1, (1 << 31) - 8193])
+def test_cross_entropy_of_the_most_rows(rows):
+    """Up to 2^31 - 1 rows (26 GB with their scratch): where the rows are counted and summed, steps end beyond the
+    last one.  All but the first three and the last five are ignored, and each of those is one of two equal logits."""
+    from yufmusicgen_amd.ops import cross_entropy_grad
+
+    x = torch.zeros(rows, 2, device="cuda", dtype=torch.bfloat16)
+    t = torch.full((rows,), -100, device="cuda", dtype=torch.int32)
+    t[:3], t[-5:] = 0, 1
+    for reduction, scale in (("mean", 8), ("sum", 1)):
+        loss, grad = cross_entropy_grad(x, t, reduction=reduction, inplace=True)
+        assert abs(loss.item() - np.log(2) * 8 / scale) <= 60 * EPS32 * 8 / scale
+        assert (grad[:3] == torch.tensor([-0.5, 0.5], device="cuda") / scale).all()
+        assert (grad[-5:] == torch.tensor([0.5, -0.5], device="cuda") / scale).all()
+        assert not grad[3:4096].any() and not grad[-(1 << 20) : -5].any()
+        x.zero_()

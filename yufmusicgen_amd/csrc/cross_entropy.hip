@@ -85,15 +85,16 @@ __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 
 // all of them is `all` (its sum is 0 and has to stay so where it saw no finite logit).
 __device__ __forceinline__ float rescale(float m, float all) { return m == -INFINITY ? 0.0f : expf(m - all); }
 
-template <typename I> __device__ __forceinline__ int count_mine(const I *targets, int M, int64_t ignore) {
+template <typename I> __device__ __forceinline__ int count_mine(const I *targets, uint32_t M, int64_t ignore) {
     int mine = 0;
-    // kBatch loads in flight: one at a time, each waits for memory (16384 rows: 10.5 us, so 6.2).
-    for (int i0 = threadIdx.x; i0 < M; i0 += kBatch * blockDim.x) {
+    // kBatch loads in flight: one at a time, each waits for memory (16384 rows: 10.5 us, so 6.2).  Unsigned,
+    // since the last step goes beyond M, which may be 2^31 - 1.
+    for (uint32_t i0 = threadIdx.x; i0 < M; i0 += kBatch * blockDim.x) {
         I t[kBatch];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) t[e] = targets[min(i0 + e * (int)blockDim.x, M - 1)];
+        for (int e = 0; e < kBatch; ++e) t[e] = targets[min(i0 + e * blockDim.x, M - 1)];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) mine += i0 + e * (int)blockDim.x < M && (int64_t)t[e] != ignore;
+        for (int e = 0; e < kBatch; ++e) mine += i0 + e * blockDim.x < M && (int64_t)t[e] != ignore;
     }
     return mine;
 }
@@ -262,12 +263,13 @@ __global__ void __launch_bounds__(kReduceThreads) loss_sum_kernel(LossParams p, 
     __shared__ double sums[kReduceThreads / kWave];
     __shared__ int partial[kReduceThreads / kWave];
     double s = 0.0;
-    for (int i0 = threadIdx.x; i0 < p.M; i0 += kBatch * kReduceThreads) {
+    const uint32_t M = p.M;  // unsigned, as where the rows are counted
+    for (uint32_t i0 = threadIdx.x; i0 < M; i0 += kBatch * kReduceThreads) {
         float v[kBatch];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) v[e] = p.row_loss[min(i0 + e * kReduceThreads, p.M - 1)];
+        for (int e = 0; e < kBatch; ++e) v[e] = p.row_loss[min(i0 + e * kReduceThreads, M - 1)];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) s += i0 + e * kReduceThreads < p.M ? (double)v[e] : 0.0;
+        for (int e = 0; e < kBatch; ++e) s += i0 + e * kReduceThreads < M ? (double)v[e] : 0.0;
     }
     s = wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
