@@ -212,3 +212,46 @@ def test_outputs_that_share_memory_are_refused():
         for by in (1, 49, -1, -49, 51, -51, 99, 6 * 100 + 49, -6 * 100 - 49):
             refused(grad(by), "not overlap")
         refused(grad(50, 99), "not overlap")  # strides that differ: some row meets another
+
+
+def test_scans_refuse_vectors_of_other_sizes():
+    """The kernels read D elements of decay and direction and B D of the memory: fewer lie beyond their ends."""
+    seq, vec, memory = torch.zeros(2, 4, 64), torch.zeros(64), torch.zeros(2, 64)
+    for what, args in (("decay", (vec[:1], vec, memory)), ("decay", (vec[0], vec, memory)),
+                       ("direction", (vec, vec[:63], memory)), ("direction", (vec, memory, memory)),
+                       ("memory", (vec, vec, memory[:1])), ("memory", (vec, vec, torch.zeros(3, 64)))):
+        with pytest.raises(ValueError, match=f"ROSA {what} must have"):
+            ops.rosa_householder_scan(seq, seq, seq, *args)
+    with pytest.raises(ValueError, match="GPU"):  # their own sizes, in any shape
+        ops.rosa_householder_scan(seq, seq, seq, vec.reshape(1, 64), vec.reshape(64, 1), memory.reshape(128))
+
+
+def test_operators_refuse_tensors_of_two_gpus():
+    """Stand-ins for tensors of two GPUs: each input in turn on the other one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def on(k, *shapes):
+            return [torch.empty(*s, device=f"cuda:{int(i == k)}") for i, s in enumerate(shapes)]
+
+        token, vec, state = (1, 4, 2, 40), (64,), (1, 2, 40, 40)
+        for k in range(1, 7):
+            *x, s = on(k, *[token] * 6, state)
+            with pytest.raises(ValueError, match="same GPU"):
+                ops.rwkv7_scan(*x, state=s)
+        for k in range(1, 9):
+            *x, s, ds = on(k, *[token] * 7, state, state)
+            with pytest.raises(ValueError, match="inputs' GPU"):
+                ops.rwkv7_scan_backward(*x, state=s, dstate=ds)
+        seq, memory = (1, 4, 64), (1, 64)
+        for k in range(1, 6):
+            with pytest.raises(ValueError, match="same GPU"):
+                ops.rosa_householder_scan(*on(k, seq, seq, seq, vec, vec, memory))
+        for k in range(1, 8):
+            with pytest.raises(ValueError, match="inputs' GPU"):
+                ops.rosa_householder_scan_backward(*on(k, seq, seq, seq, vec, vec, memory, seq, memory))
+        x, other = on(1, (3, 5), (3, 5))
+        with pytest.raises(ValueError, match="inputs' GPU"):
+            ops.dropout(x, 0.5, 1, residual=other)
+        with pytest.raises(ValueError, match="same GPU"):
+            ops.cross_entropy(x, torch.empty(3, dtype=torch.int64, device="cuda:1"))

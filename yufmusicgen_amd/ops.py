@@ -63,6 +63,11 @@ def _not_captured(name: str) -> None:
         raise RuntimeError(f"{name}: backward() cannot be captured into a graph; capture the gradient operators")
 
 
+def _check_one_device(name: str, first, *others) -> None:
+    if any(x is not None and x.device != first.device for x in others):
+        raise ValueError(f"{name} must be on the same GPU")
+
+
 def _check_like(name: str, x, shape, device, dtype=torch.float32) -> None:
     if not x.is_cuda or x.device != device:
         raise ValueError(f"{name} must be on the inputs' GPU")
@@ -97,6 +102,7 @@ def rwkv7_scan(r, w, k, v, a, b, state=None):
         if state.shape != (batch, heads, size, size) or state.dtype != torch.float32 or not state.is_cuda:
             raise ValueError("state must be a float32 GPU tensor of shape [B, H, N, N]")
         state = state.contiguous()
+    _check_one_device("RWKV-7 inputs", *tensors, state)
     if _needs_grad(*tensors, state):
         return _Rwkv7Scan.apply(*tensors, state)
     return _rwkv7_forward(*tensors, state)
@@ -128,11 +134,15 @@ def rosa_householder_scan(cand, write, read_raw, decay, direction, memory, gated
         raise ValueError("ROSA per-step inputs must have shape [B, T, D]")
     if len({tuple(x.shape) for x in (cand, write, read_raw)}) != 1:
         raise ValueError("ROSA per-step inputs must have identical shapes")
+    batch, _, dim = cand.shape
+    for name, x, elements in (("decay", decay, dim), ("direction", direction, dim), ("memory", memory, batch * dim)):
+        if x.numel() != elements:
+            raise ValueError(f"ROSA {name} must have {elements} elements, got shape {list(x.shape)}")
     tensors = [x.float().contiguous() for x in (cand, write, read_raw, decay, direction, memory)]
     if not all(x.is_cuda for x in tensors):
         raise ValueError("ROSA inputs must be on the GPU")
+    _check_one_device("ROSA inputs", *tensors)
     if _needs_grad(*tensors):
-        batch, _, dim = cand.shape
         cand, write, read_raw, decay, direction, memory = tensors
         return _RosaScan.apply(cand, write, read_raw, decay.reshape(dim), direction.reshape(dim),
                                memory.reshape(batch, dim), gated)
