@@ -1007,3 +1007,13 @@ def test_cross_entropy_of_the_most_rows(rows):
         assert (grad[-5:] == torch.tensor([0.5, -0.5], device="cuda") / scale).all()
         assert not grad[3:4096].any() and not grad[-(1 << 20) : -5].any()
         x.zero_()
+
+
+def test_philox_words_of_published_counters_and_keys():
+    """The generator's other two published known answers: every bit of counter and key set, and words that all
+    differ (digits of pi), which pin the order of the counter's and the key's words."""
+    for (block, counter, seed), words in (
+        ((2**64 - 1, 2**64 - 1, 2**64 - 1), "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+        ((0x85A308D3243F6A88, 0x0370734413198A2E, 0x299F31D0A4093822), "d16cfe09 94fdcceb 5001e420 24126ea1"),
+    ):
+        assert " ".join(f"{w:08x}" for w in philox_block(block, counter, seed)) == words
