@@ -1017,3 +1017,63 @@ def test_philox_words_of_published_counters_and_keys():
         ((0x85A308D3243F6A88, 0x0370734413198A2E, 0x299F31D0A4093822), "d16cfe09 94fdcceb 5001e420 24126ea1"),
     ):
         assert " ".join(f"{w:08x}" for w in philox_block(block, counter, seed)) == words
+
+
+def test_autograd_over_no_tokens_and_no_sequences():
+    """The scans, dropout and their backward passes over empty tensors: the carried state's gradient passes through."""
+    from yufmusicgen_amd import ops
+
+    for batch, steps in ((2, 0), (0, 5)):
+        x = [torch.empty(batch, steps, 3, 40, device="cuda", requires_grad=True) for _ in range(6)]
+        state = torch.randn(batch, 3, 40, 40, device="cuda", requires_grad=True)
+        y, final = ops.rwkv7_scan(*x, state=state)
+        dfinal = torch.randn_like(final)
+        grads = torch.autograd.grad((y, final), [*x, state], (torch.ones_like(y), dfinal))
+        assert torch.equal(final, state) and torch.equal(grads[6], dfinal) and all(g.shape == z.shape for g, z in zip(grads, x))
+        seq = [torch.empty(batch, steps, 64, device="cuda", requires_grad=True) for _ in range(3)]
+        vec = [torch.full((64,), 0.125, device="cuda", requires_grad=True) for _ in range(2)]
+        memory = torch.randn(batch, 64, device="cuda", requires_grad=True)
+        read, last = ops.rosa_householder_scan(*seq, *vec, memory, gated=True)
+        dlast = torch.randn_like(last)
+        grads = torch.autograd.grad((read, last), [*seq, *vec, memory], (torch.ones_like(read), dlast))
+        assert torch.equal(last, memory) and torch.equal(grads[5], dlast) and not grads[3].any() and not grads[4].any()
+    h = torch.empty(0, 7, device="cuda", requires_grad=True)
+    ops.dropout(h, 0.5, 1, residual=h).sum().backward()
+    assert h.grad.shape == (0, 7)
+
+
+@pytest.mark.parametrize("batch,steps,heads,size", [(700, 3, 8, 32), (40, 17, 33, 128), (1, 9, 2000, 8)])
+def test_wkv7_gradients_of_more_heads_than_segments(batch, steps, heads, size):
+    """More than 1024 heads, one segment each: the last ones' gradients are those of the last ones alone."""
+    print(f"wkv7 gradients {batch} x {steps} x {heads} x {size}", flush=True)
+    arrs, s0, dy, ds = wkv_case(size, batch, steps, heads, size)
+    many = wkv_grads(arrs, s0, dy, ds)
+    alone = wkv_grads([x[-1:, :, -2:] for x in arrs], s0[-1:, -2:], dy[-1:, :, -2:], ds[-1:, -2:])
+    for name, m, x in zip(WKV_NAMES, many, alone):
+        close(m[-1:, -2:] if name == "state" else m[-1:, :, -2:], x, 2 * (size + 32), name)
+
+
+@pytest.mark.parametrize("dim", [64, 300, 700])
+def test_rosa_gradients_of_many_sequences(dim):
+    from yufmusicgen_amd.ops import rosa_householder_scan_backward
+
+    batch, steps = 1500, 40
+    arrs, dread, dmem = rosa_case(dim, batch, steps, dim)
+    cand, write, rr, decay, u, memory = (cuda(x) for x in arrs)
+    many = rosa_householder_scan_backward(cand, write, rr, decay, u, memory, cuda(dread), cuda(dmem), gated=True)
+    cut = slice(batch - 3, None)
+    alone = rosa_householder_scan_backward(cand[cut], write[cut], rr[cut], decay, u, memory[cut], cuda(dread)[cut],
+                                           cuda(dmem)[cut], gated=True)
+    for i in (0, 1, 2, 5):
+        assert torch.equal(many[i][cut], alone[i]), ROSA_NAMES[i]
+
+
+def test_gradient_over_logits_in_inference_mode():
+    from yufmusicgen_amd.ops import cross_entropy_grad
+
+    logits, targets = loss_case(6, 100)
+    expect = cross_entropy_grad(logits.cuda(), targets.cuda())
+    with torch.inference_mode():
+        x = logits.cuda()
+        loss, grad = cross_entropy_grad(x, targets.cuda(), inplace=True)
+        assert grad is x and torch.equal(grad, expect[1]) and torch.equal(loss, expect[0])

@@ -255,3 +255,12 @@ def test_operators_refuse_tensors_of_two_gpus():
             ops.dropout(x, 0.5, 1, residual=other)
         with pytest.raises(ValueError, match="same GPU"):
             ops.cross_entropy(x, torch.empty(3, dtype=torch.int64, device="cuda:1"))
+
+
+def test_scans_of_no_sequences():
+    """An empty batch's tensors are null: nothing to do, for the scans as for their gradients."""
+    assert lib().yuf_wkv7_scan_f32(0, 5, 3, 40, *[None] * 10) == 0 and lib().yuf_wkv7_scan_f32(5, 5, 0, 40, *[None] * 10) == 0
+    for name in ("yuf_rosa_scan_f32", "yuf_rosa_scan_f32_noalloc"):
+        assert getattr(lib(), name)(0, 5, 64, None, None, None, DUMMY, DUMMY, *[None] * 4) == 0
+    refused(lib().yuf_wkv7_scan_f32(1, 5, 3, 40, *[None] * 10), "null")
+    refused(lib().yuf_rosa_scan_f32(1, 5, 64, None, None, None, DUMMY, DUMMY, *[None] * 4), "null")

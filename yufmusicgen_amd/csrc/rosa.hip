@@ -1166,7 +1166,7 @@ int rosa_operator(int B, int T, int D, const float *cand, const float *write, co
     if (B < 0 || T < 0) return fail(YUF_ERR_INVALID, "rosa: negative size");
     if (D < 1 || D > 1024) return fail(YUF_ERR_INVALID, "rosa: D must be in [1, 1024], got " + std::to_string(D));
     if (!decay || !direction) return fail(YUF_ERR_INVALID, "rosa: null decay/direction");
-    if (T > 0 && (!cand || !write || !read_out)) return fail(YUF_ERR_INVALID, "rosa: null input/output pointer");
+    if (B > 0 && T > 0 && (!cand || !write || !read_out)) return fail(YUF_ERR_INVALID, "rosa: null input/output pointer");
     RosaParams p;
     p.B = B; p.T = T; p.D = D; p.ld = D;
     p.cand = cand; p.write = write; p.read_raw = read_raw;

@@ -614,7 +614,7 @@ extern "C" int yuf_wkv7_scan_f32(int B, int T, int H, int N, const float *r, con
     using namespace yuf;
     if (B < 0 || T < 0 || H < 0) return fail(YUF_ERR_INVALID, "wkv7: negative size");
     if (!wkv7_supported(N)) return fail(YUF_ERR_INVALID, "wkv7: unsupported head size N=" + std::to_string(N));
-    if (T > 0 && (!r || !w_raw || !k || !v || !a || !b || !y))
+    if (B > 0 && T > 0 && H > 0 && (!r || !w_raw || !k || !v || !a || !b || !y))
         return fail(YUF_ERR_INVALID, "wkv7: null input/output pointer");
     WkvParams p;
     p.B = B; p.T = T; p.H = H;
