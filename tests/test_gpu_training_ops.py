@@ -1077,3 +1077,18 @@ def test_gradient_over_logits_in_inference_mode():
         x = logits.cuda()
         loss, grad = cross_entropy_grad(x, targets.cuda(), inplace=True)
         assert grad is x and torch.equal(grad, expect[1]) and torch.equal(loss, expect[0])
+
+
+@pytest.mark.parametrize("rows,vocab", [(8192, 33), (8193, 33), (2048, 1100), (2049, 1100), (1024, 5000), (1025, 5000),
+                                        (512, 10300), (513, 10300)])
+def test_cross_entropy_where_rows_are_counted_apart(rows, vocab):
+    """As many rows as the workgroups count by themselves, and one more, for each number of a row's waves."""
+    from yufmusicgen_amd.ops import cross_entropy, cross_entropy_grad
+
+    print(f"cross entropy count {rows} x {vocab}", flush=True)
+    logits, targets = loss_case(rows, vocab, ignored=0.4)
+    got = cross_entropy_grad(logits.cuda(), targets.cuda())
+    loss_close(got, loss_exact(logits, targets, -100, "mean"), torch.float32, vocab)
+    x = logits.cuda().requires_grad_()
+    loss = cross_entropy(x, targets.cuda())
+    assert torch.equal(loss, got[0]) and torch.equal(torch.autograd.grad(loss, x)[0], got[1])

@@ -23,7 +23,11 @@ constexpr int kWave = 64;
 constexpr int kRowsPerWg = 4;    // rows of a workgroup where a row is one wave
 constexpr int kMaxWaves = 16;
 constexpr int kBatch = 8;        // loads of a lane in flight where rows are counted and summed
-constexpr int kCountInline = 4096;  // up to so many rows each workgroup counts the valid targets itself
+// Up to kCountInline / (a row's waves) rows each workgroup counts the valid targets itself.  The whole call so
+// and with a count before it, rows x vocabulary: a wave, 673: 6144 17.5 and 20.0, 8192 20.2 and 20.2, 16384 44 and
+// 25 us; 4 waves, 2048: 2048 17.1 and 19.9, 4096 22.8 and 21.5; 8 waves, 20480 bf16: 1024 33.3 and 33.6,
+// 2048 54 and 52; 16 waves, 20480: 512 26.6 and 25.9, 1024 47 and 42, 4096 171 and 151.
+constexpr int kCountInline = 8192;
 
 // Vectors with the alignment of their elements: a row of an odd vocabulary starts anywhere.
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
@@ -295,14 +299,17 @@ void launch_form(LossParams p, hipStream_t s) {
 }
 
 // The fewest waves whose registers hold the row.
+int row_waves(int vecs) { return vecs <= 4 * kWave ? 1 : vecs <= 4 * 4 * kWave ? 4 : vecs <= 8 * 5 * kWave ? 8 : 16; }
+template <typename T> int row_vecs(int V) { return (V + Vec<T>::kN - 1) / Vec<T>::kN; }
+
 template <typename T>
 void launch_rows(const LossParams &p, hipStream_t s) {
-    const int vecs = (p.V + Vec<T>::kN - 1) / Vec<T>::kN;
+    const int vecs = row_vecs<T>(p.V), waves = row_waves(vecs);
     if (vecs <= 1 * kWave) launch_form<T, 1, 1>(p, s);
     else if (vecs <= 2 * kWave) launch_form<T, 1, 2>(p, s);
-    else if (vecs <= 4 * kWave) launch_form<T, 1, 4>(p, s);
-    else if (vecs <= 4 * 4 * kWave) launch_form<T, 4, 4>(p, s);
-    else if (vecs <= 8 * 5 * kWave) launch_form<T, 8, 5>(p, s);
+    else if (waves == 1) launch_form<T, 1, 4>(p, s);
+    else if (waves == 4) launch_form<T, 4, 4>(p, s);
+    else if (waves == 8) launch_form<T, 8, 5>(p, s);
     else if (vecs <= 16 * 5 * kWave) launch_form<T, 16, 5>(p, s);
     else if (vecs <= 16 * 8 * kWave) launch_form<T, 16, 8>(p, s);
     else {
@@ -351,7 +358,7 @@ int cross_entropy(int M, int V, const T *logits, int64_t ld, const void *targets
     p.row_loss = loss ? (reduced ? workspace + 1 : loss) : nullptr;
     p.dloss = dloss; p.dlogits = dlogits; p.ld_out = ld_out;
     // A mean's gradient needs the number of rows before any is written.
-    if (reduction == YUF_LOSS_MEAN && M > kCountInline) {
+    if (reduction == YUF_LOSS_MEAN && M > kCountInline / row_waves(row_vecs<T>(V))) {
         hipLaunchKernelGGL(loss_count_kernel, dim3(1), dim3(kReduceThreads), 0, s, p, workspace);
         p.count = workspace;
     }
