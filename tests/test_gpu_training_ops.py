@@ -1092,3 +1092,30 @@ def test_cross_entropy_where_rows_are_counted_apart(rows, vocab):
     x = logits.cuda().requires_grad_()
     loss = cross_entropy(x, targets.cuda())
     assert torch.equal(loss, got[0]) and torch.equal(torch.autograd.grad(loss, x)[0], got[1])
+
+
+@pytest.mark.parametrize("blocks", [128, 129, 768, 769, 4096, 4097, 12288, 12289])
+def test_rosa_gradients_at_the_limits_of_the_ranges(blocks):
+    """The longest sequences of each range length and the next ones, by pieces of other cuts joined by the memory and
+    its gradient (decay's and direction's sums over all tokens in fp64)."""
+    from yufmusicgen_amd.ops import rosa_householder_scan, rosa_householder_scan_backward
+
+    steps, dim = 32 * blocks - 5, 24
+    print(f"rosa gradients of {blocks} blocks", flush=True)
+    arrs, dread, dmem = rosa_case(7, 1, steps, dim)
+    *seq, decay, u, memory = (cuda(x) for x in arrs)
+    dread, dmem = cuda(dread), cuda(dmem)
+    whole = rosa_householder_scan_backward(*seq, decay, u, memory, dread, dmem, gated=True)
+    cuts = [0, steps // 3 + 1, steps * 3 // 4, steps]
+    pieces = [slice(a, b) for a, b in zip(cuts, cuts[1:])]
+    starts = [memory]
+    for piece in pieces[:-1]:
+        starts.append(rosa_householder_scan(*(x[:, piece] for x in seq), decay, u, starts[-1], gated=True)[1])
+    parts, end = [], dmem
+    for piece, start in zip(pieces[::-1], starts[::-1]):
+        parts.append(rosa_householder_scan_backward(*(x[:, piece] for x in seq), decay, u, start, dread[:, piece], end, gated=True))
+        end = parts[-1][5]
+    parts = parts[::-1]
+    for i, name in enumerate(ROSA_NAMES):
+        joined = torch.cat([p[i] for p in parts], 1) if i < 3 else sum(p[i].double() for p in parts) if i < 5 else end
+        close(whole[i], joined, 2 * (dim + 32), name)  # the errors of both

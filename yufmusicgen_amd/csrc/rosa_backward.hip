@@ -505,9 +505,17 @@ __global__ void __launch_bounds__(1024) rosa_grad_sum_kernel(const double *sums,
 
 int epl_of(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : D <= 512 ? 8 : 16; }
 
-// Blocks of a sequence and of a range.  A range costs the carry a step (0.33 us at D = 128) and its blocks
-// cost the local pass and the walk a block (about 3 us with its neighbours beside it) each, so R grows with
-// the sequence; without a walk up to 128 blocks.
+// Blocks of a sequence and of a range.  A range costs the carry a step (0.33 us at D = 128) and each of its
+// blocks costs the local pass and the walk, which one-block ranges need not, one (12 us together): R grows as
+// the root of the sequence.  The whole call, one sequence of D = 128 with the gate, us:
+//     blocks    128   160   256   512   768  1024  2048  3072  4096  8192 16384
+//     R = 1      65    75   105   188   275   360
+//     R = 4      80    84    92   117   145   172   280   440   550
+//     R = 8     124   126   131   152   167   183   245   327   403   827
+//     R = 16    219   221   224   247   259   271   313   368   411   689  1429
+//     R = 32    412   413   417   453   464   474   516   558   588   811  1283
+// R = 2 gains 5 to 13 us on both up to 256.  D = 64 and 256 cross at the same places.  Eight sequences, whose
+// blocks fill the GPU, are within 5 % from R = 4 to 16 (512 blocks: 316, 282, 269, 346, 559).
 struct Cut {
     int S, R, NR;
 };
@@ -515,7 +523,7 @@ Cut cut_of(int T, int D) {
     const int tok = block_tokens(epl_of(D));
     Cut c{};
     c.S = std::max(1, T / tok + (T % tok != 0));
-    c.R = D > kMaxCarryDim ? c.S : c.S <= 128 ? 1 : c.S <= 1024 ? 8 : 32;
+    c.R = D > kMaxCarryDim ? c.S : c.S <= 128 ? 1 : c.S <= 768 ? 4 : c.S <= 4096 ? 8 : c.S <= 12288 ? 16 : 32;
     c.NR = (c.S + c.R - 1) / c.R;
     return c;
 }
