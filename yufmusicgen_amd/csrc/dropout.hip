@@ -11,8 +11,9 @@
 // Bound: memory, 8 or 12 bytes an element in fp32 (half of it in bf16).  Philox costs
 // 20 32 x 32 -> 64-bit products per four elements.  A thread handles kUnits groups
 // of a 16-byte vector, all loads issued before the first product.  16384 x 640 fp32
-// with the residual: 19.4 us = 6.5 TB/s, as long as an addition of the two tensors
-// (they fit the memory-side cache).
+// with the residual: 19.0 us = 6.6 TB/s, as long as an addition of the two tensors
+// (they fit the memory-side cache).  In bf16 the products are twice as many per byte and bound it:
+// 14.8 us with the residual, 12.4 without (an addition: 10.1).
 #include "common.h"
 
 #include <cmath>

@@ -22,9 +22,10 @@
 //   5  those sums over the blocks, in fp64 and one order.
 // With R = 1 the carry's states are the blocks' and 3 is left out; with one range (D > 256, whose
 // power does not fit a workgroup's registers) 1 and 2 are, and a sequence of one block is 4 and 5.
-// 8 x 2048 x 128 with the gate (64 blocks a sequence): 13.0 + 22.6 + 22.2 + 4.1 us, 59 MB at 0.95 TB/s;
-// 3 x 777 x 256: 11.0 + 22.1 + 18.5 + 4.0.  Whole segments of 64 tokens by one wave, elementwise parts
-// included, took 39 + 12.6 + 93 + 6.4 us of the former.
+// 8 x 2048 x 128 with the gate (64 blocks a sequence): 12.6 + 22.2 + 16.4 + 4.0 us, 59 MB at 1.08 TB/s;
+// 3 x 777 x 256: 11.9 + 21.6 + 16.6 + 3.8.  Whole segments of 64 tokens by one wave, elementwise parts
+// included, took 39 + 12.6 + 93 + 6.4 us of the former.  D > 256 goes token by token along the whole sequence, twice:
+// 1 x 2048 x 512 1.22 ms, x 1024 2.37 ms (eight sequences 1.35 and 3.23).
 #include "common.h"
 #include "kernels.h"
 

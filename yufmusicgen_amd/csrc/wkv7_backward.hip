@@ -44,10 +44,11 @@
 // One segment needs the first and the last alone, two no carry.  Four-chunk segments take the first two
 // as one (wkv7_grad_block_kernel, block_form).
 //
-// 8 x 2048 x 16 x 40 (four segments): 77 + 136 + 6 + 341 us; 3 x 777 x 16 x 64 (ten): 16 + 46 + 18 + 66;
-// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 55.  The first is bound by memory (300 MB at 3.9
-// TB/s), the second and the last by their SIMDs' issue: an fp32 MFMA takes 32 cycles of one, a VALU instruction 4 and a 16-byte
-// LDS read about 18, none beside another, and a wave's chunk in the last kernel has 266 of the first at N = 64.
+// 8 x 2048 x 16 x 40 (four segments): 76 + 128 + 6 + 358 us; 3 x 777 x 16 x 64 (ten): 17 + 44 + 17 + 66;
+// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 57.  The first kernel is bound by memory (200 MB at 2.7
+// TB/s, its writes half of them), the second and the last by latency and issue together: an fp32 MFMA takes 32
+// cycles of a SIMD, a VALU instruction 4 and a 16-byte LDS read about 18, none beside another, and with two waves a
+// SIMD at most nothing else fills a wave's waits.
 //
 // MFMA layouts (16x16x4 f32; lane l, g = l / 16, li = l % 16): A[m = li][k = g],
 // B[k = g][n = li], register r of the result D[m = 4 g + r][n = li].  k-step r of a
@@ -779,9 +780,11 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_carry_k
     }
 }
 
-// A workgroup of NB waves per segment of a head.  Two waves per SIMD saturate it (the fp32 MFMAs, the VALU
-// and LDS instructions of a SIMD go one after the other: 60, 15 and 15 % of its time), and scheduled for two
-// instead of three the operands come from LDS in time: 8 x 2048 x 16 x 40 360 us, so 345.
+// A workgroup of NB waves per segment of a head.  Scheduled for two waves per SIMD instead of three the operands
+// come from LDS in time: the call of 8 x 2048 x 16 x 40 600 us, so 569.  By counters a SIMD's time goes, at N = 64 with
+// two waves on each (1 x 2048 x 16 x 64), 42 % to MFMAs, 11 to VALU and 12 to LDS instructions; at N = 40 (8 x 2048 x
+// 16), whose two three-wave workgroups leave two of a CU's SIMDs with one wave, 36, 10 and 10 on average and 48, 14 and 14
+// on the other two, and a wave waits 38 % of its time for memory, LDS and barriers.
 template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) wkv7_grad_kernel(GradParams p, int units, int per_xcd) {
     constexpr int NP = 16 * NB, SA = NP + 4, kTok = kC * SA;
     // Backward: B, K, V, Y', U, E, G [value][key] and the four 16 x 16 gradients.
@@ -948,10 +951,10 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
 
 // Whether the segments' local pass and the chunks' matrices are one kernel: four-chunk segments (at most 1024,
 // segment_chunks), and for N > 64, whose LDS leaves room for one a CU, at most 256 of them.  The whole call without
-// it and with it, one sequence of 2048 tokens in 256 / 512 / 768 / 1024 segments: N = 16 39 / 43 / 50 / 63 and
-// 34 / 38 / 44 / 47 us; N = 40 66 / 91 / 142 / 153 and 58 / 85 / 133 / 152; N = 64 87 / 130 / 193 / 224 and
-// 78 / 110 / 169 / 216; N = 128 241 / 368 / 559 / 668 and 210 / 376 / 588 / 759.  (512 tokens, 1024 segments of
-// N = 40: 137 and 143.)
+// it and with it, one sequence of 2048 tokens in 256 / 512 / 768 / 1024 segments: N = 16 40 / 44 / 51 / 65 and
+// 36 / 40 / 45 / 47 us; N = 40 67 / 93 / 144 / 154 and 59 / 87 / 135 / 154; N = 64 89 / 133 / 199 / 224 and
+// 79 / 112 / 175 / 216; N = 128 243 / 374 / 567 / 676 and 212 / 383 / 596 / 769.  (512 tokens, 1024 segments of
+// N = 40: 139 and 144.)
 bool block_form(int64_t heads, int segments, int seg_chunks, int N) {
     return segments > 1 && seg_chunks == kBlock && (N <= 64 || heads * segments <= 256);
 }
@@ -960,8 +963,8 @@ bool block_form(int64_t heads, int segments, int seg_chunks, int N) {
 // workgroups of c chunks, a third longer alone on it (5.6 us a chunk at N = 40, 7.4 alone); the local pass
 // adds 0.45 of that (a quarter of it for two segments, which have no Pi; 0.25 with the chunks' matrices in
 // the block form), the carry 4 us and 0.35 a segment.  Measured so: 8 x 2048 x 16 x 40, 2 / 4 / 8 /
-// 16 segments: 682 / 587 / 608 / 625 us; 3 x 777 x 16 x 64, 8 / 10 / 13: 160 / 143 / 169 (13 with the chunks'
-// matrices apart); 1 x 2048 x 16 x 64, 8 / 16 / 32: 190 / 143 / 116.
+// 16 segments: 644 / 568 / 603 / 626 us; 3 x 777 x 16 x 64, 8 / 10 / 13: 161 / 145 / 156 (13 with the chunks'
+// matrices apart: 171); 1 x 2048 x 16 x 64, 8 / 16 / 32: 181 / 131 / 112.
 int segment_chunks(int B, int T, int H, int N) {
     const int64_t heads = (int64_t)B * H;
     const int chunks = T / kC + (T % kC != 0);
