@@ -44,8 +44,8 @@
 // One segment needs the first and the last alone, two no carry.  Four-chunk segments take the first two
 // as one (wkv7_grad_block_kernel, block_form).
 //
-// 8 x 2048 x 16 x 40 (four segments): 76 + 128 + 6 + 358 us; 3 x 777 x 16 x 64 (ten): 17 + 44 + 17 + 66;
-// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 57.  The first kernel is bound by memory (200 MB at 2.7
+// 8 x 2048 x 16 x 40 (four segments): 76 + 126 + 6 + 354 us; 3 x 777 x 16 x 64 (ten): 17 + 44 + 17 + 66;
+// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 56.  The first kernel is bound by memory (200 MB at 2.7
 // TB/s, its writes half of them), the second and the last by latency and issue together: an fp32 MFMA takes 32
 // cycles of a SIMD, a VALU instruction 4 and a 16-byte LDS read about 18, none beside another, and with two waves a
 // SIMD at most nothing else fills a wave's waits.
@@ -781,7 +781,7 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) wkv7_grad_carry_k
 }
 
 // A workgroup of NB waves per segment of a head.  Scheduled for two waves per SIMD instead of three the operands
-// come from LDS in time: the call of 8 x 2048 x 16 x 40 600 us, so 569.  By counters a SIMD's time goes, at N = 64 with
+// come from LDS in time: the call of 8 x 2048 x 16 x 40 600 us, so 562.  By counters a SIMD's time goes, at N = 64 with
 // two waves on each (1 x 2048 x 16 x 64), 42 % to MFMAs, 11 to VALU and 12 to LDS instructions; at N = 40 (8 x 2048 x
 // 16), whose two three-wave workgroups leave two of a CU's SIMDs with one wave, 36, 10 and 10 on average and 48, 14 and 14
 // on the other two, and a wave waits 38 % of its time for memory, LDS and barriers.
@@ -880,6 +880,8 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
 #pragma unroll
             for (int r = 0; r < 4; ++r) out[(4 * g + r) * kST + li] = li < 4 * g + r + !strict ? m[r] : 0.0f;
         };
+        const floatx4 pr = R * dR, in = B * dB + K * dK;
+        float before = rows_sum(share) + Around(sum4(in), g).before;
         if (q == 0) gram(sY, sU, sMrb, false);
         if (q == (NB > 1 ? 1 : 0)) gram(sY, sV, sMrk, false);
         lds_barrier();
@@ -908,23 +910,24 @@ template <int NB> __global__ void __launch_bounds__(NB *kWave) __attribute__((am
                 dA1 = mfma(e4[r + 1], S0[t][r + 1], dA1);
             }
         }
+        const floatx4 yr = R * iR;
+        tile.store(p.dr, (dR + iR) * d.now);
         lds_barrier();
         dA += dA1;
+        const floatx4 pa = A * dA;
+        float after = Around(sum4(pr + pa), g).after;
         mul16(ld4(sLab + li * kST + 4 * g), B, iA, ldcol(sLab + 4 * g * kST + li, kST), A, iB);
         mul16(ld4(sLak + li * kST + 4 * g), K, iA1, ldcol(sLak + 4 * g * kST + li, kST), A, iK);
         iA += iA1;
-        tile.store(p.dr, (dR + iR) * d.now);
         tile.store(p.da, (dA + iA) * d.before);
         tile.store(p.db, (dB + iB) * d.inv);
         tile.store(p.dk, (dK + iK) * d.inv);
         // (log d_t)', in the tokens' order forward for what enters the state and backward for what takes from it.
-        const floatx4 pr = R * dR, pa = A * dA, in = B * dB + K * dK;
-        const floatx4 yr = R * iR, ya = A * iA, yb = B * iB + K * iK, rest = yr - yb, z = rest + ya;
+        const floatx4 ya = A * iA, yb = B * iB + K * iK, rest = yr - yb, z = rest + ya;
         floatx4 m;  // magnitude of a token's terms
 #pragma unroll
         for (int r = 0; r < 4; ++r) m[r] = fabsf(yr[r]) + fabsf(yb[r]) + fabsf(ya[r]);
         const Around az(sum4(z), g), am(sum4(m), g);
-        float before = rows_sum(share) + Around(sum4(in), g).before, after = Around(sum4(pr + pa), g).after;
         float z_before = az.before, m_before = am.before, z_after = az.after, m_after = am.after;
         floatx4 dw, inner, low;  // low: magnitude on the start's side
 #pragma unroll
