@@ -264,3 +264,8 @@ def test_scans_of_no_sequences():
         assert getattr(lib(), name)(0, 5, 64, None, None, None, DUMMY, DUMMY, *[None] * 4) == 0
     refused(lib().yuf_wkv7_scan_f32(1, 5, 3, 40, *[None] * 10), "null")
     refused(lib().yuf_rosa_scan_f32(1, 5, 64, None, None, None, DUMMY, DUMMY, *[None] * 4), "null")
+
+
+def test_gradients_of_no_sequences_take_any_other_size():
+    assert lib().yuf_wkv7_scan_backward_f32(0, 5, 1 << 20, 40, *[None] * 18) == 0
+    assert lib().yuf_wkv7_scan_backward_workspace(0, 5, 1 << 20, 40) == 0

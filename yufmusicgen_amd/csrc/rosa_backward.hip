@@ -515,8 +515,8 @@ int epl_of(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : D <= 512 
 //     R = 8     124   126   131   152   167   183   245   327   403   827
 //     R = 16    219   221   224   247   259   271   313   368   411   689  1429
 //     R = 32    412   413   417   453   464   474   516   558   588   811  1283
-// R = 2 gains 5 to 13 us on both up to 256.  D = 64 and 256 cross at the same places.  Eight sequences, whose
-// blocks fill the GPU, are within 5 % from R = 4 to 16 (512 blocks: 316, 282, 269, 346, 559).
+// (R = 2 would gain 4 to 15 us around 160 blocks.)  D = 64 and 256 cross near the same places, and for eight
+// sequences, whose blocks fill the GPU, the R picked is within 6 % of the best.
 struct Cut {
     int S, R, NR;
 };

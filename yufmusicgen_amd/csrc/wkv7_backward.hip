@@ -45,8 +45,8 @@
 // as one (wkv7_grad_block_kernel, block_form).
 //
 // 8 x 2048 x 16 x 40 (four segments): 76 + 126 + 6 + 354 us; 3 x 777 x 16 x 64 (ten): 17 + 44 + 17 + 66;
-// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 56.  The first kernel is bound by memory (200 MB at 2.7
-// TB/s, its writes half of them), the second and the last by latency and issue together: an fp32 MFMA takes 32
+// 1 x 2048 x 16 x 64 (32, the first two as one): 33 + 22 + 56.  The first kernel is bound by memory (306 MB at 4.0
+// TB/s, a third of them written), the second and the last by latency and issue together: an fp32 MFMA takes 32
 // cycles of a SIMD, a VALU instruction 4 and a 16-byte LDS read about 18, none beside another, and with two waves a
 // SIMD at most nothing else fills a wave's waits.
 //
@@ -1020,6 +1020,7 @@ Scratch scratch_of(int B, int T, int H, int N) {
 std::string unsupported(int B, int T, int H, int N) {
     if (B < 0 || T < 0 || H < 0) return "wkv7 backward: negative size";
     if (!wkv7_supported(N)) return "wkv7 backward: unsupported head size N=" + std::to_string(N);
+    if (B == 0 || H == 0) return "";
     // Offsets inside a chunk of one head are 32-bit.
     if ((int64_t)H * N > (1 << 24)) return "wkv7 backward: H * N above 2^24";
     const int64_t heads = (int64_t)B * H;
