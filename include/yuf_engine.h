@@ -186,8 +186,8 @@ int yuf_ln_linear_bf16w(int M, int N, int K, const float *A, const float *gamma,
                         void *stream);
 
 /* ---------------------------------------------------------------------------
- * Operators of the training pass: the gradients of the two scans, dropout and
- * the loss.  Device pointers, asynchronous on `stream`, no allocation: scratch
+ * Operators of the training pass: the gradients of the two scans, dropout, the
+ * loss, the token embedding and the update of weight matrices.  Device pointers, asynchronous on `stream`, no allocation: scratch
  * is a caller-owned device buffer (256-byte aligned) of the size that the
  * matching *_workspace function gives (0 for sizes that the operator refuses).
  * It holds nothing between calls; calls that may overlap (other streams, other
@@ -299,6 +299,41 @@ int yuf_cross_entropy_bf16(int M, int V, const uint16_t *logits, int64_t ld, con
                            int target_bits, int64_t ignore_index, int reduction, float *loss,
                            const float *dloss, uint16_t *dlogits, int64_t ld_out, void *workspace,
                            void *stream);
+
+/*
+ * Token embedding with a scale (the reference's nn.Embedding,
+ * yufmusicgen/model.py:390-391, :406): out[i] = scale W[t_i].
+ *   table      : device [V, D] fp32, or bf16 bit patterns.
+ *   tokens     : device [M] int32 or int64 (token_bits 32 or 64).  An id outside
+ *                [0, V) gives a row of NaN.
+ *   out        : device [M, D] of the table's type, rounded once.
+ * V, D <= 2^24, M < 2^31.  Pointers need their elements' alignment only.
+ */
+int yuf_embedding_f32(int64_t M, int V, int D, const float *table, const void *tokens,
+                      int token_bits, double scale, float *out, void *stream);
+int yuf_embedding_bf16(int64_t M, int V, int D, const uint16_t *table, const void *tokens,
+                       int token_bits, double scale, uint16_t *out, void *stream);
+
+/*
+ * Its gradient by the table: out[v] (+)= scale sum of dout[i] over t_i = v, in the
+ * order of positions, in fp32, rounded once.
+ *   dout       : device [M, D].
+ *   padding    : an id whose row gets no gradient, or -1.  Ids outside [0, V) have
+ *                no row to give theirs to.
+ *   accumulate : 1: added to what out holds (the gradient that a tied LM head left);
+ *                0: every row of out is written.
+ *   out        : device [V, D] of dout's type.  Neither out nor the workspace may
+ *                share memory with an input or with each other.
+ *   workspace  : yuf_embedding_grad_workspace(M, V, D) bytes, for either type.
+ * V, D <= 2^24, M <= 2^30.
+ */
+size_t yuf_embedding_grad_workspace(int64_t M, int V, int D);
+int yuf_embedding_grad_f32(int64_t M, int V, int D, const void *tokens, int token_bits,
+                           const float *dout, double scale, int64_t padding, int accumulate,
+                           float *out, void *workspace, void *stream);
+int yuf_embedding_grad_bf16(int64_t M, int V, int D, const void *tokens, int token_bits,
+                            const uint16_t *dout, double scale, int64_t padding, int accumulate,
+                            uint16_t *out, void *workspace, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Checkpoints (.yuf).  Replaces `Checkpoint::load / tensor / tensor_dims`

@@ -61,6 +61,15 @@ SIGNATURES = {
     "yuf_cross_entropy_bf16": (ctypes.c_int, [ctypes.c_int] * 2 + [c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int,
                                                                    ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3 +
                                [ctypes.c_int64, c_void_p, c_void_p]),
+    "yuf_embedding_f32": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, ctypes.c_int,
+                                         ctypes.c_double, c_void_p, c_void_p]),
+    "yuf_embedding_bf16": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, ctypes.c_int,
+                                          ctypes.c_double, c_void_p, c_void_p]),
+    "yuf_embedding_grad_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
+    "yuf_embedding_grad_f32": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int, c_void_p,
+                                              ctypes.c_double, ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3),
+    "yuf_embedding_grad_bf16": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int, c_void_p,
+                                               ctypes.c_double, ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3),
     "yuf_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 3 + [ctypes.c_int] + [c_void_p] * 3),
     "yuf_ln_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 9),
     "yuf_x3_planes_elems": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),

@@ -7,14 +7,15 @@ validation errors; they run the gfx950 kernels of ``libyufhip.so`` through the
 C ABI on torch's current HIP stream.  Tensors are torch plumbing (device
 memory and streams); there is no CPU fallback.
 
-Both scans, ``dropout`` and ``cross_entropy`` are differentiable once, as the
+Both scans, ``dropout``, ``cross_entropy`` and ``embedding`` are differentiable once, as the
 reference's autograd functions are (cuda_ops.py:189-253, rosa_cuda.py:73-154).
 Their gradients are operators too (``rwkv7_scan_backward``,
-``rosa_householder_scan_backward``, ``dropout`` itself, ``cross_entropy_grad``):
-a HIP graph captures those.  Captured ``backward()`` calls through these
+``rosa_householder_scan_backward``, ``dropout`` itself, ``cross_entropy_grad``,
+``embedding_grad``): a HIP graph captures those.  Captured ``backward()`` calls through these
 operators raise, because torch ends the process when a capture meets gradient
 accumulators that another, still living autograd graph made on a stream outside
-of it.
+of it.  A capture that holds a backward pass but not its forward pass ends the
+process inside torch before an operator is asked.
 """
 
 from __future__ import annotations
@@ -442,3 +443,103 @@ class _CrossEntropy(torch.autograd.Function):
         dlogits = torch.empty(rows.shape, device=rows.device, dtype=rows.dtype)
         _loss_call(rows, targets, *ctx.how, dloss.contiguous(), dlogits, False)
         return dlogits, None, None, None
+
+
+# ------------------------------------------------------------------ embedding
+def _check_tokens(tokens, device) -> None:
+    if tokens.device != device:
+        raise ValueError("tokens must be on the same GPU")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError("tokens must be int32 or int64")
+
+
+def _check_padding(padding_idx, vocab: int) -> int:
+    if padding_idx is None:
+        return -1
+    if not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx must be in [0, {vocab}), got {padding_idx}")
+    return int(padding_idx)
+
+
+def embedding(tokens, weight, scale: float = 1.0, padding_idx=None):
+    """``scale * weight[tokens]``: [..., D] for ``tokens`` [...] and ``weight`` [V, D], in
+    the weight's type (float32 or bfloat16).  Differentiable by the weight.
+
+    int32 or int64 tokens.  One outside [0, V) gives a row of NaN, and no gradient.
+    The row of ``padding_idx`` is looked up like any other and gets no gradient.
+    """
+    if weight.ndim != 2:
+        raise ValueError("weight must have shape [V, D]")
+    if not weight.is_cuda:
+        raise ValueError("weight must be on the GPU")
+    if weight.dtype not in _FLOATS:
+        raise TypeError("embedding takes float32 or bfloat16 weights")
+    if not weight.is_contiguous():
+        raise ValueError("weight must be contiguous")
+    _check_tokens(tokens, weight.device)
+    padding = _check_padding(padding_idx, weight.shape[0])
+    if _needs_grad(weight):
+        return _Embedding.apply(tokens, weight, float(scale), padding)
+    return _embedding_forward(tokens, weight, scale)
+
+
+def _embedding_forward(tokens, weight, scale):
+    tokens = tokens.contiguous()
+    vocab, dim = weight.shape
+    with _on(weight.device) as stream:
+        out = torch.empty(*tokens.shape, dim, device=weight.device, dtype=weight.dtype)
+        entry = lib().yuf_embedding_f32 if weight.dtype == torch.float32 else lib().yuf_embedding_bf16
+        check(entry(tokens.numel(), vocab, dim, weight.data_ptr(), tokens.data_ptr(), 8 * tokens.element_size(),
+                    float(scale), out.data_ptr(), stream))
+    return out
+
+
+def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=None, out=None):
+    """Gradient of ``embedding`` by its weight: [vocab, D] for ``dout`` [..., D], in dout's type.
+
+    ``out`` (a contiguous [vocab, D] tensor of that type, such as the gradient that a
+    tied LM head left): the gradient is added to it, and it is returned.  Each row's
+    sum runs over its positions in order, in float32.
+    """
+    if dout.ndim < 1 or tuple(dout.shape[:-1]) != tuple(tokens.shape):
+        raise ValueError(f"dout must have shape {list(tokens.shape) + ['D']}, got {list(dout.shape)}")
+    if not dout.is_cuda:
+        raise ValueError("dout must be on the GPU")
+    if dout.dtype not in _FLOATS:
+        raise TypeError("embedding takes float32 or bfloat16 gradients")
+    if vocab < 0:
+        raise ValueError(f"vocab must not be negative, got {vocab}")
+    _check_tokens(tokens, dout.device)
+    padding = _check_padding(padding_idx, vocab)
+    if out is not None:
+        _check_like("out", out, (vocab, dout.shape[-1]), dout.device, dout.dtype)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        if _needs_grad(out):
+            raise ValueError("out is written in place: it may not require a gradient")
+    tokens, dout = tokens.contiguous(), dout.contiguous()
+    dim, count = dout.shape[-1], tokens.numel()
+    with _on(dout.device) as stream:
+        grad = torch.empty(vocab, dim, device=dout.device, dtype=dout.dtype) if out is None else out
+        space = _scratch(lib().yuf_embedding_grad_workspace(count, vocab, dim), dout.device)
+        entry = lib().yuf_embedding_grad_f32 if dout.dtype == torch.float32 else lib().yuf_embedding_grad_bf16
+        check(entry(count, vocab, dim, tokens.data_ptr(), 8 * tokens.element_size(), dout.data_ptr(), float(scale), padding,
+                    int(out is not None), grad.data_ptr(), space.data_ptr(), stream))
+    if out is not None:
+        torch.autograd.graph.increment_version(out)  # as an in-place operation of torch's does
+    return grad
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding):
+        ctx.how = (weight.shape[0], scale, None if padding < 0 else padding)
+        ctx.save_for_backward(tokens)
+        return _embedding_forward(tokens, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        _not_captured("embedding")
+        (tokens,) = ctx.saved_tensors
+        return None, embedding_grad(tokens, dout, *ctx.how), None, None
