@@ -335,6 +335,52 @@ int yuf_embedding_grad_bf16(int64_t M, int V, int D, const void *tokens, int tok
                             const uint16_t *dout, double scale, int64_t padding, int accumulate,
                             uint16_t *out, void *workspace, void *stream);
 
+/*
+ * Matrices orthogonalised by Newton-Schulz products, as the Muon optimiser takes its
+ * updates (no counterpart in the reference, whose optimiser is AdamW,
+ * yufmusicgen/training.py): X = x / (|x|_F + eps), then `steps` times
+ * A = X X^T, X <- a X + (b A + c A A) X, on the transpose where rows > cols.
+ *   x, out     : host arrays of `count` device pointers to [rows, cols] matrices of
+ *                one type; out[i] may be x[i].  They and the workspace may not overlap
+ *                otherwise.  Any element alignment.
+ *   steps      : 1 to 64.  a, b, c: coefficients under which no singular value of a
+ *                matrix of norm 1 grows past 256.  eps >= 0.
+ *   workspace  : yuf_newton_schulz_workspace(count, rows, cols) bytes.
+ * fp32: products of operands with 22 bits, summed in fp32 (about 1.5 times an
+ * fp32 product's error).  bf16: the same up to 128 rows (the smaller side) or beyond 6
+ * steps, else operands with 11 bits and a X with 22; rounded to bf16 once.
+ * X's elements are held in steps of at least 2^-38, so a matrix whose norm is far below
+ * eps keeps fewer digits.  A matrix with a NaN or an infinity gives NaN.  Padded to multiples of 128, a matrix
+ * may have 2^28 elements.  Matrices are taken in groups, of which the workspace holds one.
+ */
+size_t yuf_newton_schulz_workspace(int count, int rows, int cols);
+int yuf_newton_schulz_f32(int count, int rows, int cols, const float *const *x, float *const *out,
+                          int steps, double a, double b, double c, double eps, void *workspace,
+                          void *stream);
+int yuf_newton_schulz_bf16(int count, int rows, int cols, const uint16_t *const *x,
+                           uint16_t *const *out, int steps, double a, double b, double c,
+                           double eps, void *workspace, void *stream);
+
+/*
+ * One update of `count` weight matrices by orthogonalised momenta, in place:
+ *     m <- momentum m + (1 - momentum) g,
+ *     u = nesterov ? momentum m + (1 - momentum) g : m,
+ *     p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) X(u),
+ * X(u) as above.
+ *   params, grads, momenta : host arrays of `count` device pointers to [rows, cols]
+ *                matrices; params and grads of one type, momenta fp32.  None may
+ *                overlap another or the workspace, except grads each other.
+ *   workspace  : yuf_newton_schulz_workspace(count, rows, cols) bytes.
+ */
+int yuf_muon_step_f32(int count, int rows, int cols, float *const *params, const float *const *grads,
+                      float *const *momenta, double lr, double momentum, int nesterov,
+                      double weight_decay, int steps, double a, double b, double c, double eps,
+                      void *workspace, void *stream);
+int yuf_muon_step_bf16(int count, int rows, int cols, uint16_t *const *params,
+                       const uint16_t *const *grads, float *const *momenta, double lr,
+                       double momentum, int nesterov, double weight_decay, int steps, double a,
+                       double b, double c, double eps, void *workspace, void *stream);
+
 /* ---------------------------------------------------------------------------
  * Checkpoints (.yuf).  Replaces `Checkpoint::load / tensor / tensor_dims`
  * (vulkan/src/checkpoint.rs:90-176).

@@ -261,3 +261,259 @@ def test_embedding_in_graphs_and_on_streams():
             got = ops.embedding_grad(tokens, dout, 400)
         torch.cuda.current_stream().wait_stream(side)
         check_grad(got, tokens, dout, 400, 1.0)
+
+
+# ----------------------------------------------------------------------- weight update
+# The polynomial amplifies what a step's rounding adds, by up to a = 3.4 each step and by how much depends on the
+# matrix: the error is compared with that of the same formula in float32 products.  fp32's operands here have
+# 22 bits for 24, so each rounding is at most 4 times as large: 4 times that error, and 2^-22 where it has
+# none.  bf16's products, of 11 bits or 22, are held to the half step of its output, 2^-8 in the 2-norm,
+# whose rounding alone takes up to 0.6 of that.
+ABC = (3.4445, -4.7750, 2.0315)
+
+
+def polynomial(x, steps=5, abc=ABC, eps=1e-7):
+    """In x's type, of products as they stand."""
+    a, b, c = abc
+    wide = x.shape[-2] <= x.shape[-1]
+    X = x if wide else x.mT.contiguous()
+    X = (X.double() / (X.double().square().sum((-1, -2), keepdim=True).sqrt() + eps)).to(x.dtype)
+    for _ in range(steps):
+        A = X @ X.mT.contiguous()
+        X = a * X + (b * A + c * (A @ A)) @ X
+    return X if wide else X.mT
+
+
+def gradient(seed, *shape, noise=0.1):
+    few = max(1, min(shape[-2:]) // 16)
+    g = gen(seed)
+    left = torch.randn(*shape[:-1], few, generator=g, device="cuda") * torch.logspace(0, -2, few, device="cuda")
+    return 1e-3 * (left @ torch.randn(*shape[:-2], few, shape[-1], generator=g, device="cuda") +
+                   noise * torch.randn(*shape, generator=g, device="cuda"))
+
+
+def norms(x):
+    return x.double().square().sum((-1, -2)).sqrt()
+
+
+def allowed(x, kind, **how):
+    """float64's result for x and, for each matrix, how far one may be from it in the 2-norm."""
+    expect = polynomial(x.double(), **how)
+    if kind == "bf16":
+        return expect, 2.0**-8 * norms(expect)
+    return expect, 4 * norms(polynomial(x.float(), **how).double() - expect) + 2.0**-22 * norms(expect)
+
+
+def check_ns(got, x, kind, floor=0.0, **how):
+    expect, off = allowed(x, kind, **how)
+    off = off + floor
+    assert got.shape == x.shape and got.dtype == x.dtype
+    err = norms(got.double() - expect)
+    assert (err <= off + 1e-30).all(), (err / norms(expect), off / norms(expect))
+
+
+NS_SHAPES = [(1, 1, 1), (2, 1, 7), (2, 7, 1), (3, 3, 5), (3, 16, 16), (2, 31, 33), (1, 64, 64), (2, 65, 64), (1, 640, 64),
+             (2, 64, 640), (1, 127, 129), (2, 256, 257), (2, 257, 256), (1, 300, 700), (3, 640, 640), (1, 1000, 129),
+             (1, 129, 1000), (1, 333, 1111), (2, 1111, 333), (1, 2560, 640), (33, 20, 30), (70, 9, 5)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count,rows,cols", NS_SHAPES)
+def test_newton_schulz(count, rows, cols, kind):
+    from yufmusicgen_amd import ops
+
+    print(f"newton schulz {count} x {rows} x {cols} {kind}", flush=True)
+    x = gradient(count + rows, count, rows, cols).to(TYPES[kind])
+    kept = x.clone()
+    got = ops.newton_schulz(x)
+    check_ns(got, x, kind)
+    assert torch.equal(x, kept)
+    check_ns(ops.newton_schulz(x.mT), x.mT, kind)  # the other orientation, and a strided input
+    one = ops.newton_schulz(x[-1])
+    assert torch.equal(one, got[-1])  # a matrix alone as among others
+    for a, b in zip(ops.newton_schulz(list(x)), got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("steps,abc", [(1, ABC), (3, ABC), (10, ABC), (20, (1.5, -0.5, 0.0)), (12, (15 / 8, -10 / 8, 3 / 8)),
+                                       (5, (0.5, 0.0, 0.0)), (2, (0.0, 1.0, -1.0)), (3, (-2.0, 1.0, 0.25))])
+def test_newton_schulz_of_other_coefficients(steps, abc, kind):
+    from yufmusicgen_amd import ops
+
+    print(f"newton schulz {steps} steps of {abc} {kind}", flush=True)
+    x = torch.randn(2, 96, 200, generator=gen(1), device="cuda").to(TYPES[kind])
+    check_ns(ops.newton_schulz(x, steps=steps, coefficients=abc), x, kind, steps=steps, abc=abc)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_newton_schulz_of_extreme_matrices(kind):
+    """Scales over the type's range, zeros, ranks of one, and non-finite matrices among finite ones."""
+    from yufmusicgen_amd import ops
+
+    x = gradient(5, 9, 70, 90).to(TYPES[kind])
+    x[1] *= 1e30
+    x[2] *= 1e-30  # eps leaves nothing of it
+    x[3] = 0
+    x[4] = x[4, :, :1] @ x[4, :1, :]
+    x[5, 3, 4] = float("nan")
+    x[6, 69, 89] = float("inf")
+    x[7] = 0
+    x[7, 69, 89] = -3.0
+    got = ops.newton_schulz(x)
+    assert got[5].isnan().all() and got[6].isnan().all()
+    rest = [0, 1, 2, 3, 4, 7, 8]
+    # X is held in steps of fp16's subnormals, 2^-24, times 2^-14: an element is off by at most 2^-39, a matrix by
+    # the root of its size times that, and a step makes at most 4 times as much of it, after adding its own.
+    check_ns(got[rest], x[rest], kind, floor=(70 * 90) ** 0.5 * 2.0**-39 * 4**5 * 4 / 3)
+    assert (got[3] == 0).all()
+    got = ops.newton_schulz(x[2], eps=0.0)  # without eps the scale does not matter
+    check_ns(got, x[2], kind, eps=0.0)
+    assert ops.newton_schulz(x[3], eps=0.0).isnan().all()
+    assert ops.newton_schulz(x[:0]).shape == (0, 70, 90) and ops.newton_schulz(x[:, :0]).shape == (9, 0, 90)
+    assert ops.newton_schulz(x.view(3, 3, 70, 90)).shape == (3, 3, 70, 90)
+
+
+def muon_reference(p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0):
+    m = momentum * m.double() + (1 - momentum) * g.double()
+    u = momentum * m + (1 - momentum) * g.double() if nesterov else m
+    rate = lr * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5
+    step = polynomial(u)
+    loose = polynomial(u.float()).double() - step
+    return p.double() * (1 - lr * weight_decay) - rate * step, m, rate * norms(step), rate * norms(loose)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("nesterov,weight_decay", [(True, 0.1), (False, 0.0)])
+@pytest.mark.parametrize("count,rows,cols", [(1, 1, 1), (3, 40, 64), (2, 200, 77), (33, 12, 9), (2, 640, 640), (1, 300, 2000)])
+def test_muon_step(count, rows, cols, nesterov, weight_decay, kind):
+    from yufmusicgen_amd import ops
+
+    print(f"muon step {count} x {rows} x {cols} {kind}", flush=True)
+    dtype = TYPES[kind]
+    p, g, m = table(1, count * rows, cols, dtype).view(count, rows, cols), gradient(2, count, rows, cols).to(dtype), gradient(3, count, rows, cols)
+    new_p, new_m, step, loose = muon_reference(p, g, m, 0.3, nesterov=nesterov, weight_decay=weight_decay)
+    ps, gs, ms = list(p.clone().unbind()), list(g.unbind()), [t.clone() for t in m]
+    ops.muon_step(ps, gs, ms, 0.3, nesterov=nesterov, weight_decay=weight_decay)
+    ps, ms = torch.stack(ps), torch.stack(ms)
+    # Two products and a sum, and a rounded coefficient in each product.
+    assert ((ms.double() - new_m).abs() <= 4 * EPS32 * (0.95 * m.double().abs() + 0.05 * g.double().abs())).all()
+    off = (2.0**-8 if kind == "bf16" else 0) * (step + norms(new_p)) + 4 * loose + 2.0**-22 * (step + norms(p))
+    assert (norms(ps.double() - new_p) <= off).all(), (norms(ps.double() - new_p), off)
+
+
+def test_muon_step_over_a_models_matrices():
+    """Matrices of several shapes and types in one call, parameters that require gradients, an odd layout of a gradient."""
+    from yufmusicgen_amd import ops
+
+    shapes = [(40, 64), (64, 40), (40, 64), (7, 7), (64, 40)]
+    params = [torch.nn.Parameter(table(i, *s, torch.bfloat16 if i == 4 else torch.float32)) for i, s in enumerate(shapes)]
+    for i, p in enumerate(params):
+        p.grad = gradient(10 + i, *p.shape).to(p.dtype)
+    params[1].grad = params[1].grad.t().contiguous().t()
+    momenta = [torch.zeros(p.shape, device="cuda") for p in params]
+    expect = [muon_reference(p.detach(), p.grad, m, 0.1) for p, m in zip(params, momenta)]
+    versions = [p._version for p in params]
+    ops.muon_step(params, [p.grad for p in params], momenta, 0.1)
+    for p, m, v, (new_p, new_m, step, loose) in zip(params, momenta, versions, expect):
+        assert p._version > v and p.requires_grad and p.is_leaf
+        off = (2.0**-8 if p.dtype == torch.bfloat16 else 0) * (step + norms(new_p)) + 4 * loose + 2.0**-22 * (step + norms(p.detach()))
+        assert norms(p.detach().double() - new_p) <= off
+        assert ((m.double() - new_m).abs() <= 4 * EPS32 * new_m.abs()).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count,rows,cols", [(2, 33, 70), (1, 300, 257)])
+def test_newton_schulz_writes_stay_inside(count, rows, cols, kind):
+    """What lies around the outputs and behind the workspace stays as it was; matrices may start at any element."""
+    import ctypes
+
+    from yufmusicgen_amd._lib import check, lib
+
+    dtype, n = TYPES[kind], rows * cols
+    x = gradient(6, count, rows, cols).to(dtype)
+    from yufmusicgen_amd import ops
+
+    expect = ops.newton_schulz(x)
+    size = lib().yuf_newton_schulz_workspace(count, rows, cols)
+    call = lib().yuf_newton_schulz_f32 if kind == "f32" else lib().yuf_newton_schulz_bf16
+    for start in (0, 1, 3):
+        space = torch.full((size + 4096,), 7, device="cuda", dtype=torch.uint8)
+        gap = n + 5
+        held, given = (torch.full((start + count * gap + 50,), 7.0, device="cuda", dtype=dtype) for _ in range(2))
+        at = [start + i * gap for i in range(count)]
+        for i, a in enumerate(at):
+            given[a : a + n] = x[i].reshape(-1)
+        lists = [(ctypes.c_void_p * count)(*[t[a:].data_ptr() for a in at]) for t in (given, held)]
+        check(call(count, rows, cols, *lists, 5, *ABC, 1e-7, space.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        untouched = torch.ones_like(held, dtype=torch.bool)
+        for i, a in enumerate(at):
+            assert torch.equal(held[a : a + n], expect[i].reshape(-1))
+            untouched[a : a + n] = False
+        assert (held[untouched] == 7).all() and (space[size:] == 7).all()
+        check(call(count, rows, cols, lists[0], lists[0], 5, *ABC, 1e-7, space.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        assert all(torch.equal(given[a : a + n], expect[i].reshape(-1)) for i, a in enumerate(at))  # in place
+
+
+def test_weight_updates_in_graphs_and_on_streams():
+    """Two captured graphs with eager calls between their replays, and a side stream."""
+    from yufmusicgen_amd import ops
+
+    x, p, m = gradient(7, 3, 70, 130), table(8, 64, 200, torch.float32), torch.zeros(64, 200, device="cuda")
+    g = gradient(9, 64, 200)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.newton_schulz(x), ops.muon_step([p.clone()], [g], [m.clone()], 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for k in range(2):
+        weights, momenta = p.clone(), m.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.newton_schulz(x)
+            ops.muon_step([weights], [g], [momenta], 0.1 * (k + 1))
+        weights.copy_(p), momenta.copy_(m)
+        graphs.append((graph, out, weights, momenta, p.clone(), m.clone(), 0.1 * (k + 1)))
+    for k in range(4):
+        x.copy_(gradient(20 + k, 3, 70, 130)), g.copy_(gradient(30 + k, 64, 200))
+        for graph, out, weights, momenta, wp, wm, lr in graphs if k % 2 else graphs[::-1]:
+            graph.replay()
+            torch.cuda.synchronize()
+            ops.muon_step([wp], [g], [wm], lr)
+            assert torch.equal(out, ops.newton_schulz(x)) and torch.equal(weights, wp) and torch.equal(momenta, wm)
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            got = ops.newton_schulz(x)
+        torch.cuda.current_stream().wait_stream(side)
+        check_ns(got, x, "f32")
+
+
+def test_a_training_step_of_these_operators():
+    """Embedding, a projection, the loss over the tied table, and the updates: the gradients are those of float64."""
+    from yufmusicgen_amd import ops
+
+    vocab, dim = 300, 64
+    weight = (0.1 * table(40, vocab, dim, torch.float32)).requires_grad_()
+    square = (table(41, dim, dim, torch.float32) / 8).requires_grad_()
+    tokens, targets = ids(42, (4, 50), vocab, 3), ids(43, (4, 50), vocab, 3)
+    targets[:, 45:] = -100
+    tokens[:, 45:] = 0
+
+    def loss_of(e, w, s, cross):
+        return cross((torch.tanh(e @ s) @ w.t()).reshape(-1, vocab), targets.reshape(-1))
+
+    loss = loss_of(ops.embedding(tokens, weight, scale=dim**0.5, padding_idx=0), weight, square, ops.cross_entropy)
+    loss.backward()
+    w64, s64 = (t.detach().double().requires_grad_() for t in (weight, square))
+    e64 = torch.nn.functional.embedding(tokens, w64, padding_idx=0) * dim**0.5
+    loss64 = loss_of(e64, w64, s64, torch.nn.functional.cross_entropy)
+    loss64.backward()
+    # Sums of up to vocab + 200 terms, twice.
+    assert abs(loss.item() - loss64.item()) <= 1000 * EPS32 * loss64.item()
+    for t, e in ((weight, w64), (square, s64)):
+        assert (t.grad.double() - e.grad).norm() <= 1000 * EPS32 * e.grad.norm()
+    momenta = [torch.zeros_like(square)]
+    new_p, _, step, loose = muon_reference(square.detach(), square.grad, momenta[0], 0.02)
+    ops.muon_step([square], [square.grad], momenta, 0.02)
+    assert norms(square.detach().double() - new_p) <= 4 * loose + 2.0**-22 * (step + norms(new_p))

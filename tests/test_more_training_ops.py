@@ -114,3 +114,115 @@ def test_embedding_refuses_what_the_kernels_do_not_take():
                                       ("require", (tokens, dout, 5), dict(out=torch.empty(5, 4, device="cuda:0", requires_grad=True)), ValueError)):
             with pytest.raises(kind, match=match):
                 ops.embedding_grad(*args, **kw)
+
+
+# ------------------------------------------------------------------- weight update
+import ctypes  # noqa: E402
+
+
+def pointers(*at):
+    return (ctypes.c_void_p * len(at))(*at)
+
+
+GOOD = (5, 3.4445, -4.7750, 2.0315, 1e-7)
+
+
+@pytest.mark.parametrize("name", ["yuf_newton_schulz_f32", "yuf_newton_schulz_bf16"])
+def test_newton_schulz_refusals(name):
+    call = getattr(lib(), name)
+    size = 64 * 40 * (4 if name.endswith("f32") else 2)
+    space = lib().yuf_newton_schulz_workspace(2, 64, 40)
+    assert space > 0 and space % 8 == 0
+
+    def bad(*words, count=2, rows=64, cols=40, x=pointers(FAR[0], FAR[1]), out=pointers(FAR[2], FAR[3]), how=GOOD, at=FAR[7]):
+        refused(call(count, rows, cols, x, out, *how, at, None), *words)
+
+    bad("negative", count=-1)
+    bad("negative", rows=-1)
+    bad("negative", cols=-1)
+    bad("2^28", rows=1 << 14, cols=(1 << 14) + 1)
+    bad("2^22", rows=1, cols=(1 << 22) + 1)
+    for steps in (0, -1, 65):
+        bad("steps", how=(steps, *GOOD[1:]))
+    for eps in (-1.0, float("nan"), float("inf")):
+        bad("eps", how=(*GOOD[:4], eps))
+    for abc in ((30.0, 0.0, 0.0), (3.4445, -4.7750, 4.0), (float("nan"), 0.0, 0.0), (float("inf"), 0.0, 0.0), (0.0, 1e300, 1e300)):
+        bad("grow", how=(5, *abc, 1e-7))
+    bad("null", x=None)
+    bad("null", out=None)
+    bad("null", x=pointers(FAR[0], None))
+    bad("null", out=pointers(None, FAR[3]))
+    bad("workspace", at=None)
+    bad("aligned", at=FAR[7] + 128)
+    for out in ((FAR[1], FAR[0]), (FAR[0] + 4, FAR[3]), (FAR[2], FAR[2]), (FAR[2], FAR[2] + size - 4), (FAR[7], FAR[3]),
+                (FAR[7] + space - 4, FAR[3]), (FAR[2], FAR[1] - size + 4)):
+        bad("overlap", out=pointers(*out))
+    bad("overlap", at=FAR[1])
+    for sizes in ((0, 64, 40), (2, 0, 40), (2, 64, 0)):
+        assert call(*sizes, None, None, *GOOD, None, None) == 0
+
+
+def test_newton_schulz_scratch():
+    space = lib().yuf_newton_schulz_workspace
+    for sizes in ((-1, 4, 4), (0, 4, 4), (1, 0, 4), (1, 4, 0), (1, 1 << 14, (1 << 14) + 1), (1, (1 << 22) + 1, 1)):
+        assert space(*sizes) == 0, sizes
+    assert space(1, 1, 1 << 20) > 0 and space(1, 1 << 14, 1 << 14) > 0
+    assert space(1000, 640, 640) == space(100, 640, 640)  # a group's, however many there are
+
+
+@pytest.mark.parametrize("name", ["yuf_muon_step_f32", "yuf_muon_step_bf16"])
+def test_muon_step_refusals(name):
+    call = getattr(lib(), name)
+    size = 64 * 40 * (4 if name.endswith("f32") else 2)
+
+    def bad(*words, p=(FAR[0], FAR[1]), g=(FAR[2], FAR[3]), m=(FAR[4], FAR[5]), lr=0.02, beta=0.95, nesterov=1, decay=0.0, how=GOOD, at=FAR[7]):
+        lists = [None if x is None else pointers(*x) for x in (p, g, m)]
+        refused(call(2, 64, 40, *lists, lr, beta, nesterov, decay, *how, at, None), *words)
+
+    for x in (float("nan"), float("inf")):
+        bad("finite", lr=x)
+        bad("finite", beta=x)
+        bad("finite", decay=x)
+    bad("nesterov", nesterov=2)
+    bad("steps", how=(0, *GOOD[1:]))
+    for which in "pgm":
+        bad("null", **{which: None})
+        bad("null", **{which: (FAR[6], None)})
+    bad("workspace", at=None)
+    bad("overlap", p=(FAR[0], FAR[0]))  # the same matrix twice
+    bad("overlap", m=(FAR[4], FAR[4] + 64 * 40 * 4 - 4))
+    bad("overlap", g=(FAR[0], FAR[3]))  # a gradient in its weight's place
+    bad("overlap", g=(FAR[4] + 64 * 40 * 4 - 4, FAR[3]))
+    bad("overlap", m=(FAR[1] + size - 4, FAR[5]))
+    assert call(0, 64, 40, None, None, None, 0.02, 0.95, 1, 0.0, *GOOD, None, None) == 0
+
+
+def test_weight_update_python_refusals():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x = torch.zeros(4, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.newton_schulz(x)
+    with pytest.raises(ValueError, match="shape"):
+        ops.newton_schulz(x[0])
+    with pytest.raises(ValueError, match="shape"):
+        ops.newton_schulz([x[None], x[None]])
+    with pytest.raises(ValueError, match="one shape"):
+        ops.newton_schulz([x, x[:2]])
+    with pytest.raises(ValueError, match="GPU"):
+        ops.muon_step([x], [x], [x], 0.1)
+    with pytest.raises(ValueError, match="as many"):
+        ops.muon_step([x], [x, x], [x], 0.1)
+    assert ops.newton_schulz([]) == [] and ops.muon_step([], [], [], 0.1) is None
+    with FakeTensorMode():
+        g = torch.empty(4, 6, device="cuda:0")
+        for kind, match, arg in ((TypeError, "float32", g.half()), (ValueError, "same GPU", [g, g.to("cuda:1")]), (TypeError, "x must be", [g, g.bfloat16()]),
+                                 (ValueError, "differentiable", torch.empty(4, 6, device="cuda:0", requires_grad=True))):
+            with pytest.raises(kind, match=match):
+                ops.newton_schulz(arg)
+        for kind, match, args in ((ValueError, "matrices", (g[0], g[0], g[0])), (TypeError, "float32", (g.half(), g, g)),
+                                  (TypeError, "grads", (g, g.bfloat16(), g)), (TypeError, "momenta", (g.bfloat16(), g.bfloat16(), g.bfloat16())),
+                                  (ValueError, "grads", (g, g[:2], g)), (ValueError, "momenta", (g, g, g.to("cuda:1"))),
+                                  (ValueError, "contiguous", (g.t(), g.t(), g.t())), (ValueError, "contiguous", (g, g, torch.empty(6, 4, device="cuda:0").t()))):
+            with pytest.raises(kind, match=match):
+                ops.muon_step(*([x] for x in args), 0.1)

@@ -70,6 +70,15 @@ SIGNATURES = {
                                               ctypes.c_double, ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3),
     "yuf_embedding_grad_bf16": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int, c_void_p,
                                                ctypes.c_double, ctypes.c_int64, ctypes.c_int] + [c_void_p] * 3),
+    "yuf_newton_schulz_workspace": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "yuf_newton_schulz_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 2 + [ctypes.c_int] + [ctypes.c_double] * 4 +
+                              [c_void_p] * 2),
+    "yuf_newton_schulz_bf16": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 2 + [ctypes.c_int] + [ctypes.c_double] * 4 +
+                               [c_void_p] * 2),
+    "yuf_muon_step_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 3 + [ctypes.c_double] * 2 + [ctypes.c_int] +
+                          [ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 4 + [c_void_p] * 2),
+    "yuf_muon_step_bf16": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 3 + [ctypes.c_double] * 2 + [ctypes.c_int] +
+                           [ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 4 + [c_void_p] * 2),
     "yuf_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 3 + [ctypes.c_int] + [c_void_p] * 3),
     "yuf_ln_linear_f32": (ctypes.c_int, [ctypes.c_int] * 3 + [c_void_p] * 9),
     "yuf_x3_planes_elems": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),

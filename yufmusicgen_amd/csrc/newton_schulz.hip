@@ -1,0 +1,612 @@
+// Orthogonalising matrices by Newton-Schulz products, and the weight update around it:
+//     X <- x / (|x|_F + eps);   `steps` times:  A = X X^T,  X <- a X + (b A + c A A) X,
+// of the transpose where x has more rows than columns (p: the smaller side, q: the larger).
+//
+// Bound: the matrix cores.  Per step p^2 q + p^3 + 2 p^2 q operations, since A and A A are symmetric: only
+// tiles on and above the diagonal are multiplied, and each is written to both its places.
+//
+// Operands are fp16 pairs.  A value v scaled by a power of two is held as hi = fp16(v), lo = fp16(v - hi),
+// |v - hi - lo| <= 2^-22 |v|.  The scale of each matrix follows from a bound of its singular values (X starts
+// with a Frobenius norm of 1, and the polynomial's largest value bounds each next step), which bounds its elements, so
+// nothing overflows and what is lost below fp16's subnormals is under 2^-38 of the bound.
+// fp32 matrices take three products, hi hi + hi lo + lo hi (the one left out is below 2^-22): the polynomial amplifies
+// what a step adds along small singular values by up to a each step, so fp32 results need operands near
+// fp32's precision (2-norm errors on the CPU, 640 x 640: 1.8e-6; fp32 products 2.9e-6).
+// bf16 matrices take hi hi alone in the products, but a X from both parts, and A and P = b A + c A A keep 32-bit sums
+// until they are rounded: what a rounded product adds stays in the row space of X and is not amplified
+// (640 x 640: 1.7e-4 against the 1.7e-3 of the output's rounding).  Near singular values of 1 the polynomial has slopes
+// of up to 4, so few of them, whose errors do not average, and many steps go astray: 1 x 7 1.2e-2, 129 x 129 after 10
+// steps 4.6e-3.  So this form is taken for more than kOnePartRows rows and up to kOnePartSteps steps (there at most 0.8
+// of 2^-8, the output's half step, for matrices of 96 to 640 rows), and three products elsewhere.
+//
+// Layout: every operand lies in 1 KB blocks of 16 rows x 32 k in the order in which the lanes of
+// v_mfma_f32_16x16x32_f16 hold them (lane l: row l % 16, k = 8 (l / 16) + j), hi blocks and then lo blocks.
+// Blocks go from memory to LDS and from LDS to registers as they lie, without bank conflicts.  X is kept along both sides:
+// X X^T runs over q, P X over p.
+#include "common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+namespace yuf {
+namespace {
+
+typedef _Float16 f16;
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr int kWave = 64;
+constexpr int kThreads = 256;
+constexpr int kXcds = 8;
+constexpr int kGroup = 32;      // matrices of a launch: their pointers are kernel arguments
+constexpr int kSumParts = 64;   // workgroups of a matrix's norm, at most
+constexpr int kSumRun = 4096;   // elements of such a workgroup, at least
+constexpr int kPrepTile = 64;
+constexpr int kStepsMost = 64;
+constexpr int kOnePartRows = 128, kOnePartSteps = 6;
+constexpr double kGrowthMost = 256.0;  // of the singular values' bound
+constexpr double kBelow = 30000.0;     // scaled values stay below this (fp16 holds 65504)
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+__device__ __forceinline__ void narrow(float x, float &out) { out = x; }
+__device__ __forceinline__ void narrow(float x, uint16_t &out) {
+    // Round to nearest even; NaN stays a (quiet) NaN.
+    const uint32_t u = __float_as_uint(x);
+    out = x != x ? (uint16_t)((u >> 16) | 0x40) : (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// The matrices of a launch.  update: x are gradients, m momenta, out the weights; else out the results.
+template <typename T> struct Matrices {
+    const T *x[kGroup];
+    float *m[kGroup];
+    T *out[kGroup];
+    int count, rows, cols;
+    bool update, nesterov;
+    float beta, rest;    // of the momentum: m <- beta m + rest g
+    float keep, rate;    // out <- keep out - rate X
+};
+
+// The value that is orthogonalised, from its gradient and the updated momentum.
+template <typename T>
+__device__ __forceinline__ float direction(const Matrices<T> &t, float g, float m) {
+    return t.nesterov ? fmaf(t.beta, m, t.rest * g) : m;
+}
+
+// ------------------------------------------------------------------- norm and momentum
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ns_norm_kernel(Matrices<T> t, int parts, double *sums) {
+    __shared__ double waves[kThreads / kWave];
+    const int matrix = blockIdx.y;
+    const int64_t n = (int64_t)t.rows * t.cols, run = (n + parts - 1) / parts;
+    const int64_t first = blockIdx.x * run, last = min(n, first + run);
+    const T *x = t.x[matrix];
+    float *m = t.update ? t.m[matrix] : nullptr;
+    double sum = 0.0;
+    for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
+        float v = widen(x[i]);
+        if (m) {
+            const float next = fmaf(t.beta, m[i], t.rest * v);
+            m[i] = next;
+            v = direction(t, v, next);
+        }
+        sum = fma((double)v, (double)v, sum);
+    }
+    sum = wave_sum_f64(sum);
+    if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / kWave; ++w) sum += waves[w];
+        sums[(int64_t)matrix * parts + blockIdx.x] = sum;
+    }
+}
+
+// -------------------------------------------------------------------- operand blocks
+// Where element (row, k) of an operand of `kblocks` blocks along k lies.
+__device__ __forceinline__ int64_t block_at(int row, int k, int kblocks) {
+    return ((int64_t)(row >> 4) * kblocks + (k >> 5)) * 512 + ((((k & 31) >> 3) * 16 + (row & 15)) << 3) + (k & 7);
+}
+
+template <int N, typename V> __device__ __forceinline__ void split(const float (&x)[N], V &hi, V &lo) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        hi[e] = (f16)x[e];
+        lo[e] = (f16)(x[e] - (float)hi[e]);
+    }
+}
+
+struct Buffers {        // of one matrix, in f16 elements from its base
+    int64_t x, xt[2], gram, poly, stride;
+    int64_t long_plane, short_plane;  // lo blocks lie that far behind the hi blocks: of X, and of A and P
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ns_prepare_kernel(Matrices<T> t, int parts, const double *sums, double eps,
+                                                               float scale, f16 *space, Buffers b, int pp, int qp) {
+    __shared__ float tile[kPrepTile][kPrepTile + 1];
+    const int matrix = blockIdx.z, tid = threadIdx.x;
+    const bool wide = t.rows <= t.cols;
+    double sum = 0.0;
+    for (int i = 0; i < parts; ++i) sum += sums[(int64_t)matrix * parts + i];
+    const double factor = 1.0 / (sqrt(sum) + eps);
+    const int r0 = (wide ? blockIdx.y : blockIdx.x) * kPrepTile, c0 = (wide ? blockIdx.x : blockIdx.y) * kPrepTile;
+    const T *x = t.x[matrix];
+    const float *m = t.update ? t.m[matrix] : nullptr;
+#pragma unroll
+    for (int i = 0; i < kPrepTile * kPrepTile / kThreads; ++i) {
+        const int r = i * (kThreads / kPrepTile) + tid / kPrepTile, c = tid % kPrepTile;
+        float v = 0.0f;
+        if (r0 + r < t.rows && c0 + c < t.cols) {
+            const int64_t at = (int64_t)(r0 + r) * t.cols + c0 + c;
+            v = widen(x[at]);
+            if (m) v = direction(t, v, m[at]);
+            v = (float)(v * factor) * scale;
+        }
+        tile[r][c] = v;
+    }
+    __syncthreads();
+    f16 *base = space + matrix * b.stride;
+    const int i0 = blockIdx.y * kPrepTile, j0 = blockIdx.x * kPrepTile;  // of X
+#pragma unroll
+    for (int u = 0; u < 2 * kPrepTile * kPrepTile / 8 / kThreads; ++u) {
+        const bool along = u >= kPrepTile * kPrepTile / 8 / kThreads;  // XT: rows are X's columns
+        const int chunk = (u * kThreads + tid) % (kPrepTile * kPrepTile / 8);
+        const int lane = chunk % kWave, block = chunk / kWave;
+        const int row = (block >> 1) * 16 + lane % 16, k = (block & 1) * 32 + lane / 16 * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = along ? k + e : row, j = along ? row : k + e;
+            v[e] = wide ? tile[i][j] : tile[j][i];
+        }
+        f16x8 hi, lo;
+        split(v, hi, lo);
+        f16 *to = base + (along ? b.xt[0] + block_at(j0 + row, i0 + k, pp / 32) : b.x + block_at(i0 + row, j0 + k, qp / 32));
+        *reinterpret_cast<f16x8 *>(to) = hi;
+        *reinterpret_cast<f16x8 *>(to + b.long_plane) = lo;
+    }
+}
+
+// ---------------------------------------------------------------------------- products
+enum { NS_GRAM, NS_POLY, NS_APPLY, NS_LAST };
+
+template <typename T> struct Product {
+    f16 *space;
+    Buffers b;
+    int pp, qp, xt;         // xt: which of the two X^T is read
+    int tiles_m, tiles_n, total, per_xcd;
+    float factor, linear, diagonal;  // value = factor sum + linear (A or X) + diagonal on the diagonal
+    Matrices<T> t;          // NS_LAST
+};
+
+// C = L R^T of one tile; L and R rows of K in blocks.  NP: products of a pair (1 or 3).
+template <typename T, int MODE, int NP, int TILE, int ST>
+__global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
+    constexpr int PL = NP == 1 ? 1 : 2;         // parts that are multiplied
+    constexpr int KB = NP == 1 ? 2 : 1;         // k blocks of a stage
+    constexpr int RB = TILE / 16;               // row blocks of a tile
+    constexpr int NB = 2 * RB * KB * PL;        // blocks of a stage: L's, then R's
+    constexpr int PER = NB / 4;                 // of a wave
+    constexpr int MI = TILE / 32;               // 16 x 16 blocks of a wave along each side
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    constexpr bool HALF = NP == 1;
+    __shared__ __attribute__((aligned(1024))) f16 lds[ST * NB * 512];
+
+    const int flat = (blockIdx.x % kXcds) * p.per_xcd + blockIdx.x / kXcds;  // a matrix's tiles on one XCD
+    if (flat >= p.total) return;
+    int matrix, bm, bn;
+    if (SYM) {
+        const int tiles = p.tiles_m * (p.tiles_m + 1) / 2;
+        matrix = flat / tiles;
+        int rest = flat - matrix * tiles;
+        for (bm = 0; rest >= p.tiles_m - bm; ++bm) rest -= p.tiles_m - bm;
+        bn = bm + rest;
+    } else {
+        const int tiles = p.tiles_m * p.tiles_n;
+        matrix = flat / tiles;
+        const int rest = flat - matrix * tiles;
+        bn = rest / p.tiles_m;
+        bm = rest - bn * p.tiles_m;
+    }
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = wave >> 1, wn = wave & 1, g4 = lane >> 4, li = lane & 15;
+    f16 *const base = p.space + (int64_t)matrix * p.b.stride;
+    const Buffers &b = p.b;
+    const int K = MODE == NS_GRAM ? p.qp : p.pp, KT = K / 32 / KB;
+    const int64_t left = MODE == NS_GRAM ? b.x : MODE == NS_POLY ? b.gram : b.poly;
+    const int64_t right = SYM ? left : b.xt[p.xt];
+    const int64_t plane_l = MODE == NS_GRAM ? b.long_plane : b.short_plane, plane_r = SYM ? plane_l : b.long_plane;
+    const auto rl = make_rsrc(base + left, (uint32_t)(plane_l * PL * 2)), rr = make_rsrc(base + right, (uint32_t)(plane_r * PL * 2));
+
+    uint32_t off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int x = wave + 4 * i, at = x % (NB / 2);  // part, row block, k block
+        const int part = at / (RB * KB), rb = at / KB % RB, kb = at % KB;
+        const int row = (x < NB / 2 ? bm : bn) * RB + rb;
+        off[i] = (uint32_t)((row * (K / 32) + kb) * 1024 + part * (int)((x < NB / 2 ? plane_l : plane_r) * 2) + lane * 16);
+    }
+    auto issue = [&](int kt, int buf) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            lds_void_t *dst = (lds_void_t *)(lds + (buf * NB + wave + 4 * i) * 512);
+            // 4 divides NB / 2: a load is of one operand for every wave.
+            const uint32_t o = off[i];
+            if (4 * i < NB / 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, dst, 16, o, kt * (KB * 1024), 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 16, o, kt * (KB * 1024), 0, 0);
+        }
+    };
+    auto arrive = [&](bool all, auto stages) {
+        constexpr int n = decltype(stages)::value;
+        if (all) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n * PER) : "memory");
+    };
+
+    floatx4 acc[MI][MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s)
+        if (s < KT) issue(s, s);
+    int buf = 0;
+    for (int kt = 0; kt < KT; ++kt) {
+        // Stage kt is in LDS for every wave, and every wave has read stage kt - 1.
+        arrive(kt + ST - 1 > KT, std::integral_constant<int, ST - 2>{});
+        if (kt + ST - 1 < KT) issue(kt + ST - 1, buf == 0 ? ST - 1 : buf - 1);
+        const f16 *l = lds + buf * NB * 512 + lane * 8, *r = l + NB / 2 * 512;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            f16x8 fl[PL][MI], fr[PL][MI];
+#pragma unroll
+            for (int q = 0; q < PL; ++q)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    fl[q][i] = *reinterpret_cast<const f16x8 *>(l + ((q * RB + wm * MI + i) * KB + kb) * 512);
+                    fr[q][i] = *reinterpret_cast<const f16x8 *>(r + ((q * RB + wn * MI + i) * KB + kb) * 512);
+                }
+#pragma unroll
+            for (int q = 0; q < NP; ++q)  // the small products first
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < MI; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[NP == 3 && q == 0][i], fr[NP == 3 && q == 1][j],
+                                                                           acc[i][j], 0, 0, 0);
+        }
+        buf = buf == ST - 1 ? 0 : buf + 1;
+    }
+
+    // Lane (g4, li) holds rows i0 + 4 g4 + r and column j0 + li of block (i, j).
+    const int row0 = (bm * RB + wm * MI) * 16, col0 = (bn * RB + wn * MI) * 16;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            const int row = row0 + i * 16 + 4 * g4, col = col0 + j * 16 + li;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] *= p.factor;
+            if (MODE == NS_POLY || (HALF && !SYM)) {  // A, which is symmetric, or X: four elements along k of X^T
+                const f16 *at = base + (MODE == NS_POLY ? b.gram : b.xt[p.xt]) + block_at(col, row, p.pp / 32);
+                const f16x4 hi = *reinterpret_cast<const f16x4 *>(at);
+                const f16x4 lo = *reinterpret_cast<const f16x4 *>(at + (MODE == NS_POLY ? b.short_plane : b.long_plane));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(p.linear, (float)hi[r] + (float)lo[r], acc[i][j][r]);
+            }
+            if (MODE == NS_POLY && !HALF) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row + r == col) acc[i][j][r] += p.diagonal;
+            }
+        }
+    if constexpr (MODE == NS_LAST) {
+        const Matrices<T> &t = p.t;
+        T *out = t.out[matrix];
+        const int P = min(t.rows, t.cols), Q = max(t.rows, t.cols);
+        const bool wide = t.rows <= t.cols;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = row0 + i * 16 + 4 * g4 + r, col = col0 + j * 16 + li;
+                    if (row >= P || col >= Q) continue;
+                    T *to = out + (wide ? (int64_t)row * t.cols + col : (int64_t)col * t.cols + row);
+                    float v = acc[i][j][r];
+                    if (t.update) v = fmaf(t.keep, widen(*to), -t.rate * v);
+                    T o;
+                    narrow(v, o);
+                    *to = o;
+                }
+        return;
+    }
+    // Column-major blocks, straight from the registers: rows are the tile's columns.
+    const int64_t to_t = MODE == NS_GRAM ? b.gram : MODE == NS_POLY ? b.poly : b.xt[p.xt ^ 1];
+    const int64_t to_n = SYM ? to_t : b.x, plane = SYM ? b.short_plane : b.long_plane;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
+            f16x4 hi, lo;
+            split(v, hi, lo);
+            f16 *at = base + to_t + block_at(col0 + j * 16 + li, row0 + i * 16 + 4 * g4, p.pp / 32);
+            *reinterpret_cast<f16x4 *>(at) = hi;
+            if (!(MODE == NS_POLY && HALF)) *reinterpret_cast<f16x4 *>(at + plane) = lo;
+        }
+    if (SYM && bm == bn) return;
+    // Row-major blocks, through wave-private LDS.
+    lds_barrier();  // every wave has read its last stage
+    constexpr int kPitch = 36;
+    float *stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
+    const int kblocks = (SYM ? p.pp : p.qp) / 32;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; j += 2) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) stage[(4 * g4 + r) * kPitch + x * 16 + li] = acc[i][j + x][r];
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = stage[li * kPitch + g4 * 8 + e];
+            f16x8 hi, lo;
+            split(v, hi, lo);
+            f16 *at = base + to_n + block_at(row0 + i * 16 + li, col0 + j * 16 + g4 * 8, kblocks);
+            *reinterpret_cast<f16x8 *>(at) = hi;
+            if (!HALF || MODE == NS_GRAM) *reinterpret_cast<f16x8 *>(at + plane) = lo;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        }
+}
+
+// -------------------------------------------------------------------------------- host
+struct Plan {
+    int p, q, pp, qp, tile, parts, group;
+    Buffers b;
+    size_t sums, bytes;
+};
+
+template <int N> using Int = std::integral_constant<int, N>;
+
+int round_up(int x, int to) { return (x + to - 1) / to * to; }
+
+Plan ns_plan(int count, int rows, int cols) {
+    Plan s{};
+    s.p = std::min(rows, cols);
+    s.q = std::max(rows, cols);
+    s.tile = s.p <= 256 ? 64 : 128;
+    s.pp = round_up(s.p, s.tile);
+    s.qp = round_up(s.q, s.tile);
+    s.group = std::min(count, kGroup);
+    const int64_t n = (int64_t)rows * cols;
+    s.parts = (int)std::min<int64_t>(kSumParts, (n + kSumRun - 1) / kSumRun);
+    s.b.long_plane = (int64_t)s.pp * s.qp;
+    s.b.short_plane = (int64_t)s.pp * s.pp;
+    s.b.x = 0;
+    s.b.xt[0] = 2 * s.b.long_plane;
+    s.b.xt[1] = 4 * s.b.long_plane;
+    s.b.gram = 6 * s.b.long_plane;
+    s.b.poly = s.b.gram + 2 * s.b.short_plane;
+    s.b.stride = s.b.poly + 2 * s.b.short_plane;
+    s.sums = (size_t)s.b.stride * sizeof(f16) * s.group;
+    s.bytes = s.sums + (size_t)s.group * s.parts * sizeof(double);
+    return s;
+}
+
+const char *ns_refusal(int count, int rows, int cols) {
+    if (count < 0 || rows < 0 || cols < 0) return "newton schulz: negative size";
+    if (count == 0 || rows == 0 || cols == 0) return nullptr;
+    // Offsets inside an operand are 32-bit: two parts of two bytes for each padded element.
+    if (rows > 1 << 22 || cols > 1 << 22 || (int64_t)round_up(rows, 128) * round_up(cols, 128) > (int64_t)1 << 28)
+        return "newton schulz: a matrix may have 2^28 elements, in sides padded to 128, and sides of 2^22";
+    return nullptr;
+}
+
+// For each step, the scales of X, A and P (powers of two), from a bound of X's singular values.
+struct Scales {
+    float x[kStepsMost + 1], gram[kStepsMost], poly[kStepsMost];
+};
+
+const char *ns_scales(int steps, double a, double b, double c, bool half, Scales &s) {
+    const auto scale = [](double bound) {
+        return (float)std::ldexp(1.0, std::min(40, (int)std::floor(std::log2(kBelow / std::max(bound, 1e-30)))));
+    };
+    const double base = half ? 0.0 : a;  // P holds a I where X is multiplied by it in whole
+    double bound = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        s.x[k] = scale(bound);
+        const double top = bound * bound;  // of X's squared singular values
+        s.gram[k] = scale(top);
+        // Extremes of base + b u + c u^2 and of t (a + b t^2 + c t^4) over the bound: ends and stationary points.
+        double poly = std::max(std::fabs(base), std::fabs(base + b * top + c * top * top)), next = std::fabs(bound * (a + b * top + c * top * top));
+        if (c != 0.0) {
+            const double u = -b / (2 * c);
+            if (u > 0 && u < top) poly = std::max(poly, std::fabs(base + b * u + c * u * u));
+        }
+        const double disc = 9 * b * b - 20 * a * c;
+        if (disc >= 0) {
+            // Both roots of 5 c u^2 + 3 b u + a, without cancellation.
+            const double h = -0.5 * (3 * b + std::copysign(std::sqrt(disc), b));
+            for (const double u : {c != 0 ? h / (5 * c) : -1.0, h != 0 ? a / h : -1.0})
+                if (u > 0 && u < top) next = std::max(next, std::fabs(std::sqrt(u) * (a + b * u + c * u * u)));
+        }
+        s.poly[k] = scale(poly);
+        bound = next * (1.0 + 1e-3);  // rounding
+        if (!(bound <= kGrowthMost)) return "newton schulz: these coefficients let singular values grow past 256";
+    }
+    s.x[steps] = 1.0f;
+    return nullptr;
+}
+
+template <typename T, int MODE, int NP, int TILE, int ST>
+hipError_t launch_product(Product<T> &p, int tiles_m, int tiles_n, int count, hipStream_t s) {
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    p.tiles_m = tiles_m; p.tiles_n = tiles_n;
+    p.total = count * (SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n);
+    p.per_xcd = ceil_div(p.total, kXcds);
+    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TILE, ST>), dim3(p.per_xcd * kXcds), dim3(kThreads), 0, s, p);
+    return hipGetLastError();
+}
+
+template <typename T, int NP, int TILE, int ST>
+int ns_group(const Plan &plan, const Matrices<T> &t, const Scales &scales, int steps, float a, float b, float c, double eps,
+             char *space, hipStream_t s) {
+    double *sums = reinterpret_cast<double *>(space + plan.sums);
+    f16 *halves = reinterpret_cast<f16 *>(space);
+    hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(plan.parts, t.count), dim3(kThreads), 0, s, t, plan.parts, sums);
+    hipLaunchKernelGGL((ns_prepare_kernel<T>), dim3(plan.qp / kPrepTile, plan.pp / kPrepTile, t.count), dim3(kThreads), 0, s, t,
+                       plan.parts, sums, eps, scales.x[0], halves, plan.b, plan.pp, plan.qp);
+    YUF_LAUNCH_CHECK("newton schulz");
+    const int tm = plan.pp / TILE, tn = plan.qp / TILE;
+    Product<T> p{};
+    p.space = halves; p.b = plan.b; p.pp = plan.pp; p.qp = plan.qp; p.t = t;
+    for (int k = 0; k < steps; ++k) {
+        const float x = scales.x[k], gram = scales.gram[k], poly = scales.poly[k], next = scales.x[k + 1];
+        p.xt = k & 1;
+        p.factor = gram / (x * x);
+        YUF_HIP_TRY((launch_product<T, NS_GRAM, NP, TILE, ST>(p, tm, tm, t.count, s)));
+        p.factor = c * (poly / (gram * gram)); p.linear = b * (poly / gram); p.diagonal = a * poly;
+        YUF_HIP_TRY((launch_product<T, NS_POLY, NP, TILE, ST>(p, tm, tm, t.count, s)));
+        p.factor = next / (poly * x); p.linear = a * (next / x);
+        if (k + 1 < steps) YUF_HIP_TRY((launch_product<T, NS_APPLY, NP, TILE, ST>(p, tm, tn, t.count, s)));
+        else YUF_HIP_TRY((launch_product<T, NS_LAST, NP, TILE, ST>(p, tm, tn, t.count, s)));
+    }
+    return YUF_OK;
+}
+
+// Whether something that is written shares memory with anything else.  A matrix may be replaced by its result.
+template <typename T>
+const char *ns_overlap(int count, size_t n, const T *const *x, float *const *m, T *const *out, void *workspace, size_t bytes) {
+    struct Run {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::vector<Run> runs;
+    runs.reserve((size_t)count * 3 + 1);
+    const auto add = [&](const void *p, size_t size, bool written) {
+        runs.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + size, written});
+    };
+    add(workspace, bytes, true);
+    for (int i = 0; i < count; ++i) {
+        if (!x[i] || !out[i] || (m && !m[i])) return "newton schulz: null matrix";
+        if (m || x[i] != out[i]) add(x[i], n * sizeof(T), false);
+        add(out[i], n * sizeof(T), true);
+        if (m) add(m[i], n * sizeof(float), true);
+    }
+    std::sort(runs.begin(), runs.end(), [](const Run &a, const Run &b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;  // where the runs so far end
+    for (const Run &r : runs) {
+        if (r.begin < written || (r.written && r.begin < any)) return "newton schulz: matrices may not overlap each other or the workspace";
+        any = std::max(any, r.end);
+        if (r.written) written = std::max(written, r.end);
+    }
+    return nullptr;
+}
+
+template <typename T>
+int newton_schulz(int count, int rows, int cols, const T *const *x, float *const *m, T *const *out, Matrices<T> t, int steps,
+                  double a, double b, double c, double eps, void *workspace, void *stream) {
+    if (const char *why = ns_refusal(count, rows, cols)) return fail(YUF_ERR_INVALID, why);
+    if (steps < 1 || steps > kStepsMost) return fail(YUF_ERR_INVALID, "newton schulz: steps must be 1 to 64");
+    if (!(eps >= 0.0) || !std::isfinite(eps)) return fail(YUF_ERR_INVALID, "newton schulz: eps must be finite and not negative");
+    const bool one_part = sizeof(T) == 2 && std::min(rows, cols) > kOnePartRows && steps <= kOnePartSteps;
+    Scales scales{};
+    if (const char *why = ns_scales(steps, a, b, c, one_part, scales)) return fail(YUF_ERR_INVALID, why);
+    if (count == 0 || rows == 0 || cols == 0) return YUF_OK;
+    if (!x || !out || (t.update && !m)) return fail(YUF_ERR_INVALID, "newton schulz: null list of matrices");
+    if (!workspace || !scratch_aligned(workspace))
+        return fail(YUF_ERR_INVALID, "newton schulz: the workspace must be given and 256-byte aligned");
+    const Plan plan = ns_plan(count, rows, cols);
+    try {
+        if (const char *why = ns_overlap(count, (size_t)rows * cols, x, m, out, workspace, plan.bytes)) return fail(YUF_ERR_INVALID, why);
+    } catch (const std::bad_alloc &) {
+        return fail(YUF_ERR_OOM, "newton schulz: no host memory for the list of matrices");
+    }
+    t.rows = rows; t.cols = cols;
+    for (int first = 0; first < count; first += plan.group) {
+        t.count = std::min(plan.group, count - first);
+        for (int i = 0; i < t.count; ++i) {
+            t.x[i] = x[first + i];
+            t.out[i] = out[first + i];
+            t.m[i] = t.update ? m[first + i] : nullptr;
+        }
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        char *at = static_cast<char *>(workspace);
+        const auto run = [&](auto np, auto tile, auto stages) {
+            return ns_group<T, decltype(np)::value, decltype(tile)::value, decltype(stages)::value>(
+                plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
+        };
+        int rc;
+        if constexpr (sizeof(T) == 2) {
+            if (one_part) {
+                rc = plan.tile == 64 ? run(Int<1>{}, Int<64>{}, Int<4>{}) : run(Int<1>{}, Int<128>{}, Int<2>{});
+                if (rc != YUF_OK) return rc;
+                continue;
+            }
+        }
+        rc = plan.tile == 64 ? run(Int<3>{}, Int<64>{}, Int<4>{}) : run(Int<3>{}, Int<128>{}, Int<2>{});
+        if (rc != YUF_OK) return rc;
+    }
+    return YUF_OK;
+}
+
+template <typename T>
+int muon_step(int count, int rows, int cols, const T *const *grads, float *const *momenta, T *const *params, double lr,
+              double momentum, int nesterov, double weight_decay, int steps, double a, double b, double c, double eps,
+              void *workspace, void *stream) {
+    if (nesterov != 0 && nesterov != 1) return fail(YUF_ERR_INVALID, "muon step: nesterov must be 0 or 1");
+    if (!std::isfinite(lr) || !std::isfinite(momentum) || !std::isfinite(weight_decay))
+        return fail(YUF_ERR_INVALID, "muon step: lr, momentum and weight decay must be finite");
+    Matrices<T> t{};
+    t.update = true;
+    t.nesterov = nesterov != 0;
+    t.beta = (float)momentum; t.rest = (float)(1.0 - momentum);
+    t.keep = (float)(1.0 - lr * weight_decay);
+    t.rate = (float)(lr * std::sqrt(std::max(1.0, cols > 0 ? (double)rows / cols : 1.0)));
+    return newton_schulz<T>(count, rows, cols, grads, momenta, params, t, steps, a, b, c, eps, workspace, stream);
+}
+
+}  // namespace
+}  // namespace yuf
+
+extern "C" size_t yuf_newton_schulz_workspace(int count, int rows, int cols) {
+    if (yuf::ns_refusal(count, rows, cols) || count == 0 || rows == 0 || cols == 0) return 0;
+    return yuf::ns_plan(count, rows, cols).bytes;
+}
+
+extern "C" int yuf_newton_schulz_f32(int count, int rows, int cols, const float *const *x, float *const *out, int steps, double a,
+                                     double b, double c, double eps, void *workspace, void *stream) {
+    return yuf::newton_schulz<float>(count, rows, cols, x, nullptr, out, {}, steps, a, b, c, eps, workspace, stream);
+}
+
+extern "C" int yuf_newton_schulz_bf16(int count, int rows, int cols, const uint16_t *const *x, uint16_t *const *out, int steps,
+                                      double a, double b, double c, double eps, void *workspace, void *stream) {
+    return yuf::newton_schulz<uint16_t>(count, rows, cols, x, nullptr, out, {}, steps, a, b, c, eps, workspace, stream);
+}
+
+extern "C" int yuf_muon_step_f32(int count, int rows, int cols, float *const *params, const float *const *grads,
+                                 float *const *momenta, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                                 double a, double b, double c, double eps, void *workspace, void *stream) {
+    return yuf::muon_step<float>(count, rows, cols, grads, momenta, params, lr, momentum, nesterov, weight_decay, steps, a, b, c,
+                                 eps, workspace, stream);
+}
+
+extern "C" int yuf_muon_step_bf16(int count, int rows, int cols, uint16_t *const *params, const uint16_t *const *grads,
+                                  float *const *momenta, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                                  double a, double b, double c, double eps, void *workspace, void *stream) {
+    return yuf::muon_step<uint16_t>(count, rows, cols, grads, momenta, params, lr, momentum, nesterov, weight_decay, steps, a, b,
+                                    c, eps, workspace, stream);
+}

@@ -20,6 +20,8 @@ process inside torch before an operator is asked.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from ._lib import check, lib
@@ -543,3 +545,107 @@ class _Embedding(torch.autograd.Function):
         _not_captured("embedding")
         (tokens,) = ctx.saved_tensors
         return None, embedding_grad(tokens, dout, *ctx.how), None, None
+
+
+# ------------------------------------------------------------- weight update
+_NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # Jordan's, of the Muon optimiser
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _check_matrices(name: str, matrices, device, dtype) -> None:
+    for x in matrices:
+        if x.ndim != 2:
+            raise ValueError(f"{name} must be matrices, got shape {list(x.shape)}")
+        if not x.is_cuda or x.device != device:
+            raise ValueError(f"{name} must be on the same GPU")
+        if x.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}")
+
+
+def newton_schulz(x, steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float = 1e-7):
+    """Matrices orthogonalised by Newton-Schulz products: ``X = x / (|x|_F + eps)``, then
+    ``steps`` times ``A = X X^T, X <- a X + (b A + c A A) X``, on the transpose where there
+    are more rows than columns.
+
+    ``x``: [..., R, C], or a list of [R, C] of one shape (and a list is returned); float32
+    or bfloat16.  float32 matrices are multiplied to about float32's precision, large bfloat16
+    ones to 11 bits; the result is rounded once.  Not differentiable.
+    """
+    several = isinstance(x, (list, tuple))
+    if several:
+        if not x:
+            return []
+        first = x[0]
+        if any(m.shape != first.shape for m in x):
+            raise ValueError("matrices of a list must have one shape")
+    else:
+        first = x
+    if first.ndim < 2 or (several and first.ndim != 2):
+        raise ValueError("x must have shape [..., R, C], or be a list of [R, C]")
+    if not first.is_cuda:
+        raise ValueError("x must be on the GPU")
+    if first.dtype not in _FLOATS:
+        raise TypeError("newton_schulz takes float32 or bfloat16")
+    if several:
+        _check_matrices("x", x, first.device, first.dtype)
+    if _needs_grad(*(x if several else (x,))):
+        raise ValueError("newton_schulz is not differentiable: detach its input")
+    a, b, c = coefficients
+    rows, cols = first.shape[-2:]
+    with _on(first.device) as stream:
+        if several:
+            taken = [m.contiguous() for m in x]
+            out = [torch.empty_like(m) for m in taken]
+            sources, targets, count = _pointers(taken), _pointers(out), len(x)
+        else:
+            taken = x.contiguous()
+            out = torch.empty_like(taken)
+            count = out.numel() // (rows * cols) if out.numel() else 0
+            size = rows * cols * out.element_size()
+            sources, targets = ((ctypes.c_void_p * count)(*[t.data_ptr() + i * size for i in range(count)]) for t in (taken, out))
+        space = _scratch(lib().yuf_newton_schulz_workspace(count, rows, cols), first.device)
+        entry = lib().yuf_newton_schulz_f32 if first.dtype == torch.float32 else lib().yuf_newton_schulz_bf16
+        check(entry(count, rows, cols, sources, targets, int(steps), float(a), float(b), float(c), float(eps),
+                    space.data_ptr(), stream))
+    return out
+
+
+def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+              steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float = 1e-7) -> None:
+    """One update of weight matrices by their orthogonalised momenta, in place:
+    ``m <- momentum m + (1 - momentum) g``; ``u = momentum m + (1 - momentum) g`` (or ``m`` without
+    ``nesterov``); ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``.
+
+    Lists of matrices, of any shapes; those of one shape are updated together.  ``params`` and
+    ``grads`` float32 or bfloat16, ``momenta`` float32.  ``params`` and ``momenta`` must be
+    contiguous.  Parameters that require a gradient are updated like an optimiser does, without
+    being recorded.
+    """
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"as many grads and momenta as params: got {len(params)}, {len(grads)} and {len(momenta)}")
+    a, b, c = coefficients
+    groups = {}
+    for p, g, m in zip(params, grads, momenta):
+        if not p.is_cuda:
+            raise ValueError("params must be on the GPU")
+        if p.dtype not in _FLOATS:
+            raise TypeError("muon_step takes float32 or bfloat16 params")
+        _check_matrices("params", (p,), p.device, p.dtype)
+        _check_like("grads", g, p.shape, p.device, p.dtype)
+        _check_like("momenta", m, p.shape, p.device)
+        if not p.is_contiguous() or not m.is_contiguous():
+            raise ValueError("params and momenta must be contiguous")
+        groups.setdefault((p.shape, p.dtype, p.device), []).append((p, g.contiguous(), m))
+    for ((rows, cols), dtype, device), members in groups.items():
+        ps, gs, ms = zip(*members)
+        with _on(device) as stream:
+            space = _scratch(lib().yuf_newton_schulz_workspace(len(ps), rows, cols), device)
+            entry = lib().yuf_muon_step_f32 if dtype == torch.float32 else lib().yuf_muon_step_bf16
+            check(entry(len(ps), rows, cols, _pointers(ps), _pointers(gs), _pointers(ms), float(lr), float(momentum),
+                        int(bool(nesterov)), float(weight_decay), int(steps), float(a), float(b), float(c), float(eps),
+                        space.data_ptr(), stream))
+        for x in (*ps, *ms):
+            torch.autograd.graph.increment_version(x)  # as an in-place operation of torch's does
