@@ -6,10 +6,12 @@
 //
 // The gradient's sums run over each token's positions in order, so they do not depend on timing: no
 // atomics on values.  Three launches:
-//   sort:  a workgroup owns a range of tokens and reads all ids twice.  Each of its waves takes a run of
-//          positions: it counts the tokens of the range, and the ids below it (which gives where the range's
-//          positions begin without asking another workgroup); after a scan over tokens and waves it
-//          places its positions, in order.
+//   sort:  a workgroup owns a range of tokens and lists its positions by token.  Its waves take runs of
+//          positions: each counts its tokens, and after a scan over tokens and waves places its positions, in order.
+//          Of few positions the workgroup reads all ids twice (and counts those below the range, which
+//          gives where the range's positions begin without asking another workgroup).  Of many, a launch before
+//          writes the number of each id's range as a byte and counts them by blocks of positions, and the
+//          workgroup picks its positions by comparing 16 bytes at a time.
 //   sum:   a wave walks a chunk of the sorted positions for up to 64 vectors of columns and writes a
 //          token's row where its run ends.  Runs that leave the chunk go to the workspace as fp32 parts.
 //          Further waves clear the rows of tokens that do not occur.
@@ -28,13 +30,22 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortRanges = 256;  // workgroups of the sort: one per CU
 constexpr int kRangeMost = 960;   // tokens of a range: their counters fill 60 KB of LDS
+// Of more than kManyPositions positions the ranges are written down first, where they are at most kNoRange of at
+// most kWidthMost tokens each.
+constexpr int kManyPositions = 4096;
+constexpr int kNoRange = 255, kWidthMost = 512;
+constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
+constexpr int kPicks = 4;         // such reads of a wave in flight
+constexpr int kHeld = 3584;       // positions of a range that are kept in LDS, beside 32 KB of counters
 constexpr int kBatch = 8;         // rows of a wave in flight
+constexpr int kWalks = 3000;     // about 12 waves a CU
 constexpr int kClearRows = 8;     // table rows that a wave looks over for tokens without positions
 constexpr int kJoinWaves = kThreads / kWave;
 constexpr int kVocabMost = 1 << 24, kColsMost = 1 << 24;
 
 // Vectors with the alignment of their elements: rows of odd widths start anywhere.
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 
 template <typename T> struct Vec;
@@ -173,18 +184,102 @@ struct Place {
     int position, token;
 };
 
+// Tokens are numbered by their ranges: a range holds `width` numbers, some of the last ones unused.  Of many positions
+// range r holds the tokens r + 255 j, so that frequent neighbours fall into different ranges.
+struct Numbering {
+    int width;
+    bool spread;
+    __device__ __forceinline__ int number(int token) const { return spread ? token % kNoRange * width + token / kNoRange : token; }
+};
+
 struct SortParams {
     int64_t M;
     int vocab, width, bits;  // tokens of a range, bits of an index into it
+    int numbers;             // of all ranges
     const void *tokens;
     bool wide;
     int64_t padding;  // or -1
     Place *order;     // [M]
-    int *start;       // [V + 1]
+    int *start;       // [numbers + 1]
+    // Of many positions:
+    int64_t block;    // positions of a block
+    int blocks;
+    uint8_t *ranges;  // [blocks block]
+    int *below;       // [blocks][256]
+    Place *picked;    // [M]: a range's positions, if they are more than LDS holds
 };
 
+// The token of a position, or -1: not to be counted.
+__device__ __forceinline__ int counted_token(const SortParams &p, int64_t at) {
+    const int64_t t = token_at(p.tokens, p.wide, at);
+    return t >= 0 && t < p.vocab && t != p.padding ? (int)t : -1;
+}
+
+// Lanes with the same j as this one, among those that are `in`.
+__device__ __forceinline__ uint64_t same_lanes(bool in, int j, int bits) {
+    uint64_t same = __ballot(in);
+    for (int bit = 0; bit < bits; ++bit) {
+        const uint64_t set = __ballot(in && (j >> bit & 1));
+        same &= j >> bit & 1 ? set : ~set;
+    }
+    return same;
+}
+
+// counts [waves][p.width] of the range's tokens -> where each wave's first position of each token goes, the range's
+// positions beginning at `first`; p.start of the range.  The workgroup, between barriers.
+__device__ __forceinline__ void sort_places(const SortParams &p, int range, int first, int *counts, int *sums) {
+    const int low = range * p.width, width = min(p.width, p.numbers - low);
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    for (int base = 0; base < width; base += kSortThreads) {
+        const int j = base + threadIdx.x;
+        int here = 0;
+        if (j < width)
+            for (int w = 0; w < kSortWaves; ++w) here += counts[w * p.width + j];
+        int upto = here;  // inclusive scan over the workgroup
+        for (int step = 1; step < kWave; step *= 2) {
+            const int other = __shfl_up(upto, step);
+            if (lane >= step) upto += other;
+        }
+        if (lane == kWave - 1) sums[wave] = upto;
+        __syncthreads();
+        int before = first, all = 0;
+        for (int w = 0; w < kSortWaves; ++w) {
+            if (w < wave) before += sums[w];
+            all += sums[w];
+        }
+        int next = before + upto - here;
+        if (j < width) {
+            p.start[low + j] = next;
+            for (int w = 0; w < kSortWaves; ++w) {
+                const int n = counts[w * p.width + j];
+                counts[w * p.width + j] = next;
+                next += n;
+            }
+        }
+        first += all;
+        __syncthreads();
+    }
+    if (low + width < p.numbers) return;
+    if (threadIdx.x == 0) p.start[p.numbers] = first;
+    for (int64_t i = first + threadIdx.x; i < p.M; i += kSortThreads) p.order[i] = {0, -1};  // positions that are not counted
+}
+
+// Lanes of the same token rank themselves by comparing its bits; `mine`: the wave's places.
+__device__ __forceinline__ void sort_place(const SortParams &p, bool in, int j, int token, int position, int *mine) {
+    const uint64_t same = same_lanes(in, j, p.bits);
+    const int lane = threadIdx.x % kWave;
+    if (in) {
+        const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+        const int at = mine[j];
+        __builtin_amdgcn_wave_barrier();
+        p.order[at + rank] = {position, token};
+        if (rank == 0) mine[j] = at + __popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams p) {
-    extern __shared__ int counts[];  // [waves][width]: counts, then where a wave's next position goes
+    extern __shared__ int counts[];  // [waves][width]
     __shared__ int below[kSortWaves], sums[kSortWaves];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int low = blockIdx.x * p.width, width = min(p.width, p.vocab - low);
@@ -194,11 +289,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
     // This wave's run of positions, in whole waves of them.
     const int64_t tiles = (p.M + kWave - 1) / kWave;
     const int64_t first = tiles * wave / kSortWaves * kWave, last = min(p.M, tiles * (wave + 1) / kSortWaves * kWave);
-    const auto read = [&](int64_t at) -> int {  // the token, or -1: not to be counted
-        if (at + lane >= last) return -1;
-        const int64_t t = token_at(p.tokens, p.wide, at + lane);
-        return t >= 0 && t < p.vocab && t != p.padding ? (int)t : -1;
-    };
+    const auto read = [&](int64_t at) { return at + lane < last ? counted_token(p, at + lane) : -1; };
     int less = 0;
     for (int64_t at = first; at < last; at += kBatch * kWave) {
         int t[kBatch];
@@ -213,40 +304,9 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
     for (int step = 1; step < kWave; step *= 2) less += __shfl_xor(less, step);
     if (lane == 0) below[wave] = less;
     __syncthreads();
-    // Counts of a token before each wave, then of the tokens before each token.
     int total = 0;
     for (int w = 0; w < kSortWaves; ++w) total += below[w];
-    for (int base = 0; base < width; base += kSortThreads) {
-        const int j = base + threadIdx.x;
-        int here = 0;
-        if (j < width)
-            for (int w = 0; w < kSortWaves; ++w) here += counts[w * p.width + j];
-        int upto = here;  // inclusive scan over the workgroup
-        for (int step = 1; step < kWave; step *= 2) {
-            const int other = __shfl_up(upto, step);
-            if (lane >= step) upto += other;
-        }
-        if (lane == kWave - 1) sums[wave] = upto;
-        __syncthreads();
-        int before = total, all = 0;
-        for (int w = 0; w < kSortWaves; ++w) {
-            if (w < wave) before += sums[w];
-            all += sums[w];
-        }
-        int next = before + upto - here;
-        if (j < width) {
-            p.start[low + j] = next;
-            for (int w = 0; w < kSortWaves; ++w) {
-                const int n = counts[w * p.width + j];
-                counts[w * p.width + j] = next;
-                next += n;
-            }
-        }
-        total += all;
-        __syncthreads();
-    }
-    if (low + width == p.vocab && threadIdx.x == 0) p.start[p.vocab] = total;
-    // Places, in the order of positions: lanes of the same token rank themselves by comparing its bits.
+    sort_places(p, blockIdx.x, total, counts, sums);
     for (int64_t at = first; at < last; at += kBatch * kWave) {
         int t[kBatch];
 #pragma unroll
@@ -254,37 +314,176 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const bool in = t[u] >= low && t[u] < low + width;
-            uint64_t same = __ballot(in);
-            if (same == 0) continue;
-            const int j = t[u] - low;
-            for (int bit = 0; bit < p.bits; ++bit) {
-                const uint64_t set = __ballot(in && (j >> bit & 1));
-                same &= j >> bit & 1 ? set : ~set;
-            }
-            if (in) {
-                const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
-                const int at0 = mine[j];
-                __builtin_amdgcn_wave_barrier();
-                p.order[at0 + rank] = {(int)(at + u * kWave) + lane, t[u]};
-                if (rank == 0) mine[j] = at0 + __popcll(same);
-            }
-            __builtin_amdgcn_wave_barrier();
+            if (__ballot(in) != 0) sort_place(p, in, t[u] - low, t[u], (int)(at + u * kWave) + lane, mine);
         }
     }
 }
 
+// The byte of each position: its range, or 255, of 16 positions e in word e % 4 and byte e / 4; and for each block of positions, how many lie in ranges below each.
+__global__ void __launch_bounds__(kThreads) embedding_ranges_kernel(SortParams p) {
+    __shared__ int counts[kThreads], sums[kThreads / kWave];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    counts[tid] = 0;
+    __syncthreads();
+    const int64_t first = (int64_t)blockIdx.x * p.block;
+    for (int64_t at = first + tid * 4; at < first + p.block; at += kThreads * 4) {
+        uint8_t *to = p.ranges + at / 16 * 16 + at % 16 / 4;
+        int t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = at + e < p.M ? counted_token(p, at + e) : -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int range = t[e] < 0 ? kNoRange : t[e] % kNoRange;
+            if (t[e] >= 0) atomicAdd(&counts[range], 1);
+            to[e * 4] = (uint8_t)range;
+        }
+    }
+    __syncthreads();
+    const int here = counts[tid];
+    int upto = here;
+    for (int step = 1; step < kWave; step *= 2) {
+        const int other = __shfl_up(upto, step);
+        if (lane >= step) upto += other;
+    }
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += sums[w];
+    p.below[blockIdx.x * kThreads + tid] = upto - here;
+}
+
+__global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams p) {
+    extern __shared__ int counts[];  // [waves][width]
+    __shared__ int sums[kSortWaves], offsets[kBlocksMost + 1], bases[kSortWaves];
+    __shared__ Place held[kHeld];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int range = blockIdx.x;
+    int *mine = counts + wave * p.width;
+    for (int i = tid; i < kSortWaves * p.width; i += kSortThreads) counts[i] = 0;
+    // Where the range's positions begin, and where each block's do among them.
+    int before = 0, here = 0;
+    if (tid < p.blocks) {
+        before = p.below[tid * kThreads + range];
+        here = p.below[tid * kThreads + range + 1] - before;
+    }
+    int upto = here;
+    for (int step = 1; step < kWave; step *= 2) {
+        const int other = __shfl_up(upto, step);
+        if (lane >= step) upto += other;
+        before += __shfl_xor(before, step);
+    }
+    if (lane == kWave - 1) sums[wave] = upto;
+    if (lane == 0) bases[wave] = before;
+    __syncthreads();
+    int first = 0, n = 0;
+    for (int w = 0; w < kSortWaves; ++w) {
+        first += bases[w];
+        if (w < wave) upto += sums[w];
+        n += sums[w];
+    }
+    if (tid < p.blocks) offsets[tid] = upto - here;
+    if (tid == 0) offsets[p.blocks] = n;
+    __syncthreads();
+    // The range's positions in order: in LDS where they fit, else in memory.
+    const bool fits = n <= kHeld;
+    const uint32_t pattern = (uint32_t)range * 0x01010101u;
+    const int block0 = p.blocks * wave / kSortWaves, block1 = p.blocks * (wave + 1) / kSortWaves;
+    int next = offsets[block0];
+    for (int64_t at = block0 * p.block; at < block1 * p.block; at += kPicks * kBlockRun) {
+        uint4 bytes[kPicks];
+#pragma unroll
+        for (int u = 0; u < kPicks; ++u)
+            bytes[u] = *reinterpret_cast<const uint4 *>(p.ranges + min(at + u * kBlockRun, block1 * p.block - kBlockRun) + lane * 16);
+#pragma unroll
+        for (int u = 0; u < kPicks; ++u) {
+            if (at + u * kBlockRun >= block1 * p.block) break;
+            // Bit 8 b + w of match: byte b of word w is the range.  In ascending order they are the positions 4 b + w.
+            const uint32_t words[4] = {bytes[u].x, bytes[u].y, bytes[u].z, bytes[u].w};
+            uint32_t match = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t x = words[w] ^ pattern;
+                match |= (~(((x & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | x) & 0x80808080u) >> (7 - w);
+            }
+            if (__ballot(match != 0) == 0) continue;
+            int upto = __popc(match);
+            const int own = upto;
+            for (int step = 1; step < kWave; step *= 2) {
+                const int other = __shfl_up(upto, step);
+                if (lane >= step) upto += other;
+            }
+            int to = next + upto - own;
+            for (; match; match &= match - 1, ++to) {
+                const int bit = __ffs(match) - 1, position = (int)(at + u * kBlockRun) + lane * 16 + (bit >> 3) * 4 + (bit & 7);
+                if (fits) held[to].position = position;
+                else p.picked[first + to].position = position;
+            }
+            next += __builtin_amdgcn_readlane(upto, kWave - 1);
+        }
+    }
+    __syncthreads();
+    const int tiles = (n + kWave - 1) / kWave;
+    const int from = tiles * wave / kSortWaves * kWave, end = min(n, tiles * (wave + 1) / kSortWaves * kWave);
+    Place *list = p.picked + first;
+    for (int at = from; at < end; at += kBatch * kWave) {
+        int position[kBatch], j[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = min(at + u * kWave + lane, end - 1);
+            position[u] = fits ? held[i].position : list[i].position;
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) j[u] = (int)token_at(p.tokens, p.wide, position[u]) / kNoRange;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = at + u * kWave + lane;
+            const bool in = i < end;
+            if (in) (fits ? held[i].token : list[i].token) = j[u];
+            const uint64_t same = same_lanes(in, j[u], p.bits);
+            if (in && (same & (((uint64_t)1 << lane) - 1)) == 0) mine[j[u]] += __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    __syncthreads();
+    sort_places(p, range, first, counts, sums);
+    for (int at = from; at < end; at += kBatch * kWave) {
+        Place place[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = min(at + u * kWave + lane, end - 1);
+            place[u] = fits ? held[i] : list[i];
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (at + u * kWave < end)
+                sort_place(p, at + u * kWave + lane < end, place[u].token, place[u].token * kNoRange + range, place[u].position, mine);
+    }
+}
+
 template <typename T> struct SumParams {
+    int64_t M;
     int vocab, cols, slices;  // slices: of the columns, one vector a lane
+    Numbering numbering;
     int chunk, chunks;        // sorted positions of a wave's walk, and the most such walks
     int clears;               // waves that look for tokens without positions
     float scale;
     const Place *order;
     const int *start;
     const T *dout;
-    float *parts;  // [chunks][2][cols]: of a run that began before the chunk, and of one that goes on behind it
+    float *parts;  // [chunks][2][slices][lanes' columns]: of a run that began before the chunk, and of one that goes on behind it
     T *out;
     bool add;
 };
+
+// A lane's part of a run that enters (0) or leaves (1) a chunk.
+template <typename T>
+__device__ __forceinline__ floatx4 *part_at(const SumParams<T> &p, int64_t chunk, int which, int slice, int lane) {
+    return reinterpret_cast<floatx4 *>(p.parts + (((chunk * 2 + which) * p.slices + slice) * kWave + lane) * Vec<T>::kN);
+}
+template <typename T>
+__device__ __forceinline__ void store_part(floatx4 *to, const float (&x)[Vec<T>::kN]) {
+#pragma unroll
+    for (int e = 0; e < Vec<T>::kN; e += 4) to[e / 4] = floatx4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+}
 
 // Writes a token's finished row: scale x sum, added to what is there where `old` is given.
 template <typename T, bool ADD>
@@ -304,31 +503,32 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
     if (task >= walks) {  // the rows of tokens that have no position
         const int64_t clear = task - walks;
         if (ADD || clear >= p.clears) return;  // the last workgroup's spare waves
-        for (int r = 0; r < kClearRows; ++r) {
-            const int row = (int)clear * kClearRows + r;
-            if (row >= p.vocab) return;
-            if (p.start[row + 1] != p.start[row]) continue;
-            float zero[kN] = {};
-            for (int first = lane * kN; first < p.cols; first += kWave * kN)
-                Columns<T>(first, p.cols).store(p.out + (int64_t)row * p.cols, zero);
+        const int row0 = (int)clear * kClearRows, mine = min(row0 + lane, p.vocab - 1);
+        uint64_t empty = __ballot(lane < kClearRows && row0 + lane < p.vocab && p.start[p.numbering.number(mine) + 1] == p.start[p.numbering.number(mine)]);
+        float zero[kN] = {};
+        for (; empty; empty &= empty - 1) {
+            T *row = p.out + (int64_t)(row0 + __ffsll((unsigned long long)empty) - 1) * p.cols;
+            for (int first = lane * kN; first < p.cols; first += kWave * kN) Columns<T>(first, p.cols).store(row, zero);
         }
         return;
     }
     const int chunk = (int)(task / p.slices), slice = (int)(task - (int64_t)chunk * p.slices);
-    const int all = p.start[p.vocab];
-    const int begin = chunk * p.chunk, end = min(all, begin + p.chunk);
-    if (begin >= end) return;
+    const int begin = chunk * p.chunk, end = (int)min(p.M, (int64_t)begin + p.chunk);
     const Columns<T> c((slice * kWave + lane) * kN, p.cols);
-    const bool goes_on = end < all && p.order[end].token == p.order[end - 1].token;
-    bool came = begin > 0 && p.order[begin - 1].token == p.order[begin].token;  // the present run began before the chunk
+    const int previous = begin > 0 ? p.order[begin - 1].token : -1;
+    bool came = false, goes_on = false;  // the present run began before the chunk; the last one goes on behind it
     float sum[kN] = {};
     for (int base = begin; base < end; base += kWave) {
-        const int n = min(kWave, end - base);
         const Place place = p.order[min(base + lane, end - 1)];
-        // Whether this lane's position ends its token's run.
-        const int next = __shfl_down(place.token, 1);
-        const bool closes = base + lane == end - 1 ? !goes_on : lane == kWave - 1 ? p.order[base + kWave].token != place.token : next != place.token;
-        const uint64_t ends = __ballot(lane < n && closes);
+        const int next = (int64_t)base + lane + 1 < p.M ? p.order[base + lane + 1].token : -1;
+        const bool in = base + lane < end && place.token >= 0;
+        const int n = __popcll(__ballot(in));  // the counted positions come first
+        if (n == 0) break;
+        if (base == begin) came = __builtin_amdgcn_readlane(place.token, 0) == previous;
+        // The positions that end their token's run; the chunk's last one leaves it unfinished where it goes on.
+        const uint64_t more = __ballot(in && next == place.token);
+        goes_on = base + n == end && (more >> (n - 1) & 1);
+        const uint64_t ends = __ballot(in) & ~more;
         for (int j0 = 0; j0 < n; j0 += kBatch) {
             float row[kBatch][kN], old[kBatch][kN];
 #pragma unroll
@@ -350,10 +550,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
                 if (ends >> j & 1) {
                     if (c.any()) {
                         if (came) {
-                            float *part = p.parts + (int64_t)chunk * 2 * p.cols + c.at;
-#pragma unroll
-                            for (int e = 0; e < kN; ++e)
-                                if (e >= c.own && e < c.end) part[e] = sum[e];
+                            store_part<T>(part_at(p, chunk, 0, slice, lane), sum);
                         } else {
                             write_row<T, ADD>(p, c, __builtin_amdgcn_readlane(place.token, j), sum, old[u]);
                         }
@@ -365,12 +562,8 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
             }
         }
     }
-    if (goes_on && c.any()) {  // a run through the whole chunk counts as begun before it
-        float *part = p.parts + ((int64_t)chunk * 2 + (came ? 0 : 1)) * p.cols + c.at;
-#pragma unroll
-        for (int e = 0; e < kN; ++e)
-            if (e >= c.own && e < c.end) part[e] = sum[e];
-    }
+    // A run through the whole chunk counts as begun before it.
+    if (goes_on && c.any()) store_part<T>(part_at(p, chunk, came ? 0 : 1, slice, lane), sum);
 }
 
 // The parts of a run that began in this workgroup's chunk: each wave sums every kJoinWaves-th, then they are joined.
@@ -380,17 +573,17 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumParams<T> p
     __shared__ float joined[kJoinWaves][kN][kWave];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int chunk = blockIdx.x / p.slices, slice = blockIdx.x - chunk * p.slices;
-    const int64_t end = (int64_t)(chunk + 1) * p.chunk;
-    if (end >= p.start[p.vocab]) return;
+    const int64_t begin = (int64_t)chunk * p.chunk, end = begin + p.chunk;
+    if (end >= p.M) return;
     const int token = p.order[end - 1].token;
-    const int from = p.start[token], to = p.start[token + 1];
-    if (from < end - p.chunk || to <= end) return;
+    if (token < 0 || p.order[end].token != token || (begin > 0 && p.order[begin - 1].token == token)) return;
+    const int to = p.start[p.numbering.number(token) + 1];
     const int last = (to - 1) / p.chunk;  // its last chunk
     const Columns<T> c((slice * kWave + lane) * kN, p.cols);
     const auto part = [&](int k, float (&x)[kN]) {  // the run's k-th part
-        const float *at = p.parts + ((int64_t)(chunk + k) * 2 + (k == 0 ? 1 : 0)) * p.cols + c.at;
+        const floatx4 *at = part_at(p, chunk + k, k == 0, slice, lane);
 #pragma unroll
-        for (int e = 0; e < kN; ++e) x[e] = e >= c.own && e < c.end ? at[e] : 0.0f;
+        for (int e = 0; e < kN; ++e) x[e] = at[e / 4][e % 4];
     };
     const int count = last - chunk + 1;
     float sum[kN] = {};
@@ -419,20 +612,31 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumParams<T> p
 }
 
 struct GradPlan {
-    int width, ranges, slices, chunk, chunks, clears;
+    int width, ranges, bits, numbers, slices, chunk, chunks, clears;
+    int blocks;                     // 0: the ranges are not written down
+    int64_t block;
     int64_t sums, joins;            // workgroups
-    size_t order, start, parts, bytes;  // offsets into the workspace, and its size
+    size_t order, start, parts, bytes_of, below, picked, bytes;  // offsets into the workspace, and its size
 };
 
-// Sorted positions of a wave's walk: as many as leave 16 waves a CU, so that short batches still fill the card.
+// Sorted positions of a wave's walk: as many as leave kWalks waves, so that short batches still fill the card.
 GradPlan grad_plan(int64_t M, int V, int D, int vec) {
     GradPlan g{};
     g.ranges = std::max(std::min(V, kSortRanges), ceil_div(V, kRangeMost));
     g.width = ceil_div(V, g.ranges);
     g.ranges = ceil_div(V, g.width);
+    if (M > kManyPositions && V <= kNoRange * kWidthMost) {
+        g.ranges = std::min(V, kNoRange);
+        g.width = ceil_div(V, kNoRange);
+        const int64_t run = (M + kBlocksMost - 1) / kBlocksMost;
+        g.block = (run + kBlockRun - 1) / kBlockRun * kBlockRun;
+        g.blocks = (int)((M + g.block - 1) / g.block);
+    }
+    while (1 << g.bits < g.width) ++g.bits;
+    g.numbers = g.blocks ? g.ranges * g.width : V;
     g.slices = ceil_div(D, kWave * vec);
-    g.chunk = 16;
-    while (g.chunk < 256 && (M + 2 * g.chunk - 1) / (2 * g.chunk) * g.slices >= 4096) g.chunk *= 2;
+    g.chunk = 8;
+    while (g.chunk < 256 && (M + 2 * g.chunk - 1) / (2 * g.chunk) * g.slices >= kWalks) g.chunk *= 2;
     g.chunks = (int)((M + g.chunk - 1) / g.chunk);
     g.clears = ceil_div(V, kClearRows);
     g.joins = (int64_t)g.chunks * g.slices;
@@ -440,8 +644,11 @@ GradPlan grad_plan(int64_t M, int V, int D, int vec) {
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     g.order = 0;
     g.start = round((size_t)M * sizeof(Place));
-    g.parts = g.start + round(((size_t)V + 1) * sizeof(int));
-    g.bytes = g.parts + round((size_t)g.chunks * 2 * D * sizeof(float));
+    g.parts = g.start + round(((size_t)g.numbers + 1) * sizeof(int));
+    g.bytes_of = g.parts + round((size_t)g.chunks * 2 * g.slices * kWave * vec * sizeof(float));
+    g.below = g.bytes_of + round((size_t)(g.blocks * g.block));
+    g.picked = g.below + round((size_t)g.blocks * kThreads * sizeof(int));
+    g.bytes = g.picked + (g.blocks ? round((size_t)M * sizeof(Place)) : 0);
     return g;
 }
 
@@ -458,7 +665,13 @@ const char *grad_refusal(int64_t M, int V, int D, int vec) {
 
 template <typename T, bool ADD>
 int launch_grad(const GradPlan &g, const SortParams &sort, const SumParams<T> &sum, hipStream_t s) {
-    hipLaunchKernelGGL(embedding_sort_kernel, dim3(g.ranges), dim3(kSortThreads), kSortWaves * g.width * sizeof(int), s, sort);
+    const size_t counters = kSortWaves * g.width * sizeof(int);
+    if (g.blocks) {
+        hipLaunchKernelGGL(embedding_ranges_kernel, dim3(g.blocks), dim3(kThreads), 0, s, sort);
+        hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
+    } else {
+        hipLaunchKernelGGL(embedding_sort_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
+    }
     const int64_t sums = ADD ? (g.joins + kThreads / kWave - 1) / (kThreads / kWave) : g.sums;
     hipLaunchKernelGGL((embedding_sum_kernel<T, ADD>), dim3((uint32_t)sums), dim3(kThreads), 0, s, sum);
     if (g.chunks > 1) hipLaunchKernelGGL((embedding_join_kernel<T, ADD>), dim3((uint32_t)g.joins), dim3(kThreads), 0, s, sum);
@@ -482,13 +695,17 @@ int embedding_grad(int64_t M, int V, int D, const void *tokens, int token_bits, 
         return fail(YUF_ERR_INVALID, "embedding gradient: the output and the workspace may not be an input or each other, nor a part of them");
     char *space = static_cast<char *>(workspace);
     SortParams sort{};
-    sort.M = M; sort.vocab = V; sort.width = g.width;
-    while (1 << sort.bits < g.width) ++sort.bits;
+    sort.M = M; sort.vocab = V; sort.width = g.width; sort.bits = g.bits; sort.numbers = g.numbers;
+    sort.block = g.block; sort.blocks = g.blocks;
+    sort.ranges = reinterpret_cast<uint8_t *>(space + g.bytes_of);
+    sort.below = reinterpret_cast<int *>(space + g.below);
+    sort.picked = reinterpret_cast<Place *>(space + g.picked);
     sort.tokens = tokens; sort.wide = token_bits == 64; sort.padding = padding;
     sort.order = reinterpret_cast<Place *>(space + g.order);
     sort.start = reinterpret_cast<int *>(space + g.start);
     SumParams<T> sum{};
-    sum.vocab = V; sum.cols = D; sum.slices = g.slices; sum.chunk = g.chunk; sum.chunks = g.chunks;
+    sum.numbering = {g.width, g.blocks > 0};
+    sum.M = M; sum.vocab = V; sum.cols = D; sum.slices = g.slices; sum.chunk = g.chunk; sum.chunks = g.chunks;
     sum.clears = g.clears;
     sum.scale = (float)scale;
     sum.order = sort.order; sum.start = sort.start; sum.dout = dout;
