@@ -21,8 +21,8 @@
 //
 // Layout: every operand lies in 1 KB blocks of 16 rows x 32 k in the order in which the lanes of
 // v_mfma_f32_16x16x32_f16 hold them (lane l: row l % 16, k = 8 (l / 16) + j), hi blocks and then lo blocks.
-// Blocks go from memory to LDS and from LDS to registers as they lie, without bank conflicts.  X is kept along both sides:
-// X X^T runs over q, P X over p.
+// Blocks go from memory to LDS as they lie, and from LDS to registers without bank conflicts.  X is kept as X^T
+// (rows of q, k over p), as P X takes it; X X^T, which runs over q, reads the same blocks from LDS transposed.
 #include "common.h"
 
 #include <algorithm>
@@ -78,24 +78,73 @@ __device__ __forceinline__ float direction(const Matrices<T> &t, float g, float 
     return t.nesterov ? fmaf(t.beta, m, t.rest * g) : m;
 }
 
+// Four elements of which `count` exist, with the alignment of one.
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { using type = f32x4_u; };
+template <> struct Vec4<uint16_t> { using type = u16x4_u; };
+template <typename T> __device__ __forceinline__ void load4(const T *from, int count, float (&x)[4]) {
+    if (count >= 4) {
+        const auto v = *reinterpret_cast<const typename Vec4<T>::type *>(from);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = widen(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = e < count ? widen(from[e]) : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store4(T *to, int count, const float (&x)[4]) {
+    typename Vec4<T>::type v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        T o;
+        narrow(x[e], o);
+        v[e] = o;
+    }
+    if (count >= 4) {
+        *reinterpret_cast<typename Vec4<T>::type *>(to) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < count) to[e] = v[e];
+    }
+}
+
 // ------------------------------------------------------------------- norm and momentum
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ns_norm_kernel(Matrices<T> t, int parts, double *sums) {
+    constexpr int kBatch = 4;  // vectors of a lane in flight
     __shared__ double waves[kThreads / kWave];
     const int matrix = blockIdx.y;
-    const int64_t n = (int64_t)t.rows * t.cols, run = (n + parts - 1) / parts;
+    const int64_t n = (int64_t)t.rows * t.cols, run = ((n + parts - 1) / parts + 3) / 4 * 4;
     const int64_t first = blockIdx.x * run, last = min(n, first + run);
     const T *x = t.x[matrix];
     float *m = t.update ? t.m[matrix] : nullptr;
     double sum = 0.0;
-    for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
-        float v = widen(x[i]);
-        if (m) {
-            const float next = fmaf(t.beta, m[i], t.rest * v);
-            m[i] = next;
-            v = direction(t, v, next);
+    for (int64_t i = first + threadIdx.x * 4; i < last; i += kBatch * kThreads * 4) {
+        float v[kBatch][4], old[kBatch][4];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t at = i + u * kThreads * 4;
+            load4(x + at, (int)min((int64_t)4, last - at), v[u]);
+            if (m) load4(m + at, (int)min((int64_t)4, last - at), old[u]);
         }
-        sum = fma((double)v, (double)v, sum);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t at = i + u * kThreads * 4;
+            if (m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    old[u][e] = fmaf(t.beta, old[u][e], t.rest * v[u][e]);
+                    v[u][e] = direction(t, v[u][e], old[u][e]);
+                }
+                store4(m + at, (int)min((int64_t)4, last - at), old[u]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e < last) sum = fma((double)v[u][e], (double)v[u][e], sum);
+        }
     }
     sum = wave_sum_f64(sum);
     if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = sum;
@@ -120,14 +169,21 @@ template <int N, typename V> __device__ __forceinline__ void split(const float (
     }
 }
 
+// Four elements of LDS from each lane of a group of 16; lane t gets element t of each run of four lanes' sixteen.
+__device__ __forceinline__ f16x4 transposed(f16 *at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at));
+}
+
 struct Buffers {        // of one matrix, in f16 elements from its base
-    int64_t x, xt[2], gram, poly, stride;
-    int64_t long_plane, short_plane;  // lo blocks lie that far behind the hi blocks: of X, and of A and P
+    int64_t xt[2], gram, poly, stride;
+    int64_t long_plane, short_plane;  // lo blocks lie that far behind the hi blocks: of X^T, and of A and P
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ns_prepare_kernel(Matrices<T> t, int parts, const double *sums, double eps,
-                                                               float scale, f16 *space, Buffers b, int pp, int qp) {
+                                                               float scale, f16 *space, Buffers b, int pp) {
     __shared__ float tile[kPrepTile][kPrepTile + 1];
     const int matrix = blockIdx.z, tid = threadIdx.x;
     const bool wide = t.rows <= t.cols;
@@ -137,36 +193,36 @@ __global__ void __launch_bounds__(kThreads) ns_prepare_kernel(Matrices<T> t, int
     const int r0 = (wide ? blockIdx.y : blockIdx.x) * kPrepTile, c0 = (wide ? blockIdx.x : blockIdx.y) * kPrepTile;
     const T *x = t.x[matrix];
     const float *m = t.update ? t.m[matrix] : nullptr;
+    constexpr int kRows = kPrepTile * kPrepTile / kThreads / 4;
+    float v[kRows][4], u[kRows][4];
+    const int c = tid % (kPrepTile / 4) * 4;
 #pragma unroll
-    for (int i = 0; i < kPrepTile * kPrepTile / kThreads; ++i) {
-        const int r = i * (kThreads / kPrepTile) + tid / kPrepTile, c = tid % kPrepTile;
-        float v = 0.0f;
-        if (r0 + r < t.rows && c0 + c < t.cols) {
-            const int64_t at = (int64_t)(r0 + r) * t.cols + c0 + c;
-            v = widen(x[at]);
-            if (m) v = direction(t, v, m[at]);
-            v = (float)(v * factor) * scale;
-        }
-        tile[r][c] = v;
+    for (int i = 0; i < kRows; ++i) {
+        const int r = (tid / (kPrepTile / 4)) * kRows + i, count = r0 + r < t.rows ? t.cols - c0 - c : 0;
+        const int64_t at = (int64_t)(r0 + r) * t.cols + c0 + c;
+        load4(x + at, count, v[i]);
+        if (m) load4(m + at, count, u[i]);
     }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (m) v[i][e] = direction(t, v[i][e], u[i][e]);
+            tile[(tid / (kPrepTile / 4)) * kRows + i][c + e] = (float)(v[i][e] * factor) * scale;
+        }
     __syncthreads();
     f16 *base = space + matrix * b.stride;
     const int i0 = blockIdx.y * kPrepTile, j0 = blockIdx.x * kPrepTile;  // of X
 #pragma unroll
-    for (int u = 0; u < 2 * kPrepTile * kPrepTile / 8 / kThreads; ++u) {
-        const bool along = u >= kPrepTile * kPrepTile / 8 / kThreads;  // XT: rows are X's columns
-        const int chunk = (u * kThreads + tid) % (kPrepTile * kPrepTile / 8);
-        const int lane = chunk % kWave, block = chunk / kWave;
-        const int row = (block >> 1) * 16 + lane % 16, k = (block & 1) * 32 + lane / 16 * 8;
-        float v[8];
+    for (int w = 0; w < kPrepTile * kPrepTile / 8 / kThreads; ++w) {
+        const int chunk = w * kThreads + tid, lane = chunk % kWave, block = chunk / kWave;
+        const int j = (block >> 1) * 16 + lane % 16, i = (block & 1) * 32 + lane / 16 * 8;
+        float x8[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = along ? k + e : row, j = along ? row : k + e;
-            v[e] = wide ? tile[i][j] : tile[j][i];
-        }
+        for (int e = 0; e < 8; ++e) x8[e] = wide ? tile[i + e][j] : tile[j][i + e];
         f16x8 hi, lo;
-        split(v, hi, lo);
-        f16 *to = base + (along ? b.xt[0] + block_at(j0 + row, i0 + k, pp / 32) : b.x + block_at(i0 + row, j0 + k, qp / 32));
+        split(x8, hi, lo);
+        f16 *to = base + b.xt[0] + block_at(j0 + j, i0 + i, pp / 32);
         *reinterpret_cast<f16x8 *>(to) = hi;
         *reinterpret_cast<f16x8 *>(to + b.long_plane) = lo;
     }
@@ -184,18 +240,23 @@ template <typename T> struct Product {
     Matrices<T> t;          // NS_LAST
 };
 
-// C = L R^T of one tile; L and R rows of K in blocks.  NP: products of a pair (1 or 3).
-template <typename T, int MODE, int NP, int TILE, int ST>
-__global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
+// C = L R^T of one tile of TM x TN; L and R rows of K in blocks.  NP: products of a pair (1 or 3).  WM x WN x SK waves:
+// each has TM / WM x TN / WN of the tile, over every SK-th k block.  A stage holds KB k blocks, ST stages lie in LDS.
+template <typename T, int MODE, int NP, int TM, int TN, int WM, int WN, int SK, int KB, int ST>
+__global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Product<T> p) {
+    constexpr int NW = WM * WN * SK;
     constexpr int PL = NP == 1 ? 1 : 2;         // parts that are multiplied
-    constexpr int KB = NP == 1 ? 2 : 1;         // k blocks of a stage
-    constexpr int RB = TILE / 16;               // row blocks of a tile
-    constexpr int NB = 2 * RB * KB * PL;        // blocks of a stage: L's, then R's
-    constexpr int PER = NB / 4;                 // of a wave
-    constexpr int MI = TILE / 32;               // 16 x 16 blocks of a wave along each side
+    constexpr int LR = TM / 16, RR = TN / 16;   // row blocks
+    constexpr int LB = LR * KB * PL, NB = LB + RR * KB * PL;  // blocks of a stage: L's, then R's
+    constexpr int PER = NB / NW;                // of a wave
+    constexpr int MI = LR / WM, NI = RR / WN;   // 16 x 16 blocks of a wave along each side
+    constexpr int KW = KB / SK;                 // k blocks of a wave in a stage
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     constexpr bool HALF = NP == 1;
-    __shared__ __attribute__((aligned(1024))) f16 lds[ST * NB * 512];
+    static_assert(!SYM || TM == TN, "a symmetric product's tiles are square");
+    static_assert(LB % NW == 0 && NB % NW == 0 && KB % SK == 0 && (SK == 1 || MI % (2 * SK) == 0) && NI % 2 == 0, "shares of a wave");
+    constexpr int kStages = ST * NB * 512, kSplit = SK == 1 ? 0 : WM * WN * SK * (MI / SK) * NI * 256 * 2;  // in f16
+    __shared__ __attribute__((aligned(1024))) f16 lds[kStages > kSplit ? kStages : kSplit];
 
     const int flat = (blockIdx.x % kXcds) * p.per_xcd + blockIdx.x / kXcds;  // a matrix's tiles on one XCD
     if (flat >= p.total) return;
@@ -214,11 +275,11 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
         bm = rest - bn * p.tiles_m;
     }
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wm = wave >> 1, wn = wave & 1, g4 = lane >> 4, li = lane & 15;
+    const int sk = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN, g4 = lane >> 4, li = lane & 15;
     f16 *const base = p.space + (int64_t)matrix * p.b.stride;
     const Buffers &b = p.b;
     const int K = MODE == NS_GRAM ? p.qp : p.pp, KT = K / 32 / KB;
-    const int64_t left = MODE == NS_GRAM ? b.x : MODE == NS_POLY ? b.gram : b.poly;
+    const int64_t left = MODE == NS_GRAM ? b.xt[p.xt] : MODE == NS_POLY ? b.gram : b.poly;
     const int64_t right = SYM ? left : b.xt[p.xt];
     const int64_t plane_l = MODE == NS_GRAM ? b.long_plane : b.short_plane, plane_r = SYM ? plane_l : b.long_plane;
     const auto rl = make_rsrc(base + left, (uint32_t)(plane_l * PL * 2)), rr = make_rsrc(base + right, (uint32_t)(plane_r * PL * 2));
@@ -226,19 +287,27 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
     uint32_t off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int x = wave + 4 * i, at = x % (NB / 2);  // part, row block, k block
-        const int part = at / (RB * KB), rb = at / KB % RB, kb = at % KB;
-        const int row = (x < NB / 2 ? bm : bn) * RB + rb;
-        off[i] = (uint32_t)((row * (K / 32) + kb) * 1024 + part * (int)((x < NB / 2 ? plane_l : plane_r) * 2) + lane * 16);
+        const int x = wave + NW * i, of_r = x >= LB, at = x - of_r * LB;  // part, row block, k block
+        const int rows = of_r ? RR : LR, part = at / (rows * KB), tile = of_r ? bn : bm;
+        int block;
+        if (MODE == NS_GRAM) {  // [k block][its 16 rows of X^T][32 of the tile's rows, which are k there]
+            const int kr = at % (rows * KB) / (rows / 2), ic = at % (rows / 2);
+            block = kr * (p.pp / 32) + tile * (rows / 2) + ic;
+        } else {  // [row block][k block]
+            const int rb = at / KB % rows, kb = at % KB;
+            block = (tile * rows + rb) * (K / 32) + kb;
+        }
+        off[i] = (uint32_t)(block * 1024 + part * (int)((of_r ? plane_r : plane_l) * 2) + lane * 16);
     }
+    const int step = MODE == NS_GRAM ? KB * 2 * (p.pp / 32) * 1024 : KB * 1024;  // of a stage
     auto issue = [&](int kt, int buf) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            lds_void_t *dst = (lds_void_t *)(lds + (buf * NB + wave + 4 * i) * 512);
-            // 4 divides NB / 2: a load is of one operand for every wave.
+            lds_void_t *dst = (lds_void_t *)(lds + (buf * NB + wave + NW * i) * 512);
             const uint32_t o = off[i];
-            if (4 * i < NB / 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, dst, 16, o, kt * (KB * 1024), 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 16, o, kt * (KB * 1024), 0, 0);
+            // NW divides LB: a load is of one operand for every wave.
+            if (NW * i < LB) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, dst, 16, o, kt * step, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 16, o, kt * step, 0, 0);
         }
     };
     auto arrive = [&](bool all, auto stages) {
@@ -247,11 +316,28 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n * PER) : "memory");
     };
 
-    floatx4 acc[MI][MI];
+    // Rows 16 m .. of an operand's part in a stage.  For X X^T lane li of group g4 gives the address of four elements
+    // along the rows, at k = 8 g4 + 4 h + li / 4, and gets its row's four along k.
+    const int turned = (g4 >> 1) * (MODE == NS_GRAM ? 1 : 0), inside = (li % 4 / 2) * 128 + ((g4 & 1) * 8 + li / 4) * 8 + li % 2 * 4;
+    auto fragment = [&](f16 *from, int rows, int part, int m, int kb) -> f16x8 {
+        if constexpr (MODE == NS_GRAM) {
+            f16 *at = from + ((part * KB + kb) * 2 * (rows / 2) + turned * (rows / 2) + m / 2) * 512 + m % 2 * 256 + inside;
+            const f16x4 a = transposed(at), c = transposed(at + 32);
+            return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const f16x8 *>(from + ((part * rows + m) * KB + kb) * 512 + lane * 8);
+        }
+    };
+
+    // The products with a low part are summed apart: a third of the roundings in the large sum.
+    floatx4 acc[MI][NI], low[NP == 3 ? MI : 1][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NI; ++j) {
+            acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (NP == 3) low[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
         if (s < KT) issue(s, s);
@@ -259,37 +345,87 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
     for (int kt = 0; kt < KT; ++kt) {
         // Stage kt is in LDS for every wave, and every wave has read stage kt - 1.
         arrive(kt + ST - 1 > KT, std::integral_constant<int, ST - 2>{});
-        if (kt + ST - 1 < KT) issue(kt + ST - 1, buf == 0 ? ST - 1 : buf - 1);
-        const f16 *l = lds + buf * NB * 512 + lane * 8, *r = l + NB / 2 * 512;
+        f16 *const l = lds + buf * NB * 512, *const r = l + LB * 512;
+        f16x8 fl[KW][PL][MI], fr[KW][PL][NI];
+        const auto next = [&] {
+            if (kt + ST - 1 < KT) issue(kt + ST - 1, buf == 0 ? ST - 1 : buf - 1);
+        };
+        const auto read = [&](int kw) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            f16x8 fl[PL][MI], fr[PL][MI];
+            for (int q = 0; q < PL; ++q) {
 #pragma unroll
-            for (int q = 0; q < PL; ++q)
+                for (int i = 0; i < MI; ++i) fl[kw][q][i] = fragment(l, LR, q, wm * MI + i, kw * SK + sk);
 #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    fl[q][i] = *reinterpret_cast<const f16x8 *>(l + ((q * RB + wm * MI + i) * KB + kb) * 512);
-                    fr[q][i] = *reinterpret_cast<const f16x8 *>(r + ((q * RB + wn * MI + i) * KB + kb) * 512);
-                }
+                for (int j = 0; j < NI; ++j) fr[kw][q][j] = fragment(r, RR, q, wn * NI + j, kw * SK + sk);
+            }
+        };
+        if constexpr (MODE == NS_GRAM) {
+            // The compiler lets the transposing reads wait for every load into LDS: they come before the next ones.
+            static_assert(MODE != NS_GRAM || ST == 2, "loads of one stage in flight");
 #pragma unroll
-            for (int q = 0; q < NP; ++q)  // the small products first
+            for (int kw = 0; kw < KW; ++kw) read(kw);
+            __builtin_amdgcn_sched_barrier(0);
+            next();
+        } else {
+            next();
+        }
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+        for (int kw = 0; kw < KW; ++kw) {
+            if (MODE != NS_GRAM) read(kw);
 #pragma unroll
-                    for (int j = 0; j < MI; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[NP == 3 && q == 0][i], fr[NP == 3 && q == 1][j],
-                                                                           acc[i][j], 0, 0, 0);
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kw][0][i], fr[kw][0][j], acc[i][j], 0, 0, 0);
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NI; ++j)
+                            low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kw][1 - q][i], fr[kw][q][j], low[i][j], 0, 0, 0);
+            }
         }
         buf = buf == ST - 1 ? 0 : buf + 1;
     }
+    if constexpr (NP == 3) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] += low[i][j];
+    }
+    // The waves of a part of the tile give each other their sums of all row blocks but their own ones.
+    constexpr int EI = MI / SK;  // row blocks that a wave finishes: from sk EI on, in acc[0 .. EI)
+    if constexpr (SK == 2) {
+        floatx4 *swap = reinterpret_cast<floatx4 *>(lds) + lane;
+        lds_barrier();  // every wave has read its last stage
+#pragma unroll
+        for (int i = 0; i < EI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                if (sk == 0) swap[((wave * EI + i) * NI + j) * kWave] = acc[EI + i][j];
+                else swap[((wave * EI + i) * NI + j) * kWave] = acc[i][j];
+            }
+        lds_barrier();
+        const int other = (wave + WM * WN) % NW;
+#pragma unroll
+        for (int i = 0; i < EI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const floatx4 theirs = swap[((other * EI + i) * NI + j) * kWave];
+                acc[i][j] = sk == 0 ? acc[i][j] + theirs : theirs + acc[EI + i][j];
+            }
+    }
 
     // Lane (g4, li) holds rows i0 + 4 g4 + r and column j0 + li of block (i, j).
-    const int row0 = (bm * RB + wm * MI) * 16, col0 = (bn * RB + wn * MI) * 16;
+    const int row0 = (bm * LR + wm * MI + sk * EI) * 16, col0 = (bn * RR + wn * NI) * 16;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < EI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) {
+        for (int j = 0; j < NI; ++j) {
             const int row = row0 + i * 16 + 4 * g4, col = col0 + j * 16 + li;
+            if (EI * NI > 16 && j == 0) __builtin_amdgcn_sched_barrier(0);  // a row of blocks' loads at a time: registers
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] *= p.factor;
             if (MODE == NS_POLY || (HALF && !SYM)) {  // A, which is symmetric, or X: four elements along k of X^T
@@ -305,35 +441,67 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
                     if (row + r == col) acc[i][j][r] += p.diagonal;
             }
         }
+    constexpr int kPitch = 36;
+    float *stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
     if constexpr (MODE == NS_LAST) {
         const Matrices<T> &t = p.t;
-        T *out = t.out[matrix];
-        const int P = min(t.rows, t.cols), Q = max(t.rows, t.cols);
-        const bool wide = t.rows <= t.cols;
+        T *const out = t.out[matrix];
+        const int P = min(t.rows, t.cols), Q = max(t.rows, t.cols), cols = t.cols;
+        const bool wide = t.rows <= t.cols, update = t.update;
+        const float keep = t.keep, rate = t.rate;
+        const auto put = [&](T *to, int count, float (&v)[4]) {
+            if (update) {
+                float old[4];
+                load4(to, count, old);
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(keep, old[e], -rate * v[e]);
+            }
+            store4(to, count, v);
+        };
+        if (!wide) {  // rows of the output are columns here
 #pragma unroll
-            for (int j = 0; j < MI; ++j)
+            for (int j = 0; j < NI; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = row0 + i * 16 + 4 * g4 + r, col = col0 + j * 16 + li;
-                    if (row >= P || col >= Q) continue;
-                    T *to = out + (wide ? (int64_t)row * t.cols + col : (int64_t)col * t.cols + row);
-                    float v = acc[i][j][r];
-                    if (t.update) v = fmaf(t.keep, widen(*to), -t.rate * v);
-                    T o;
-                    narrow(v, o);
-                    *to = o;
+                for (int i = 0; i < EI; ++i) {
+                    const int row = row0 + i * 16 + 4 * g4, col = col0 + j * 16 + li;
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
+                    if (col < Q) put(out + (int64_t)col * cols + row, P - row, v);
                 }
+            return;
+        }
+        lds_barrier();  // every wave has read its last stage, and what it was given
+#pragma unroll
+        for (int i = 0; i < EI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; j += 2) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) stage[(4 * g4 + r) * kPitch + x * 16 + li] = acc[i][j + x][r];
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {  // eight lanes a row of 32 columns
+                    const int row = x * 8 + lane / 8, col = col0 + j * 16 + lane % 8 * 4;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = stage[row * kPitch + lane % 8 * 4 + e];
+                    if (row0 + i * 16 + row < P) put(out + (int64_t)(row0 + i * 16 + row) * cols + col, Q - col, v);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            }
         return;
     }
     // Column-major blocks, straight from the registers: rows are the tile's columns.
     const int64_t to_t = MODE == NS_GRAM ? b.gram : MODE == NS_POLY ? b.poly : b.xt[p.xt ^ 1];
-    const int64_t to_n = SYM ? to_t : b.x, plane = SYM ? b.short_plane : b.long_plane;
+    const int64_t plane = SYM ? b.short_plane : b.long_plane;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < EI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) {
+        for (int j = 0; j < NI; ++j) {
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
@@ -343,16 +511,13 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
             *reinterpret_cast<f16x4 *>(at) = hi;
             if (!(MODE == NS_POLY && HALF)) *reinterpret_cast<f16x4 *>(at + plane) = lo;
         }
-    if (SYM && bm == bn) return;
-    // Row-major blocks, through wave-private LDS.
+    if (!SYM || bm == bn) return;
+    // The mirrored tile's blocks, through wave-private LDS.
     lds_barrier();  // every wave has read its last stage
-    constexpr int kPitch = 36;
-    float *stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
-    const int kblocks = (SYM ? p.pp : p.qp) / 32;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < EI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; j += 2) {
+        for (int j = 0; j < NI; j += 2) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -364,7 +529,7 @@ __global__ void __launch_bounds__(kThreads) ns_product_kernel(Product<T> p) {
             for (int e = 0; e < 8; ++e) v[e] = stage[li * kPitch + g4 * 8 + e];
             f16x8 hi, lo;
             split(v, hi, lo);
-            f16 *at = base + to_n + block_at(row0 + i * 16 + li, col0 + j * 16 + g4 * 8, kblocks);
+            f16 *at = base + to_t + block_at(row0 + i * 16 + li, col0 + j * 16 + g4 * 8, p.pp / 32);
             *reinterpret_cast<f16x8 *>(at) = hi;
             if (!HALF || MODE == NS_GRAM) *reinterpret_cast<f16x8 *>(at + plane) = lo;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -379,15 +544,15 @@ struct Plan {
     size_t sums, bytes;
 };
 
-template <int N> using Int = std::integral_constant<int, N>;
-
 int round_up(int x, int to) { return (x + to - 1) / to * to; }
 
 Plan ns_plan(int count, int rows, int cols) {
     Plan s{};
     s.p = std::min(rows, cols);
     s.q = std::max(rows, cols);
-    s.tile = s.p <= 256 ? 64 : 128;
+    // Tiles of the products of one part are larger, so the workspace's paddings are theirs for either kind.
+    const int small = getenv("NTL") ? atoi(getenv("NTL")) : 256, big = getenv("NTB") ? atoi(getenv("NTB")) : 1 << 30;
+    s.tile = s.p <= small ? 64 : s.p >= big ? 256 : 128;
     s.pp = round_up(s.p, s.tile);
     s.qp = round_up(s.q, s.tile);
     s.group = std::min(count, kGroup);
@@ -395,10 +560,9 @@ Plan ns_plan(int count, int rows, int cols) {
     s.parts = (int)std::min<int64_t>(kSumParts, (n + kSumRun - 1) / kSumRun);
     s.b.long_plane = (int64_t)s.pp * s.qp;
     s.b.short_plane = (int64_t)s.pp * s.pp;
-    s.b.x = 0;
-    s.b.xt[0] = 2 * s.b.long_plane;
-    s.b.xt[1] = 4 * s.b.long_plane;
-    s.b.gram = 6 * s.b.long_plane;
+    s.b.xt[0] = 0;
+    s.b.xt[1] = 2 * s.b.long_plane;
+    s.b.gram = 4 * s.b.long_plane;
     s.b.poly = s.b.gram + 2 * s.b.short_plane;
     s.b.stride = s.b.poly + 2 * s.b.short_plane;
     s.sums = (size_t)s.b.stride * sizeof(f16) * s.group;
@@ -451,38 +615,49 @@ const char *ns_scales(int steps, double a, double b, double c, bool half, Scales
     return nullptr;
 }
 
-template <typename T, int MODE, int NP, int TILE, int ST>
-hipError_t launch_product(Product<T> &p, int tiles_m, int tiles_n, int count, hipStream_t s) {
+template <typename T, int MODE, int NP, int TM, int TN, int WM, int WN, int SK, int KB, int ST>
+hipError_t launch_product(Product<T> &p, hipStream_t s) {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    p.tiles_m = tiles_m; p.tiles_n = tiles_n;
-    p.total = count * (SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n);
+    p.tiles_m = p.pp / TM; p.tiles_n = SYM ? p.tiles_m : p.qp / TN;
+    p.total = p.t.count * (SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n);
     p.per_xcd = ceil_div(p.total, kXcds);
-    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TILE, ST>), dim3(p.per_xcd * kXcds), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TM, TN, WM, WN, SK, KB, ST>), dim3(p.per_xcd * kXcds),
+                       dim3(WM * WN * SK * kWave), 0, s, p);
     return hipGetLastError();
 }
 
-template <typename T, int NP, int TILE, int ST>
+// A product in the tiles that its plan names.
+template <typename T, int MODE, int NP> hipError_t launch_mode(const Plan &plan, Product<T> &p, hipStream_t s) {
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    constexpr int ST = MODE == NS_GRAM ? 2 : 4;
+    if (plan.tile == 64) return launch_product<T, MODE, NP, 64, 64, 2, 2, 1, NP == 1 ? 2 : 1, ST>(p, s);
+    if constexpr (NP == 1) {
+        if (plan.tile == 256) return launch_product<T, MODE, NP, 256, 256, 2, 4, 1, 1, ST>(p, s);
+    }
+    return launch_product<T, MODE, NP, 128, 128, 2, 2, 1, NP == 1 ? 2 : 1, 2>(p, s);
+}
+
+template <typename T, int NP>
 int ns_group(const Plan &plan, const Matrices<T> &t, const Scales &scales, int steps, float a, float b, float c, double eps,
              char *space, hipStream_t s) {
     double *sums = reinterpret_cast<double *>(space + plan.sums);
     f16 *halves = reinterpret_cast<f16 *>(space);
     hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(plan.parts, t.count), dim3(kThreads), 0, s, t, plan.parts, sums);
     hipLaunchKernelGGL((ns_prepare_kernel<T>), dim3(plan.qp / kPrepTile, plan.pp / kPrepTile, t.count), dim3(kThreads), 0, s, t,
-                       plan.parts, sums, eps, scales.x[0], halves, plan.b, plan.pp, plan.qp);
+                       plan.parts, sums, eps, scales.x[0], halves, plan.b, plan.pp);
     YUF_LAUNCH_CHECK("newton schulz");
-    const int tm = plan.pp / TILE, tn = plan.qp / TILE;
     Product<T> p{};
     p.space = halves; p.b = plan.b; p.pp = plan.pp; p.qp = plan.qp; p.t = t;
     for (int k = 0; k < steps; ++k) {
         const float x = scales.x[k], gram = scales.gram[k], poly = scales.poly[k], next = scales.x[k + 1];
         p.xt = k & 1;
         p.factor = gram / (x * x);
-        YUF_HIP_TRY((launch_product<T, NS_GRAM, NP, TILE, ST>(p, tm, tm, t.count, s)));
+        YUF_HIP_TRY((launch_mode<T, NS_GRAM, NP>(plan, p, s)));
         p.factor = c * (poly / (gram * gram)); p.linear = b * (poly / gram); p.diagonal = a * poly;
-        YUF_HIP_TRY((launch_product<T, NS_POLY, NP, TILE, ST>(p, tm, tm, t.count, s)));
+        YUF_HIP_TRY((launch_mode<T, NS_POLY, NP>(plan, p, s)));
         p.factor = next / (poly * x); p.linear = a * (next / x);
-        if (k + 1 < steps) YUF_HIP_TRY((launch_product<T, NS_APPLY, NP, TILE, ST>(p, tm, tn, t.count, s)));
-        else YUF_HIP_TRY((launch_product<T, NS_LAST, NP, TILE, ST>(p, tm, tn, t.count, s)));
+        if (k + 1 < steps) YUF_HIP_TRY((launch_mode<T, NS_APPLY, NP>(plan, p, s)));
+        else YUF_HIP_TRY((launch_mode<T, NS_LAST, NP>(plan, p, s)));
     }
     return YUF_OK;
 }
@@ -545,19 +720,13 @@ int newton_schulz(int count, int rows, int cols, const T *const *x, float *const
         }
         hipStream_t s = static_cast<hipStream_t>(stream);
         char *at = static_cast<char *>(workspace);
-        const auto run = [&](auto np, auto tile, auto stages) {
-            return ns_group<T, decltype(np)::value, decltype(tile)::value, decltype(stages)::value>(
-                plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
-        };
         int rc;
         if constexpr (sizeof(T) == 2) {
-            if (one_part) {
-                rc = plan.tile == 64 ? run(Int<1>{}, Int<64>{}, Int<4>{}) : run(Int<1>{}, Int<128>{}, Int<2>{});
-                if (rc != YUF_OK) return rc;
-                continue;
-            }
+            rc = one_part ? ns_group<T, 1>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s)
+                          : ns_group<T, 3>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
+        } else {
+            rc = ns_group<T, 3>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
         }
-        rc = plan.tile == 64 ? run(Int<3>{}, Int<64>{}, Int<4>{}) : run(Int<3>{}, Int<128>{}, Int<2>{});
         if (rc != YUF_OK) return rc;
     }
     return YUF_OK;
