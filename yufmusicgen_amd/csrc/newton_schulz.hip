@@ -43,7 +43,7 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 constexpr int kWave = 64;
 constexpr int kThreads = 256;
 constexpr int kXcds = 8;
-constexpr int kGroup = 32;      // matrices of a launch: their pointers are kernel arguments
+constexpr int kGroup = 64;      // matrices of a launch: their pointers are kernel arguments
 constexpr int kSumParts = 64;   // workgroups of a matrix's norm, at most
 constexpr int kSumRun = 4096;   // elements of such a workgroup, at least
 constexpr int kPrepTile = 64;
@@ -169,11 +169,58 @@ template <int N, typename V> __device__ __forceinline__ void split(const float (
     }
 }
 
-// Four elements of LDS from each lane of a group of 16; lane t gets element t of each run of four lanes' sixteen.
-__device__ __forceinline__ f16x4 transposed(f16 *at) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at));
+// Transposing reads of the fragments of 16 N rows of each of two operands, 32 k.  A lane gives the address (in LDS) of
+// four elements along the rows; lane t of a group of 16 gets element t of each run of four lanes' sixteen.  Blocks of
+// 16 rows are 512 bytes apart, the second four k 64.  The wait is part of the block: the compiler, which knows
+// of no loads in it, would let such reads by its builtin wait for every load into LDS that is on its way.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int N> __device__ __forceinline__ void read_transposed(uint32_t left, uint32_t right, f16x8 (&l)[N], f16x8 (&r)[N]) {
+    static_assert(N == 2 || N == 4, "fragments of a wave");
+    u32x2 x[4 * N];
+    if constexpr (N == 2) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\t"
+            "ds_read_b64_tr_b16 %1, %8 offset:64\n\t"
+            "ds_read_b64_tr_b16 %2, %8 offset:512\n\t"
+            "ds_read_b64_tr_b16 %3, %8 offset:576\n\t"
+            "ds_read_b64_tr_b16 %4, %9\n\t"
+            "ds_read_b64_tr_b16 %5, %9 offset:64\n\t"
+            "ds_read_b64_tr_b16 %6, %9 offset:512\n\t"
+            "ds_read_b64_tr_b16 %7, %9 offset:576\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+            : "v"(left), "v"(right)
+            : "memory");
+    } else {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %16\n\t"
+            "ds_read_b64_tr_b16 %1, %16 offset:64\n\t"
+            "ds_read_b64_tr_b16 %2, %16 offset:512\n\t"
+            "ds_read_b64_tr_b16 %3, %16 offset:576\n\t"
+            "ds_read_b64_tr_b16 %4, %16 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %5, %16 offset:1088\n\t"
+            "ds_read_b64_tr_b16 %6, %16 offset:1536\n\t"
+            "ds_read_b64_tr_b16 %7, %16 offset:1600\n\t"
+            "ds_read_b64_tr_b16 %8, %17\n\t"
+            "ds_read_b64_tr_b16 %9, %17 offset:64\n\t"
+            "ds_read_b64_tr_b16 %10, %17 offset:512\n\t"
+            "ds_read_b64_tr_b16 %11, %17 offset:576\n\t"
+            "ds_read_b64_tr_b16 %12, %17 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %13, %17 offset:1088\n\t"
+            "ds_read_b64_tr_b16 %14, %17 offset:1536\n\t"
+            "ds_read_b64_tr_b16 %15, %17 offset:1600\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7]),
+              "=&v"(x[8]), "=&v"(x[9]), "=&v"(x[10]), "=&v"(x[11]), "=&v"(x[12]), "=&v"(x[13]), "=&v"(x[14]), "=&v"(x[15])
+            : "v"(left), "v"(right)
+            : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        l[i] = __builtin_shufflevector(__builtin_bit_cast(f16x4, x[2 * i]), __builtin_bit_cast(f16x4, x[2 * i + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        r[i] = __builtin_shufflevector(__builtin_bit_cast(f16x4, x[2 * N + 2 * i]), __builtin_bit_cast(f16x4, x[2 * N + 2 * i + 1]), 0, 1, 2, 3,
+                                       4, 5, 6, 7);
+    }
 }
 
 struct Buffers {        // of one matrix, in f16 elements from its base
@@ -240,23 +287,21 @@ template <typename T> struct Product {
     Matrices<T> t;          // NS_LAST
 };
 
-// C = L R^T of one tile of TM x TN; L and R rows of K in blocks.  NP: products of a pair (1 or 3).  WM x WN x SK waves:
-// each has TM / WM x TN / WN of the tile, over every SK-th k block.  A stage holds KB k blocks, ST stages lie in LDS.
-template <typename T, int MODE, int NP, int TM, int TN, int WM, int WN, int SK, int KB, int ST>
-__global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Product<T> p) {
-    constexpr int NW = WM * WN * SK;
-    constexpr int PL = NP == 1 ? 1 : 2;         // parts that are multiplied
-    constexpr int LR = TM / 16, RR = TN / 16;   // row blocks
-    constexpr int LB = LR * KB * PL, NB = LB + RR * KB * PL;  // blocks of a stage: L's, then R's
-    constexpr int PER = NB / NW;                // of a wave
-    constexpr int MI = LR / WM, NI = RR / WN;   // 16 x 16 blocks of a wave along each side
-    constexpr int KW = KB / SK;                 // k blocks of a wave in a stage
+// C = L R^T of one tile of TILE x TILE; L and R rows of K in blocks.  NP: products of a pair (1 or 3).  Four waves have a
+// quarter of the tile each.  A stage holds KB k blocks, ST stages lie in LDS.
+template <typename T, int MODE, int NP, int TILE, int KB, int ST>
+__global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
+    constexpr int NW = kThreads / kWave;
+    constexpr int PL = NP == 1 ? 1 : 2;       // parts that are multiplied
+    constexpr int RB = TILE / 16;             // row blocks of an operand
+    constexpr int HB = RB * KB * PL;          // blocks of a stage: L's, then R's
+    constexpr int PER = 2 * HB / NW;          // of a wave
+    constexpr int MI = RB / 2;                // 16 x 16 blocks of a wave along each side
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     constexpr bool HALF = NP == 1;
-    static_assert(!SYM || TM == TN, "a symmetric product's tiles are square");
-    static_assert(LB % NW == 0 && NB % NW == 0 && KB % SK == 0 && (SK == 1 || MI % (2 * SK) == 0) && NI % 2 == 0, "shares of a wave");
-    constexpr int kStages = ST * NB * 512, kSplit = SK == 1 ? 0 : WM * WN * SK * (MI / SK) * NI * 256 * 2;  // in f16
-    __shared__ __attribute__((aligned(1024))) f16 lds[kStages > kSplit ? kStages : kSplit];
+    static_assert(HB % NW == 0 && MI % 2 == 0, "shares of a wave");
+    constexpr int kStages = ST * 2 * HB * 512;
+    __shared__ __attribute__((aligned(1024))) f16 lds[kStages];
 
     const int flat = (blockIdx.x % kXcds) * p.per_xcd + blockIdx.x / kXcds;  // a matrix's tiles on one XCD
     if (flat >= p.total) return;
@@ -275,7 +320,7 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
         bm = rest - bn * p.tiles_m;
     }
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int sk = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN, g4 = lane >> 4, li = lane & 15;
+    const int wm = wave >> 1, wn = wave & 1, g4 = lane >> 4, li = lane & 15;
     f16 *const base = p.space + (int64_t)matrix * p.b.stride;
     const Buffers &b = p.b;
     const int K = MODE == NS_GRAM ? p.qp : p.pp, KT = K / 32 / KB;
@@ -287,28 +332,29 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
     uint32_t off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int x = wave + NW * i, of_r = x >= LB, at = x - of_r * LB;  // part, row block, k block
-        const int rows = of_r ? RR : LR, part = at / (rows * KB), tile = of_r ? bn : bm;
+        const int x = wave + NW * i, of_r = x >= HB, at = x - of_r * HB;
+        const int part = at / (RB * KB), tile = of_r ? bn : bm;
         int block;
         if (MODE == NS_GRAM) {  // [k block][its 16 rows of X^T][32 of the tile's rows, which are k there]
-            const int kr = at % (rows * KB) / (rows / 2), ic = at % (rows / 2);
-            block = kr * (p.pp / 32) + tile * (rows / 2) + ic;
+            const int kr = at % (RB * KB) / (RB / 2), ic = at % (RB / 2);
+            block = kr * (p.pp / 32) + tile * (RB / 2) + ic;
         } else {  // [row block][k block]
-            const int rb = at / KB % rows, kb = at % KB;
-            block = (tile * rows + rb) * (K / 32) + kb;
+            const int rb = at / KB % RB, kb = at % KB;
+            block = (tile * RB + rb) * (K / 32) + kb;
         }
         off[i] = (uint32_t)(block * 1024 + part * (int)((of_r ? plane_r : plane_l) * 2) + lane * 16);
     }
     const int step = MODE == NS_GRAM ? KB * 2 * (p.pp / 32) * 1024 : KB * 1024;  // of a stage
+    auto issue_one = [&](int i, int kt, int buf) {
+        lds_void_t *dst = (lds_void_t *)(lds + (buf * 2 * HB + wave + NW * i) * 512);
+        const uint32_t o = off[i];
+        // NW divides HB: a load is of one operand for every wave.
+        if (NW * i < HB) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, dst, 16, o, kt * step, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 16, o, kt * step, 0, 0);
+    };
     auto issue = [&](int kt, int buf) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            lds_void_t *dst = (lds_void_t *)(lds + (buf * NB + wave + NW * i) * 512);
-            const uint32_t o = off[i];
-            // NW divides LB: a load is of one operand for every wave.
-            if (NW * i < LB) __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, dst, 16, o, kt * step, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 16, o, kt * step, 0, 0);
-        }
+        for (int i = 0; i < PER; ++i) issue_one(i, kt, buf);
     };
     auto arrive = [&](bool all, auto stages) {
         constexpr int n = decltype(stages)::value;
@@ -316,25 +362,20 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n * PER) : "memory");
     };
 
-    // Rows 16 m .. of an operand's part in a stage.  For X X^T lane li of group g4 gives the address of four elements
-    // along the rows, at k = 8 g4 + 4 h + li / 4, and gets its row's four along k.
-    const int turned = (g4 >> 1) * (MODE == NS_GRAM ? 1 : 0), inside = (li % 4 / 2) * 128 + ((g4 & 1) * 8 + li / 4) * 8 + li % 2 * 4;
-    auto fragment = [&](f16 *from, int rows, int part, int m, int kb) -> f16x8 {
-        if constexpr (MODE == NS_GRAM) {
-            f16 *at = from + ((part * KB + kb) * 2 * (rows / 2) + turned * (rows / 2) + m / 2) * 512 + m % 2 * 256 + inside;
-            const f16x4 a = transposed(at), c = transposed(at + 32);
-            return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-            return *reinterpret_cast<const f16x8 *>(from + ((part * rows + m) * KB + kb) * 512 + lane * 8);
-        }
+    // Where a lane's transposing reads begin in a k block of 32 rows of X^T: for group g4 at k = 8 g4 + li / 4, four
+    // of its 16 rows' elements from 4 (li % 4) on.
+    const auto turned = [&](int part, int m, int kb) {
+        const int block = ((part * KB + kb) * 2 + (g4 >> 1)) * (RB / 2) + m / 2;
+        return block * 512 + li % 4 / 2 * 128 + ((g4 & 1) * 8 + li / 4) * 8 + li % 2 * 4;
     };
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void_t *)lds;
 
     // The products with a low part are summed apart: a third of the roundings in the large sum.
-    floatx4 acc[MI][NI], low[NP == 3 ? MI : 1][NI];
+    floatx4 acc[MI][MI], low[NP == 3 ? MI : 1][MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
+        for (int j = 0; j < MI; ++j) {
             acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
             if (NP == 3) low[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
@@ -342,182 +383,167 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
     for (int s = 0; s < ST - 1; ++s)
         if (s < KT) issue(s, s);
     int buf = 0;
-    for (int kt = 0; kt < KT; ++kt) {
+    const auto multiply = [&](int kt, auto loads) {
+        constexpr bool kLoads = decltype(loads)::value;
         // Stage kt is in LDS for every wave, and every wave has read stage kt - 1.
         arrive(kt + ST - 1 > KT, std::integral_constant<int, ST - 2>{});
-        f16 *const l = lds + buf * NB * 512, *const r = l + LB * 512;
-        f16x8 fl[KW][PL][MI], fr[KW][PL][NI];
-        const auto next = [&] {
-            if (kt + ST - 1 < KT) issue(kt + ST - 1, buf == 0 ? ST - 1 : buf - 1);
-        };
-        const auto read = [&](int kw) {
+        const f16 *const l = lds + buf * 2 * HB * 512, *const r = l + HB * 512;
+        f16x8 fl[KB][PL][MI], fr[KB][PL][MI];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int q = 0; q < PL; ++q) {
+                if constexpr (MODE == NS_GRAM) {
+                    const uint32_t at = lds_at + buf * 2 * HB * 1024;
+                    read_transposed<MI>(at + turned(q, wm * MI, kb) * 2, at + HB * 1024 + turned(q, wn * MI, kb) * 2, fl[kb][q], fr[kb][q]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < MI; ++i) fl[kw][q][i] = fragment(l, LR, q, wm * MI + i, kw * SK + sk);
-#pragma unroll
-                for (int j = 0; j < NI; ++j) fr[kw][q][j] = fragment(r, RR, q, wn * NI + j, kw * SK + sk);
+                    for (int i = 0; i < MI; ++i) {
+                        fl[kb][q][i] = *reinterpret_cast<const f16x8 *>(l + ((q * RB + wm * MI + i) * KB + kb) * 512 + lane * 8);
+                        fr[kb][q][i] = *reinterpret_cast<const f16x8 *>(r + ((q * RB + wn * MI + i) * KB + kb) * 512 + lane * 8);
+                    }
+                }
             }
-        };
-        if constexpr (MODE == NS_GRAM) {
-            // The compiler lets the transposing reads wait for every load into LDS: they come before the next ones.
-            static_assert(MODE != NS_GRAM || ST == 2, "loads of one stage in flight");
+        // The next loads go between the products: a wave that issues its loads one after the other waits for about 80
+        // cycles each, in which it multiplies nothing.
+        const int target = buf == 0 ? ST - 1 : buf - 1;
+        constexpr int kProducts = KB * NP * MI * MI, kEvery = kProducts / PER;
+        static_assert(kProducts % PER == 0, "products between loads");
 #pragma unroll
-            for (int kw = 0; kw < KW; ++kw) read(kw);
-            __builtin_amdgcn_sched_barrier(0);
-            next();
-        } else {
-            next();
-        }
-#pragma unroll
-        for (int kw = 0; kw < KW; ++kw) {
-            if (MODE != NS_GRAM) read(kw);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kw][0][i], fr[kw][0][j], acc[i][j], 0, 0, 0);
-            if constexpr (NP == 3) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int i = 0; i < MI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NI; ++j)
-                            low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kw][1 - q][i], fr[kw][q][j], low[i][j], 0, 0, 0);
+        for (int n = 0; n < kProducts; ++n) {
+            if (kLoads && n % kEvery == 0) {
+                __builtin_amdgcn_sched_barrier(0);
+                issue_one(n / kEvery, kt + ST - 1, target);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            const int kb = n / (NP * MI * MI), q = n / (MI * MI) % NP, i = n / MI % MI, j = n % MI;
+            if (q == 0) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kb][0][i], fr[kb][0][j], acc[i][j], 0, 0, 0);
+            else low[NP == 3 ? i : 0][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kb][NP == 3 ? 2 - q : 0][i], fr[kb][NP == 3 ? q - 1 : 0][j],
+                                                                                  low[NP == 3 ? i : 0][j], 0, 0, 0);
         }
         buf = buf == ST - 1 ? 0 : buf + 1;
-    }
+    };
+    int kt = 0;
+    for (; kt < KT - (ST - 1); ++kt) multiply(kt, std::true_type{});
+    for (; kt < KT; ++kt) multiply(kt, std::false_type{});
     if constexpr (NP == 3) {
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] += low[i][j];
+            for (int j = 0; j < MI; ++j) acc[i][j] += low[i][j];
     }
-    // The waves of a part of the tile give each other their sums of all row blocks but their own ones.
-    constexpr int EI = MI / SK;  // row blocks that a wave finishes: from sk EI on, in acc[0 .. EI)
-    if constexpr (SK == 2) {
-        floatx4 *swap = reinterpret_cast<floatx4 *>(lds) + lane;
-        lds_barrier();  // every wave has read its last stage
+    // Lane (g4, li) holds rows 4 g4 + r and column li of block (i, j).  As rows of an operand the tile's columns' four
+    // elements are neighbours: at a wave's block of 16 columns x 32 rows and at `mine` in it.
+    const int row0 = (bm * RB + wm * MI) * 16, col0 = (bn * RB + wn * MI) * 16;
+    const int kblocks = p.pp / 32;
+    const int mine = (g4 >> 1) * 128 + li * 8 + (g4 & 1) * 4;
+    const auto turned_block = [&](int i, int j) { return ((col0 / 16 + j) * kblocks + row0 / 32 + i / 2) * 512 + i % 2 * 256; };
+    const f16 *const addend = base + (MODE == NS_POLY ? b.gram : b.xt[p.xt]);  // A, which is symmetric, or X
+    const int64_t plane = SYM ? b.short_plane : b.long_plane;
+    const float factor = p.factor, linear = p.linear, diagonal = p.diagonal;
 #pragma unroll
-        for (int i = 0; i < EI; ++i)
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                if (sk == 0) swap[((wave * EI + i) * NI + j) * kWave] = acc[EI + i][j];
-                else swap[((wave * EI + i) * NI + j) * kWave] = acc[i][j];
-            }
-        lds_barrier();
-        const int other = (wave + WM * WN) % NW;
+        for (int j = 0; j < MI; ++j) {
+            if (MODE == NS_POLY || (HALF && !SYM)) {
+                const f16 *at = addend + turned_block(i, j);
+                const f16x4 hi = *reinterpret_cast<const f16x4 *>(at + mine), lo = *reinterpret_cast<const f16x4 *>(at + plane + mine);
 #pragma unroll
-        for (int i = 0; i < EI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                const floatx4 theirs = swap[((other * EI + i) * NI + j) * kWave];
-                acc[i][j] = sk == 0 ? acc[i][j] + theirs : theirs + acc[EI + i][j];
-            }
-    }
-
-    // Lane (g4, li) holds rows i0 + 4 g4 + r and column j0 + li of block (i, j).
-    const int row0 = (bm * LR + wm * MI + sk * EI) * 16, col0 = (bn * RR + wn * NI) * 16;
-#pragma unroll
-    for (int i = 0; i < EI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            const int row = row0 + i * 16 + 4 * g4, col = col0 + j * 16 + li;
-            if (EI * NI > 16 && j == 0) __builtin_amdgcn_sched_barrier(0);  // a row of blocks' loads at a time: registers
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] *= p.factor;
-            if (MODE == NS_POLY || (HALF && !SYM)) {  // A, which is symmetric, or X: four elements along k of X^T
-                const f16 *at = base + (MODE == NS_POLY ? b.gram : b.xt[p.xt]) + block_at(col, row, p.pp / 32);
-                const f16x4 hi = *reinterpret_cast<const f16x4 *>(at);
-                const f16x4 lo = *reinterpret_cast<const f16x4 *>(at + (MODE == NS_POLY ? b.short_plane : b.long_plane));
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(p.linear, (float)hi[r] + (float)lo[r], acc[i][j][r]);
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(linear, (float)hi[r] + (float)lo[r], factor * acc[i][j][r]);
+            } else {
+                acc[i][j] *= factor;
             }
             if (MODE == NS_POLY && !HALF) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (row + r == col) acc[i][j][r] += p.diagonal;
+                    if (row0 + i * 16 + 4 * g4 + r == col0 + j * 16 + li) acc[i][j][r] += diagonal;
             }
         }
-    constexpr int kPitch = 36;
-    float *stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
+    }
     if constexpr (MODE == NS_LAST) {
+        // Through wave-private LDS, 16 lines of the output at a time, so that they are read and written in long runs.
         const Matrices<T> &t = p.t;
         T *const out = t.out[matrix];
-        const int P = min(t.rows, t.cols), Q = max(t.rows, t.cols), cols = t.cols;
+        const int lines = t.rows, cols = t.cols;
         const bool wide = t.rows <= t.cols, update = t.update;
         const float keep = t.keep, rate = t.rate;
-        const auto put = [&](T *to, int count, float (&v)[4]) {
+        // Lane `lane` has four columns of every kLines-th line, of the 16 lines of each of kParts parts.
+        const auto finish = [&](auto run, auto parts, int line0, int at0, auto &&fill) {
+            constexpr int kRun = decltype(run)::value, kParts = decltype(parts)::value, kPitch = kRun + 4;
+            constexpr int kLanes = kRun / 4, kLines = kWave / kLanes, kEach = 16 / kLines;
+            static_assert(NW * 16 * kPitch * 2 <= kStages, "the lines fit the stages' LDS");
+            float *const stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
+            const int line = lane / kLanes, at = lane % kLanes * 4;
+            float old[kParts][kEach][4];  // loaded before the first is waited for
             if (update) {
-                float old[4];
-                load4(to, count, old);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = fmaf(keep, old[e], -rate * v[e]);
+                for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                    for (int u = 0; u < kEach; ++u) {
+                        const int row = line0 + part * 16 + u * kLines + line;
+                        load4(out + (int64_t)row * cols + at0 + at, row < lines ? cols - at0 - at : 0, old[part][u]);
+                    }
             }
-            store4(to, count, v);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                fill(part, stage, kPitch);
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+#pragma unroll
+                for (int u = 0; u < kEach; ++u) {
+                    const int row = line0 + part * 16 + u * kLines + line;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = stage[(u * kLines + line) * kPitch + at + e];
+                        if (update) v[e] = fmaf(keep, old[part][u][e], -rate * v[e]);
+                    }
+                    store4(out + (int64_t)row * cols + at0 + at, row < lines ? cols - at0 - at : 0, v);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            }
         };
-        if (!wide) {  // rows of the output are columns here
-#pragma unroll
-            for (int j = 0; j < NI; ++j)
-#pragma unroll
-                for (int i = 0; i < EI; ++i) {
-                    const int row = row0 + i * 16 + 4 * g4, col = col0 + j * 16 + li;
-                    float v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
-                    if (col < Q) put(out + (int64_t)col * cols + row, P - row, v);
-                }
-            return;
-        }
         lds_barrier();  // every wave has read its last stage, and what it was given
+        if (wide) {
+            finish(std::integral_constant<int, MI * 16>{}, std::integral_constant<int, MI>{}, row0, col0, [&](int i, float *stage, int pitch) {
 #pragma unroll
-        for (int i = 0; i < EI; ++i)
+                for (int j = 0; j < MI; ++j)
 #pragma unroll
-            for (int j = 0; j < NI; j += 2) {
+                    for (int r = 0; r < 4; ++r) stage[(4 * g4 + r) * pitch + j * 16 + li] = acc[i][j][r];
+            });
+        } else {  // lines of the output are columns here
+            finish(std::integral_constant<int, MI * 16>{}, std::integral_constant<int, MI>{}, col0, row0, [&](int j, float *stage, int pitch) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) stage[(4 * g4 + r) * kPitch + x * 16 + li] = acc[i][j + x][r];
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {  // eight lanes a row of 32 columns
-                    const int row = x * 8 + lane / 8, col = col0 + j * 16 + lane % 8 * 4;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = stage[row * kPitch + lane % 8 * 4 + e];
-                    if (row0 + i * 16 + row < P) put(out + (int64_t)(row0 + i * 16 + row) * cols + col, Q - col, v);
-                }
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-            }
+                for (int i = 0; i < MI; ++i) *reinterpret_cast<floatx4 *>(stage + li * pitch + i * 16 + 4 * g4) = acc[i][j];
+            });
+        }
         return;
     }
-    // Column-major blocks, straight from the registers: rows are the tile's columns.
-    const int64_t to_t = MODE == NS_GRAM ? b.gram : MODE == NS_POLY ? b.poly : b.xt[p.xt ^ 1];
-    const int64_t plane = SYM ? b.short_plane : b.long_plane;
+    // Blocks of rows that are the tile's columns, straight from the registers.
+    f16 *const to = base + (MODE == NS_GRAM ? b.gram : MODE == NS_POLY ? b.poly : b.xt[p.xt ^ 1]);
 #pragma unroll
-    for (int i = 0; i < EI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
+        for (int j = 0; j < MI; ++j) {
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
             f16x4 hi, lo;
             split(v, hi, lo);
-            f16 *at = base + to_t + block_at(col0 + j * 16 + li, row0 + i * 16 + 4 * g4, p.pp / 32);
-            *reinterpret_cast<f16x4 *>(at) = hi;
-            if (!(MODE == NS_POLY && HALF)) *reinterpret_cast<f16x4 *>(at + plane) = lo;
+            f16 *at = to + turned_block(i, j);
+            *reinterpret_cast<f16x4 *>(at + mine) = hi;
+            if (!(MODE == NS_POLY && HALF)) *reinterpret_cast<f16x4 *>(at + plane + mine) = lo;
         }
     if (!SYM || bm == bn) return;
     // The mirrored tile's blocks, through wave-private LDS.
     lds_barrier();  // every wave has read its last stage
+    constexpr int kPitch = 36;
+    float *const stage = reinterpret_cast<float *>(lds) + wave * 16 * kPitch;
 #pragma unroll
-    for (int i = 0; i < EI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; j += 2) {
+        for (int j = 0; j < MI; j += 2) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -529,9 +555,9 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
             for (int e = 0; e < 8; ++e) v[e] = stage[li * kPitch + g4 * 8 + e];
             f16x8 hi, lo;
             split(v, hi, lo);
-            f16 *at = base + to_t + block_at(row0 + i * 16 + li, col0 + j * 16 + g4 * 8, p.pp / 32);
-            *reinterpret_cast<f16x8 *>(at) = hi;
-            if (!HALF || MODE == NS_GRAM) *reinterpret_cast<f16x8 *>(at + plane) = lo;
+            f16 *at = to + ((row0 / 16 + i) * kblocks + col0 / 32 + j / 2) * 512;
+            *reinterpret_cast<f16x8 *>(at + lane * 8) = hi;
+            if (!HALF || MODE == NS_GRAM) *reinterpret_cast<f16x8 *>(at + plane + lane * 8) = lo;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
         }
@@ -539,23 +565,34 @@ __global__ void __launch_bounds__(WM * WN * SK * kWave, 2) ns_product_kernel(Pro
 
 // -------------------------------------------------------------------------------- host
 struct Plan {
-    int p, q, pp, qp, tile, parts, group;
+    int p, q, pp, qp, parts, group;
+    bool small_sym, small_apply, many;
     Buffers b;
     size_t sums, bytes;
 };
 
 int round_up(int x, int to) { return (x + to - 1) / to * to; }
 
-Plan ns_plan(int count, int rows, int cols) {
+// Tiles of 128 x 128 load least for their products; of 64 x 64 four times as many, which counts where 128 x 128 ones
+// do not fill the card.  Launches in us, 128 and 64, by tiles of 128 (bf16, one part):
+//   X X^T: 60 x 2560 29 and 17, 120 x 2560 31 and 21, 144 x 4096 46 and 45, 210 x 2560 34 and 38, 288 x 4096 57 and 73;
+//   P X: 100 x 640 11.5 and 8.3, 256 x 1024 17.7 and 18.0, 350 x 640 16.6 and 19.0, 400 x 640 17.3 and 22.5;
+// three products: X X^T 210 x 640 24 and 21, 288 x 1024 38 and 43; A A 288 x 1024 41 and 37; 420 x 640 33 and 36;
+//   P X 100 x 640 18 and 11, 350 x 640 26 and 28.  (Rows of the sum: tiles x k.)
+// Many tiles of one part take stages of one k block, so that three workgroups share a CU: P X 400 x 640 17.3 and 18.7,
+// 1400 x 640 53 and 51, 2800 x 640 116 and 107, 6144 x 1024 303 and 275.
+Plan ns_plan(int count, int rows, int cols, bool one_part) {
     Plan s{};
     s.p = std::min(rows, cols);
     s.q = std::max(rows, cols);
-    // Tiles of the products of one part are larger, so the workspace's paddings are theirs for either kind.
-    const int small = getenv("NTL") ? atoi(getenv("NTL")) : 256, big = getenv("NTB") ? atoi(getenv("NTB")) : 1 << 30;
-    s.tile = s.p <= small ? 64 : s.p >= big ? 256 : 128;
-    s.pp = round_up(s.p, s.tile);
-    s.qp = round_up(s.q, s.tile);
     s.group = std::min(count, kGroup);
+    const int64_t tiles = (s.p + 127) / 128, sym = s.group * (tiles * (tiles + 1) / 2), apply = s.group * tiles * ((s.q + 127) / 128);
+    s.small_sym = s.p <= 128 || sym <= (one_part ? 144 : 256);
+    s.small_apply = s.p <= 128 || apply <= 200;
+    s.many = apply > 1536;
+    const int unit = s.small_sym && s.small_apply ? 64 : 128;
+    s.pp = round_up(s.p, unit);
+    s.qp = round_up(s.q, unit);
     const int64_t n = (int64_t)rows * cols;
     s.parts = (int)std::min<int64_t>(kSumParts, (n + kSumRun - 1) / kSumRun);
     s.b.long_plane = (int64_t)s.pp * s.qp;
@@ -615,26 +652,23 @@ const char *ns_scales(int steps, double a, double b, double c, bool half, Scales
     return nullptr;
 }
 
-template <typename T, int MODE, int NP, int TM, int TN, int WM, int WN, int SK, int KB, int ST>
-hipError_t launch_product(Product<T> &p, hipStream_t s) {
+template <typename T, int MODE, int NP, int TILE, int KB, int ST> hipError_t launch_product(Product<T> &p, hipStream_t s) {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    p.tiles_m = p.pp / TM; p.tiles_n = SYM ? p.tiles_m : p.qp / TN;
+    p.tiles_m = p.pp / TILE; p.tiles_n = SYM ? p.tiles_m : p.qp / TILE;
     p.total = p.t.count * (SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n);
     p.per_xcd = ceil_div(p.total, kXcds);
-    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TM, TN, WM, WN, SK, KB, ST>), dim3(p.per_xcd * kXcds),
-                       dim3(WM * WN * SK * kWave), 0, s, p);
+    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TILE, KB, ST>), dim3(p.per_xcd * kXcds), dim3(kThreads), 0, s, p);
     return hipGetLastError();
 }
 
 // A product in the tiles that its plan names.
 template <typename T, int MODE, int NP> hipError_t launch_mode(const Plan &plan, Product<T> &p, hipStream_t s) {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    constexpr int ST = MODE == NS_GRAM ? 2 : 4;
-    if (plan.tile == 64) return launch_product<T, MODE, NP, 64, 64, 2, 2, 1, NP == 1 ? 2 : 1, ST>(p, s);
-    if constexpr (NP == 1) {
-        if (plan.tile == 256) return launch_product<T, MODE, NP, 256, 256, 2, 4, 1, 1, ST>(p, s);
-    }
-    return launch_product<T, MODE, NP, 128, 128, 2, 2, 1, NP == 1 ? 2 : 1, 2>(p, s);
+    if (SYM ? plan.small_sym : plan.small_apply) return launch_product<T, MODE, NP, 64, NP == 1 ? 2 : 1, 4>(p, s);
+    if constexpr (NP == 3) return launch_product<T, MODE, NP, 128, 1, 2>(p, s);
+    else if constexpr (SYM) return launch_product<T, MODE, NP, 128, 1, 4>(p, s);
+    else if constexpr (MODE == NS_LAST) return launch_product<T, MODE, NP, 128, 1, 3>(p, s);
+    else return plan.many ? launch_product<T, MODE, NP, 128, 1, 2>(p, s) : launch_product<T, MODE, NP, 128, 2, 2>(p, s);
 }
 
 template <typename T, int NP>
@@ -704,7 +738,7 @@ int newton_schulz(int count, int rows, int cols, const T *const *x, float *const
     if (!x || !out || (t.update && !m)) return fail(YUF_ERR_INVALID, "newton schulz: null list of matrices");
     if (!workspace || !scratch_aligned(workspace))
         return fail(YUF_ERR_INVALID, "newton schulz: the workspace must be given and 256-byte aligned");
-    const Plan plan = ns_plan(count, rows, cols);
+    const Plan plan = ns_plan(count, rows, cols, one_part);
     try {
         if (const char *why = ns_overlap(count, (size_t)rows * cols, x, m, out, workspace, plan.bytes)) return fail(YUF_ERR_INVALID, why);
     } catch (const std::bad_alloc &) {
@@ -753,7 +787,7 @@ int muon_step(int count, int rows, int cols, const T *const *grads, float *const
 
 extern "C" size_t yuf_newton_schulz_workspace(int count, int rows, int cols) {
     if (yuf::ns_refusal(count, rows, cols) || count == 0 || rows == 0 || cols == 0) return 0;
-    return yuf::ns_plan(count, rows, cols).bytes;
+    return std::max(yuf::ns_plan(count, rows, cols, false).bytes, yuf::ns_plan(count, rows, cols, true).bytes);  // of either type
 }
 
 extern "C" int yuf_newton_schulz_f32(int count, int rows, int cols, const float *const *x, float *const *out, int steps, double a,
