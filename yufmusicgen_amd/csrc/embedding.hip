@@ -31,8 +31,8 @@ constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortRanges = 256;  // workgroups of the sort: one per CU
 constexpr int kRangeMost = 960;   // tokens of a range: their counters fill 60 KB of LDS
 // Of more than kManyPositions positions the ranges are written down first, where they are at most kNoRange of at
-// most kWidthMost tokens each.
-constexpr int kManyPositions = 4096;
+// most kWidthMost tokens each.  Both forms, us without and with: 4111 of 673 8.4 and 12.0, 16384 of 20480 24 and 16.7.
+constexpr int kManyPositions = 8192;
 constexpr int kNoRange = 255, kWidthMost = 512;
 constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
 constexpr int kPicks = 4;         // such reads of a wave in flight

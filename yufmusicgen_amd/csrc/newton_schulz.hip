@@ -72,6 +72,11 @@ template <typename T> struct Matrices {
     float keep, rate;    // out <- keep out - rate X
 };
 
+// For each step, the scales of X, A and P: powers of two.
+struct Scales {
+    float x[kStepsMost + 1], gram[kStepsMost], poly[kStepsMost];
+};
+
 // The value that is orthogonalised, from its gradient and the updated momentum.
 template <typename T>
 __device__ __forceinline__ float direction(const Matrices<T> &t, float g, float m) {
@@ -563,9 +568,242 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
         }
 }
 
+// ------------------------------------------------------------------------- small matrices
+// Matrices of up to 64 rows (the smaller side) and 768 columns as one workgroup each, from the norm to the result: a
+// step's three products depend on each other, and as launches of their own each is mostly waiting.  A wave owns every
+// kSmallWaves-th block of 32 columns of X and keeps it in registers, in fp32 and in the accumulators' order; it
+// turns a block into operands through its own part of LDS.  X X^T is summed over the waves in order; A and P lie in LDS.
+constexpr int kSmallWaves = 8, kSmallRows = 64, kSmallBlocks = 3;  // blocks of a wave
+constexpr int kSmallThreads = kSmallWaves * kWave, kSmallColumns = kSmallBlocks * kSmallWaves * 32;
+constexpr int kUpper = 10;  // 16 x 16 blocks of A on and above the diagonal: (i, j) is block j (j + 1) / 2 + i
+
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kSmallThreads, 2) ns_small_kernel(Matrices<T> t, Scales scales, int steps, float a, float b, float c,
+                                                                     double eps) {
+    constexpr int KB = kSmallRows / 32, MI = kSmallRows / 16;  // k blocks and row blocks of A and P
+    constexpr int kPlane = kSmallRows * kSmallRows;            // f16 of a part of A or P
+    constexpr int kPitch = 36;                                 // floats of a row of a block in LDS
+    __shared__ __attribute__((aligned(1024))) f16 gram[2 * kPlane], poly[2 * kPlane];
+    __shared__ __attribute__((aligned(16))) floatx4 sums[kSmallWaves][kUpper][kWave];
+    __shared__ double norms[kSmallWaves];
+    static_assert(sizeof(sums[0]) >= kSmallRows * kPitch * sizeof(float), "a wave's sums' place holds a block");
+    const int matrix = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int g4 = lane >> 4, li = lane & 15;
+    const bool wide = t.rows <= t.cols, update = t.update;
+    const int P = min(t.rows, t.cols), Q = max(t.rows, t.cols), cols = t.cols;
+    const T *const x = t.x[matrix];
+    float *const m = update ? t.m[matrix] : nullptr;
+    // Elements (row + r, col), r < 4, of X: a lane's are rows 16 i + 4 g4 + r and columns 32 block + 16 j + li.  In a
+    // matrix of more rows than columns they are neighbours.
+    const auto fetch = [&](const auto *from, int row, int col, float (&v)[4]) {
+        if (!wide) return load4(from + (int64_t)col * cols + row, col < Q ? P - row : 0, v);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = row + r < P && col < Q ? widen(from[(int64_t)(row + r) * cols + col]) : 0.0f;
+    };
+    const auto keep = [&](auto *to, int row, int col, const float (&v)[4]) {
+        using E = std::remove_reference_t<decltype(*to)>;
+        if (!wide) return store4<E>(to + (int64_t)col * cols + row, col < Q ? P - row : 0, v);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            E o;
+            narrow(v[r], o);
+            if (row + r < P && col < Q) to[(int64_t)(row + r) * cols + col] = o;
+        }
+    };
+    floatx4 X[BLOCKS][MI][2];
+    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < BLOCKS; ++w)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = i * 16 + 4 * g4, col = (wave + w * kSmallWaves) * 32 + j * 16 + li;
+                float v[4];
+                fetch(x, row, col, v);
+                if (update) {
+                    float moved[4];
+                    fetch(m, row, col, moved);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        moved[r] = fmaf(t.beta, moved[r], t.rest * v[r]);
+                        v[r] = direction(t, v[r], moved[r]);
+                    }
+                    keep(m, row, col, moved);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sum = fma((double)v[r], (double)v[r], sum);
+                    X[w][i][j][r] = v[r];
+                }
+            }
+    sum = wave_sum_f64(sum);
+    if (lane == 0) norms[wave] = sum;
+    __syncthreads();
+    sum = norms[0];
+    for (int w = 1; w < kSmallWaves; ++w) sum += norms[w];
+    const double factor = 1.0 / (sqrt(sum) + eps);
+#pragma unroll
+    for (int w = 0; w < BLOCKS; ++w)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {  // beyond the matrix 0, also where the factor is infinite
+                    const bool in = i * 16 + 4 * g4 + r < P && (wave + w * kSmallWaves) * 32 + j * 16 + li < Q;
+                    X[w][i][j][r] = in ? (float)(X[w][i][j][r] * factor) * scales.x[0] : 0.0f;
+                }
+    float *const stage = reinterpret_cast<float *>(sums[wave]);
+    const auto fence = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    const auto lay = [&](const floatx4 (&block)[MI][2]) {
+        fence();
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) stage[(i * 16 + 4 * g4 + r) * kPitch + j * 16 + li] = block[i][j][r];
+        fence();
+    };
+    // Writes block (i, j) of a symmetric matrix into both its places in LDS.
+    const auto put = [&](f16 *to, int i, int j, const floatx4 &value) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = value[r];
+        f16x4 hi, lo;
+        split(v, hi, lo);
+        const int row = i * 16 + 4 * g4, col = j * 16 + li;
+        f16 *at = to + block_at(col, row, KB);
+        *reinterpret_cast<f16x4 *>(at) = hi;
+        *reinterpret_cast<f16x4 *>(at + kPlane) = lo;
+        if (i == j) return;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            to[block_at(row + r, col, KB)] = hi[r];
+            to[block_at(row + r, col, KB) + kPlane] = lo[r];
+        }
+    };
+    const auto of = [&](int block, int &i, int &j) {  // block -> (i, j)
+        j = block >= 6 ? 3 : block >= 3 ? 2 : block >= 1 ? 1 : 0;
+        i = block - j * (j + 1) / 2;
+    };
+    const auto mfma3 = [](const f16x8 &lh, const f16x8 &ll, const f16x8 &rh, const f16x8 &rl, floatx4 &high, floatx4 &low) {
+        high = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh, high, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh, low, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl, low, 0, 0, 0);
+    };
+    for (int step = 0; step < steps; ++step) {
+        const float sx = scales.x[step], sa = scales.gram[step], sp = scales.poly[step], next = scales.x[step + 1];
+        {
+            floatx4 high[kUpper], low[kUpper];
+#pragma unroll
+            for (int u = 0; u < kUpper; ++u) high[u] = low[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < BLOCKS; ++w) {
+                lay(X[w]);
+                f16x8 f[2][MI];
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = stage[(i * 16 + li) * kPitch + g4 * 8 + e];
+                    split(v, f[0][i], f[1][i]);
+                }
+#pragma unroll
+                for (int j = 0; j < MI; ++j)
+#pragma unroll
+                    for (int i = 0; i <= j; ++i)
+                        mfma3(f[0][i], f[1][i], f[0][j], f[1][j], high[j * (j + 1) / 2 + i], low[j * (j + 1) / 2 + i]);
+            }
+            fence();
+#pragma unroll
+            for (int u = 0; u < kUpper; ++u) sums[wave][u][lane] = high[u] + low[u];
+        }
+        __syncthreads();
+        for (int u = wave; u < kUpper; u += kSmallWaves) {
+            floatx4 v = sums[0][u][lane];
+            for (int w = 1; w < kSmallWaves; ++w) v += sums[w][u][lane];
+            int i, j;
+            of(u, i, j);
+            put(gram, i, j, v * (sa / (sx * sx)));
+        }
+        __syncthreads();
+        for (int u = wave; u < kUpper; u += kSmallWaves) {
+            int i, j;
+            of(u, i, j);
+            floatx4 high{0.f, 0.f, 0.f, 0.f}, low{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                const f16 *l = gram + (i * KB + k) * 512 + lane * 8, *r = gram + (j * KB + k) * 512 + lane * 8;
+                mfma3(*reinterpret_cast<const f16x8 *>(l), *reinterpret_cast<const f16x8 *>(l + kPlane), *reinterpret_cast<const f16x8 *>(r),
+                      *reinterpret_cast<const f16x8 *>(r + kPlane), high, low);
+            }
+            const f16 *at = gram + block_at(j * 16 + li, i * 16 + 4 * g4, KB);  // A, which is symmetric
+            floatx4 v = (high + low) * (c * (sp / (sa * sa)));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[r] = fmaf(b * (sp / sa), (float)at[r] + (float)at[kPlane + r], v[r]);
+                if (i == j && 4 * g4 + r == li) v[r] += a * sp;
+            }
+            put(poly, i, j, v);
+        }
+        __syncthreads();
+        const float scale = next / (sp * sx);
+#pragma unroll
+        for (int w = 0; w < BLOCKS; ++w) {
+            lay(X[w]);
+            f16x8 f[2][2][KB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = stage[(k * 32 + g4 * 8 + e) * kPitch + j * 16 + li];
+                    split(v, f[0][j][k], f[1][j][k]);
+                }
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                floatx4 high[2], low[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) high[j] = low[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const f16 *l = poly + (i * KB + k) * 512 + lane * 8;
+                    const f16x8 lh = *reinterpret_cast<const f16x8 *>(l), ll = *reinterpret_cast<const f16x8 *>(l + kPlane);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) mfma3(lh, ll, f[0][j][k], f[1][j][k], high[j], low[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) X[w][i][j] = (high[j] + low[j]) * scale;
+            }
+        }
+    }
+    int again = lane;  // its places are computed again: kept from the loads they would take registers all along
+    asm volatile("" : "+v"(again));
+#pragma unroll
+    for (int w = 0; w < BLOCKS; ++w)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = i * 16 + 4 * (again >> 4), col = (wave + w * kSmallWaves) * 32 + j * 16 + (again & 15);
+                float v[4], old[4];
+                if (update) fetch(t.out[matrix], row, col, old);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = update ? fmaf(t.keep, old[r], -t.rate * X[w][i][j][r]) : X[w][i][j][r];
+                keep(t.out[matrix], row, col, v);
+            }
+}
+
 // -------------------------------------------------------------------------------- host
 struct Plan {
     int p, q, pp, qp, parts, group;
+    bool whole;  // a workgroup for each matrix
     bool small_sym, small_apply, many;
     Buffers b;
     size_t sums, bytes;
@@ -587,6 +825,7 @@ Plan ns_plan(int count, int rows, int cols, bool one_part) {
     s.q = std::max(rows, cols);
     s.group = std::min(count, kGroup);
     const int64_t tiles = (s.p + 127) / 128, sym = s.group * (tiles * (tiles + 1) / 2), apply = s.group * tiles * ((s.q + 127) / 128);
+    s.whole = s.p <= kSmallRows && s.q <= kSmallColumns;
     s.small_sym = s.p <= 128 || sym <= (one_part ? 144 : 256);
     s.small_apply = s.p <= 128 || apply <= 200;
     s.many = apply > 1536;
@@ -604,6 +843,7 @@ Plan ns_plan(int count, int rows, int cols, bool one_part) {
     s.b.stride = s.b.poly + 2 * s.b.short_plane;
     s.sums = (size_t)s.b.stride * sizeof(f16) * s.group;
     s.bytes = s.sums + (size_t)s.group * s.parts * sizeof(double);
+    if (s.whole) s.bytes = 256;  // nothing
     return s;
 }
 
@@ -616,11 +856,7 @@ const char *ns_refusal(int count, int rows, int cols) {
     return nullptr;
 }
 
-// For each step, the scales of X, A and P (powers of two), from a bound of X's singular values.
-struct Scales {
-    float x[kStepsMost + 1], gram[kStepsMost], poly[kStepsMost];
-};
-
+// For each step, the scales of X, A and P, from a bound of X's singular values.
 const char *ns_scales(int steps, double a, double b, double c, bool half, Scales &s) {
     const auto scale = [](double bound) {
         return (float)std::ldexp(1.0, std::min(40, (int)std::floor(std::log2(kBelow / std::max(bound, 1e-30)))));
@@ -676,6 +912,20 @@ int ns_group(const Plan &plan, const Matrices<T> &t, const Scales &scales, int s
              char *space, hipStream_t s) {
     double *sums = reinterpret_cast<double *>(space + plan.sums);
     f16 *halves = reinterpret_cast<f16 *>(space);
+    if constexpr (NP == 3) {
+        if (plan.whole) {
+            const int blocks = ceil_div(plan.q, 32 * kSmallWaves);  // of a wave
+            const auto run = [&](auto n) {
+                hipLaunchKernelGGL((ns_small_kernel<T, decltype(n)::value>), dim3(t.count), dim3(kSmallThreads), 0, s, t, scales, steps, a, b,
+                                   c, eps);
+            };
+            if (blocks == 1) run(std::integral_constant<int, 1>{});
+            else if (blocks == 2) run(std::integral_constant<int, 2>{});
+            else run(std::integral_constant<int, kSmallBlocks>{});
+            YUF_LAUNCH_CHECK("newton schulz");
+            return YUF_OK;
+        }
+    }
     hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(plan.parts, t.count), dim3(kThreads), 0, s, t, plan.parts, sums);
     hipLaunchKernelGGL((ns_prepare_kernel<T>), dim3(plan.qp / kPrepTile, plan.pp / kPrepTile, t.count), dim3(kThreads), 0, s, t,
                        plan.parts, sums, eps, scales.x[0], halves, plan.b, plan.pp);

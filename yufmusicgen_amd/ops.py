@@ -519,6 +519,10 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
             raise ValueError("out must be contiguous")
         if _needs_grad(out):
             raise ValueError("out is written in place: it may not require a gradient")
+    return _embedding_backward(tokens, dout, vocab, scale, padding, out)
+
+
+def _embedding_backward(tokens, dout, vocab, scale, padding, out=None):
     tokens, dout = tokens.contiguous(), dout.contiguous()
     dim, count = dout.shape[-1], tokens.numel()
     with _on(dout.device) as stream:
@@ -535,7 +539,7 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
-        ctx.how = (weight.shape[0], scale, None if padding < 0 else padding)
+        ctx.how = (weight.shape[0], scale, padding)
         ctx.save_for_backward(tokens)
         return _embedding_forward(tokens, weight, scale)
 
@@ -544,7 +548,7 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, dout):
         _not_captured("embedding")
         (tokens,) = ctx.saved_tensors
-        return None, embedding_grad(tokens, dout, *ctx.how), None, None
+        return None, _embedding_backward(tokens, dout, *ctx.how), None, None
 
 
 # ------------------------------------------------------------- weight update
