@@ -319,7 +319,8 @@ def check_ns(got, x, kind, floor=0.0, **how):
 
 NS_SHAPES = [(1, 1, 1), (2, 1, 7), (2, 7, 1), (3, 3, 5), (3, 16, 16), (2, 31, 33), (1, 64, 64), (2, 65, 64), (1, 640, 64),
              (2, 64, 640), (1, 127, 129), (2, 256, 257), (2, 257, 256), (1, 300, 700), (3, 640, 640), (1, 1000, 129),
-             (1, 129, 1000), (1, 333, 1111), (2, 1111, 333), (1, 2560, 640), (33, 20, 30), (70, 9, 5)]
+             (1, 129, 1000), (1, 333, 1111), (2, 1111, 333), (1, 2560, 640), (33, 20, 30), (70, 9, 5), (1, 64, 256), (1, 64, 257), (2, 64, 513),
+             (1, 64, 768), (1, 64, 769), (1, 769, 33), (65, 65, 65), (12, 640, 640), (18, 640, 640), (26, 640, 640), (11, 640, 1200)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -334,8 +335,9 @@ def test_newton_schulz(count, rows, cols, kind):
     check_ns(got, x, kind)
     assert torch.equal(x, kept)
     check_ns(ops.newton_schulz(x.mT), x.mT, kind)  # the other orientation, and a strided input
-    one = ops.newton_schulz(x[-1])
-    assert torch.equal(one, got[-1])  # a matrix alone as among others
+    assert torch.equal(got, ops.newton_schulz(x))
+    # A matrix alone: other tiles, and with them the order in which the low parts of A's lower half are summed.
+    check_ns(ops.newton_schulz(x[-1]), x[-1], kind)
     for a, b in zip(ops.newton_schulz(list(x)), got):
         assert torch.equal(a, b)
 
@@ -425,6 +427,26 @@ def test_muon_step_over_a_models_matrices():
         off = (2.0**-8 if p.dtype == torch.bfloat16 else 0) * (step + norms(new_p)) + 4 * loose + LAST * (step + norms(p.detach()))
         assert norms(p.detach().double() - new_p) <= off
         assert ((m.double() - new_m).abs() <= 4 * EPS32 * new_m.abs()).all()
+
+
+def test_muon_step_refuses_before_it_updates():
+    """Matrices that share memory, in one shape or in two: nothing is updated."""
+    from yufmusicgen_amd import ops
+    from yufmusicgen_amd._lib import YufError
+
+    p, g, m = table(50, 12, 8, torch.float32), gradient(51, 12, 8), torch.zeros(12, 8, device="cuda")
+    q, h, n = table(52, 6, 8, torch.float32), gradient(53, 6, 8), torch.zeros(6, 8, device="cuda")
+    before = [t.clone() for t in (p, m, q, n)]
+    for params, grads, momenta in (([q, p, p], [h, g, g], [n, m, m.clone()]), ([q, p, p.view(8, 12)], [h, g, g.view(8, 12)], [n, m, m.clone().view(8, 12)]),
+                                   ([q, p], [h, g], [n, p]), ([q, p], [q, g], [n, m]), ([p, p[:6]], [g, h], [m, n])):
+        with pytest.raises((ValueError, YufError), match="overlap"):
+            ops.muon_step(params, grads, momenta, 0.1)
+    for refused in (dict(steps=0), dict(eps=-1.0), dict(coefficients=(30.0, 0.0, 0.0)), dict(lr=float("nan"))):
+        with pytest.raises(YufError):
+            ops.muon_step([q, p], [h, g], [n, m], **{"lr": 0.1, **refused})
+    assert all(torch.equal(a, b) for a, b in zip(before, (p, m, q, n)))
+    ops.muon_step([q, p], [h, g], [n, m], 0.1)
+    assert not torch.equal(p, before[0]) and not torch.equal(q, before[2])
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])

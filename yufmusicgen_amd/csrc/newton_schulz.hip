@@ -44,12 +44,14 @@ constexpr int kWave = 64;
 constexpr int kThreads = 256;
 constexpr int kXcds = 8;
 constexpr int kGroup = 64;      // matrices of a launch: their pointers are kernel arguments
+constexpr size_t kSpaceMost = (size_t)2 << 30;  // bytes of a group's operands, if it is more than one matrix
 constexpr int kSumParts = 64;   // workgroups of a matrix's norm, at most
 constexpr int kSumRun = 4096;   // elements of such a workgroup, at least
 constexpr int kPrepTile = 64;
 constexpr int kStepsMost = 64;
 constexpr int kOnePartRows = 128, kOnePartSteps = 6;
 constexpr double kGrowthMost = 256.0;  // of the singular values' bound
+constexpr double kPolyMost = 1e6;      // of P's; no polynomial with the former bound comes near it
 constexpr double kBelow = 30000.0;     // scaled values stay below this (fp16 holds 65504)
 
 __device__ __forceinline__ float widen(float x) { return x; }
@@ -823,7 +825,9 @@ Plan ns_plan(int count, int rows, int cols, bool one_part) {
     Plan s{};
     s.p = std::min(rows, cols);
     s.q = std::max(rows, cols);
-    s.group = std::min(count, kGroup);
+    // Operands in the padding of the larger tiles: two of X, and A and P, of two parts each.
+    const size_t most = ((size_t)4 * round_up(s.p, 128) * round_up(s.q, 128) + (size_t)4 * round_up(s.p, 128) * round_up(s.p, 128)) * sizeof(f16);
+    s.group = std::min({count, kGroup, (int)std::max<size_t>(1, std::min<size_t>(kGroup, kSpaceMost / most))});
     const int64_t tiles = (s.p + 127) / 128, sym = s.group * (tiles * (tiles + 1) / 2), apply = s.group * tiles * ((s.q + 127) / 128);
     s.whole = s.p <= kSmallRows && s.q <= kSmallColumns;
     s.small_sym = s.p <= 128 || sym <= (one_part ? 144 : 256);
@@ -864,9 +868,7 @@ const char *ns_scales(int steps, double a, double b, double c, bool half, Scales
     const double base = half ? 0.0 : a;  // P holds a I where X is multiplied by it in whole
     double bound = 1.0;
     for (int k = 0; k < steps; ++k) {
-        s.x[k] = scale(bound);
         const double top = bound * bound;  // of X's squared singular values
-        s.gram[k] = scale(top);
         // Extremes of base + b u + c u^2 and of t (a + b t^2 + c t^4) over the bound: ends and stationary points.
         double poly = std::max(std::fabs(base), std::fabs(base + b * top + c * top * top)), next = std::fabs(bound * (a + b * top + c * top * top));
         if (c != 0.0) {
@@ -880,9 +882,11 @@ const char *ns_scales(int steps, double a, double b, double c, bool half, Scales
             for (const double u : {c != 0 ? h / (5 * c) : -1.0, h != 0 ? a / h : -1.0})
                 if (u > 0 && u < top) next = std::max(next, std::fabs(std::sqrt(u) * (a + b * u + c * u * u)));
         }
+        if (!(next <= kGrowthMost) || !(poly <= kPolyMost)) return "newton schulz: these coefficients let singular values grow past 256";
+        s.x[k] = scale(bound);
+        s.gram[k] = scale(top);
         s.poly[k] = scale(poly);
         bound = next * (1.0 + 1e-3);  // rounding
-        if (!(bound <= kGrowthMost)) return "newton schulz: these coefficients let singular values grow past 256";
     }
     s.x[steps] = 1.0f;
     return nullptr;

@@ -569,6 +569,23 @@ def _check_matrices(name: str, matrices, device, dtype) -> None:
             raise TypeError(f"{name} must be {dtype}")
 
 
+def _check_apart(written, read) -> None:
+    """Contiguous tensors that are written share memory with none of the others."""
+    def end(x):
+        return x.data_ptr() + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+    runs = sorted((x.device.index, x.data_ptr(), end(x), kind) for kind, xs in ((True, written), (False, read)) for x in xs if x.numel())
+    device, any_end, written_end = None, 0, 0
+    for index, begin, stop, kind in runs:
+        if index != device:
+            device, any_end, written_end = index, 0, 0
+        if begin < written_end or (kind and begin < any_end):
+            raise ValueError("params, grads and momenta may not overlap")
+        any_end = max(any_end, stop)
+        if kind:
+            written_end = max(written_end, stop)
+
+
 def newton_schulz(x, steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float = 1e-7):
     """Matrices orthogonalised by Newton-Schulz products: ``X = x / (|x|_F + eps)``, then
     ``steps`` times ``A = X X^T, X <- a X + (b A + c A A) X``, on the transpose where there
@@ -642,10 +659,15 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
         _check_like("momenta", m, p.shape, p.device)
         if not p.is_contiguous() or not m.is_contiguous():
             raise ValueError("params and momenta must be contiguous")
-        groups.setdefault((p.shape, p.dtype, p.device), []).append((p, g.contiguous(), m))
+        if p.numel() and not lib().yuf_newton_schulz_workspace(1, *p.shape):
+            raise ValueError(f"matrices of shape {list(p.shape)} are too large")
+        groups.setdefault((p.shape, p.dtype, p.device), []).append((p, g, m))
+    if len(groups) > 1:  # the library sees one group at a time, and all are refused before one is updated
+        _check_apart((*params, *momenta), grads)
     for ((rows, cols), dtype, device), members in groups.items():
         ps, gs, ms = zip(*members)
         with _on(device) as stream:
+            gs = [g.contiguous() for g in gs]
             space = _scratch(lib().yuf_newton_schulz_workspace(len(ps), rows, cols), device)
             entry = lib().yuf_muon_step_f32 if dtype == torch.float32 else lib().yuf_muon_step_bf16
             check(entry(len(ps), rows, cols, _pointers(ps), _pointers(gs), _pointers(ms), float(lr), float(momentum),
