@@ -36,7 +36,7 @@ constexpr int kManyPositions = 8192;
 constexpr int kNoRange = 255, kWidthMost = 512;
 constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
 constexpr int kPicks = 4;         // such reads of a wave in flight
-constexpr int kHeld = 3584;       // positions of a range that are kept in LDS, beside 32 KB of counters
+constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (96 KB), beside 32 KB of counters
 constexpr int kBatch = 8;         // rows of a wave in flight
 constexpr int kWalks = 3000;     // about 12 waves a CU
 constexpr int kClearRows = 8;     // table rows that a wave looks over for tokens without positions
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads) embedding_ranges_kernel(SortParams p
 }
 
 __global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams p) {
-    extern __shared__ int counts[];  // [waves][width]
+    __shared__ int counts[kSortWaves * kWidthMost];  // [waves][width]
     __shared__ int sums[kSortWaves], offsets[kBlocksMost + 1], bases[kSortWaves];
     __shared__ Place held[kHeld];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -668,7 +668,7 @@ int launch_grad(const GradPlan &g, const SortParams &sort, const SumParams<T> &s
     const size_t counters = kSortWaves * g.width * sizeof(int);
     if (g.blocks) {
         hipLaunchKernelGGL(embedding_ranges_kernel, dim3(g.blocks), dim3(kThreads), 0, s, sort);
-        hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
+        hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.ranges), dim3(kSortThreads), 0, s, sort);
     } else {
         hipLaunchKernelGGL(embedding_sort_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
     }
