@@ -87,7 +87,9 @@ def check_grad(got, tokens, dout, vocab, scale, padding=None, out=None):
                                                    (300, 1, 640, 1), (2331, 673, 333, 3), (4111, 673, 1024, 8), (5000, 4, 9, 8),
                                                    (1000, 65536, 8, 1), (777, 20480, 2047, 3), (40000, 300, 40, 3),
                                                    (8192, 255, 12, 1), (8193, 255, 12, 1), (9001, 256, 12, 3), (9000, 130560, 4, 1),
-                                                   (9000, 130561, 4, 1), (70000, 65536, 4, 3), (300000, 20480, 4, 8), (270000, 1, 3, 1)])
+                                                   (9000, 130561, 4, 1), (70000, 65536, 4, 3), (300000, 20480, 4, 8), (270000, 1, 3, 1),
+                                                   (65536, 2, 3, 1), (65537, 2, 3, 1), (100000, 3, 5, 1), (90000, 256, 4, 8),
+                                                   (200000, 673, 33, 8), (530000, 600, 2, 8)])
 def test_embedding_gradient(rows, vocab, cols, skew, kind, add):
     from yufmusicgen_amd import ops
 
@@ -115,6 +117,20 @@ def test_embedding_gradient_of_runs_at_the_chunks_ends(rows, kind):
         tokens = torch.arange(rows, device="cuda") // length
         tokens = tokens[torch.randperm(rows, generator=gen(7), device="cuda")]
         check_grad(ops.embedding_grad(tokens, dout, rows + 3), tokens, dout, rows + 3, 1.0)
+
+
+@pytest.mark.parametrize("tokens,vocab", [(lambda n: n // 20000, 300), (lambda n: n // 20000 * 255, 2000), (lambda n: n % 3 * 255 + 254, 1000),
+                                          (lambda n: (n % 70000 == 0) * 5, 700)], ids=["runs", "runs of a range", "last range", "one id"])
+def test_embedding_gradient_of_many_positions_in_few_ranges(tokens, vocab):
+    """Ranges that several workgroups share, their positions in one place and all over, some shares empty."""
+    from yufmusicgen_amd import ops
+
+    rows = 140001
+    print(f"embedding gradient of {rows} positions in few ranges, {vocab} tokens", flush=True)
+    tokens, dout = tokens(torch.arange(rows, device="cuda")), table(8, rows, 6, torch.float32)
+    got = ops.embedding_grad(tokens, dout, vocab)
+    check_grad(got, tokens, dout, vocab, 1.0)
+    assert torch.equal(got, ops.embedding_grad(tokens, dout, vocab))
 
 
 def test_embedding_gradient_of_paddings_and_wild_ids():

@@ -37,6 +37,10 @@ constexpr int kNoRange = 255, kWidthMost = 512;
 constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
 constexpr int kPicks = 4;         // such reads of a wave in flight
 constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (96 KB), beside 32 KB of counters
+// Of more than kSplitPositions positions, ranges with more than kHeavy of them (or a kHeavyShare-th of all) are shared
+// by helpers of half as many each, which costs a launch.
+constexpr int64_t kSplitPositions = 65536;
+constexpr int kHeavy = 16384, kHeavyShare = 64;
 constexpr int kBatch = 8;         // rows of a wave in flight
 constexpr int kWalks = 3000;     // about 12 waves a CU
 constexpr int kClearRows = 8;     // table rows that a wave looks over for tokens without positions
@@ -207,6 +211,10 @@ struct SortParams {
     uint8_t *ranges;  // [blocks block]
     int *below;       // [blocks][256]
     Place *picked;    // [M]: a range's positions, if they are more than LDS holds
+    int heavy;        // a range with more positions than this is shared by helpers, two for each `heavy` of them
+    int helpers;      // the most there can be; 0: no range is shared
+    int *shares;      // [helpers][width]: a helper's positions of each token
+    int *assigned;    // [helpers][3]: a helper's range (or -1), part and parts
 };
 
 // The token of a position, or -1: not to be counted.
@@ -226,15 +234,24 @@ __device__ __forceinline__ uint64_t same_lanes(bool in, int j, int bits) {
 }
 
 // counts [waves][p.width] of the range's tokens -> where each wave's first position of each token goes, the range's
-// positions beginning at `first`; p.start of the range.  The workgroup, between barriers.
-__device__ __forceinline__ void sort_places(const SortParams &p, int range, int first, int *counts, int *sums) {
+// positions beginning at `first`; p.start of the range.  The workgroup, between barriers.  Helper `part` of `parts` has its
+// counts here and those of all in `shares`.
+__device__ __forceinline__ void sort_places(const SortParams &p, int range, int first, int *counts, int *sums,
+                                            const int *shares = nullptr, int part = 0, int parts = 1) {
     const int low = range * p.width, width = min(p.width, p.numbers - low);
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     for (int base = 0; base < width; base += kSortThreads) {
         const int j = base + threadIdx.x;
-        int here = 0;
-        if (j < width)
+        int here = 0, earlier = 0;  // of all helpers, and of those before this one
+        if (j < width && shares) {
+            for (int q = 0; q < parts; ++q) {
+                const int n = shares[q * p.width + j];
+                here += n;
+                if (q < part) earlier += n;
+            }
+        } else if (j < width) {
             for (int w = 0; w < kSortWaves; ++w) here += counts[w * p.width + j];
+        }
         int upto = here;  // inclusive scan over the workgroup
         for (int step = 1; step < kWave; step *= 2) {
             const int other = __shfl_up(upto, step);
@@ -249,7 +266,8 @@ __device__ __forceinline__ void sort_places(const SortParams &p, int range, int 
         }
         int next = before + upto - here;
         if (j < width) {
-            p.start[low + j] = next;
+            if (part == 0) p.start[low + j] = next;
+            next += earlier;
             for (int w = 0; w < kSortWaves; ++w) {
                 const int n = counts[w * p.width + j];
                 counts[w * p.width + j] = next;
@@ -259,7 +277,7 @@ __device__ __forceinline__ void sort_places(const SortParams &p, int range, int 
         first += all;
         __syncthreads();
     }
-    if (low + width < p.numbers) return;
+    if (low + width < p.numbers || part > 0) return;
     if (threadIdx.x == 0) p.start[p.numbers] = first;
     for (int64_t i = first + threadIdx.x; i < p.M; i += kSortThreads) p.order[i] = {0, -1};  // positions that are not counted
 }
@@ -351,15 +369,9 @@ __global__ void __launch_bounds__(kThreads) embedding_ranges_kernel(SortParams p
     p.below[blockIdx.x * kThreads + tid] = upto - here;
 }
 
-__global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams p) {
-    __shared__ int counts[kSortWaves * kWidthMost];  // [waves][width]
-    __shared__ int sums[kSortWaves], offsets[kBlocksMost + 1], bases[kSortWaves];
-    __shared__ Place held[kHeld];
+// Where the range's positions begin, and where each block's do among them (offsets, with their number at the end).
+__device__ __forceinline__ int range_offsets(const SortParams &p, int range, int *offsets, int *sums, int *bases) {
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const int range = blockIdx.x;
-    int *mine = counts + wave * p.width;
-    for (int i = tid; i < kSortWaves * p.width; i += kSortThreads) counts[i] = 0;
-    // Where the range's positions begin, and where each block's do among them.
     int before = 0, here = 0;
     if (tid < p.blocks) {
         before = p.below[tid * kThreads + range];
@@ -383,11 +395,13 @@ __global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams
     if (tid < p.blocks) offsets[tid] = upto - here;
     if (tid == 0) offsets[p.blocks] = n;
     __syncthreads();
-    // The range's positions in order: in LDS where they fit, else in memory.
-    const bool fits = n <= kHeld;
+    return first;
+}
+
+// A wave's blocks' positions of the range, in order, from list[next] on.
+__device__ __forceinline__ void pick_positions(const SortParams &p, int range, int block0, int block1, int next, Place *list) {
+    const int lane = threadIdx.x % kWave;
     const uint32_t pattern = (uint32_t)range * 0x01010101u;
-    const int block0 = p.blocks * wave / kSortWaves, block1 = p.blocks * (wave + 1) / kSortWaves;
-    int next = offsets[block0];
     for (int64_t at = block0 * p.block; at < block1 * p.block; at += kPicks * kBlockRun) {
         uint4 bytes[kPicks];
 #pragma unroll
@@ -413,50 +427,170 @@ __global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams
             }
             int to = next + upto - own;
             for (; match; match &= match - 1, ++to) {
-                const int bit = __ffs(match) - 1, position = (int)(at + u * kBlockRun) + lane * 16 + (bit >> 3) * 4 + (bit & 7);
-                if (fits) held[to].position = position;
-                else p.picked[first + to].position = position;
+                const int bit = __ffs(match) - 1;
+                list[to].position = (int)(at + u * kBlockRun) + lane * 16 + (bit >> 3) * 4 + (bit & 7);
             }
             next += __builtin_amdgcn_readlane(upto, kWave - 1);
         }
     }
-    __syncthreads();
-    const int tiles = (n + kWave - 1) / kWave;
-    const int from = tiles * wave / kSortWaves * kWave, end = min(n, tiles * (wave + 1) / kSortWaves * kWave);
-    Place *list = p.picked + first;
+}
+
+// A wave's positions from list[from] to list[end]: their tokens (numbered in the range) are looked up, if LOOK, and counted.
+template <bool LOOK>
+__device__ __forceinline__ void count_positions(const SortParams &p, Place *list, int from, int end, int *mine) {
+    const int lane = threadIdx.x % kWave;
     for (int at = from; at < end; at += kBatch * kWave) {
-        int position[kBatch], j[kBatch];
+        int j[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int i = min(at + u * kWave + lane, end - 1);
-            position[u] = fits ? held[i].position : list[i].position;
+            const Place &place = list[min(at + u * kWave + lane, end - 1)];
+            j[u] = LOOK ? place.position : place.token;
         }
+        if (LOOK)
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) j[u] = (int)token_at(p.tokens, p.wide, position[u]) / kNoRange;
+            for (int u = 0; u < kBatch; ++u) j[u] = (int)token_at(p.tokens, p.wide, j[u]) / kNoRange;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const int i = at + u * kWave + lane;
             const bool in = i < end;
-            if (in) (fits ? held[i].token : list[i].token) = j[u];
+            if (LOOK && in) list[i].token = j[u];
             const uint64_t same = same_lanes(in, j[u], p.bits);
             if (in && (same & (((uint64_t)1 << lane) - 1)) == 0) mine[j[u]] += __popcll(same);
             __builtin_amdgcn_wave_barrier();
         }
     }
-    __syncthreads();
-    sort_places(p, range, first, counts, sums);
+}
+
+__device__ __forceinline__ void place_positions(const SortParams &p, int range, const Place *list, int from, int end, int *mine) {
+    const int lane = threadIdx.x % kWave;
     for (int at = from; at < end; at += kBatch * kWave) {
         Place place[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = min(at + u * kWave + lane, end - 1);
-            place[u] = fits ? held[i] : list[i];
-        }
+        for (int u = 0; u < kBatch; ++u) place[u] = list[min(at + u * kWave + lane, end - 1)];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
             if (at + u * kWave < end)
                 sort_place(p, at + u * kWave + lane < end, place[u].token, place[u].token * kNoRange + range, place[u].position, mine);
     }
+}
+
+// Sorts a range's positions by token: into `list`, where the wave's blocks begin at `next`, and from there into p.order.
+__device__ __forceinline__ void sort_range(const SortParams &p, int range, int first, int n, int block0, int block1, int next,
+                                           Place *list, int *counts, int *sums) {
+    const int wave = threadIdx.x / kWave, tiles = (n + kWave - 1) / kWave;
+    const int from = tiles * wave / kSortWaves * kWave, end = min(n, tiles * (wave + 1) / kSortWaves * kWave);
+    int *mine = counts + wave * p.width;
+    pick_positions(p, range, block0, block1, next, list);
+    __syncthreads();
+    count_positions<true>(p, list, from, end, mine);
+    __syncthreads();
+    sort_places(p, range, first, counts, sums);
+    place_positions(p, range, list, from, end, mine);
+}
+
+// A helper's range and its part of it.  Helpers are numbered through the heavy ranges; at most 3 M / heavy are needed, since
+// ceil(2 n / heavy) < 3 n / heavy for n > heavy.
+struct Share {
+    int range, part, parts;
+};
+__device__ __forceinline__ Share find_share(const SortParams &p, int helper, int *firsts, int *sums) {
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    if (tid < kThreads) firsts[tid] = 0;
+    __syncthreads();
+    constexpr int kQuarters = kSortThreads / kThreads, kReads = 16;
+    int first = 0;  // positions of ranges below this thread's, in a quarter of the blocks
+    for (int b0 = tid / kThreads; b0 < p.blocks; b0 += kReads * kQuarters) {
+        int below[kReads];
+#pragma unroll
+        for (int u = 0; u < kReads; ++u) below[u] = p.below[min(b0 + u * kQuarters, p.blocks - 1) * kThreads + tid % kThreads];
+#pragma unroll
+        for (int u = 0; u < kReads; ++u)
+            if (b0 + u * kQuarters < p.blocks) first += below[u];
+    }
+    atomicAdd(&firsts[tid % kThreads], first);
+    __syncthreads();
+    const int n = tid < kThreads - 1 ? firsts[tid + 1] - firsts[tid] : 0;
+    const int here = n > p.heavy ? min((int)((2 * (int64_t)n + p.heavy - 1) / p.heavy), p.blocks) : 0;
+    int upto = here;
+    for (int step = 1; step < kWave; step *= 2) {
+        const int other = __shfl_up(upto, step);
+        if (lane >= step) upto += other;
+    }
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += sums[w];
+    __syncthreads();
+    if (tid == 0) sums[0] = -1;
+    __syncthreads();
+    if (helper >= upto - here && helper < upto) {  // one thread at most
+        sums[0] = tid;
+        sums[1] = helper - (upto - here);
+        sums[2] = here;
+    }
+    __syncthreads();
+    const Share share{sums[0], sums[1], sums[2]};
+    if (tid < 3) p.assigned[helper * 3 + tid] = sums[tid];
+    __syncthreads();
+    return share;
+}
+
+// Range blockIdx.x - helpers, unless helpers share it; of a helper's part the positions with their tokens and the counts.
+__global__ void __launch_bounds__(kSortThreads) embedding_pick_kernel(SortParams p) {
+    __shared__ int counts[kSortWaves * kWidthMost];  // [waves][width]
+    __shared__ int sums[kSortWaves], offsets[kBlocksMost + 1], bases[kSortWaves];
+    __shared__ Place held[kHeld];
+    const int tid = threadIdx.x, wave = tid / kWave;
+    for (int i = tid; i < kSortWaves * p.width; i += kSortThreads) counts[i] = 0;
+    if ((int)blockIdx.x >= p.helpers) {
+        const int range = blockIdx.x - p.helpers;
+        const int first = range_offsets(p, range, offsets, sums, bases), n = offsets[p.blocks];
+        if (p.helpers && n > p.heavy) return;
+        const int block0 = p.blocks * wave / kSortWaves, block1 = p.blocks * (wave + 1) / kSortWaves;
+        if (n <= kHeld) {
+            sort_range(p, range, first, n, block0, block1, offsets[block0], held, counts, sums);
+        } else {
+            sort_range(p, range, first, n, block0, block1, offsets[block0], p.picked + first, counts, sums);
+        }
+        return;
+    }
+    const Share share = find_share(p, blockIdx.x, offsets, sums);
+    if (share.range < 0) return;
+    const int first = range_offsets(p, share.range, offsets, sums, bases);
+    const int begin = p.blocks * share.part / share.parts, blocks = p.blocks * (share.part + 1) / share.parts - begin;
+    const int block0 = begin + blocks * wave / kSortWaves, block1 = begin + blocks * (wave + 1) / kSortWaves;
+    const int base = offsets[begin], n = offsets[begin + blocks] - base, tiles = (n + kWave - 1) / kWave;
+    const int from = tiles * wave / kSortWaves * kWave, end = min(n, tiles * (wave + 1) / kSortWaves * kWave);
+    Place *list = p.picked + first + base;
+    pick_positions(p, share.range, block0, block1, offsets[block0] - base, list);
+    __syncthreads();
+    count_positions<true>(p, list, from, end, counts + wave * p.width);
+    __syncthreads();
+    for (int j = tid; j < p.width; j += kSortThreads) {
+        int here = 0;
+        for (int w = 0; w < kSortWaves; ++w) here += counts[w * p.width + j];
+        p.shares[blockIdx.x * p.width + j] = here;
+    }
+}
+
+// The helpers' second half: their places, from the counts of all.
+__global__ void __launch_bounds__(kSortThreads) embedding_share_kernel(SortParams p) {
+    __shared__ int counts[kSortWaves * kWidthMost];  // [waves][width]
+    __shared__ int sums[kSortWaves], offsets[kBlocksMost + 1], bases[kSortWaves];
+    const int tid = threadIdx.x, wave = tid / kWave;
+    const int *assigned = p.assigned + blockIdx.x * 3;
+    const Share share{assigned[0], assigned[1], assigned[2]};
+    if (share.range < 0) return;
+    for (int i = tid; i < kSortWaves * p.width; i += kSortThreads) counts[i] = 0;
+    const int first = range_offsets(p, share.range, offsets, sums, bases);
+    const int begin = p.blocks * share.part / share.parts, after = p.blocks * (share.part + 1) / share.parts;
+    const int base = offsets[begin], n = offsets[after] - base, tiles = (n + kWave - 1) / kWave;
+    const int from = tiles * wave / kSortWaves * kWave, end = min(n, tiles * (wave + 1) / kSortWaves * kWave);
+    Place *list = p.picked + first + base;
+    int *mine = counts + wave * p.width;
+    count_positions<false>(p, list, from, end, mine);
+    __syncthreads();
+    sort_places(p, share.range, first, counts, sums, p.shares + (blockIdx.x - share.part) * p.width, share.part, share.parts);
+    place_positions(p, share.range, list, from, end, mine);
 }
 
 template <typename T> struct SumParams {
@@ -531,12 +665,13 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
         const uint64_t ends = __ballot(in) & ~more;
         for (int j0 = 0; j0 < n; j0 += kBatch) {
             float row[kBatch][kN], old[kBatch][kN];
+            const bool finishes = ADD && (ends >> j0 & ((1u << kBatch) - 1));
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const int j = min(j0 + u, n - 1);
                 const T *from = p.dout + (int64_t)__builtin_amdgcn_readlane(place.position, j) * p.cols;
                 if (c.any()) c.load(from, row[u]);
-                if (ADD) {  // where no row is finished, dout's own row once more, which is near
+                if (finishes) {  // where no row is finished, dout's own row once more, which is near
                     const T *there = p.out + (int64_t)__builtin_amdgcn_readlane(place.token, j) * p.cols;
                     if (c.any()) c.load(ends >> j & 1 ? there : from, old[u]);
                 }
@@ -615,8 +750,9 @@ struct GradPlan {
     int width, ranges, bits, numbers, slices, chunk, chunks, clears;
     int blocks;                     // 0: the ranges are not written down
     int64_t block;
+    int heavy, helpers;             // no helpers: no range is shared
     int64_t sums, joins;            // workgroups
-    size_t order, start, parts, bytes_of, below, picked, bytes;  // offsets into the workspace, and its size
+    size_t order, start, parts, bytes_of, below, picked, shares, assigned, bytes;  // offsets into the workspace, and its size
 };
 
 // Sorted positions of a wave's walk: as many as leave kWalks waves, so that short batches still fill the card.
@@ -631,6 +767,10 @@ GradPlan grad_plan(int64_t M, int V, int D, int vec) {
         const int64_t run = (M + kBlocksMost - 1) / kBlocksMost;
         g.block = (run + kBlockRun - 1) / kBlockRun * kBlockRun;
         g.blocks = (int)((M + g.block - 1) / g.block);
+        if (M > kSplitPositions) {
+            g.heavy = (int)std::max<int64_t>(kHeavy, M / kHeavyShare);
+            g.helpers = (int)(3 * M / g.heavy);
+        }
     }
     while (1 << g.bits < g.width) ++g.bits;
     g.numbers = g.blocks ? g.ranges * g.width : V;
@@ -648,7 +788,9 @@ GradPlan grad_plan(int64_t M, int V, int D, int vec) {
     g.bytes_of = g.parts + round((size_t)g.chunks * 2 * g.slices * kWave * vec * sizeof(float));
     g.below = g.bytes_of + round((size_t)(g.blocks * g.block));
     g.picked = g.below + round((size_t)g.blocks * kThreads * sizeof(int));
-    g.bytes = g.picked + (g.blocks ? round((size_t)M * sizeof(Place)) : 0);
+    g.shares = g.picked + (g.blocks ? round((size_t)M * sizeof(Place)) : 0);
+    g.assigned = g.shares + round((size_t)g.helpers * g.width * sizeof(int));
+    g.bytes = g.assigned + round((size_t)g.helpers * 3 * sizeof(int));
     return g;
 }
 
@@ -668,7 +810,8 @@ int launch_grad(const GradPlan &g, const SortParams &sort, const SumParams<T> &s
     const size_t counters = kSortWaves * g.width * sizeof(int);
     if (g.blocks) {
         hipLaunchKernelGGL(embedding_ranges_kernel, dim3(g.blocks), dim3(kThreads), 0, s, sort);
-        hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.ranges), dim3(kSortThreads), 0, s, sort);
+        hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.helpers + g.ranges), dim3(kSortThreads), 0, s, sort);
+        if (g.helpers) hipLaunchKernelGGL(embedding_share_kernel, dim3(g.helpers), dim3(kSortThreads), 0, s, sort);
     } else {
         hipLaunchKernelGGL(embedding_sort_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
     }
@@ -700,6 +843,8 @@ int embedding_grad(int64_t M, int V, int D, const void *tokens, int token_bits, 
     sort.ranges = reinterpret_cast<uint8_t *>(space + g.bytes_of);
     sort.below = reinterpret_cast<int *>(space + g.below);
     sort.picked = reinterpret_cast<Place *>(space + g.picked);
+    sort.heavy = g.heavy; sort.helpers = g.helpers; sort.shares = reinterpret_cast<int *>(space + g.shares);
+    sort.assigned = reinterpret_cast<int *>(space + g.assigned);
     sort.tokens = tokens; sort.wide = token_bits == 64; sort.padding = padding;
     sort.order = reinterpret_cast<Place *>(space + g.order);
     sort.start = reinterpret_cast<int *>(space + g.start);
