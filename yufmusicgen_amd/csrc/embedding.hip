@@ -42,9 +42,9 @@ constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (
 constexpr int64_t kSplitPositions = 65536;
 constexpr int kHeavy = 16384, kHeavyShare = 64;
 constexpr int kBatch = 8;         // rows of a wave in flight
-constexpr int kWalks = 3000;     // about 12 waves a CU
+constexpr int kWalks = 5120;      // 20 waves a CU, which run together (4096 of bf16 32 x 8192 x 1024: 140 -> 132 us)
 constexpr int kClearRows = 8;     // table rows that a wave looks over for tokens without positions
-constexpr int kJoinWaves = kThreads / kWave;
+constexpr int kJoinWaves = 8, kJoinAlone = 16;  // and parts that a wave joins alone
 constexpr int kVocabMost = 1 << 24, kColsMost = 1 << 24;
 
 // Vectors with the alignment of their elements: rows of odd widths start anywhere.
@@ -82,16 +82,20 @@ template <typename T> struct Columns {
         if (first >= cols) own = end;
     }
     __device__ __forceinline__ bool any() const { return own < end; }
-    __device__ __forceinline__ void load(const T *row, float (&x)[Vec<T>::kN]) const {
+    __device__ __forceinline__ void load(const T *row, typename Vec<T>::type &x) const {
         constexpr int kN = Vec<T>::kN;
         if (end == kN) {
-            const auto v = *reinterpret_cast<const typename Vec<T>::type *>(row + at);
-#pragma unroll
-            for (int e = 0; e < kN; ++e) x[e] = widen(v[e]);
+            x = *reinterpret_cast<const typename Vec<T>::type *>(row + at);
         } else {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) x[e] = e < end ? widen(row[at + e]) : 0.0f;
+            for (int e = 0; e < kN; ++e) x[e] = e < end ? row[at + e] : T(0);
         }
+    }
+    __device__ __forceinline__ void load(const T *row, float (&x)[Vec<T>::kN]) const {
+        typename Vec<T>::type v;
+        load(row, v);
+#pragma unroll
+        for (int e = 0; e < Vec<T>::kN; ++e) x[e] = widen(v[e]);
     }
     __device__ __forceinline__ void store(T *row, const float (&x)[Vec<T>::kN]) const {
         constexpr int kN = Vec<T>::kN;
@@ -622,14 +626,14 @@ __device__ __forceinline__ void store_part(floatx4 *to, const float (&x)[Vec<T>:
 // Writes a token's finished row: scale x sum, added to what is there where `old` is given.
 template <typename T, bool ADD>
 __device__ __forceinline__ void write_row(const SumParams<T> &p, const Columns<T> &c, int token, float (&sum)[Vec<T>::kN],
-                                          const float (&old)[Vec<T>::kN]) {
+                                          const typename Vec<T>::type &old) {
 #pragma unroll
-    for (int e = 0; e < Vec<T>::kN; ++e) sum[e] = ADD ? fmaf(p.scale, sum[e], old[e]) : p.scale * sum[e];
+    for (int e = 0; e < Vec<T>::kN; ++e) sum[e] = ADD ? fmaf(p.scale, sum[e], widen(old[e])) : p.scale * sum[e];
     c.store(p.out + (int64_t)token * p.cols, sum);
 }
 
 template <typename T, bool ADD>
-__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p) {
+__global__ void __launch_bounds__(kThreads, 5) embedding_sum_kernel(SumParams<T> p) {
     constexpr int kN = Vec<T>::kN;
     const int lane = threadIdx.x % kWave;
     const int64_t task = (int64_t)blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -664,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
         goes_on = base + n == end && (more >> (n - 1) & 1);
         const uint64_t ends = __ballot(in) & ~more;
         for (int j0 = 0; j0 < n; j0 += kBatch) {
-            float row[kBatch][kN], old[kBatch][kN];
+            typename Vec<T>::type row[kBatch], old[kBatch];  // as they are, until they are summed
             const bool finishes = ADD && (ends >> j0 & ((1u << kBatch) - 1));
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
                 const int j = j0 + u;
                 if (j >= n) break;
 #pragma unroll
-                for (int e = 0; e < kN; ++e) sum[e] += row[u][e];
+                for (int e = 0; e < kN; ++e) sum[e] += widen(row[u][e]);
                 if (ends >> j & 1) {
                     if (c.any()) {
                         if (came) {
@@ -701,49 +705,75 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams<T> p)
     if (goes_on && c.any()) store_part<T>(part_at(p, chunk, came ? 0 : 1, slice, lane), sum);
 }
 
-// The parts of a run that began in this workgroup's chunk: each wave sums every kJoinWaves-th, then they are joined.
+// The number of parts of a run that began in a chunk and left it, or 0.
+template <typename T> __device__ __forceinline__ int parts_of(const SumParams<T> &p, int chunk) {
+    const int64_t begin = (int64_t)chunk * p.chunk, end = begin + p.chunk;
+    if (end >= p.M) return 0;
+    const int token = p.order[end - 1].token;
+    if (token < 0 || p.order[end].token != token || (begin > 0 && p.order[begin - 1].token == token)) return 0;
+    return (p.start[p.numbering.number(token) + 1] - 1) / p.chunk - chunk + 1;
+}
+
+// The parts of such runs.  A wave joins the few of its own; many are shared by the workgroup, each wave summing every
+// kJoinWaves-th.  8 waves: a run of 80 thousand positions 44 -> 27 us against 4 waves that share every run.
 template <typename T, bool ADD>
-__global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumParams<T> p) {
+__global__ void __launch_bounds__(kJoinWaves * kWave) embedding_join_kernel(SumParams<T> p) {
     constexpr int kN = Vec<T>::kN;
     __shared__ float joined[kJoinWaves][kN][kWave];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int chunk = blockIdx.x / p.slices, slice = blockIdx.x - chunk * p.slices;
-    const int64_t begin = (int64_t)chunk * p.chunk, end = begin + p.chunk;
-    if (end >= p.M) return;
-    const int token = p.order[end - 1].token;
-    if (token < 0 || p.order[end].token != token || (begin > 0 && p.order[begin - 1].token == token)) return;
-    const int to = p.start[p.numbering.number(token) + 1];
-    const int last = (to - 1) / p.chunk;  // its last chunk
-    const Columns<T> c((slice * kWave + lane) * kN, p.cols);
-    const auto part = [&](int k, float (&x)[kN]) {  // the run's k-th part
-        const floatx4 *at = part_at(p, chunk + k, k == 0, slice, lane);
+    __shared__ int many[kJoinWaves];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int first = blockIdx.x * kJoinWaves, tasks = p.chunks * p.slices;  // a long run's slices in different workgroups
+    const auto sum_parts = [&](int chunk, int slice, int from, int step, int count, float (&sum)[kN]) {
+        for (int k0 = from; k0 < count; k0 += kBatch * step) {
+            floatx4 x[kBatch][kN / 4];
 #pragma unroll
-        for (int e = 0; e < kN; ++e) x[e] = at[e / 4][e % 4];
-    };
-    const int count = last - chunk + 1;
-    float sum[kN] = {};
-    if (c.any()) {
-        for (int k0 = wave; k0 < count; k0 += kBatch * kJoinWaves) {
-            float x[kBatch][kN];
+            for (int u = 0; u < kBatch; ++u) {
+                const int k = min(k0 + u * step, count - 1);
+                const floatx4 *at = part_at(p, chunk + k, k == 0, slice, lane);
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) part(min(k0 + u * kJoinWaves, count - 1), x[u]);
+                for (int e = 0; e < kN / 4; ++e) x[u][e] = at[e];
+            }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u)
 #pragma unroll
                 for (int e = 0; e < kN; ++e)
-                    if (k0 + u * kJoinWaves < count) sum[e] += x[u][e];
+                    if (k0 + u * step < count) sum[e] += x[u][e / 4][e % 4];
         }
+    };
+    const auto write = [&](const Columns<T> &c, int chunk, float (&sum)[kN]) {
+        const int token = p.order[(int64_t)(chunk + 1) * p.chunk - 1].token;
+        typename Vec<T>::type old{};
+        if (ADD) c.load(p.out + (int64_t)token * p.cols, old);
+        write_row<T, ADD>(p, c, token, sum, old);
+    };
+    const int task = first + wave, slice = task / p.chunks, chunk = task - slice * p.chunks;
+    const int count = task < tasks ? parts_of(p, chunk) : 0;
+    const Columns<T> c((slice * kWave + lane) * kN, p.cols);
+    if (count > 0 && count <= kJoinAlone && c.any()) {
+        float sum[kN] = {};
+        sum_parts(chunk, slice, 0, 1, count, sum);
+        write(c, chunk, sum);
     }
-#pragma unroll
-    for (int e = 0; e < kN; ++e) joined[wave][e][lane] = sum[e];
+    if (lane == 0) many[wave] = count > kJoinAlone ? count : 0;
     __syncthreads();
-    if (wave != 0 || !c.any()) return;
-    float old[kN] = {};
-    if (ADD) c.load(p.out + (int64_t)token * p.cols, old);
+    for (int w = 0; w < kJoinWaves; ++w) {
+        const int count = many[w];
+        if (count == 0) continue;
+        const int slice = (first + w) / p.chunks, chunk = first + w - slice * p.chunks;
+        const Columns<T> c((slice * kWave + lane) * kN, p.cols);
+        float sum[kN] = {};
+        if (c.any()) sum_parts(chunk, slice, wave, kJoinWaves, count, sum);
 #pragma unroll
-    for (int e = 0; e < kN; ++e)
-        for (int w = 1; w < kJoinWaves; ++w) sum[e] += joined[w][e][lane];
-    write_row<T, ADD>(p, c, token, sum, old);
+        for (int e = 0; e < kN; ++e) joined[wave][e][lane] = sum[e];
+        __syncthreads();
+        if (wave == 0 && c.any()) {
+#pragma unroll
+            for (int e = 0; e < kN; ++e)
+                for (int v = 1; v < kJoinWaves; ++v) sum[e] += joined[v][e][lane];
+            write(c, chunk, sum);
+        }
+        __syncthreads();
+    }
 }
 
 struct GradPlan {
@@ -775,8 +805,8 @@ GradPlan grad_plan(int64_t M, int V, int D, int vec) {
     while (1 << g.bits < g.width) ++g.bits;
     g.numbers = g.blocks ? g.ranges * g.width : V;
     g.slices = ceil_div(D, kWave * vec);
-    g.chunk = 8;
-    while (g.chunk < 256 && (M + 2 * g.chunk - 1) / (2 * g.chunk) * g.slices >= kWalks) g.chunk *= 2;
+    const int64_t each = (M * g.slices + kWalks - 1) / kWalks;
+    g.chunk = (int)std::min<int64_t>(256, std::max<int64_t>(8, (each + 7) / 8 * 8));
     g.chunks = (int)((M + g.chunk - 1) / g.chunk);
     g.clears = ceil_div(V, kClearRows);
     g.joins = (int64_t)g.chunks * g.slices;
@@ -817,7 +847,7 @@ int launch_grad(const GradPlan &g, const SortParams &sort, const SumParams<T> &s
     }
     const int64_t sums = ADD ? (g.joins + kThreads / kWave - 1) / (kThreads / kWave) : g.sums;
     hipLaunchKernelGGL((embedding_sum_kernel<T, ADD>), dim3((uint32_t)sums), dim3(kThreads), 0, s, sum);
-    if (g.chunks > 1) hipLaunchKernelGGL((embedding_join_kernel<T, ADD>), dim3((uint32_t)g.joins), dim3(kThreads), 0, s, sum);
+    if (g.chunks > 1) hipLaunchKernelGGL((embedding_join_kernel<T, ADD>), dim3((uint32_t)((g.joins + kJoinWaves - 1) / kJoinWaves)), dim3(kJoinWaves * kWave), 0, s, sum);
     YUF_LAUNCH_CHECK("embedding gradient");
     return YUF_OK;
 }
