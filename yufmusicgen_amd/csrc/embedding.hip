@@ -2,20 +2,25 @@
 //     out[i] = scale W[t_i],    dW[v] (+)= scale sum_{i: t_i = v} dout[i].
 //
 // Bound: HBM -- the looked-up rows and the outputs once; for the gradient dout once and the whole table
-// once (twice where it is added to).
+// once (twice where it is added to).  A thread of the lookup has four vectors of 16 bytes in flight: 16384 rows of
+// 20480 x 640 fp32 take 13.4 us, 6.3 TB/s (they fit the memory-side cache).
 //
 // The gradient's sums run over each token's positions in order, so they do not depend on timing: no
-// atomics on values.  Three launches:
+// atomics on values.  Three to five launches:
 //   sort:  a workgroup owns a range of tokens and lists its positions by token.  Its waves take runs of
 //          positions: each counts its tokens, and after a scan over tokens and waves places its positions, in order.
 //          Of few positions the workgroup reads all ids twice (and counts those below the range, which
 //          gives where the range's positions begin without asking another workgroup).  Of many, a launch before
 //          writes the number of each id's range as a byte and counts them by blocks of positions, and the
-//          workgroup picks its positions by comparing 16 bytes at a time.
+//          workgroup picks its positions by comparing 16 bytes at a time.  Of very many, ranges with a large share of
+//          them are picked and counted by several workgroups, and placed by a launch behind.
 //   sum:   a wave walks a chunk of the sorted positions for up to 64 vectors of columns and writes a
 //          token's row where its run ends.  Runs that leave the chunk go to the workspace as fp32 parts.
 //          Further waves clear the rows of tokens that do not occur.
 //   join:  the parts of such a run, in order.
+// us of the sort, the sum and the join: 16384 of 20480 x 640 fp32, added, 16, 17.5, 4.7; 262144 of 20480 x 1024 bf16,
+// with a token that has 3.7 % of them, 47, 133 (4.4 TB/s of rows in random order) and 10; 4111 of 673 x 333 bf16,
+// where each is a chain of latencies, 8.5, 8.8, 4.5.
 #include "common.h"
 
 #include <algorithm>
@@ -38,7 +43,8 @@ constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and 
 constexpr int kPicks = 4;         // such reads of a wave in flight
 constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (96 KB), beside 32 KB of counters
 // Of more than kSplitPositions positions, ranges with more than kHeavy of them (or a kHeavyShare-th of all) are shared
-// by helpers of half as many each, which costs a launch.
+// by helpers of half as many each, which costs a launch.  The sort of 187747 of 673, one of them in 44 % of the places:
+// 125 us without and 39 with; with even frequencies 22 and 29.
 constexpr int64_t kSplitPositions = 65536;
 constexpr int kHeavy = 16384, kHeavyShare = 64;
 constexpr int kBatch = 8;         // rows of a wave in flight
@@ -341,7 +347,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
     }
 }
 
-// The byte of each position: its range, or 255, of 16 positions e in word e % 4 and byte e / 4; and for each block of positions, how many lie in ranges below each.
+// The byte of each position: its range, or 255, of 16 positions e in word e % 4 and byte e / 4; and for each block of
+// positions, how many lie in ranges below each.
 __global__ void __launch_bounds__(kThreads) embedding_ranges_kernel(SortParams p) {
     __shared__ int counts[kThreads], sums[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -785,7 +792,8 @@ struct GradPlan {
     size_t order, start, parts, bytes_of, below, picked, shares, assigned, bytes;  // offsets into the workspace, and its size
 };
 
-// Sorted positions of a wave's walk: as many as leave kWalks waves, so that short batches still fill the card.
+// Sorted positions of a wave's walk: as many as leave kWalks waves, so that short batches still fill the card and long ones
+// do so in one round.
 GradPlan grad_plan(int64_t M, int V, int D, int vec) {
     GradPlan g{};
     g.ranges = std::max(std::min(V, kSortRanges), ceil_div(V, kRangeMost));
