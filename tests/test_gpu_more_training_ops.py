@@ -221,6 +221,12 @@ def test_embedding_through_autograd():
     (grad,) = torch.autograd.grad(ops.embedding(tokens, weight, scale=3.0, padding_idx=4), weight, dout)
     terms = (ops.embedding(tokens, step, scale=3.0).double() * dout.double()).abs().sum()
     assert abs((grad.double() * step.double()).sum() - value) <= 60 * EPS32 * terms
+    # Once differentiable: a recorded gradient is the same and cannot be differentiated again.
+    (recorded,) = torch.autograd.grad(ops.embedding(tokens, weight, scale=3.0, padding_idx=4), weight, dout.requires_grad_(),
+                                      create_graph=True)
+    assert recorded.requires_grad and torch.equal(recorded, grad)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        recorded.sum().backward()
 
 
 def test_a_captured_backward_pass_of_the_embedding_is_refused():

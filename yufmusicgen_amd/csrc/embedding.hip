@@ -9,7 +9,7 @@
 // atomics on values.  Three to five launches:
 //   sort:  a workgroup owns a range of tokens and lists its positions by token.  Its waves take runs of
 //          positions: each counts its tokens, and after a scan over tokens and waves places its positions, in order.
-//          Of few positions the workgroup reads all ids twice (and counts those below the range, which
+//          Of few positions the workgroup reads all ids (and counts those below the range, which
 //          gives where the range's positions begin without asking another workgroup).  Of many, a launch before
 //          writes the number of each id's range as a byte and counts them by blocks of positions, and the
 //          workgroup picks its positions by comparing 16 bytes at a time.  Of very many, ranges with a large share of
@@ -20,7 +20,7 @@
 //   join:  the parts of such a run, in order.
 // us of the sort, the sum and the join: 16384 of 20480 x 640 fp32, added, 16, 17.5, 4.7; 262144 of 20480 x 1024 bf16,
 // with a token that has 3.7 % of them, 47, 133 (4.4 TB/s of rows in random order) and 10; 4111 of 673 x 333 bf16,
-// where each is a chain of latencies, 8.5, 8.8, 4.5.
+// where each is a chain of latencies, 6.7, 8.8, 4.5.
 #include "common.h"
 
 #include <algorithm>
@@ -36,7 +36,7 @@ constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortRanges = 256;  // workgroups of the sort: one per CU
 constexpr int kRangeMost = 960;   // tokens of a range: their counters fill 60 KB of LDS
 // Of more than kManyPositions positions the ranges are written down first, where they are at most kNoRange of at
-// most kWidthMost tokens each.  Both forms, us without and with: 4111 of 673 8.4 and 12.0, 16384 of 20480 24 and 16.7.
+// most kWidthMost tokens each.  Both forms, us without and with: 4111 of 673 6.7 and 12.0, 16384 of 20480 24 and 15.6.
 constexpr int kManyPositions = 8192;
 constexpr int kNoRange = 255, kWidthMost = 512;
 constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
@@ -48,6 +48,7 @@ constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (
 constexpr int64_t kSplitPositions = 65536;
 constexpr int kHeavy = 16384, kHeavyShare = 64;
 constexpr int kBatch = 8;         // rows of a wave in flight
+static_assert(kSortWaves * kBatch * kWave >= kManyPositions, "a batch of each wave holds them");
 constexpr int kWalks = 5120;      // 20 waves a CU, which run together (4096 of bf16 32 x 8192 x 1024: 140 -> 132 us)
 constexpr int kClearRows = 8;     // table rows that a wave looks over for tokens without positions
 constexpr int kJoinWaves = 8, kJoinAlone = 16;  // and parts that a wave joins alone
@@ -253,6 +254,10 @@ __device__ __forceinline__ void sort_places(const SortParams &p, int range, int 
     for (int base = 0; base < width; base += kSortThreads) {
         const int j = base + threadIdx.x;
         int here = 0, earlier = 0;  // of all helpers, and of those before this one
+        int mine[kSortWaves];
+        if (j < width)
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) mine[w] = counts[w * p.width + j];
         if (j < width && shares) {
             for (int q = 0; q < parts; ++q) {
                 const int n = shares[q * p.width + j];
@@ -260,7 +265,8 @@ __device__ __forceinline__ void sort_places(const SortParams &p, int range, int 
                 if (q < part) earlier += n;
             }
         } else if (j < width) {
-            for (int w = 0; w < kSortWaves; ++w) here += counts[w * p.width + j];
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) here += mine[w];
         }
         int upto = here;  // inclusive scan over the workgroup
         for (int step = 1; step < kWave; step *= 2) {
@@ -278,10 +284,10 @@ __device__ __forceinline__ void sort_places(const SortParams &p, int range, int 
         if (j < width) {
             if (part == 0) p.start[low + j] = next;
             next += earlier;
+#pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
-                const int n = counts[w * p.width + j];
                 counts[w * p.width + j] = next;
-                next += n;
+                next += mine[w];
             }
         }
         first += all;
@@ -306,6 +312,9 @@ __device__ __forceinline__ void sort_place(const SortParams &p, bool in, int j, 
     __builtin_amdgcn_wave_barrier();
 }
 
+// ONCE: a wave's positions are one batch, whose tokens stay in registers (M <= kManyPositions; 4111 of 673 8.5 -> 6.7 us,
+// 8192 of 20480 12.8 -> 11.1).
+template <bool ONCE>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams p) {
     extern __shared__ int counts[];  // [waves][width]
     __shared__ int below[kSortWaves], sums[kSortWaves];
@@ -317,12 +326,18 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
     // This wave's run of positions, in whole waves of them.
     const int64_t tiles = (p.M + kWave - 1) / kWave;
     const int64_t first = tiles * wave / kSortWaves * kWave, last = min(p.M, tiles * (wave + 1) / kSortWaves * kWave);
-    const auto read = [&](int64_t at) { return at + lane < last ? counted_token(p, at + lane) : -1; };
-    int less = 0;
-    for (int64_t at = first; at < last; at += kBatch * kWave) {
-        int t[kBatch];
+    int t[kBatch];
+    const auto read = [&](int64_t from) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) t[u] = read(at + u * kWave);
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t at = from + u * kWave + lane;
+            t[u] = at < last ? counted_token(p, at) : -1;
+        }
+    };
+    if (ONCE) read(first);
+    int less = 0;
+    for (int64_t at = first; at < (ONCE ? first + 1 : last); at += kBatch * kWave) {
+        if (!ONCE) read(at);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             less += t[u] >= 0 && t[u] < low;
@@ -335,10 +350,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortParams
     int total = 0;
     for (int w = 0; w < kSortWaves; ++w) total += below[w];
     sort_places(p, blockIdx.x, total, counts, sums);
-    for (int64_t at = first; at < last; at += kBatch * kWave) {
-        int t[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) t[u] = read(at + u * kWave);
+    for (int64_t at = first; at < (ONCE ? first + 1 : last); at += kBatch * kWave) {
+        if (!ONCE) read(at);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const bool in = t[u] >= low && t[u] < low + width;
@@ -851,7 +864,8 @@ int launch_grad(const GradPlan &g, const SortParams &sort, const SumParams<T> &s
         hipLaunchKernelGGL(embedding_pick_kernel, dim3(g.helpers + g.ranges), dim3(kSortThreads), 0, s, sort);
         if (g.helpers) hipLaunchKernelGGL(embedding_share_kernel, dim3(g.helpers), dim3(kSortThreads), 0, s, sort);
     } else {
-        hipLaunchKernelGGL(embedding_sort_kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
+        const auto kernel = sort.M <= kManyPositions ? embedding_sort_kernel<true> : embedding_sort_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3(g.ranges), dim3(kSortThreads), counters, s, sort);
     }
     const int64_t sums = ADD ? (g.joins + kThreads / kWave - 1) / (kThreads / kWave) : g.sums;
     hipLaunchKernelGGL((embedding_sum_kernel<T, ADD>), dim3((uint32_t)sums), dim3(kThreads), 0, s, sum);
