@@ -346,9 +346,9 @@ int yuf_embedding_grad_bf16(int64_t M, int V, int D, const void *tokens, int tok
  *   steps      : 1 to 64.  a, b, c: coefficients under which no singular value of a
  *                matrix of norm 1 grows past 256.  eps >= 0.
  *   workspace  : yuf_newton_schulz_workspace(count, rows, cols) bytes.
- * fp32: products of operands with 22 bits, summed in fp32 (the error of fp32
- * products).  bf16: the same up to 128 rows (the smaller side) or beyond 6
- * steps, else operands with 11 bits and a X with 22; rounded to bf16 once.
+ * Products of operands with 22 bits, summed in fp32, for either type; the result is
+ * rounded to it once.  About the error of fp32 products (an operand's rounding is up to
+ * four times fp32's), which the polynomial amplifies as it does theirs.
  * X's elements are held in steps of at least 2^-38, so a matrix whose norm is far below
  * eps keeps fewer digits.  A matrix with a NaN or an infinity gives NaN.  Padded to multiples of 128, a matrix
  * may have 2^28 elements.  Matrices are taken in groups, of which the workspace holds one.

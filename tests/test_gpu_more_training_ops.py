@@ -293,8 +293,8 @@ def test_embedding_in_graphs_and_on_streams():
 # 22 bits for 24, so each rounding is at most 4 times as large: 4 times that error.  A small matrix has few
 # roundings, and float32's may cancel; then the last step's remain: its terms a X, b A X and c A A X are
 # together up to (3.4 + 4.8 * 1.2^2 + 2.0 * 1.2^4) = 14.6 times X, each with up to three operands off by 2^-22 of
-# themselves, 44 times 2^-22 in all, of which LAST = 16 are allowed.  bf16's products, of 11 bits or 22, are held to the half step of its output, 2^-8 in the 2-norm,
-# whose rounding alone takes up to 0.6 of that.
+# themselves, 44 times 2^-22 in all, of which LAST = 16 are allowed.  bf16's products, of 22 bits too, are held to the half
+# step of its output, 2^-8 in the 2-norm, whose rounding alone takes up to 0.6 of that.
 ABC = (3.4445, -4.7750, 2.0315)
 LAST = 16 * 2.0**-22
 
@@ -566,3 +566,107 @@ def test_a_training_step_of_these_operators():
     new_p, _, step, loose = muon_reference(square.detach(), square.grad, momenta[0], 0.02)
     ops.muon_step([square], [square.grad], momenta, 0.02)
     assert norms(square.detach().double() - new_p) <= 4 * loose + LAST * (step + norms(new_p))
+
+
+# ------------------------------------------------------- weight updates: spectra, coefficients, launches
+STEEP = (4.0848, -6.8946, 2.9270)  # slopes of up to 4 near the values that the steps settle at
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=gen(seed), device="cuda")
+
+
+def of_singular_values(seed, values, rows, cols):
+    """A [rows, cols] matrix of these singular values."""
+    few = min(rows, cols)
+    left, right = (torch.linalg.qr(normal(seed + i, n, few).double())[0] for i, n in enumerate((rows, cols)))
+    return (left * values.to(left)) @ right.mT.contiguous()
+
+
+def one_row(seed, rows, cols, few=None):
+    x = torch.zeros(rows, cols, device="cuda")
+    x[rows // 2, :few] = normal(seed, cols if few is None else few)
+    return x
+
+
+SPECTRA = {
+    "normal": lambda r, c: normal(60, r, c),
+    "equal": lambda r, c: of_singular_values(61, torch.ones(min(r, c)), r, c),
+    "near": lambda r, c: of_singular_values(63, torch.logspace(0, -0.3, min(r, c)), r, c),
+    "one row": lambda r, c: one_row(65, r, c),
+    "seven elements": lambda r, c: one_row(66, r, c, 7),
+    "ones": lambda r, c: torch.ones(r, c, device="cuda"),
+}
+
+
+@pytest.mark.parametrize("steps,abc", [(5, ABC), (6, ABC), (5, STEEP)], ids=["5", "6", "steep"])
+@pytest.mark.parametrize("rows,cols", [(129, 200), (160, 160), (333, 1111), (640, 2560), (1024, 1024)])
+@pytest.mark.parametrize("spectrum", SPECTRA)
+def test_newton_schulz_bf16_of_any_spectrum(spectrum, rows, cols, steps, abc):
+    """Before its rounding a bf16 result is as near as a float32 one, whatever the matrix: the rounding's half step, 2^-8 of each
+    element, is all that is seen.  (Operands of 11 bits are not enough: amplified in few directions near 1 their errors reached 1.2e-2
+    with seven elements, 2^-8 = 3.9e-3, and 8.5e-2 with equal singular values and steep coefficients.)"""
+    from yufmusicgen_amd import ops
+
+    print(f"newton schulz bf16 {spectrum} {rows} x {cols}, {steps} steps of {abc}", flush=True)
+    x = SPECTRA[spectrum](rows, cols).bfloat16()
+    expect = polynomial(x.double(), steps, abc)
+    off = 2.0**-8 * norms(expect) + 4 * norms(polynomial(x.float(), steps, abc).double() - expect) + LAST * norms(expect)
+    err = norms(ops.newton_schulz(x, steps=steps, coefficients=abc).double() - expect)
+    print(f"  {(err / norms(expect)).item():.2e}, allowed {(off / norms(expect)).item():.2e}", flush=True)
+    assert err <= off
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("steps,abc", [(1, ABC), (3, ABC), (6, ABC), (7, ABC), (20, (1.5, -0.5, 0.0)), (5, (0.5, 0.0, 0.0)),
+                                       (2, (0.0, 1.0, -1.0)), (3, (-2.0, 1.0, 0.25))])
+def test_newton_schulz_of_other_coefficients_in_tiles(steps, abc, kind):
+    from yufmusicgen_amd import ops
+
+    print(f"newton schulz in tiles, {steps} steps of {abc} {kind}", flush=True)
+    x = normal(67, 2, 200, 300).to(TYPES[kind])
+    check_ns(ops.newton_schulz(x, steps=steps, coefficients=abc), x, kind, steps=steps, abc=abc)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_newton_schulz_of_extreme_matrices_in_tiles(kind):
+    """As of small ones: scales over the type's range, zeros, a rank of one, non-finite matrices among finite ones."""
+    from yufmusicgen_amd import ops
+
+    x = gradient(68, 7, 200, 300).to(TYPES[kind])
+    x[1] *= 1e30
+    x[2] *= 1e-20
+    x[3] = 0
+    x[4] = x[4, :, :1] @ x[4, :1, :]
+    x[5, 3, 4] = float("nan")
+    x[6, 199, 299] = float("inf")
+    got = ops.newton_schulz(x, eps=0.0)
+    assert got[[3, 5, 6]].isnan().all()
+    check_ns(got[[0, 1, 2, 4]], x[[0, 1, 2, 4]], kind, eps=0.0)
+    assert (ops.newton_schulz(x)[3] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count,rows,cols", [(60, 256, 256), (64, 640, 640), (49, 256, 256)])
+def test_newton_schulz_of_many_matrices(count, rows, cols, kind):
+    """Launches whose symmetric products take other tiles than their last product, and full groups of 64."""
+    from yufmusicgen_amd import ops
+
+    print(f"newton schulz {count} x {rows} x {cols} {kind}", flush=True)
+    x = gradient(69, count, rows, cols).to(TYPES[kind])
+    check_ns(ops.newton_schulz(x), x, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_newton_schulz_of_more_matrices_than_a_workspace_holds(kind):
+    """2 GB of operands are 8 matrices of this size: the ninth is taken alone, in the same memory."""
+    from yufmusicgen_amd import ops
+    from yufmusicgen_amd._lib import lib
+
+    count, rows, cols = 9, 4000, 4090
+    assert lib().yuf_newton_schulz_workspace(count, rows, cols) == lib().yuf_newton_schulz_workspace(count - 1, rows, cols)
+    print(f"newton schulz {count} x {rows} x {cols} {kind}", flush=True)
+    x = gradient(70, count, rows, cols).to(TYPES[kind])
+    got = ops.newton_schulz(list(x))
+    for i in (0, 7, 8):
+        check_ns(got[i], x[i], kind)

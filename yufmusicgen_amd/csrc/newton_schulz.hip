@@ -9,27 +9,23 @@
 // |v - hi - lo| <= 2^-22 |v|.  The scale of each matrix follows from a bound of its singular values (X starts
 // with a Frobenius norm of 1, and the polynomial's largest value bounds each next step), which bounds its elements, so
 // nothing overflows and what is lost below fp16's subnormals is under 2^-38 of the bound.
-// fp32 matrices take three products, hi hi + hi lo + lo hi (the one left out is below 2^-22): the polynomial amplifies
-// what a step adds along small singular values by up to a each step, so fp32 results need operands near
-// fp32's precision (2-norm errors on the CPU, 640 x 640: 1.8e-6; fp32 products 2.9e-6).
-// bf16 matrices take hi hi alone in the products, but a X from both parts, and A and P = b A + c A A keep 32-bit sums
-// until they are rounded: what a rounded product adds stays in the row space of X and is not amplified
-// (640 x 640: 1.7e-4 against the 1.7e-3 of the output's rounding).  Near singular values of 1 the polynomial has slopes
-// of up to 4, so few of them, whose errors do not average, and many steps go astray: 1 x 7 1.2e-2, 129 x 129 after 10
-// steps 4.6e-3.  So this form is taken for more than kOnePartRows rows and up to kOnePartSteps steps (there at most 0.8
-// of 2^-8, the output's half step, for matrices of 96 to 640 rows), and three products elsewhere.
+// A product of two is three of theirs, hi hi + hi lo + lo hi (the one left out is below 2^-22): the polynomial amplifies what
+// a step's rounding adds, along small singular values by up to a each step and near 1 by slopes of up to 4, and by how much
+// in all depends on the matrix (2-norm errors of 640 x 640: 1.8e-6; of fp32 products 2.9e-6).  bf16 matrices take the
+// same: hi hi alone, 11 bits, is enough for many noisy directions (2e-4, against the 3.9e-3 of the output's half step), but was
+// off by 6e-3 for 333 equal singular values, 9.6e-3 for equal elements, 8.5e-2 with steeper coefficients, and no rule on
+// sizes, steps and coefficients tells these apart.
 //
 // Layout: every operand lies in 1 KB blocks of 16 rows x 32 k in the order in which the lanes of
 // v_mfma_f32_16x16x32_f16 hold them (lane l: row l % 16, k = 8 (l / 16) + j), hi blocks and then lo blocks.
 // Blocks go from memory to LDS as they lie, and from LDS to registers without bank conflicts.  X is kept as X^T
 // (rows of q, k over p), as P X takes it; X X^T, which runs over q, reads the same blocks from LDS transposed.
-// (Keeping X both ways would write it twice: that and loads that waited for each other took 3.5 ms for an update of
-// 24 x 1024 x 4096 bf16 matrices, against 2.7.)
+// (Keeping X both ways would write it twice.)
 //
-// Five steps of 56 x 640 x 640 fp32 (three products): X X^T 70 us, A A 65, P X 95 a step = 750, 810 and 930 TFLOP/s of
-// multiplied tiles; the whole update 1.26 ms.  24 x 1024 x 4096 bf16: 146, 45, 279 us a step, 800, 650 and 740 TFLOP/s
-// (a large bf16 matrix product of the same card: 1.2 to 1.3 PFLOP/s).  What bounds the products is their operands' way
-// into LDS: without those loads X X^T of the fp32 case takes 51 us and P X 60.
+// Five steps of 56 x 640 x 640 fp32: X X^T 68 us, A A 63, P X 91 a step = 780, 840 and 960 TFLOP/s of multiplied tiles;
+// the whole update 1.22 ms.  24 x 1024 x 4096 bf16: 332, 88, 514 us a step, 1050, 990 and 1200 TFLOP/s, 5.2 ms (a
+// large fp16 matrix product of the same card: 1.2 to 1.3 PFLOP/s).  What bounds the former is their operands' way into
+// LDS: without those loads X X^T takes 51 us and P X 60.
 #include "common.h"
 
 #include <algorithm>
@@ -56,7 +52,6 @@ constexpr int kSumParts = 64;   // workgroups of a matrix's norm, at most
 constexpr int kSumRun = 4096;   // elements of such a workgroup, at least
 constexpr int kPrepTile = 64;
 constexpr int kStepsMost = 64;
-constexpr int kOnePartRows = 128, kOnePartSteps = 6;
 constexpr double kGrowthMost = 256.0;  // of the singular values' bound
 constexpr double kPolyMost = 1e6;      // of P's; no polynomial with the former bound comes near it
 constexpr double kBelow = 30000.0;     // scaled values stay below this (fp16 holds 65504)
@@ -297,23 +292,21 @@ template <typename T> struct Product {
     Buffers b;
     int pp, qp, xt;         // xt: which of the two X^T is read
     int tiles_m, tiles_n, total, per_xcd;
-    float factor, linear, diagonal;  // value = factor sum + linear (A or X) + diagonal on the diagonal
+    float factor, linear, diagonal;  // value = factor sum, of P + linear A + diagonal on the diagonal
     Matrices<T> t;          // NS_LAST
 };
 
-// C = L R^T of one tile of TILE x TILE; L and R rows of K in blocks.  NP: products of a pair (1 or 3).  Four waves have a
-// quarter of the tile each.  A stage holds KB k blocks, ST stages lie in LDS; the loads of the stage that is ST - 1 ahead
-// are issued between the products of the present one, a few at a time.
-template <typename T, int MODE, int NP, int TILE, int KB, int ST>
+// C = L R^T of one tile of TILE x TILE; L and R rows of K in blocks.  Four waves have a quarter of the tile each.  A
+// stage holds one k block, ST stages lie in LDS; the loads of the stage that is ST - 1 ahead are issued between the
+// products of the present one, a few at a time.
+template <typename T, int MODE, int TILE, int ST>
 __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
     constexpr int NW = kThreads / kWave;
-    constexpr int PL = NP == 1 ? 1 : 2;       // parts that are multiplied
     constexpr int RB = TILE / 16;             // row blocks of an operand
-    constexpr int HB = RB * KB * PL;          // blocks of a stage: L's, then R's
+    constexpr int HB = RB * 2;                // blocks of a stage, hi and lo: L's, then R's
     constexpr int PER = 2 * HB / NW;          // of a wave
     constexpr int MI = RB / 2;                // 16 x 16 blocks of a wave along each side
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    constexpr bool HALF = NP == 1;
     static_assert(HB % NW == 0 && MI % 2 == 0, "shares of a wave");
     constexpr int kStages = ST * 2 * HB * 512;
     __shared__ __attribute__((aligned(1024))) f16 lds[kStages];
@@ -338,28 +331,27 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
     const int wm = wave >> 1, wn = wave & 1, g4 = lane >> 4, li = lane & 15;
     f16 *const base = p.space + (int64_t)matrix * p.b.stride;
     const Buffers &b = p.b;
-    const int K = MODE == NS_GRAM ? p.qp : p.pp, KT = K / 32 / KB;
+    const int K = MODE == NS_GRAM ? p.qp : p.pp, KT = K / 32;
     const int64_t left = MODE == NS_GRAM ? b.xt[p.xt] : MODE == NS_POLY ? b.gram : b.poly;
     const int64_t right = SYM ? left : b.xt[p.xt];
     const int64_t plane_l = MODE == NS_GRAM ? b.long_plane : b.short_plane, plane_r = SYM ? plane_l : b.long_plane;
-    const auto rl = make_rsrc(base + left, (uint32_t)(plane_l * PL * 2)), rr = make_rsrc(base + right, (uint32_t)(plane_r * PL * 2));
+    const auto rl = make_rsrc(base + left, (uint32_t)(plane_l * 4)), rr = make_rsrc(base + right, (uint32_t)(plane_r * 4));
 
     uint32_t off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int x = wave + NW * i, of_r = x >= HB, at = x - of_r * HB;
-        const int part = at / (RB * KB), tile = of_r ? bn : bm;
+        const int part = at / RB, tile = of_r ? bn : bm;
         int block;
-        if (MODE == NS_GRAM) {  // [k block][its 16 rows of X^T][32 of the tile's rows, which are k there]
-            const int kr = at % (RB * KB) / (RB / 2), ic = at % (RB / 2);
+        if (MODE == NS_GRAM) {  // [16 rows of X^T][32 of the tile's rows, which are k there]
+            const int kr = at % RB / (RB / 2), ic = at % (RB / 2);
             block = kr * (p.pp / 32) + tile * (RB / 2) + ic;
-        } else {  // [row block][k block]
-            const int rb = at / KB % RB, kb = at % KB;
-            block = (tile * RB + rb) * (K / 32) + kb;
+        } else {  // a row block
+            block = (tile * RB + at % RB) * (K / 32);
         }
         off[i] = (uint32_t)(block * 1024 + part * (int)((of_r ? plane_r : plane_l) * 2) + lane * 16);
     }
-    const int step = MODE == NS_GRAM ? KB * 2 * (p.pp / 32) * 1024 : KB * 1024;  // of a stage
+    const int step = MODE == NS_GRAM ? 2 * (p.pp / 32) * 1024 : 1024;  // of a stage
     auto issue_one = [&](int i, int kt, int buf) {
         lds_void_t *dst = (lds_void_t *)(lds + (buf * 2 * HB + wave + NW * i) * 512);
         const uint32_t o = off[i];
@@ -379,21 +371,18 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
 
     // Where a lane's transposing reads begin in a k block of 32 rows of X^T: for group g4 at k = 8 g4 + li / 4, four
     // of its 16 rows' elements from 4 (li % 4) on.
-    const auto turned = [&](int part, int m, int kb) {
-        const int block = ((part * KB + kb) * 2 + (g4 >> 1)) * (RB / 2) + m / 2;
+    const auto turned = [&](int part, int m) {
+        const int block = (part * 2 + (g4 >> 1)) * (RB / 2) + m / 2;
         return block * 512 + li % 4 / 2 * 128 + ((g4 & 1) * 8 + li / 4) * 8 + li % 2 * 4;
     };
     const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void_t *)lds;
 
     // The products with a low part are summed apart: a third of the roundings in the large sum.
-    floatx4 acc[MI][MI], low[NP == 3 ? MI : 1][MI];
+    floatx4 acc[MI][MI], low[MI][MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) {
-            acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (NP == 3) low[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int j = 0; j < MI; ++j) acc[i][j] = low[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
         if (s < KT) issue(s, s);
@@ -403,26 +392,24 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
         // Stage kt is in LDS for every wave, and every wave has read stage kt - 1.
         arrive(kt + ST - 1 > KT, std::integral_constant<int, ST - 2>{});
         const f16 *const l = lds + buf * 2 * HB * 512, *const r = l + HB * 512;
-        f16x8 fl[KB][PL][MI], fr[KB][PL][MI];
+        f16x8 fl[2][MI], fr[2][MI];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int q = 0; q < 2; ++q) {
+            if constexpr (MODE == NS_GRAM) {
+                const uint32_t at = lds_at + buf * 2 * HB * 1024;
+                read_transposed<MI>(at + turned(q, wm * MI) * 2, at + HB * 1024 + turned(q, wn * MI) * 2, fl[q], fr[q]);
+            } else {
 #pragma unroll
-            for (int q = 0; q < PL; ++q) {
-                if constexpr (MODE == NS_GRAM) {
-                    const uint32_t at = lds_at + buf * 2 * HB * 1024;
-                    read_transposed<MI>(at + turned(q, wm * MI, kb) * 2, at + HB * 1024 + turned(q, wn * MI, kb) * 2, fl[kb][q], fr[kb][q]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        fl[kb][q][i] = *reinterpret_cast<const f16x8 *>(l + ((q * RB + wm * MI + i) * KB + kb) * 512 + lane * 8);
-                        fr[kb][q][i] = *reinterpret_cast<const f16x8 *>(r + ((q * RB + wn * MI + i) * KB + kb) * 512 + lane * 8);
-                    }
+                for (int i = 0; i < MI; ++i) {
+                    fl[q][i] = *reinterpret_cast<const f16x8 *>(l + (q * RB + wm * MI + i) * 512 + lane * 8);
+                    fr[q][i] = *reinterpret_cast<const f16x8 *>(r + (q * RB + wn * MI + i) * 512 + lane * 8);
                 }
             }
+        }
         // The next loads go between the products: a wave that issues its loads one after the other waits for about 80
         // cycles each, in which it multiplies nothing.
         const int target = buf == 0 ? ST - 1 : buf - 1;
-        constexpr int kProducts = KB * NP * MI * MI, kEvery = kProducts / PER;
+        constexpr int kProducts = 3 * MI * MI, kEvery = kProducts / PER;
         static_assert(kProducts % PER == 0, "products between loads");
 #pragma unroll
         for (int n = 0; n < kProducts; ++n) {
@@ -431,47 +418,40 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
                 issue_one(n / kEvery, kt + ST - 1, target);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const int kb = n / (NP * MI * MI), q = n / (MI * MI) % NP, i = n / MI % MI, j = n % MI;
-            if (q == 0) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kb][0][i], fr[kb][0][j], acc[i][j], 0, 0, 0);
-            else low[NP == 3 ? i : 0][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[kb][NP == 3 ? 2 - q : 0][i], fr[kb][NP == 3 ? q - 1 : 0][j],
-                                                                                  low[NP == 3 ? i : 0][j], 0, 0, 0);
+            const int q = n / (MI * MI), i = n / MI % MI, j = n % MI;  // hi hi, lo hi, hi lo
+            floatx4 &sum = q == 0 ? acc[i][j] : low[i][j];
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[q == 1][i], fr[q == 2][j], sum, 0, 0, 0);
         }
         buf = buf == ST - 1 ? 0 : buf + 1;
     };
     int kt = 0;
     for (; kt < KT - (ST - 1); ++kt) multiply(kt, std::true_type{});
     for (; kt < KT; ++kt) multiply(kt, std::false_type{});
-    if constexpr (NP == 3) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < MI; ++j) acc[i][j] += low[i][j];
-    }
+        for (int j = 0; j < MI; ++j) acc[i][j] += low[i][j];
     // Lane (g4, li) holds rows 4 g4 + r and column li of block (i, j).  As rows of an operand the tile's columns' four
     // elements are neighbours: at a wave's block of 16 columns x 32 rows and at `mine` in it.
     const int row0 = (bm * RB + wm * MI) * 16, col0 = (bn * RB + wn * MI) * 16;
     const int kblocks = p.pp / 32;
     const int mine = (g4 >> 1) * 128 + li * 8 + (g4 & 1) * 4;
     const auto turned_block = [&](int i, int j) { return ((col0 / 16 + j) * kblocks + row0 / 32 + i / 2) * 512 + i % 2 * 256; };
-    const f16 *const addend = base + (MODE == NS_POLY ? b.gram : b.xt[p.xt]);  // A, which is symmetric, or X
     const int64_t plane = SYM ? b.short_plane : b.long_plane;
     const float factor = p.factor, linear = p.linear, diagonal = p.diagonal;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
         for (int j = 0; j < MI; ++j) {
-            if (MODE == NS_POLY || (HALF && !SYM)) {
-                const f16 *at = addend + turned_block(i, j);
-                const f16x4 hi = *reinterpret_cast<const f16x4 *>(at + mine), lo = *reinterpret_cast<const f16x4 *>(at + plane + mine);
+            acc[i][j] *= factor;
+            if (MODE == NS_POLY) {
+                const f16 *at = base + b.gram + turned_block(i, j) + mine;  // A, which is symmetric
+                const f16x4 hi = *reinterpret_cast<const f16x4 *>(at), lo = *reinterpret_cast<const f16x4 *>(at + plane);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(linear, (float)hi[r] + (float)lo[r], factor * acc[i][j][r]);
-            } else {
-                acc[i][j] *= factor;
-            }
-            if (MODE == NS_POLY && !HALF) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 4; ++r) {
+                    acc[i][j][r] = fmaf(linear, (float)hi[r] + (float)lo[r], acc[i][j][r]);
                     if (row0 + i * 16 + 4 * g4 + r == col0 + j * 16 + li) acc[i][j][r] += diagonal;
+                }
             }
         }
     }
@@ -548,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
             split(v, hi, lo);
             f16 *at = to + turned_block(i, j);
             *reinterpret_cast<f16x4 *>(at + mine) = hi;
-            if (!(MODE == NS_POLY && HALF)) *reinterpret_cast<f16x4 *>(at + plane + mine) = lo;
+            *reinterpret_cast<f16x4 *>(at + plane + mine) = lo;
         }
     if (!SYM || bm == bn) return;
     // The mirrored tile's blocks, through wave-private LDS.
@@ -572,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
             split(v, hi, lo);
             f16 *at = to + ((row0 / 16 + i) * kblocks + col0 / 32 + j / 2) * 512;
             *reinterpret_cast<f16x8 *>(at + lane * 8) = hi;
-            if (!HALF || MODE == NS_GRAM) *reinterpret_cast<f16x8 *>(at + plane + lane * 8) = lo;
+            *reinterpret_cast<f16x8 *>(at + plane + lane * 8) = lo;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
         }
@@ -814,7 +794,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) ns_small_kernel(Matrices<T> 
 struct Plan {
     int p, q, pp, qp, parts, group;
     bool whole;  // a workgroup for each matrix
-    bool small_sym, small_apply, many;
+    bool small_sym, small_apply;
     Buffers b;
     size_t sums, bytes;
 };
@@ -822,14 +802,10 @@ struct Plan {
 int round_up(int x, int to) { return (x + to - 1) / to * to; }
 
 // Tiles of 128 x 128 load least for their products; of 64 x 64 four times as many, which counts where 128 x 128 ones
-// do not fill the card.  Launches in us, 128 and 64, by tiles of 128 (bf16, one part):
-//   X X^T: 60 x 2560 29 and 17, 120 x 2560 31 and 21, 144 x 4096 46 and 45, 210 x 2560 34 and 38, 288 x 4096 57 and 73;
-//   P X: 100 x 640 11.5 and 8.3, 256 x 1024 17.7 and 18.0, 350 x 640 16.6 and 19.0, 400 x 640 17.3 and 22.5;
-// three products: X X^T 210 x 640 24 and 21, 288 x 1024 38 and 43; A A 288 x 1024 41 and 37; 420 x 640 33 and 36;
-//   P X 100 x 640 18 and 11, 350 x 640 26 and 28.  (Rows of the sum: tiles x k.)
-// Many tiles of one part take stages of one k block, so that three workgroups share a CU: P X 400 x 640 17.3 and 18.7,
-// 1400 x 640 53 and 51, 2800 x 640 116 and 107, 6144 x 1024 303 and 275.
-Plan ns_plan(int count, int rows, int cols, bool one_part) {
+// do not fill the card.  Launches in us, 128 and 64, by tiles of 128 x rows of the sum:
+//   X X^T 210 x 640 24 and 21, 288 x 1024 38 and 43; A A 288 x 1024 41 and 37, 420 x 640 33 and 36;
+//   P X 100 x 640 18 and 11, 350 x 640 26 and 28.
+Plan ns_plan(int count, int rows, int cols) {
     Plan s{};
     s.p = std::min(rows, cols);
     s.q = std::max(rows, cols);
@@ -838,9 +814,8 @@ Plan ns_plan(int count, int rows, int cols, bool one_part) {
     s.group = std::min({count, kGroup, (int)std::max<size_t>(1, std::min<size_t>(kGroup, kSpaceMost / most))});
     const int64_t tiles = (s.p + 127) / 128, sym = s.group * (tiles * (tiles + 1) / 2), apply = s.group * tiles * ((s.q + 127) / 128);
     s.whole = s.p <= kSmallRows && s.q <= kSmallColumns;
-    s.small_sym = s.p <= 128 || sym <= (one_part ? 144 : 256);
+    s.small_sym = s.p <= 128 || sym <= 256;
     s.small_apply = s.p <= 128 || apply <= 200;
-    s.many = apply > 1536;
     const int unit = s.small_sym && s.small_apply ? 64 : 128;
     s.pp = round_up(s.p, unit);
     s.qp = round_up(s.q, unit);
@@ -869,19 +844,18 @@ const char *ns_refusal(int count, int rows, int cols) {
 }
 
 // For each step, the scales of X, A and P, from a bound of X's singular values.
-const char *ns_scales(int steps, double a, double b, double c, bool half, Scales &s) {
+const char *ns_scales(int steps, double a, double b, double c, Scales &s) {
     const auto scale = [](double bound) {
         return (float)std::ldexp(1.0, std::min(40, (int)std::floor(std::log2(kBelow / std::max(bound, 1e-30)))));
     };
-    const double base = half ? 0.0 : a;  // P holds a I where X is multiplied by it in whole
     double bound = 1.0;
     for (int k = 0; k < steps; ++k) {
         const double top = bound * bound;  // of X's squared singular values
-        // Extremes of base + b u + c u^2 and of t (a + b t^2 + c t^4) over the bound: ends and stationary points.
-        double poly = std::max(std::fabs(base), std::fabs(base + b * top + c * top * top)), next = std::fabs(bound * (a + b * top + c * top * top));
+        // Extremes of a + b u + c u^2 and of t (a + b t^2 + c t^4) over the bound: ends and stationary points.
+        double poly = std::max(std::fabs(a), std::fabs(a + b * top + c * top * top)), next = std::fabs(bound * (a + b * top + c * top * top));
         if (c != 0.0) {
             const double u = -b / (2 * c);
-            if (u > 0 && u < top) poly = std::max(poly, std::fabs(base + b * u + c * u * u));
+            if (u > 0 && u < top) poly = std::max(poly, std::fabs(a + b * u + c * u * u));
         }
         const double disc = 9 * b * b - 20 * a * c;
         if (disc >= 0) {
@@ -900,45 +874,39 @@ const char *ns_scales(int steps, double a, double b, double c, bool half, Scales
     return nullptr;
 }
 
-template <typename T, int MODE, int NP, int TILE, int KB, int ST> hipError_t launch_product(Product<T> &p, hipStream_t s) {
+template <typename T, int MODE, int TILE, int ST> hipError_t launch_product(Product<T> &p, hipStream_t s) {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     p.tiles_m = p.pp / TILE; p.tiles_n = SYM ? p.tiles_m : p.qp / TILE;
     p.total = p.t.count * (SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n);
     p.per_xcd = ceil_div(p.total, kXcds);
-    hipLaunchKernelGGL((ns_product_kernel<T, MODE, NP, TILE, KB, ST>), dim3(p.per_xcd * kXcds), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((ns_product_kernel<T, MODE, TILE, ST>), dim3(p.per_xcd * kXcds), dim3(kThreads), 0, s, p);
     return hipGetLastError();
 }
 
 // A product in the tiles that its plan names.  Small tiles take four stages: with few workgroups a CU each has to cover
 // its own loads (X X^T of 4 x 640 x 640 fp32 10.3 us, of 1024 x 1024 12.8; two stages 14.2 and 20.3), and of many two
 // workgroups a CU do as well as four (14 x 640 x 640 21.4 and 22.8).
-template <typename T, int MODE, int NP> hipError_t launch_mode(const Plan &plan, Product<T> &p, hipStream_t s) {
+template <typename T, int MODE> hipError_t launch_mode(const Plan &plan, Product<T> &p, hipStream_t s) {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    if (SYM ? plan.small_sym : plan.small_apply) return launch_product<T, MODE, NP, 64, NP == 1 ? 2 : 1, 4>(p, s);
-    if constexpr (NP == 3) return launch_product<T, MODE, NP, 128, 1, 2>(p, s);
-    else if constexpr (SYM) return launch_product<T, MODE, NP, 128, 1, 4>(p, s);
-    else if constexpr (MODE == NS_LAST) return launch_product<T, MODE, NP, 128, 1, 3>(p, s);
-    else return plan.many ? launch_product<T, MODE, NP, 128, 1, 2>(p, s) : launch_product<T, MODE, NP, 128, 2, 2>(p, s);
+    return (SYM ? plan.small_sym : plan.small_apply) ? launch_product<T, MODE, 64, 4>(p, s) : launch_product<T, MODE, 128, 2>(p, s);
 }
 
-template <typename T, int NP>
+template <typename T>
 int ns_group(const Plan &plan, const Matrices<T> &t, const Scales &scales, int steps, float a, float b, float c, double eps,
              char *space, hipStream_t s) {
     double *sums = reinterpret_cast<double *>(space + plan.sums);
     f16 *halves = reinterpret_cast<f16 *>(space);
-    if constexpr (NP == 3) {
-        if (plan.whole) {
-            const int blocks = ceil_div(plan.q, 32 * kSmallWaves);  // of a wave
-            const auto run = [&](auto n) {
-                hipLaunchKernelGGL((ns_small_kernel<T, decltype(n)::value>), dim3(t.count), dim3(kSmallThreads), 0, s, t, scales, steps, a, b,
-                                   c, eps);
-            };
-            if (blocks == 1) run(std::integral_constant<int, 1>{});
-            else if (blocks == 2) run(std::integral_constant<int, 2>{});
-            else run(std::integral_constant<int, kSmallBlocks>{});
-            YUF_LAUNCH_CHECK("newton schulz");
-            return YUF_OK;
-        }
+    if (plan.whole) {
+        const int blocks = ceil_div(plan.q, 32 * kSmallWaves);  // of a wave
+        const auto run = [&](auto n) {
+            hipLaunchKernelGGL((ns_small_kernel<T, decltype(n)::value>), dim3(t.count), dim3(kSmallThreads), 0, s, t, scales, steps, a, b, c,
+                               eps);
+        };
+        if (blocks == 1) run(std::integral_constant<int, 1>{});
+        else if (blocks == 2) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, kSmallBlocks>{});
+        YUF_LAUNCH_CHECK("newton schulz");
+        return YUF_OK;
     }
     hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(plan.parts, t.count), dim3(kThreads), 0, s, t, plan.parts, sums);
     hipLaunchKernelGGL((ns_prepare_kernel<T>), dim3(plan.qp / kPrepTile, plan.pp / kPrepTile, t.count), dim3(kThreads), 0, s, t,
@@ -950,12 +918,12 @@ int ns_group(const Plan &plan, const Matrices<T> &t, const Scales &scales, int s
         const float x = scales.x[k], gram = scales.gram[k], poly = scales.poly[k], next = scales.x[k + 1];
         p.xt = k & 1;
         p.factor = gram / (x * x);
-        YUF_HIP_TRY((launch_mode<T, NS_GRAM, NP>(plan, p, s)));
+        YUF_HIP_TRY((launch_mode<T, NS_GRAM>(plan, p, s)));
         p.factor = c * (poly / (gram * gram)); p.linear = b * (poly / gram); p.diagonal = a * poly;
-        YUF_HIP_TRY((launch_mode<T, NS_POLY, NP>(plan, p, s)));
-        p.factor = next / (poly * x); p.linear = a * (next / x);
-        if (k + 1 < steps) YUF_HIP_TRY((launch_mode<T, NS_APPLY, NP>(plan, p, s)));
-        else YUF_HIP_TRY((launch_mode<T, NS_LAST, NP>(plan, p, s)));
+        YUF_HIP_TRY((launch_mode<T, NS_POLY>(plan, p, s)));
+        p.factor = next / (poly * x);
+        if (k + 1 < steps) YUF_HIP_TRY((launch_mode<T, NS_APPLY>(plan, p, s)));
+        else YUF_HIP_TRY((launch_mode<T, NS_LAST>(plan, p, s)));
     }
     return YUF_OK;
 }
@@ -995,14 +963,13 @@ int newton_schulz(int count, int rows, int cols, const T *const *x, float *const
     if (const char *why = ns_refusal(count, rows, cols)) return fail(YUF_ERR_INVALID, why);
     if (steps < 1 || steps > kStepsMost) return fail(YUF_ERR_INVALID, "newton schulz: steps must be 1 to 64");
     if (!(eps >= 0.0) || !std::isfinite(eps)) return fail(YUF_ERR_INVALID, "newton schulz: eps must be finite and not negative");
-    const bool one_part = sizeof(T) == 2 && std::min(rows, cols) > kOnePartRows && steps <= kOnePartSteps;
     Scales scales{};
-    if (const char *why = ns_scales(steps, a, b, c, one_part, scales)) return fail(YUF_ERR_INVALID, why);
+    if (const char *why = ns_scales(steps, a, b, c, scales)) return fail(YUF_ERR_INVALID, why);
     if (count == 0 || rows == 0 || cols == 0) return YUF_OK;
     if (!x || !out || (t.update && !m)) return fail(YUF_ERR_INVALID, "newton schulz: null list of matrices");
     if (!workspace || !scratch_aligned(workspace))
         return fail(YUF_ERR_INVALID, "newton schulz: the workspace must be given and 256-byte aligned");
-    const Plan plan = ns_plan(count, rows, cols, one_part);
+    const Plan plan = ns_plan(count, rows, cols);
     try {
         if (const char *why = ns_overlap(count, (size_t)rows * cols, x, m, out, workspace, plan.bytes)) return fail(YUF_ERR_INVALID, why);
     } catch (const std::bad_alloc &) {
@@ -1017,14 +984,7 @@ int newton_schulz(int count, int rows, int cols, const T *const *x, float *const
             t.m[i] = t.update ? m[first + i] : nullptr;
         }
         hipStream_t s = static_cast<hipStream_t>(stream);
-        char *at = static_cast<char *>(workspace);
-        int rc;
-        if constexpr (sizeof(T) == 2) {
-            rc = one_part ? ns_group<T, 1>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s)
-                          : ns_group<T, 3>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
-        } else {
-            rc = ns_group<T, 3>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, at, s);
-        }
+        const int rc = ns_group<T>(plan, t, scales, steps, (float)a, (float)b, (float)c, eps, static_cast<char *>(workspace), s);
         if (rc != YUF_OK) return rc;
     }
     return YUF_OK;
@@ -1051,7 +1011,7 @@ int muon_step(int count, int rows, int cols, const T *const *grads, float *const
 
 extern "C" size_t yuf_newton_schulz_workspace(int count, int rows, int cols) {
     if (yuf::ns_refusal(count, rows, cols) || count == 0 || rows == 0 || cols == 0) return 0;
-    return std::max(yuf::ns_plan(count, rows, cols, false).bytes, yuf::ns_plan(count, rows, cols, true).bytes);  // of either type
+    return yuf::ns_plan(count, rows, cols).bytes;
 }
 
 extern "C" int yuf_newton_schulz_f32(int count, int rows, int cols, const float *const *x, float *const *out, int steps, double a,

@@ -592,8 +592,8 @@ def newton_schulz(x, steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float =
     are more rows than columns.
 
     ``x``: [..., R, C], or a list of [R, C] of one shape (and a list is returned); float32
-    or bfloat16.  float32 matrices are multiplied to about float32's precision, large bfloat16
-    ones to 11 bits; the result is rounded once.  Not differentiable.
+    or bfloat16.  Products are of operands with 22 bits, summed in float32 (about the error of
+    float32 products); the result is rounded to x's type once.  Not differentiable.
     """
     several = isinstance(x, (list, tuple))
     if several:
