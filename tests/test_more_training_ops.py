@@ -229,3 +229,58 @@ def test_weight_update_python_refusals():
                                   (ValueError, "contiguous", (g.t(), g.t(), g.t())), (ValueError, "contiguous", (g, g, torch.empty(6, 4, device="cuda:0").t()))):
             with pytest.raises(kind, match=match):
                 ops.muon_step(*([x] for x in args), 0.1)
+
+
+# -------------------------------------------------------------- sizes beyond 32 bits
+def test_sizes_beyond_32_bits_reach_no_entry_point():
+    """A size whose low 32 bits are a valid one is refused where it is converted, not taken for those."""
+    big = (1 << 32) + 5
+    for call in (lambda: lib().yuf_embedding_grad_workspace(4, big, 8), lambda: lib().yuf_embedding_grad_workspace(4, 8, big),
+                 lambda: lib().yuf_newton_schulz_workspace(1, big, 4), lambda: lib().yuf_newton_schulz_workspace(1, 4, -big),
+                 lambda: lib().yuf_newton_schulz_workspace(big, 4, 4), lambda: lib().yuf_cross_entropy_workspace(big),
+                 lambda: lib().yuf_embedding_grad_workspace(4, 1 << 31, 8), lambda: lib().yuf_embedding_grad_workspace(1 << 64, 8, 8),
+                 lambda: lib().yuf_newton_schulz_f32(1, 4, 4, None, None, big, *GOOD[1:], None, None)):
+        with pytest.raises(ctypes.ArgumentError, match="bits"):
+            call()
+    for call in (lambda: lib().yuf_embedding_grad_workspace(4.0, 8, 8), lambda: lib().yuf_newton_schulz_workspace("1", 4, 4)):
+        with pytest.raises(ctypes.ArgumentError):
+            call()
+    assert lib().yuf_embedding_grad_workspace(4, (1 << 31) - 1, 8) == lib().yuf_embedding_grad_workspace(4, -(1 << 31), 8) == 0
+
+
+def test_python_refuses_sizes_beyond_the_documented_ones():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def empty(*shape):
+        return torch.empty(*shape, device="cuda:0", dtype=torch.bfloat16)
+
+    with FakeTensorMode():
+        tokens = torch.empty(3, dtype=torch.int64, device="cuda:0")
+        for size in ((1 << 24) + 1, 1 << 31, (1 << 32) + 5):
+            for weight in (empty(size, 1), empty(5, size)):
+                with pytest.raises(ValueError, match="2\\^24"):
+                    ops.embedding(tokens, weight)
+            for dout, vocab in ((empty(3, 4), size), (empty(3, size), 4)):
+                with pytest.raises(ValueError, match="2\\^24"):
+                    ops.embedding_grad(tokens, dout, vocab)
+        for size in ((1 << 22) + 1, (1 << 32) + 4):
+            for x in (empty(size, 1), empty(1, size), empty(2, size, 1)):
+                with pytest.raises(ValueError, match="too large"):
+                    ops.newton_schulz(x)
+            x, m = empty(size, 4), torch.empty(size, 4, device="cuda:0")
+            with pytest.raises(ValueError, match="too large"):
+                ops.muon_step([x], [x.clone()], [m], 0.1)
+        x = empty((1 << 14) + 1, 1 << 14)
+        with pytest.raises(ValueError, match="too large"):
+            ops.newton_schulz([x, x])
+    ops._check_size(0, 1 << 23)  # nothing is not too large
+    # The same limit as the library's.
+    for rows, cols in ((1 << 14, 1 << 14), ((1 << 14) + 1, 1 << 14), (1, 1 << 20), (1 << 21, 128), ((1 << 21) + 1, 128), (1 << 21, 129), (1 << 22, 1),
+                       ((1 << 22) + 1, 1), (1000, 260000), (127, 1 << 21)):
+        fits = lib().yuf_newton_schulz_workspace(1, rows, cols) > 0
+        try:
+            ops._check_size(rows, cols)
+        except ValueError:
+            assert not fits, (rows, cols)
+        else:
+            assert fits, (rows, cols)

@@ -129,6 +129,23 @@ SIGNATURES = {
                                          ctypes.c_uint64, ctypes.c_uint64, c_void_p, c_void_p]),
 }
 
+def _checked(kind):
+    """The argument type ``kind``, which by itself drops the bits that it does not hold."""
+    high = (1 << 8 * ctypes.sizeof(kind) - 1) - 1
+    convert = kind.from_param
+
+    class Checked:
+        @staticmethod
+        def from_param(value):
+            if not ~high <= value <= high:
+                raise ValueError(f"{value} does not fit in {8 * ctypes.sizeof(kind)} bits")
+            return convert(value)
+
+    return Checked
+
+
+_CHECKED = {kind: _checked(kind) for kind in (ctypes.c_int, ctypes.c_int64)}
+
 _LIB = None
 
 
@@ -144,7 +161,7 @@ def lib() -> ctypes.CDLL:
             if fn is None:  # reported by missing_symbols(); calling it raises AttributeError
                 continue
             fn.restype = restype
-            fn.argtypes = argtypes
+            fn.argtypes = [_CHECKED.get(kind, kind) for kind in argtypes]
         _LIB = handle
     return _LIB
 

@@ -448,6 +448,9 @@ class _CrossEntropy(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------ embedding
+_TABLE_MOST = 1 << 24  # rows, and columns
+
+
 def _check_tokens(tokens, device) -> None:
     if tokens.device != device:
         raise ValueError("tokens must be on the same GPU")
@@ -461,6 +464,11 @@ def _check_padding(padding_idx, vocab: int) -> int:
     if not 0 <= padding_idx < vocab:
         raise ValueError(f"padding_idx must be in [0, {vocab}), got {padding_idx}")
     return int(padding_idx)
+
+
+def _check_table(vocab: int, dim: int) -> None:
+    if vocab > _TABLE_MOST or dim > _TABLE_MOST:
+        raise ValueError(f"a table may have 2^24 rows and columns, got [{vocab}, {dim}]")
 
 
 def embedding(tokens, weight, scale: float = 1.0, padding_idx=None):
@@ -478,6 +486,7 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx=None):
         raise TypeError("embedding takes float32 or bfloat16 weights")
     if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
+    _check_table(*weight.shape)
     _check_tokens(tokens, weight.device)
     padding = _check_padding(padding_idx, weight.shape[0])
     if _needs_grad(weight):
@@ -511,6 +520,7 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
         raise TypeError("embedding takes float32 or bfloat16 gradients")
     if vocab < 0:
         raise ValueError(f"vocab must not be negative, got {vocab}")
+    _check_table(vocab, dout.shape[-1])
     _check_tokens(tokens, dout.device)
     padding = _check_padding(padding_idx, vocab)
     if out is not None:
@@ -569,6 +579,12 @@ def _check_matrices(name: str, matrices, device, dtype) -> None:
             raise TypeError(f"{name} must be {dtype}")
 
 
+def _check_size(rows: int, cols: int) -> None:
+    padded = (rows + 127) // 128 * ((cols + 127) // 128) << 14
+    if rows and cols and (max(rows, cols) > 1 << 22 or padded > 1 << 28):
+        raise ValueError(f"matrices of shape {[rows, cols]} are too large")
+
+
 def _check_apart(written, read) -> None:
     """Contiguous tensors that are written share memory with none of the others."""
     def end(x):
@@ -616,6 +632,7 @@ def newton_schulz(x, steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float =
         raise ValueError("newton_schulz is not differentiable: detach its input")
     a, b, c = coefficients
     rows, cols = first.shape[-2:]
+    _check_size(rows, cols)
     with _on(first.device) as stream:
         if several:
             taken = [m.contiguous() for m in x]
@@ -659,8 +676,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
         _check_like("momenta", m, p.shape, p.device)
         if not p.is_contiguous() or not m.is_contiguous():
             raise ValueError("params and momenta must be contiguous")
-        if p.numel() and not lib().yuf_newton_schulz_workspace(1, *p.shape):
-            raise ValueError(f"matrices of shape {list(p.shape)} are too large")
+        _check_size(*p.shape)
         groups.setdefault((p.shape, p.dtype, p.device), []).append((p, g, m))
     if len(groups) > 1:  # the library sees one group at a time, and all are refused before one is updated
         _check_apart((*params, *momenta), grads)
