@@ -284,3 +284,39 @@ def test_python_refuses_sizes_beyond_the_documented_ones():
             assert not fits, (rows, cols)
         else:
             assert fits, (rows, cols)
+
+
+# ------------------------------------------------------------------- forward mode
+def test_tangents_are_refused():
+    """A dual tensor's primal alone would be taken, with or without a recorded gradient: every operator raises."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+
+    with FakeTensorMode(), forward_ad.dual_level():
+        def plain(*shape):
+            return torch.empty(shape, device="cuda:0")
+
+        def dual(*shape):
+            return forward_ad.make_dual(plain(*shape), plain(*shape))
+
+        tokens = torch.empty(3, dtype=torch.int64, device="cuda:0")
+        scan, state, rosa, row = (2, 3, 2, 8), (2, 2, 8, 8), (2, 3, 4), (4,)
+        scans, rosas = [plain(*scan) for _ in range(7)], [plain(*rosa), plain(*rosa), plain(*rosa), plain(*row), plain(*row), plain(2, 4), plain(*rosa)]
+        calls = [lambda: ops.embedding(tokens, dual(5, 4)), lambda: ops.embedding_grad(tokens, dual(3, 4), 5),
+                 lambda: ops.embedding_grad(tokens, plain(3, 4), 5, out=dual(5, 4)), lambda: ops.newton_schulz(dual(4, 4)),
+                 lambda: ops.newton_schulz([plain(4, 4), dual(4, 4)]), lambda: ops.dropout(dual(4, 4), 0.5, 1),
+                 lambda: ops.dropout(plain(4, 4), 0.5, 1, residual=dual(4, 4)), lambda: ops.cross_entropy(dual(3, 5), tokens),
+                 lambda: ops.cross_entropy_grad(dual(3, 5), tokens), lambda: ops.cross_entropy_grad(plain(3, 5), tokens, dloss=dual()),
+                 lambda: ops.rwkv7_scan(*scans[:6], dual(*state)), lambda: ops.rwkv7_cuda(*scans[:5], dual(*scan)),
+                 lambda: ops.rwkv7_scan_backward(*scans[:6], dual(*scan)), lambda: ops.rwkv7_scan_backward(*scans, dstate=dual(*state)),
+                 lambda: ops.rosa_householder_scan(*rosas[:5], dual(2, 4)), lambda: ops.rosa_householder_scan_backward(*rosas[:6], dual(*rosa)),
+                 lambda: ops.rosa_householder_scan_backward(*rosas, dmemory=dual(2, 4))]
+        for k in range(3):
+            lists = [[plain(4, 4)] for _ in range(3)]
+            lists[k] = [dual(4, 4)]
+            calls.append(lambda lists=lists: ops.muon_step(*lists, 0.1))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -14,7 +14,8 @@ Their gradients are operators too (``rwkv7_scan_backward``,
 ``embedding_grad``): a HIP graph captures those.  Captured ``backward()`` calls through these
 operators raise, because torch ends the process when a capture meets gradient
 accumulators that another, still living autograd graph made on a stream outside
-of it.  A capture that holds a backward pass but not its forward pass ends the
+of it.  Forward-mode derivatives there are none: an input with a tangent raises.
+A capture that holds a backward pass but not its forward pass ends the
 process inside torch before an operator is asked.
 """
 
@@ -23,6 +24,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -54,6 +56,12 @@ class _on:
 
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_tangents(name: str, *tensors) -> None:
+    """The kernels see a dual tensor's primal alone: its tangent would be lost."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _scratch(size: int, device):
@@ -106,6 +114,7 @@ def rwkv7_scan(r, w, k, v, a, b, state=None):
             raise ValueError("state must be a float32 GPU tensor of shape [B, H, N, N]")
         state = state.contiguous()
     _check_one_device("RWKV-7 inputs", *tensors, state)
+    _no_tangents("rwkv7_scan", *tensors, state)
     if _needs_grad(*tensors, state):
         return _Rwkv7Scan.apply(*tensors, state)
     return _rwkv7_forward(*tensors, state)
@@ -145,6 +154,7 @@ def rosa_householder_scan(cand, write, read_raw, decay, direction, memory, gated
     if not all(x.is_cuda for x in tensors):
         raise ValueError("ROSA inputs must be on the GPU")
     _check_one_device("ROSA inputs", *tensors)
+    _no_tangents("rosa_householder_scan", *tensors)
     if _needs_grad(*tensors):
         cand, write, read_raw, decay, direction, memory = tensors
         return _RosaScan.apply(cand, write, read_raw, decay.reshape(dim), direction.reshape(dim),
@@ -190,6 +200,7 @@ def rwkv7_scan_backward(r, w, k, v, a, b, dy, state=None, dstate=None):
     for name, x in (("state", state), ("dstate", dstate)):
         if x is not None:
             _check_like(name, x, (batch, heads, size, size), r.device)
+    _no_tangents("rwkv7_scan_backward", *tensors, state, dstate)
     return _rwkv7_backward(*tensors, state, dstate)
 
 
@@ -247,6 +258,7 @@ def rosa_householder_scan_backward(cand, write, read_raw, decay, direction, memo
     if dmemory is not None:
         dmemory = dmemory.float().contiguous()
         _check_like("dmemory", dmemory, (batch, dim), cand.device)
+    _no_tangents("rosa_householder_scan_backward", *tensors, dmemory)
     cand, write, read_raw, decay, direction, memory, dread = tensors
     with _on(cand.device) as stream:
         dcand, dwrite, dmemory_in = torch.empty_like(cand), torch.empty_like(cand), torch.empty_like(memory)
@@ -306,6 +318,7 @@ def dropout(x, p: float, seed: int, counter=0, residual=None):
         if not counter.is_cuda or counter.device != x.device or counter.dtype != torch.int64 or counter.numel() != 1:
             raise ValueError("counter must be an int or an int64 tensor of one element on the input's GPU")
         counter, counter_dev = 0, counter
+    _no_tangents("dropout", x, residual)
     if _needs_grad(x, residual):
         return _Dropout.apply(x, residual, float(p), int(seed), int(counter), counter_dev)
     return _dropout_forward(x, residual, p, seed, counter, counter_dev)
@@ -399,6 +412,7 @@ def cross_entropy(logits, targets, ignore_index: int = -100, reduction: str = "m
     a mean over no rows.
     """
     rows, flat = _loss_rows(logits, targets, reduction)
+    _no_tangents("cross_entropy", logits)
     if _needs_grad(logits):
         loss = _CrossEntropy.apply(rows, flat, ignore_index, reduction)
     else:
@@ -417,6 +431,7 @@ def cross_entropy_grad(logits, targets, ignore_index: int = -100, reduction: str
     if dloss is not None:
         _check_like("dloss", dloss, targets.shape if reduction == "none" else (), logits.device)
         dloss = dloss.contiguous()
+    _no_tangents("cross_entropy_grad", logits, dloss)
     if inplace:
         if rows.data_ptr() != logits.data_ptr():
             raise ValueError("inplace needs logits whose rows are one stride apart")
@@ -487,6 +502,7 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx=None):
     if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
     _check_table(*weight.shape)
+    _no_tangents("embedding", weight)
     _check_tokens(tokens, weight.device)
     padding = _check_padding(padding_idx, weight.shape[0])
     if _needs_grad(weight):
@@ -529,6 +545,7 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
             raise ValueError("out must be contiguous")
         if _needs_grad(out):
             raise ValueError("out is written in place: it may not require a gradient")
+    _no_tangents("embedding_grad", dout, out)
     return _embedding_backward(tokens, dout, vocab, scale, padding, out)
 
 
@@ -628,6 +645,7 @@ def newton_schulz(x, steps: int = 5, coefficients=_NS_COEFFICIENTS, eps: float =
         raise TypeError("newton_schulz takes float32 or bfloat16")
     if several:
         _check_matrices("x", x, first.device, first.dtype)
+    _no_tangents("newton_schulz", *(x if several else (x,)))
     if _needs_grad(*(x if several else (x,))):
         raise ValueError("newton_schulz is not differentiable: detach its input")
     a, b, c = coefficients
@@ -678,6 +696,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
             raise ValueError("params and momenta must be contiguous")
         _check_size(*p.shape)
         groups.setdefault((p.shape, p.dtype, p.device), []).append((p, g, m))
+    _no_tangents("muon_step", *params, *grads, *momenta)
     if len(groups) > 1:  # the library sees one group at a time, and all are refused before one is updated
         _check_apart((*params, *momenta), grads)
     for ((rows, cols), dtype, device), members in groups.items():
