@@ -320,3 +320,18 @@ def test_tangents_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_the_embeddings_gradient_is_not_recorded_in_silence():
+    """A dout that wants a gradient would get none: refused, unless nothing is recorded."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        tokens, dout = torch.empty(3, dtype=torch.int64, device="cuda:0"), torch.empty(3, 4, device="cuda:0", requires_grad=True)
+        for d in (dout, dout * 2.0):
+            for out in (None, torch.empty(5, 4, device="cuda:0")):
+                with pytest.raises(ValueError, match="detach"):
+                    ops.embedding_grad(tokens, d, 5, out=out)
+        with torch.no_grad(), pytest.raises(Exception) as error:  # accepted: what fails is the device that is not there
+            ops.embedding_grad(tokens, dout, 5)
+        assert "detach" not in str(error.value)

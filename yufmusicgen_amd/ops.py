@@ -526,7 +526,7 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
 
     ``out`` (a contiguous [vocab, D] tensor of that type, such as the gradient that a
     tied LM head left): the gradient is added to it, and it is returned.  Each row's
-    sum runs over its positions in order, in float32.
+    sum runs over its positions in order, in float32.  Not differentiable.
     """
     if dout.ndim < 1 or tuple(dout.shape[:-1]) != tuple(tokens.shape):
         raise ValueError(f"dout must have shape {list(tokens.shape) + ['D']}, got {list(dout.shape)}")
@@ -545,6 +545,8 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
             raise ValueError("out must be contiguous")
         if _needs_grad(out):
             raise ValueError("out is written in place: it may not require a gradient")
+    if _needs_grad(dout):
+        raise ValueError("embedding_grad is not differentiable: detach dout")
     _no_tangents("embedding_grad", dout, out)
     return _embedding_backward(tokens, dout, vocab, scale, padding, out)
 
