@@ -335,3 +335,15 @@ def test_the_embeddings_gradient_is_not_recorded_in_silence():
         with torch.no_grad(), pytest.raises(Exception) as error:  # accepted: what fails is the device that is not there
             ops.embedding_grad(tokens, dout, 5)
         assert "detach" not in str(error.value)
+
+
+def test_muon_step_names_what_is_no_tensor():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(4, 6, device="cuda:0")
+        for name, k in (("params", 0), ("grads", 1), ("momenta", 2)):
+            lists = [[x, x] for _ in range(3)]
+            lists[k] = [x, None]
+            with pytest.raises(TypeError, match=f"{name} must be tensors, got NoneType"):
+                ops.muon_step(*lists, 0.1)

@@ -677,16 +677,19 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     ``m <- momentum m + (1 - momentum) g``; ``u = momentum m + (1 - momentum) g`` (or ``m`` without
     ``nesterov``); ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``.
 
-    Lists of matrices, of any shapes; those of one shape are updated together.  ``params`` and
-    ``grads`` float32 or bfloat16, ``momenta`` float32.  ``params`` and ``momenta`` must be
-    contiguous.  Parameters that require a gradient are updated like an optimiser does, without
-    being recorded.
+    Lists of matrices, of any shapes; those of one shape are updated together.  A weight
+    without a gradient is left out of all three.  ``params`` and ``grads`` float32 or bfloat16,
+    ``momenta`` float32.  ``params`` and ``momenta`` must be contiguous.  Parameters that
+    require a gradient are updated like an optimiser does, without being recorded.
     """
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f"as many grads and momenta as params: got {len(params)}, {len(grads)} and {len(momenta)}")
     a, b, c = coefficients
     groups = {}
     for p, g, m in zip(params, grads, momenta):
+        for name, x in (("params", p), ("grads", g), ("momenta", m)):
+            if not isinstance(x, torch.Tensor):
+                raise TypeError(f"{name} must be tensors, got {type(x).__name__}: leave a weight without a gradient out of all three lists")
         if not p.is_cuda:
             raise ValueError("params must be on the GPU")
         if p.dtype not in _FLOATS:
