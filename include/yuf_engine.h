@@ -315,8 +315,9 @@ int yuf_embedding_bf16(int64_t M, int V, int D, const uint16_t *table, const voi
                        int token_bits, double scale, uint16_t *out, void *stream);
 
 /*
- * Its gradient by the table: out[v] (+)= scale sum of dout[i] over t_i = v, in the
- * order of positions, in fp32, rounded once.
+ * Its gradient by the table: out[v] (+)= scale sum of dout[i] over t_i = v, in fp32,
+ * rounded once.  The order of summation follows from the sizes and ids alone: runs of
+ * positions in order, whose sums are added in an order of their own.
  *   dout       : device [M, D].
  *   padding    : an id whose row gets no gradient, or -1.  Ids outside [0, V) have
  *                no row to give theirs to.

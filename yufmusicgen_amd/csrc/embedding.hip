@@ -5,7 +5,7 @@
 // once (twice where it is added to).  A thread of the lookup has four vectors of 16 bytes in flight: 16384 rows of
 // 20480 x 640 fp32 take 13.4 us, 6.3 TB/s (they fit the memory-side cache).
 //
-// The gradient's sums run over each token's positions in order, so they do not depend on timing: no
+// The gradient's sums run over each token's positions in an order that sizes and ids fix, not timing: no
 // atomics on values.  Three to five launches:
 //   sort:  a workgroup owns a range of tokens and lists its positions by token.  Its waves take runs of
 //          positions: each counts its tokens, and after a scan over tokens and waves places its positions, in order.
@@ -17,7 +17,7 @@
 //   sum:   a wave walks a chunk of the sorted positions for up to 64 vectors of columns and writes a
 //          token's row where its run ends.  Runs that leave the chunk go to the workspace as fp32 parts.
 //          Further waves clear the rows of tokens that do not occur.
-//   join:  the parts of such a run, in order.
+//   join:  the parts of such a run: up to 16 in order, more as eight sums of every eighth, which are added in order.
 // us of the sort, the sum and the join: 16384 of 20480 x 640 fp32, added, 16, 17.5, 4.7; 262144 of 20480 x 1024 bf16,
 // with a token that has 3.7 % of them, 47, 133 (4.4 TB/s of rows in random order) and 10; 4111 of 673 x 333 bf16,
 // where each is a chain of latencies, 6.7, 8.8, 4.5.
@@ -36,7 +36,9 @@ constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortRanges = 256;  // workgroups of the sort: one per CU
 constexpr int kRangeMost = 960;   // tokens of a range: their counters fill 60 KB of LDS
 // Of more than kManyPositions positions the ranges are written down first, where they are at most kNoRange of at
-// most kWidthMost tokens each.  Both forms, us without and with: 4111 of 673 6.7 and 12.0, 16384 of 20480 24 and 15.6.
+// most kWidthMost tokens each, that is for up to 130560 tokens.  Both forms, us without and with: 4111 of 673 6.7 and 12.0,
+// 16384 of 20480 24 and 15.6, of 130560 27 and 16.2; 262144 of 130560 355 and 39.  Without, each range's workgroup reads
+// all ids, so that a larger table costs as much, and one of millions of narrow rows more than anything else (16384 of 2^24 x 8 1.6 ms).
 constexpr int kManyPositions = 8192;
 constexpr int kNoRange = 255, kWidthMost = 512;
 constexpr int kBlocksMost = 256, kBlockRun = 1024;  // blocks of positions, and positions that a wave reads at a time
@@ -44,7 +46,8 @@ constexpr int kPicks = 4;         // such reads of a wave in flight
 constexpr int kHeld = 12288;      // positions of a range that are kept in LDS (96 KB), beside 32 KB of counters
 // Of more than kSplitPositions positions, ranges with more than kHeavy of them (or a kHeavyShare-th of all) are shared
 // by helpers of half as many each, which costs a launch.  The sort of 187747 of 673, one of them in 44 % of the places:
-// 125 us without and 39 with; with even frequencies 22 and 29.
+// 125 us without and 39 with; with even frequencies 22 and 29.  262144 of 20480, the heaviest range 10500: 41.5 and 47, the
+// helpers having nothing to do.
 constexpr int64_t kSplitPositions = 65536;
 constexpr int kHeavy = 16384, kHeavyShare = 64;
 constexpr int kBatch = 8;         // rows of a wave in flight

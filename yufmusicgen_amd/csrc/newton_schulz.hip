@@ -562,7 +562,8 @@ __global__ void __launch_bounds__(kThreads, 2) ns_product_kernel(Product<T> p) {
 // Matrices of up to 64 rows (the smaller side) and 768 columns as one workgroup each, from the norm to the result: a
 // step's three products depend on each other, and as launches of their own each is mostly waiting (640 x 64 fp32: 78 us as
 // launches, 62 here; 91 with X in memory).  A wave owns every kSmallWaves-th block of 32 columns of X and keeps it in
-// registers, in fp32 and in the accumulators' order; it turns a block into operands through its own part of LDS.  X X^T is summed over the waves in order; A and P lie in LDS.
+// registers, in fp32 and in the accumulators' order; it turns a block into operands through its own part of LDS.  X X^T
+// is summed over the waves in order; A and P lie in LDS.
 constexpr int kSmallWaves = 8, kSmallRows = 64, kSmallBlocks = 3;  // blocks of a wave
 constexpr int kSmallThreads = kSmallWaves * kWave, kSmallColumns = kSmallBlocks * kSmallWaves * 32;
 constexpr int kUpper = 10;  // 16 x 16 blocks of A on and above the diagonal: (i, j) is block j (j + 1) / 2 + i

@@ -525,8 +525,8 @@ def embedding_grad(tokens, dout, vocab: int, scale: float = 1.0, padding_idx=Non
     """Gradient of ``embedding`` by its weight: [vocab, D] for ``dout`` [..., D], in dout's type.
 
     ``out`` (a contiguous [vocab, D] tensor of that type, such as the gradient that a
-    tied LM head left): the gradient is added to it, and it is returned.  Each row's
-    sum runs over its positions in order, in float32.  Not differentiable.
+    tied LM head left): the gradient is added to it, and it is returned.  Each row is
+    summed in float32, in an order that the sizes and ids fix.  Not differentiable.
     """
     if dout.ndim < 1 or tuple(dout.shape[:-1]) != tuple(tokens.shape):
         raise ValueError(f"dout must have shape {list(tokens.shape) + ['D']}, got {list(dout.shape)}")
