@@ -670,3 +670,19 @@ def test_newton_schulz_of_more_matrices_than_a_workspace_holds(kind):
     got = ops.newton_schulz(list(x))
     for i in (0, 7, 8):
         check_ns(got[i], x[i], kind)
+
+
+# ------------------------------------------------- embedding gradients of large vocabularies
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,cols,skew", [(70000, 130561, 5, 3), (100001, 151936, 12, 8), (140000, 151936, 3, 1), (9000, 1 << 24, 1, 3),
+                                                  (8192, 151936, 7, 3), (8193, 151936, 7, 8)])
+def test_embedding_gradient_of_large_vocabularies(rows, vocab, cols, skew, kind):
+    """Beyond 130560 ids, where each range's workgroup reads all positions: long batches with frequent neighbours."""
+    from yufmusicgen_amd import ops
+
+    print(f"embedding gradient {rows} of {vocab} x {cols} skew {skew} {kind}", flush=True)
+    tokens, dout, out = ids(71, (rows,), vocab, skew), table(72, rows, cols, TYPES[kind]), table(73, vocab, cols, TYPES[kind])
+    got = ops.embedding_grad(tokens, dout, vocab, scale=2.0, padding_idx=1)
+    check_grad(got, tokens, dout, vocab, 2.0, padding=1)
+    assert torch.equal(got, ops.embedding_grad(tokens.int(), dout, vocab, scale=2.0, padding_idx=1))
+    check_grad(ops.embedding_grad(tokens, dout, vocab, out=out.clone()), tokens, dout, vocab, 1.0, out=out)
